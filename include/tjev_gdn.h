@@ -304,6 +304,86 @@ int tjev_gdn_gated_rmsnorm_bwd(const tjev_gdn_norm_params* p, void* stream, cons
                                const void* d_y, void* d_x, void* d_gate, float* d_weight,
                                void* workspace, size_t workspace_bytes);
 
+/* ---- The attention layers between the GDN layers (no counterpart in the megakernel) ----
+ *
+ * Rotary positions with several axes (time, height, width), forward (inverse = 0) and its gradient
+ * (inverse = 1: the turn back, on d q and d k). q [batch, length, q_heads, dim] and k (k_heads; either may
+ * have no heads) with strides of their own, in elements, the last dim contiguous; q_out and k_out the
+ * same contiguous, aliasing neither. The first `rotary` lanes of a head are rotary / 2 pairs: lanes i and i + rotary / 2, or
+ * 2i and 2i + 1 (adjacent); the others are passed on. Pair i turns by positions[axis of i] *
+ * inv_freq[i], taken in 64 bits; positions [axes, batch, length] int32 or int64, inv_freq [rotary / 2]
+ * fp32 or fp64. The sections add up to rotary / 2: axis 0 has the first sections[0] pairs and so on;
+ * interleaved, pair i belongs to axis i mod axes while i < axes * sections[i mod axes], to axis 0 otherwise. */
+#define TJEV_GDN_MAX_AXES 4
+typedef struct tjev_gdn_rotary_params {
+  int64_t batch, length;
+  int32_t q_heads, k_heads, dim, rotary;
+  int32_t axes, sections[TJEV_GDN_MAX_AXES];
+  int32_t interleaved, adjacent, inverse;
+  int32_t dtype;                    /* tjev_gdn_dtype of q, k and the outputs */
+  int32_t position_bits, freq_bits; /* 32 or 64 */
+  int32_t reserved;
+  int64_t q_stride[3], k_stride[3]; /* batch, token, head */
+} tjev_gdn_rotary_params;
+int tjev_gdn_rotary(const tjev_gdn_rotary_params* p, void* stream, const void* q, const void* k,
+                    const void* positions, const void* inv_freq, void* q_out, void* k_out);
+
+/* The paged key/value cache of `requests` requests: k_cache and v_cache [pages, page_size, kv_heads,
+ * dim], read through strides; block_table [requests, table_width] int32, the pages of each request's tokens in order. A
+ * token's slot is its page * page_size + its place in the page. An entry outside 0 .. pages - 1 (-1) is
+ * no page. */
+typedef struct tjev_gdn_paged_params {
+  int64_t tokens;                   /* rows of q, k, v and slots */
+  int32_t requests, table_width, pages, page_size;
+  int32_t heads, kv_heads, dim;
+  int32_t dtype;                    /* tjev_gdn_dtype of q, k, v, the caches, gate and out */
+  int32_t fill;                     /* attention: 1 writes 0 to the rows of no request, 0 leaves them */
+  float scale;                      /* attention: of the products q k */
+  int64_t q_stride[2], gate_stride[2], out_stride[2]; /* elements: token, head */
+  int64_t k_stride[3], v_stride[3]; /* elements: the caches' page, slot and head (attention, append) */
+  int64_t k_new_stride[2], v_new_stride[2];           /* append: k's and v's token and head */
+} tjev_gdn_paged_params;
+
+/* Block tables and slot maps of a step: request b holds cached[b] tokens and brings new_tokens[b]
+ * (int32; negative: 0). It keeps the pages of its cached tokens and takes the further ones it needs from free_pages
+ * [n_free] int32, which request 0's, then request 1's ... follow from index taken[0] (null: 0). Writes
+ *   table_out [requests, table_width]  the pages kept, then those taken (-1 where the list is at its end),
+ *                                      -1 behind them; table_out == block_table: only the taken entries
+ *   slots     [tokens] int64           of each new token, requests in order; -1 without a page (past the list or
+ *                                      the table's width) and behind the last request
+ *   starts    [requests + 1] int32     the requests' first tokens
+ *   lengths   [requests] int32         cached + new
+ *   taken_out [1] int32                taken + the pages wanted: more than n_free means a shortage.
+ *                                      Not aliasing taken
+ * tokens, requests (up to TJEV_GDN_MAX_REQUESTS), table_width and page_size of p are read. Sums past 2^31 - 1 stay there. */
+#define TJEV_GDN_MAX_REQUESTS 8192
+int tjev_gdn_paged_tables(const tjev_gdn_paged_params* p, void* stream, const int32_t* cached,
+                          const int32_t* new_tokens, const int32_t* block_table,
+                          const int32_t* free_pages, int64_t n_free, const int32_t* taken,
+                          int32_t* table_out, int64_t* slots, int32_t* starts, int32_t* lengths,
+                          int32_t* taken_out);
+
+/* The write of new tokens: k and v [tokens, kv_heads, dim] into the slots [tokens] int64 of the caches.
+ * A slot outside 0 .. pages * page_size - 1 is skipped; the slots of one call are distinct (two tokens of
+ * one slot leave either's values, or parts of both). */
+int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const void* k, const void* v,
+                          void* k_cache, void* v_cache, const int64_t* slots);
+
+/* Causal attention of new tokens over the paged cache, their own keys and values in it already: rows
+ * starts[b] .. starts[b + 1] - 1 of q [tokens, heads, dim] are request b's last tokens, of lengths[b] in all; token j
+ * stands at lengths[b] - (starts[b + 1] - starts[b]) + j and attends to the keys up to there:
+ *   out = softmax(scale q k^T) v, times sigmoid(gate) when gate [tokens, heads, dim] is not null
+ * with heads / kv_heads query heads to a key head. Keys without a page, or past the table's width, are left out; a row
+ * without keys is 0. Rows of no request: see fill. What a cache holds in other places (NaN too) does not matter.
+ * dim in multiples of 8 up to 256; q, gate, out and the caches 16-byte aligned, with strides that keep
+ * their rows so. The workspace (tjev_gdn_paged_workspace_bytes, 256-byte aligned) needs no
+ * clearing; calls that may overlap need one each. */
+size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p);
+int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const void* q,
+                             const void* k_cache, const void* v_cache, const int32_t* block_table,
+                             const int32_t* starts, const int32_t* lengths, const void* gate,
+                             void* out, void* workspace, size_t workspace_bytes);
+
 /* Per-kernel timing (no counterpart in the reference, whose kernels are timed by xprof):
  * between tjev_gdn_profile_begin() and tjev_gdn_profile_end(), every launch of the megakernel
  * and norm calls is bracketed by a hipEvent pair on the call's stream. _end synchronizes those events

@@ -47,6 +47,11 @@ EXPORTS = (
     "tjev_gdn_norm_workspace_bytes",
     "tjev_gdn_gated_rmsnorm_fwd",
     "tjev_gdn_gated_rmsnorm_bwd",
+    "tjev_gdn_rotary",
+    "tjev_gdn_paged_tables",
+    "tjev_gdn_paged_append",
+    "tjev_gdn_paged_workspace_bytes",
+    "tjev_gdn_paged_attention",
     "tjev_gdn_profile_begin",
     "tjev_gdn_profile_end",
     "tjev_gdn_kernel_name",
@@ -72,6 +77,33 @@ class NormParams(ctypes.Structure):
 
     _fields_ = [("tokens", ctypes.c_int64), ("heads", ctypes.c_int32), ("dim", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+MAX_AXES = 4  # TJEV_GDN_MAX_AXES
+MAX_REQUESTS = 8192  # TJEV_GDN_MAX_REQUESTS
+
+
+class RotaryParams(ctypes.Structure):
+    """tjev_gdn_rotary_params"""
+
+    _fields_ = [("batch", ctypes.c_int64), ("length", ctypes.c_int64),
+                *((n, ctypes.c_int32) for n in ("q_heads", "k_heads", "dim", "rotary", "axes")),
+                ("sections", ctypes.c_int32 * MAX_AXES),
+                *((n, ctypes.c_int32) for n in ("interleaved", "adjacent", "inverse", "dtype", "position_bits",
+                                                "freq_bits", "reserved")),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3)]
+
+
+class PagedParams(ctypes.Structure):
+    """tjev_gdn_paged_params"""
+
+    _fields_ = [("tokens", ctypes.c_int64),
+                *((n, ctypes.c_int32) for n in ("requests", "table_width", "pages", "page_size", "heads", "kv_heads",
+                                                "dim", "dtype", "fill")),
+                ("scale", ctypes.c_float),
+                *((n, ctypes.c_int64 * 2) for n in ("q_stride", "gate_stride", "out_stride")),
+                *((n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride")),
+                *((n, ctypes.c_int64 * 2) for n in ("k_new_stride", "v_new_stride"))]
 
 
 class Merge(ctypes.Structure):
@@ -175,6 +207,17 @@ def open_library(path: Path) -> ctypes.CDLL:
     lib.tjev_gdn_gated_rmsnorm_fwd.restype = i32
     lib.tjev_gdn_gated_rmsnorm_bwd.argtypes = [npp, vp] + [vp] * 9 + [sz]
     lib.tjev_gdn_gated_rmsnorm_bwd.restype = i32
+    rpp, gpp, i64 = ctypes.POINTER(RotaryParams), ctypes.POINTER(PagedParams), ctypes.c_int64
+    lib.tjev_gdn_rotary.argtypes = [rpp, vp] + [vp] * 6
+    lib.tjev_gdn_rotary.restype = i32
+    lib.tjev_gdn_paged_tables.argtypes = [gpp, vp] + [vp] * 4 + [i64] + [vp] * 6
+    lib.tjev_gdn_paged_tables.restype = i32
+    lib.tjev_gdn_paged_append.argtypes = [gpp, vp] + [vp] * 5
+    lib.tjev_gdn_paged_append.restype = i32
+    lib.tjev_gdn_paged_workspace_bytes.argtypes = [gpp]
+    lib.tjev_gdn_paged_workspace_bytes.restype = sz
+    lib.tjev_gdn_paged_attention.argtypes = [gpp, vp] + [vp] * 9 + [sz]
+    lib.tjev_gdn_paged_attention.restype = i32
     lib.tjev_gdn_profile_begin.argtypes = []
     lib.tjev_gdn_profile_begin.restype = i32
     lib.tjev_gdn_profile_end.argtypes = [ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int), i32]
@@ -229,6 +272,17 @@ def current_stream(device: torch.device) -> int:
         raise ValueError(f"expected a GPU device, not {device}")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: a launch goes to the current device, whatever stream it names.
+    Nothing is entered where it is current already (1 us of a small call)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def check_status(status: int, lib: ctypes.CDLL | None = None) -> None:
