@@ -137,16 +137,17 @@ def test_attention(dtype, heads, kv_heads, dim, page, lens):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("page", [16, 10])
-def test_pages_that_are_none(dtype, page):
+@pytest.mark.parametrize("heads", [4, 16])
+def test_pages_that_are_none(dtype, page, heads):
     """A table's entries -1 or past the cache hold no keys: what is left is attended to, and a row without
     any is 0. Lengths past the table's width end there; lengths shorter than the new tokens leave rows empty."""
-    case = batch(torch.Generator().manual_seed(5), [(200, 4), (90, 20), (33, 1), (0, 7)], heads=4, kv_heads=2, dim=64, page=page, dtype=dtype)
+    case = batch(torch.Generator().manual_seed(5), [(200, 4), (90, 20), (33, 1), (0, 7)], heads=heads, kv_heads=2, dim=64, page=page, dtype=dtype)
     t = case["block_table"]
     t[0, 1], t[0, 3], t[1, 0], t[2, :] = -1, case["k_cache"].shape[0], 2 ** 31 - 1, -2 ** 31
     case["lengths"][0] += 3000  # behind the table: the keys end with it
     case["lengths"][3] = 4      # three of its seven tokens stand before the first
     t[0][t[0] == -1] = 10 ** 6
-    print(f"attention over pages that are none {dtype} page={page}", flush=True)
+    print(f"attention over pages that are none {dtype} page={page} heads={heads}", flush=True)
     want, room = attention64(*(case[n] for n in ("q", "k_cache", "v_cache", "block_table", "starts", "lengths")))
     got = _attend(case)
     compare(got, want, room)
@@ -258,6 +259,15 @@ def test_offsets_past_32_bits():
     got = paged_attention(q.cuda(), kc, vc, table.cuda(), starts.cuda(), lengths.cuda())
     want, room = attention64(q, *small, torch.tensor([[0, 1, 2]], dtype=torch.int32), starts, lengths)
     compare(got, want, room)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+def test_scales(dtype, scale):
+    case = batch(torch.Generator().manual_seed(13), [(60, 2), (30, 90), (9, 1)], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    print(f"attention {dtype} scale={scale}", flush=True)
+    want, room = attention64(*(case[n] for n in ("q", "k_cache", "v_cache", "block_table", "starts", "lengths")), scale)
+    compare(_attend(case, scale=scale), want, room)
 
 
 def test_no_tokens():

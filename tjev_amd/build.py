@@ -34,6 +34,8 @@ FLAGS = [
 # units built once: the C ABI, the gated RMSNorm, the decode step, the merged LoRA projections, and the
 # attention layers' rotary positions, page tables and paged attention
 EXTRA_UNITS = ("gdn_api", "gdn_norm", "gdn_decode", "gdn_lora", "gdn_rotary", "gdn_paged", "gdn_attention")
+# paged attention: one object per type and head dim (gdn_attn_inst.hip)
+ATTENTION = [(t, d) for t in ("bf16", "f32") for d in (64, 128, 256)]
 # object files per (chunk, head dim) pair: the launch sequences with the small kernels (part 0),
 # then one per large kernel family (gdn_inst.hip's GDN_PART)
 PARTS = 6
@@ -46,6 +48,11 @@ PART_FLAGS = {(128, 128, 3): ["-mllvm", "--amdgpu-sched-strategy=max-memory-clau
 def unit_flags(c: int, d: int, part: int) -> list[str]:
     """The defines and backend options of one gdn_inst.hip object."""
     return [f"-DGDN_C={c}", f"-DGDN_D={d}", f"-DGDN_PART={part}", *PART_FLAGS.get((c, d, part), [])]
+
+
+def attention_flags(t: str, d: int) -> list[str]:
+    """The defines of one gdn_attn_inst.hip object."""
+    return [f"-DGDN_T={t}", f"-DGDN_D={d}"]
 
 
 def shapes(lds_poison: bool = False) -> list[tuple[int, int]]:
@@ -90,6 +97,9 @@ def build(jobs: int | None = None, verbose: bool = False, verify: bool = True, l
                           str(obj)])
     for name in EXTRA_UNITS:
         units.append([hipcc, *FLAGS, *extra, "-c", str(CSRC / f"{name}.hip"), "-o", str(out / f"{name}.o")])
+    for t, d in ATTENTION:
+        units.insert(0, [hipcc, *FLAGS, *extra, *attention_flags(t, d), "-c", str(CSRC / "gdn_attn_inst.hip"), "-o",
+                         str(out / f"gdn_attn_{t}_{d}.o")])
     t0 = time.time()
     with ThreadPoolExecutor(max_workers=jobs or min(len(units), os.cpu_count() or 4)) as pool:
         checks = []
@@ -99,6 +109,7 @@ def build(jobs: int | None = None, verbose: bool = False, verify: bool = True, l
             checks = [pool.submit(check_source, CSRC / "gdn_inst.hip", [*extra, *unit_flags(c, d, part)])
                       for c, d in shapes(lds_poison) for part in range(PARTS)]
             checks += [pool.submit(check_source, CSRC / f"{name}.hip", extra) for name in EXTRA_UNITS]
+            checks += [pool.submit(check_source, CSRC / "gdn_attn_inst.hip", [*extra, *attention_flags(t, d)]) for t, d in ATTENTION]
         list(pool.map(_run, units))
         bad = [line for f in checks for line in f.result()]
     if bad:

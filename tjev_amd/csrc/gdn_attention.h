@@ -1,0 +1,1198 @@
+// Causal attention of new tokens over the paged key/value cache for gfx950 (the full-attention layers
+// that stand between the GDN layers), from one token per request to chunks of a prompt:
+//   o_r = sum_k p_rk v_k / sum_k p_rk,  p_rk = 2^(c q_r k_k - m_r),  c = scale log2(e),
+// one pass over the keys with the running maximum m_r and sum of each row in 32 bits.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "gdn_device.h"
+#include "gdn_paged.h"
+
+namespace gdn {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kNegInf = -__builtin_inff();
+
+// ---------------------------------------------------------------- the stream's plan
+// All units of a batch (gdn_paged.h) in a line (request, tile, key head, keys) are cut into G equal ranges, one
+// per workgroup, so that requests of very different lengths keep every CU busy to the end, whatever
+// the host knows of them.
+
+// a value that is the same in all lanes, held once
+__device__ __forceinline__ long uniform(long v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+  return (long)((uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Request uniform(const Request& q) {
+  return {uniform(q.s0), uniform(q.rows), uniform(q.tiles), uniform(q.tile_rows), uniform(q.keys), uniform(q.blocks), uniform(q.y),
+          uniform(q.g), uniform(q.first), uniform(q.per_head), uniform(q.cost)};
+}
+
+// The kernel's arguments read anew: what a tile needs of them is then held for the tile only, and not (spilled)
+// across the whole kernel.
+__device__ __forceinline__ const AttnArgs& arguments() {
+  auto p = (const __attribute__((address_space(4))) AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttnArgs*)p;
+}
+
+// The lane, counted anew: values taken from it are not held (or spilled: a spilled value's load waits for all
+// loads on their way) from before.
+__device__ __forceinline__ int lane_anew() {
+  int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
+// inclusive running sum over the workgroup's threads (in order); total: the sum of all
+__device__ __forceinline__ long scan_block(long v, long* swave, long& total) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long t = __shfl_up(v, d);
+    if (lane() >= d) v += t;
+  }
+  __syncthreads();
+  if (lane() == 63) swave[wave()] = v;
+  __syncthreads();
+  total = 0;
+  long before = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave()) before += swave[w];
+    total += swave[w];
+  }
+  return v + before;
+}
+
+// What a workgroup finds out of the batch: the units of each range, the request that its range begins with and that
+// request's first unit. b = -1: the range is empty.
+struct Found {
+  long total, each, unit;
+  int b;
+  Request q;
+};
+struct FoundLds {
+  long swave[kThreads / 64], unit;
+  int b;
+  Request q;
+};
+
+// Up to kThreads requests are read and summed once, more of them in turns, twice.
+template <int R, int KB>
+__device__ __forceinline__ Found find_range(const AttnArgs& A, int range, FoundLds& f) {
+  const int tid = threadIdx.x;
+  const bool once = A.B <= kThreads;
+  Found r;
+  Request q{};
+  long units = 0, sum = 0;  // the thread's inclusive sum, the batch's
+  auto load = [&](int b) {
+    q = Request{};
+    if (b < A.B) q = request<R, KB>(A, b);
+  };
+  if (tid == 0) f.b = -1;
+  if (once) {
+    load(tid);
+    units = scan_block(q.cost, f.swave, sum);
+  } else {
+    long mine = 0;
+    for (int b0 = 0; b0 < A.B; b0 += kThreads) {
+      load(b0 + tid);
+      mine += q.cost;
+    }
+    scan_block(mine, f.swave, sum);
+  }
+  r.total = sum;
+  r.each = sum ? (sum + A.G - 1) / A.G : 1;
+  const long place = range * r.each;
+  long before = 0;
+  for (int b0 = 0; b0 < A.B; b0 += kThreads) {
+    if (!once) {
+      load(b0 + tid);
+      units = scan_block(q.cost, f.swave, sum) + before;
+      before += sum;
+    }
+    if (place >= units - q.cost && place < units) {
+      f.b = b0 + tid;
+      f.q = q;
+      f.unit = units - q.cost;
+    }
+    if (!once && before > place) break;
+  }
+  __syncthreads();
+  r.b = uniform(f.b);
+  if (r.b >= 0) {
+    r.q = uniform(f.q);
+    r.unit = uniform(f.unit);
+  }
+  return r;
+}
+
+// ---------------------------------------------------------------- fragments
+// Scores are computed transposed, 16 keys by 16 rows per MFMA, K from the first operand: a lane's four
+// results are keys 4 (lane / 16) .. + 3 of row lane % 16, which is the layout of the second operand of
+// out^T += V^T P^T when the contraction takes the keys in that order; V's fragments are read in the same
+// order, straight from memory: a lane loads VE consecutive values of each of its keys, and value e of them
+// is the first operand of the e-th MFMA (rows d = VE m + e). So neither P nor V passes through LDS; in bf16
+// the 8 keys by 8 values of a lane are transposed by byte permutes.
+template <class T, int DT>
+struct Shape {
+  static constexpr bool BF = sizeof(T) == 2;
+  static constexpr int KG = BF ? 2 : 1;                 // groups of 16 keys per step of a wave
+  static constexpr int E = 16 / (int)sizeof(T);         // elements of a 16-byte piece
+  static constexpr int KS = DT / (4 * E);               // pieces of a K or Q fragment row
+  static constexpr int VE = BF && DT >= 128 ? 8 : 4;    // V's values per lane and key
+  static constexpr int VH = DT / (16 * VE);
+  static constexpr int KB = 64 * KG;                    // keys of a unit: a step of each of four waves
+  using VVec = std::conditional_t<VE * sizeof(T) == 16, uint4, uint2>;
+};
+
+typedef uint32_t u32;
+__device__ __forceinline__ u32 word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ u32 word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
+
+template <class T, int DT>
+__device__ __forceinline__ f32x4 dot_step(const uint4& k, const uint4& q, f32x4 acc) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(word(k, e)), __uint_as_float(word(q, e)), acc, 0, 0, 0);
+    return acc;
+  }
+}
+
+// max or sum over the four lanes that hold one row (lane % 16)
+__device__ __forceinline__ float rows_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+// the base of the powers: 0 where a row has seen no key yet, so that its powers are 0 and not NaN
+__device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
+
+// out += P V for one step (KG groups of 16 keys). V [key group][r]: the lane's keys 4 (lane / 16) + r
+template <class T, int DT, int NQ>
+__device__ __forceinline__ void add_pv(const typename Shape<T, DT>::VVec (&v)[Shape<T, DT>::KG][4][Shape<T, DT>::VH],
+                                       const f32x4 (&p)[Shape<T, DT>::KG][NQ],
+                                       f32x4 (&o)[NQ][Shape<T, DT>::VH][Shape<T, DT>::VE]) {
+  using S = Shape<T, DT>;
+  if constexpr (S::BF) {
+    bf16x8 pb[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)  // rounded to bf16 for the product, as V is: the sums stay in 32 bits
+      pb[n] = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[0][n][0], p[0][n][1]), pack2(p[0][n][2], p[0][n][3]),
+                                                    pack2(p[1][n][0], p[1][n][1]), pack2(p[1][n][2], p[1][n][3])));
+#pragma unroll
+    for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) {
+        const u32 sel = e % 2 ? 0x07060302u : 0x05040100u;
+        u32 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = __builtin_amdgcn_perm(word(v[i / 2][2 * (i % 2) + 1][h], e / 2), word(v[i / 2][2 * (i % 2)][h], e / 2), sel);
+        const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[n][h][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[n], o[n][h][e], 0, 0, 0);
+      }
+  } else {
+#pragma unroll
+    for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+            o[n][h][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(word(v[0][r][h], e)), p[0][n][r], o[n][h][e], 0, 0, 0);
+  }
+}
+
+template <class T, class W>
+__device__ __forceinline__ bool not_finite(const W& v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(W) / 4); ++i) {
+    const u32 w = word(v, i);
+    if constexpr (sizeof(T) == 2) {
+      bad = bad || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    } else {
+      bad = bad || (w & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  return bad;
+}
+
+// Infinities and NaN among values that some rows of a tile attend to and others do not: a product would
+// give the others 0 * NaN. They are counted instead, by a product of marks (1 for infinity, 128 for minus infinity,
+// 16384 for NaN; at most 64 of each, so the sum is exact) with ones for the keys a row attends to, and
+// the counted values added to its result; the values themselves become 0.
+__device__ __forceinline__ float special_of(float count) {
+  const int n = (int)count;
+  const float inf = __builtin_inff();
+  const bool pos = n & 127, neg = (n >> 7) & 127, nan = n >> 14;
+  return nan || (pos && neg) ? __builtin_nanf("") : pos ? inf : neg ? -inf : 0.f;
+}
+// the mark of one bf16 value (bits) as bf16 bits
+__device__ __forceinline__ u32 mark_of(u32 h) {
+  return (h & 0x7f80u) != 0x7f80u ? 0u : (h & 0x7fu) ? 0x4680u : (h & 0x8000u) ? 0x4300u : 0x3f80u;
+}
+__device__ __forceinline__ u32 marks_of(u32 w) { return mark_of(w & 0xffffu) | mark_of(w >> 16) << 16; }
+__device__ __forceinline__ u32 finite_of(u32 w) {
+  return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+
+__device__ __forceinline__ void zero_word(uint4& v) { v = make_uint4(0, 0, 0, 0); }
+__device__ __forceinline__ void zero_word(uint2& v) { v = make_uint2(0, 0); }
+
+__device__ __forceinline__ void set_word(uint4& v, int i, u32 w) { (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = w; }
+__device__ __forceinline__ void set_word(uint2& v, int i, u32 w) { (i == 0 ? v.x : v.y) = w; }
+
+template <class T, int DT>
+using VStep = typename Shape<T, DT>::VVec[Shape<T, DT>::KG][4][Shape<T, DT>::VH];
+
+template <class T, int DT, int NQ>
+__device__ __forceinline__ void add_special(VStep<T, DT>& v,
+                                            const bool (&on)[Shape<T, DT>::KG][4][NQ],
+                                            f32x4 (&o)[NQ][Shape<T, DT>::VH][Shape<T, DT>::VE]) {
+  using S = Shape<T, DT>;
+#pragma unroll
+  for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+    for (int e = 0; e < S::VE; ++e)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (S::BF) {
+          u32 w[4], p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = i / 2, r = 2 * (i % 2), sh = 16 * (e % 2);
+            w[i] = mark_of(word(v[j][r][h], e / 2) >> sh & 0xffffu) | mark_of(word(v[j][r + 1][h], e / 2) >> sh & 0xffffu) << 16;
+            p[i] = (on[j][r][n] ? 0x3f80u : 0u) | (on[j][r + 1][n] ? 0x3f800000u : 0u);
+          }
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3])),
+                                                        __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])), acc, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const u32 x = word(v[0][r][h], e);
+            const float mark = (x & 0x7f800000u) != 0x7f800000u ? 0.f : (x & 0x7fffffu) ? 16384.f : (x >> 31) ? 128.f : 1.f;
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(mark, on[0][r][n] ? 1.f : 0.f, acc, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[n][h][e][r] += special_of(acc[r]);
+      }
+#pragma unroll
+  for (int j = 0; j < S::KG; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(typename S::VVec) / 4); ++i) {
+          const u32 x = word(v[j][r][h], i);
+          set_word(v[j][r][h], i, S::BF ? finite_of(x) : (x & 0x7f800000u) == 0x7f800000u ? 0u : x);
+        }
+}
+
+// a row's 4 x VE consecutive results, divided by its sum, gated, rounded once and stored
+template <class T, int DT, bool PAD>
+__device__ __forceinline__ void store_row(const AttnArgs& A, const f32x4 (&o)[Shape<T, DT>::VH][Shape<T, DT>::VE], float l, long token,
+                                          int head) {
+  using S = Shape<T, DT>;
+  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+  for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = h * 16 * S::VE + (4 * (lane() / 16) + r) * S::VE;
+      if (PAD && d >= A.D) continue;
+      float x[S::VE];
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) x[e] = o[h][e][r] * inv;
+      if (A.gate) {
+        const T* gp = reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + d;
+#pragma unroll
+        for (int e = 0; e < S::VE; ++e) x[e] *= sigmoidf_(ldf(gp + e));
+      }
+      T* op = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d;
+      if constexpr (S::VE == 8) {
+        st8_io(op, x);
+      } else {
+        st4_io(op, x);
+      }
+    }
+}
+
+// ---------------------------------------------------------------- the workgroups' ranges
+// A range's first tile goes to slot 2 i of the workspace unless the range holds all its keys, its last, when it
+// goes on behind the range's end, to slot 2 i + 1.
+struct Part {
+  float* p;       // where the tile's rows go, or null: they are finished here
+  int tile, head;
+};
+
+template <int DT>
+constexpr int slot_floats(int rows) { return rows * (DT + 2); }
+
+// The tile that begins in a range and goes on behind it, for the kernel that joins its parts: the first lies in
+// slot `first`, the others are the first ones of the next ranges. parts = 0: there is none.
+struct Split {
+  int parts, first, s0, rows, tile_rows, tile, head, pad;
+};
+static_assert(sizeof(Split) == kSplitBytes, "the workspace's last part");
+
+// the workgroup's i-th range: consecutive ranges stay on one XCD (its L2 holds the keys that they share)
+__device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block : (block % 8) * (G / 8) + block / 8; }
+
+// ---------------------------------------------------------------- few rows: keys streamed
+// The four waves take steps of KG * 16 keys in turn, each with a running maximum, sum and result of its
+// own, joined in LDS at the end. Bound by memory: the keys and values are read once, straight into registers.
+// WHOLE: pages hold whole groups of 16 keys, whose page is then one value per wave.
+template <class T, int DT, int NQ>
+struct StreamLds {
+  static constexpr int NV = NQ * Shape<T, DT>::VH * Shape<T, DT>::VE;  // result registers of four
+  static constexpr int HALF = NV >= 32 ? NV / 2 : NV;                  // joined at a time
+  static constexpr int Q = NQ * Shape<T, DT>::KS * 64, ACC = 2 * HALF * 64;  // pieces of 16 bytes
+};
+
+template <class T, int DT, int NQ, bool PAD, bool WHOLE>
+__device__ __forceinline__ void stream_tile(const Request& q, int b, const Part& part, int kb0, int seg, uint4* sq,
+                                            f32x4* sacc, float (&sm)[4][16 * NQ], float (&sl)[4][16 * NQ]) {
+  using S = Shape<T, DT>;
+  constexpr int R = 16 * NQ, KB = S::KB, KG = S::KG, E = S::E;
+  constexpr int NV = StreamLds<T, DT, NQ>::NV, HALF = StreamLds<T, DT, NQ>::HALF;
+  const AttnArgs& A = arguments();
+  const int w = __builtin_amdgcn_readfirstlane(wave()), ln = lane(), r16 = ln & 15, g4 = ln >> 4;
+  const int row0 = part.tile * R, h = part.head;
+  // the queries, staged once for the four waves in the order of the fragments
+  for (int x = w; x < NQ * S::KS; x += 4) {
+    const int n = x / S::KS, i = x - n * S::KS, row = row0 + n * 16 + r16, e = (4 * i + g4) * E;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < q.rows && !(PAD && e >= A.D)) {
+      const int t = row / A.g;
+      v = *reinterpret_cast<const uint4*>(A.q + (long)(q.s0 + t) * A.qt + (h * A.g + (row - t * A.g)) * A.qh + e * (int)sizeof(T));
+    }
+    sq[x * 64 + ln] = v;
+  }
+  int lim[NQ];  // the lane's row of each row tile: its last key + 1
+  float m[NQ], l[NQ];
+  f32x4 o[NQ][S::VH][S::VE];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = row0 + n * 16 + r16;
+    lim[n] = row < q.rows ? row_limit(q, row, A.g) : 0;
+    m[n] = kNegInf;
+    l[n] = 0.f;
+#pragma unroll
+    for (int x = 0; x < S::VH; ++x)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) o[n][x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int lo_lim = uniform(row_limit(q, row0, A.g)), hi_lim = uniform(row_limit(q, min(row0 + R, q.rows) - 1, A.g));
+  const int32_t* table = A.table + (long)b * A.M;
+  const char *kc = A.k + h * A.kh, *vc = A.v + h * A.vh;
+  __syncthreads();
+
+  for (int kb = kb0; kb < kb0 + seg; ++kb) {
+    const int k0 = kb * KB + w * 16 * KG;
+    if (k0 >= hi_lim) break;
+    uint4 kf[KG][S::KS];
+    typename S::VVec vf[KG][4][S::VH];
+    bool ok[KG][4];  // the lane's keys 4 g4 + r have a page
+    bool all_ok = true;
+#pragma unroll
+    for (int j = 0; j < KG; ++j) {
+      const int key0 = k0 + 16 * j;
+      const char *krow, *vrow[4];
+      if constexpr (WHOLE) {
+        // the group lies in one page: its first key's, a group behind the last key the step's first one's
+        const Place at = place_of(A, table, key0 < q.keys ? key0 : k0, q.keys);
+        const long p = __builtin_amdgcn_readfirstlane(at.page), in = at.in;
+        const bool good = __builtin_amdgcn_readfirstlane(at.good);
+        all_ok = all_ok && good;
+        krow = kc + p * A.kp + (in + r16) * A.ks;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          vrow[r] = vc + p * A.vp + (in + 4 * g4 + r) * A.vs;
+          ok[j][r] = good;
+        }
+      } else {
+        const Place at = place_of(A, table, key0 + r16, q.keys);
+        krow = kc + at.page * A.kp + at.in * A.ks;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const Place pv = place_of(A, table, key0 + 4 * g4 + r, q.keys);
+          vrow[r] = vc + pv.page * A.vp + pv.in * A.vs;
+          ok[j][r] = pv.good;
+          all_ok = all_ok && pv.good;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S::KS; ++i) {
+        const int e = (4 * i + g4) * E;
+        kf[j][i] = PAD && e >= A.D ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(krow + e * (int)sizeof(T));
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int x = 0; x < S::VH; ++x) {
+          const int d = (16 * x + r16) * S::VE;
+          if (PAD && d >= A.D) {
+            zero_word(vf[j][r][x]);
+          } else {
+            vf[j][r][x] = *reinterpret_cast<const typename S::VVec*>(vrow[r] + d * (int)sizeof(T));
+          }
+        }
+    }
+    const bool bad_page = WHOLE ? !all_ok : __any(!all_ok);
+
+    f32x4 s[KG][NQ];
+#pragma unroll
+    for (int j = 0; j < KG; ++j)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < S::KS; ++i)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const uint4 qf = sq[(n * S::KS + i) * 64 + ln];
+#pragma unroll
+        for (int j = 0; j < KG; ++j) s[j][n] = dot_step<T, DT>(kf[j][i], qf, s[j][n]);
+      }
+#pragma unroll
+    for (int j = 0; j < KG; ++j)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[j][n] *= A.c;
+    const bool masked = k0 + 16 * KG > lo_lim || bad_page;
+    bool careful = false;
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < KG; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = k0 + 16 * j + 4 * g4 + r;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[j][n][r] = key < lim[n] && ok[j][r] ? s[j][n][r] : kNegInf;
+          // what no row attends to must not meet its zero weight: 0 * NaN
+          if (key >= hi_lim || !ok[j][r])
+#pragma unroll
+            for (int x = 0; x < S::VH; ++x) zero_word(vf[j][r][x]);
+        }
+      if (lo_lim < hi_lim) {
+#pragma unroll
+        for (int j = 0; j < KG; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int x = 0; x < S::VH; ++x) careful = careful || not_finite<T>(vf[j][r][x]);
+        careful = __any(careful);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float t = kNegInf;
+#pragma unroll
+      for (int j = 0; j < KG; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t = fmaxf(t, s[j][n][r]);
+      const float mn = fmaxf(m[n], rows_max(t)), base = base_of(mn), a = __builtin_amdgcn_exp2f(m[n] - base);
+      m[n] = mn;
+      l[n] *= a;
+#pragma unroll
+      for (int j = 0; j < KG; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[j][n][r] = __builtin_amdgcn_exp2f(s[j][n][r] - base);
+          l[n] += s[j][n][r];
+        }
+#pragma unroll
+      for (int x = 0; x < S::VH; ++x)
+#pragma unroll
+        for (int e = 0; e < S::VE; ++e) o[n][x][e] *= a;
+    }
+    if (careful) {
+      bool on[KG][4][NQ];
+#pragma unroll
+      for (int j = 0; j < KG; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) on[j][r][n] = k0 + 16 * j + 4 * g4 + r < lim[n];
+      add_special<T, DT, NQ>(vf, on, o);
+    }
+    add_pv<T, DT, NQ>(vf, s, o);
+  }
+
+  // the four waves' rows joined
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    l[n] = rows_sum(l[n]);
+    if (g4 == 0) sm[w][n * 16 + r16] = m[n], sl[w][n * 16 + r16] = l[n];
+  }
+  __syncthreads();
+  float mj[NQ], lj[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    mj[n] = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mj[n] = fmaxf(mj[n], sm[i][n * 16 + r16]);
+    const float base = base_of(mj[n]);
+    lj[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lj[n] += sl[i][n * 16 + r16] * __builtin_amdgcn_exp2f(sm[i][n * 16 + r16] - base);
+    const float a = __builtin_amdgcn_exp2f(m[n] - base);
+#pragma unroll
+    for (int x = 0; x < S::VH; ++x)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) o[n][x][e] *= a;
+  }
+  auto each_reg = [&](int from, auto f) {  // registers from .. from + HALF - 1
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int x = 0; x < S::VH; ++x)
+#pragma unroll
+        for (int e = 0; e < S::VE; ++e) {
+          const int v = (n * S::VH + x) * S::VE + e;
+          if (v >= from && v < from + HALF) f((v - from) * 64 + ln, o[n][x][e]);
+        }
+  };
+#pragma unroll
+  for (int from = 0; from < NV; from += HALF) {
+    if (w >= 2) each_reg(from, [&](int i, f32x4& x) { sacc[(w - 2) * HALF * 64 + i] = x; });
+    __syncthreads();
+    if (w < 2) each_reg(from, [&](int i, f32x4& x) { x += sacc[w * HALF * 64 + i]; });
+    __syncthreads();
+    if (w == 1) each_reg(from, [&](int i, f32x4& x) { sacc[i] = x; });
+    __syncthreads();
+    if (w == 0) each_reg(from, [&](int i, f32x4& x) { x += sacc[i]; });
+    __syncthreads();
+  }
+  if (w == 0) {
+    if (!part.p) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int row = row0 + n * 16 + r16, t = row / A.g;
+        if (row < q.rows) store_row<T, DT, PAD>(A, o[n], lj[n], q.s0 + t, h * A.g + (row - t * A.g));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int x = 0; x < S::VH; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {  // rows of DT values
+            float* po = part.p + (n * 16 + r16) * DT + (x * 16 + 4 * g4 + r) * S::VE;
+#pragma unroll
+            for (int e = 0; e < S::VE; e += 4)
+              *reinterpret_cast<f32x4*>(po + e) = f32x4{o[n][x][e][r], o[n][x][e + 1][r], o[n][x][e + 2][r], o[n][x][e + 3][r]};
+          }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+        if (g4 == 0) {
+          part.p[R * DT + n * 16 + r16] = mj[n];
+          part.p[R * (DT + 1) + n * 16 + r16] = lj[n];
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- many rows: tiles of 128 (bf16)
+// Four waves of 32 rows each. K and V pass through LDS, TK keys at a time in two buffers, brought there by
+// 16-byte loads that do not touch registers; scores are again transposed (32 keys by 32 rows per MFMA), so that a
+// row's weights stay in its two lanes and are the second operand of out^T += V^T P^T as they come, V's
+// fragments by transposing LDS reads. The pieces of a row of K or V lie in LDS in an order that depends on the row
+// (swz), which spreads both kinds of read over the banks.
+// The base of the powers follows the running maximum only when that has grown by more than 2^8: the rescaling
+// of the results is skipped otherwise (a softmax does not depend on its base; weights up to 2^8 have bf16's
+// relative precision like all others).
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+template <int DT>
+struct Wide {
+  static constexpr int TK = DT == 256 ? 32 : 64;  // keys per buffer
+  static constexpr int NS = TK / 32, CPR = DT / 8, RW = TK / 4, RI = 64 / CPR, NI = RW / RI;
+  static constexpr int QL = DT == 256 ? 2 : 0;  // fragments of a wave's queries kept in LDS: what the registers cannot hold
+  static constexpr int SPAN = CPR >= 16 ? 256 : 128;  // bytes within which the pieces of a row are exchanged
+  // the place of piece c of row r: c ^ swz(r)
+  static constexpr __device__ __forceinline__ int swz(int r) {
+    return CPR >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 1) << 2) | ((r >> 1) & 3);
+  }
+};
+
+__device__ __forceinline__ i16x4 read_tr(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
+}
+
+// the pieces of 16 bytes that a wave's lanes address, to consecutive places of LDS
+__device__ __forceinline__ void load_to_lds(const char* from, uint16_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <int DT, bool PAD, bool WHOLE>
+struct WideTile {
+  using W = Wide<DT>;
+  static constexpr int TK = W::TK, NS = W::NS;
+  const AttnArgs& A;
+  const Request& q;
+  const int32_t* table;
+  const char *kc, *vc;
+  int w, k_first;
+  u32 (*sbad)[4];  // [buffer][wave]: keys without a page
+
+  // The table's entry for this wave's rows of the keys k0 .. k0 + TK - 1: of all of them (WHOLE: they lie in one
+  // page; a group behind the last key stands for the range's first), or of the lane's. Loaded a buffer ahead of its use.
+  __device__ __forceinline__ int first_key(int k0) const {
+    const int key0 = k0 + w * W::RW;
+    return key0 < q.keys ? key0 : k_first;
+  }
+  __device__ __forceinline__ int lane_key(int k0) const { return min(k0 + w * W::RW + lane_anew() % W::RW, q.keys - 1); }
+  __device__ __forceinline__ int look(int k0) const { return table[page_of(A, WHOLE ? first_key(k0) : lane_key(k0))]; }
+
+  // those rows on their way to LDS
+  __device__ __forceinline__ void issue(int k0, int entry, int buf, uint16_t* sk, uint16_t* sv) const {
+    const int ln = lane_anew(), rl = ln / W::CPR, pos = ln % W::CPR;
+    const bool good = entry >= 0 && entry < A.pages;
+    const int page = good ? entry : 0;
+    const unsigned long bad = WHOLE ? (good ? 0ul : ~0ul) : __ballot(!good && ln < W::RW);
+    if (ln == 0) sbad[buf][w] = (u32)bad;
+    // a row's pieces are exchanged by swz(row): the lane's part of it, and below the part of i
+    const u32 piece = (u32)(pos ^ W::swz(w * W::RW + rl)) << 4;
+    if (WHOLE || A.page % 8 == 0) {  // the rows of a load lie in one page: a scalar base
+      const int in = WHOLE ? 0 : lane_key(k0) - page_of(A, lane_key(k0)) * A.page;
+      const int in0 = WHOLE ? first_key(k0) - page_of(A, first_key(k0)) * A.page : 0;
+#pragma unroll
+      for (int i = 0; i < W::NI; ++i) {
+        const long p = WHOLE ? __builtin_amdgcn_readfirstlane(page) : __builtin_amdgcn_readlane(page, i * W::RI);
+        const long n = WHOLE ? uniform(in0) + i * W::RI : __builtin_amdgcn_readlane(in, i * W::RI);
+        const u32 c = piece ^ (u32)(W::swz(i * W::RI) << 4);
+        // rows behind the last key: none may lie past its page
+        const u32 r = WHOLE ? rl : min(rl, (int)(A.page - 1 - n));
+        if (!PAD || (int)c < 2 * A.D) {
+          u32 ko = r * (u32)A.ks + c, vo = r * (u32)A.vs + c;
+          asm volatile("" : "+v"(ko), "+v"(vo));  // 32 bits beside a scalar base, not 64 held for each row
+          load_to_lds(kc + p * A.kp + n * A.ks + ko, sk + (w * W::RW + i * W::RI) * DT);
+          load_to_lds(vc + p * A.vp + n * A.vs + vo, sv + (w * W::RW + i * W::RI) * DT);
+        }
+      }
+    } else {
+      const int key = lane_key(k0), in = key - page_of(A, key) * A.page;
+#pragma unroll
+      for (int i = 0; i < W::NI; ++i) {
+        const u32 c = piece ^ (u32)(W::swz(i * W::RI) << 4);
+        const long p = __shfl(page, i * W::RI + rl), n = __shfl(in, i * W::RI + rl);
+        if (!PAD || (int)c < 2 * A.D) {
+          load_to_lds(kc + p * A.kp + n * A.ks + c, sk + (w * W::RW + i * W::RI) * DT);
+          load_to_lds(vc + p * A.vp + n * A.vs + c, sv + (w * W::RW + i * W::RI) * DT);
+        }
+      }
+    }
+  }
+};
+
+template <int DT, bool PAD, bool WHOLE>
+__device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& part, int kb0, int seg, uint16_t* sk0,
+                                          uint16_t* sv0, uint16_t* sk1, uint16_t* sv1, uint4* sq, u32 (*sbad)[4]) {
+  using W = Wide<DT>;
+  using T = uint16_t;
+  constexpr int TK = W::TK, NS = W::NS, KQ = DT / 16, ND = DT / 32, KB = 128, QL = W::QL;
+  const AttnArgs& A = arguments();
+  const int w = __builtin_amdgcn_readfirstlane(wave()), h = part.head, row0 = part.tile * kWideRows;
+  // the lane's row: its token and head, the byte offset of its values (a row past the last: row 0's)
+  auto place = [&](int l, bool& live, long& token, int& head) {
+    const int row = row0 + w * 32 + l % 32, t = row / A.g;
+    live = row < q.rows;
+    token = q.s0 + (live ? t : 0);
+    head = h * A.g + (live ? row - t * A.g : 0);
+  };
+  int lim;
+  {
+    const int row = row0 + w * 32 + lane_anew() % 32;
+    lim = row < q.rows ? row_limit(q, row, A.g) : 0;
+  }
+  // limits of the wave's and of the workgroup's first and last rows
+  const int wr = row0 + w * 32;
+  const bool rows_w = wr < q.rows;  // a wave without rows only helps to bring K and V
+  const int lo_w = uniform(rows_w ? row_limit(q, wr, A.g) : 0), hi_w = uniform(rows_w ? row_limit(q, min(wr + 32, q.rows) - 1, A.g) : 0);
+  const int lo_g = uniform(row_limit(q, row0, A.g)), hi_g = uniform(row_limit(q, min(row0 + kWideRows, q.rows) - 1, A.g));
+  const bool flip = A.c < 0.f;  // the scale's sign goes into q, which is exact
+  const float c = flip ? -A.c : A.c;
+
+  bf16x8 qf[KQ - QL];
+  {
+  const int lq = lane_anew();
+  bool live;
+  long token;
+  int head;
+  place(lq, live, token, head);
+#pragma unroll
+  for (int i = 0; i < KQ; ++i) {
+    const int e = i * 16 + lq / 32 * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (live && !(PAD && e >= A.D)) v = *reinterpret_cast<const uint4*>(A.q + token * A.qt + head * A.qh + e * 2);
+    if (flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+    if (i < KQ - QL) {
+      qf[i] = __builtin_bit_cast(bf16x8, v);
+    } else {
+      sq[(w * QL + i - (KQ - QL)) * 64 + lq] = v;  // read by this lane alone
+    }
+  }
+  }
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[d][x] = 0.f;
+  float m = kNegInf, l = 0.f;
+
+  const int k_first = kb0 * KB, k_end = min((kb0 + seg) * KB, hi_g);
+  const WideTile<DT, PAD, WHOLE> tile{A, q, A.table + (long)b * A.M, A.k + h * A.kh, A.v + h * A.vh, w, k_first, sbad};
+  if (PAD) {  // pieces past the head's dim are not loaded
+    for (int x = threadIdx.x; x < TK * DT / 8; x += kThreads) {
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(sk0)[x] = reinterpret_cast<uint4*>(sk1)[x] = z;
+      reinterpret_cast<uint4*>(sv0)[x] = reinterpret_cast<uint4*>(sv1)[x] = z;
+    }
+    __syncthreads();
+  }
+
+  // The lane's byte addresses in a buffer: its row of K's fragments, and of V's transposing reads. A piece's place is
+  // then one exclusive or with a constant away (the buffers' rows are aligned to their length).
+  static_assert(DT >= 64, "rows of 8 pieces and more");
+  auto k_lane = [&](int l) { return (l % 32) * DT * 2 + (((l / 32) ^ W::swz(l % 32)) << 4); };
+  auto v_lane = [&](int l) {
+    const int r = 4 * (l / 32) + (l % 16) / 4, c = (l / 16 % 2) * 2 + (l & 3) / 2;
+    return r * DT * 2 + ((c ^ W::swz(r)) << 4) + 8 * (l & 1);
+  };
+
+  // V's fragment: 32 values (d) by 16 keys, in the order of the weights' lanes
+  auto v_frag = [&](const uint16_t* sv, int vl, int d, int n, int j) {
+    i16x4 v[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      v[x] = read_tr(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(sv) +
+                                                       (vl ^ ((d * 64) & (W::SPAN - 1)) ^ (W::swz(8 * x) << 4)) +
+                                                       d * 64 / W::SPAN * W::SPAN + (n * 32 + 16 * j + 8 * x) * DT * 2));
+    return __builtin_bit_cast(bf16x8, (i16x8){v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]});
+  };
+  // what no row attends to must not meet its zero weight (0 * NaN): values of keys behind the last row's last or
+  // without a page become 0
+  auto clear_unseen = [&](int k0, int buf, uint16_t* sv) {
+    for (int x = threadIdx.x; x < TK * W::CPR; x += kThreads) {
+      const int r = x / W::CPR;
+      if (k0 + r >= hi_g || (sbad[buf][r / W::RW] >> (r % W::RW)) & 1) reinterpret_cast<uint4*>(sv)[x] = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+  };
+  bool special = false;  // infinities or NaN where some rows attend and others do not
+
+  auto compute = [&](int k0, int buf, uint16_t* sk, uint16_t* sv) {
+    u32 any_bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any_bad |= sbad[buf][i];
+    any_bad = __builtin_amdgcn_readfirstlane(any_bad);
+    if (k0 + TK > hi_g || any_bad) clear_unseen(k0, buf, sv);
+    if (k0 + TK > lo_g && lo_g < hi_g) {  // such values are left out here and counted at the end
+      bool nf = false;
+      for (int x = threadIdx.x; x < TK * W::CPR; x += kThreads) {
+        uint4& v = reinterpret_cast<uint4*>(sv)[x];
+        if (not_finite<T>(v)) {
+          nf = true;
+          v = make_uint4(finite_of(v.x), finite_of(v.y), finite_of(v.z), finite_of(v.w));
+        }
+      }
+      special = __syncthreads_or(nf) || special;
+    }
+    if (k0 >= hi_w) return;
+    // taken anew for each buffer: held across the loop, the addresses of all the reads do not fit the registers
+    const int la = lane_anew(), kl = k_lane(la), vl = v_lane(la);
+    f32x16 s[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[n][x] = 0.f;
+    // Fragments are read AHEAD products before their own: left to itself the compiler reads them all first, which
+    // runs it out of registers
+    constexpr int AHEAD = NS == 1 ? 3 : 2;
+    bf16x8 kf[AHEAD][NS];
+    auto read_k = [&](int i) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+        kf[i % AHEAD][n] = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(sk) + (kl ^ ((i * 32) & (W::SPAN - 1))) +
+                                                            i * 32 / W::SPAN * W::SPAN + n * 32 * DT * 2);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD - 1; ++i) read_k(i);
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) {
+      if (i + AHEAD - 1 < KQ) read_k(i + AHEAD - 1);
+      const bf16x8 qi = i < KQ - QL ? qf[i < KQ - QL ? i : 0] : __builtin_bit_cast(bf16x8, sq[(w * QL + i - (KQ - QL)) * 64 + la]);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD][n], qi, s[n], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (k0 + TK > lo_w) {
+      const int left = lim - k0 - 4 * (lane_anew() / 32);
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[n][x] = n * 32 + 8 * (x / 4) + x % 4 < left ? s[n][x] : kNegInf;
+    }
+    if (any_bad) {
+      const int hb = lane_anew() / 32;
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // 4 keys of one wave's rows
+          const int r = n * 32 + 8 * x + 4 * hb;
+          const u32 word = sbad[buf][r / W::RW] >> (r % W::RW);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][4 * x + i] = (word >> i) & 1 ? kNegInf : s[n][4 * x + i];
+        }
+    }
+    float t = kNegInf;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) t = fmaxf(t, s[n][x]);
+    t = fmaxf(t, __shfl_xor(t, 32)) * c;
+    if (__any(t > m + 8.f)) {
+      const float mn = fmaxf(m, t), a = __builtin_amdgcn_exp2f(m - base_of(mn));
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[d][x] *= a;
+    }
+    const float base = base_of(m);
+    bf16x8 p[NS][2];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        u32 pk[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x], c, -base));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x + 1], c, -base));
+          l += p0 + p1;
+          pk[x] = pack2(p0, p1);  // rounded for the product, as V is: the sums stay in 32 bits
+        }
+        p[n][j] = __builtin_bit_cast(bf16x8, make_uint4(pk[0], pk[1], pk[2], pk[3]));
+      }
+    bf16x8 vf[2][NS][2];
+    auto read_v = [&](int d) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vf[d % 2][n][j] = v_frag(sv, vl, d, n, j);
+    };
+    read_v(0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      if (d + 1 < ND) read_v(d + 1);
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d % 2][n][j], p[n][j], o[d], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // a buffer's loads are waited for and its readers of the step before joined by the one barrier of a step
+  auto ready = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+  if (k_first < k_end) {
+    tile.issue(k_first, tile.look(k_first), 0, sk0, sv0);
+    int entry = tile.look(k_first + TK);
+    for (int k0 = k_first; k0 < k_end; k0 += 2 * TK) {
+      ready();
+      if (k0 + TK < k_end) tile.issue(k0 + TK, entry, 1, sk1, sv1);
+      entry = tile.look(k0 + 2 * TK);
+      compute(k0, 0, sk0, sv0);
+      if (k0 + TK >= k_end) break;
+      ready();
+      if (k0 + 2 * TK < k_end) tile.issue(k0 + 2 * TK, entry, 0, sk0, sv0);
+      entry = tile.look(k0 + 3 * TK);
+      compute(k0 + TK, 1, sk1, sv1);
+    }
+  }
+  const int ln = lane_anew(), r32 = ln % 32, hf = ln / 32;
+  if (special) {  // the whole workgroup: counted per row (add_special), the values brought once more
+    for (int k0 = k_first; k0 < k_end; k0 += TK) {
+      if (k0 + TK <= lo_g) continue;
+      __syncthreads();
+      tile.issue(k0, tile.look(k0), 0, sk0, sv0);
+      ready();
+      clear_unseen(k0, 0, sv0);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        f32x16 o1;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o1[x] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 v = __builtin_bit_cast(uint4, v_frag(sv0, v_lane(ln), d, n, j));
+            u32 on[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = k0 + n * 32 + 16 * j + (x / 2) * 8 + 4 * hf + 2 * (x % 2);
+              on[x] = (key < lim ? 0x3f80u : 0u) | (key + 1 < lim ? 0x3f800000u : 0u);
+            }
+            o1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                __builtin_bit_cast(bf16x8, make_uint4(marks_of(v.x), marks_of(v.y), marks_of(v.z), marks_of(v.w))),
+                __builtin_bit_cast(bf16x8, make_uint4(on[0], on[1], on[2], on[3])), o1, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          o[d][x] += special_of(o1[x]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  // the lane's results: row r32, values 32 d + 8 x + 4 hf .. + 3
+  if (!part.p) {
+    bool live;
+    long token;
+    int head;
+    place(ln, live, token, head);
+    if (live) {
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+      const char* gp = A.gate ? A.gate + token * A.gt + head * A.gh : nullptr;
+      char* op = A.out + token * A.ot + head * A.oh;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int e = 32 * d + 8 * x + 4 * hf;
+          if (PAD && e >= A.D) continue;
+          float y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = o[d][4 * x + i] * inv;
+          if (gp) {
+            Raw4<T> gt;
+            gt.load(reinterpret_cast<const T*>(gp) + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] *= sigmoidf_(gt.elem(i));
+          }
+          st4_io(reinterpret_cast<T*>(op) + e, y);
+        }
+    }
+  } else if (rows_w) {
+    f32x4* po = reinterpret_cast<f32x4*>(part.p) + w * (ND * 4) * 64;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) po[(d * 4 + x) * 64 + ln] = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+    if (hf == 0) {
+      part.p[kWideRows * DT + w * 32 + r32] = m;
+      part.p[kWideRows * DT + kWideRows + w * 32 + r32] = l;
+    }
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------- the kernel
+// MIXED: the batch may hold requests of more than A.wide packed rows, which take the wide tiles.
+template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
+__global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
+  using S = Shape<T, DT>;
+  using L = StreamLds<T, DT, NQ>;
+  constexpr int R = 16 * NQ, KB = S::KB;
+  constexpr int BUF = MIXED ? Wide<DT>::TK * DT / 8 : 0;  // pieces of 16 bytes
+  constexpr int NA = L::ACC > 2 * BUF ? L::ACC : 2 * BUF, NB = L::Q > BUF ? L::Q : BUF;
+  __shared__ FoundLds sfound;
+  __shared__ float sm[4][R], sl[4][R];
+  __shared__ u32 sbad[2][4];
+  // the streamed tiles' sums and queries; the wide tiles' buffers
+  __shared__ __align__(16) uint4 sa[NA];
+  __shared__ __align__(16) uint4 sb[NB];
+  __shared__ __align__(16) uint4 sc[MIXED ? BUF : 1];
+  __shared__ __align__(16) uint4 sd[MIXED && Wide<DT>::QL ? 4 * Wide<DT>::QL * 64 : 1];
+  GDN_POISON_LDS(sfound, sm, sl, sbad, sa, sb, sc, sd);
+
+  if (A.fill) {  // rows of no request
+    const long b0 = A.starts[0], b1 = A.starts[A.B];
+    const long lo = b0 < 0 ? 0 : b0 > A.N ? A.N : b0, hi = b1 < lo ? lo : b1 > A.N ? A.N : b1;
+    const long rest = lo + (A.N - hi);
+    const int heads = A.Hk * A.g;
+    for (long i = blockIdx.x; i < rest; i += gridDim.x) {
+      const long row = i < lo ? i : hi + (i - lo);
+      for (int x = threadIdx.x; x < heads * (A.D / 4); x += kThreads) {
+        T* o = reinterpret_cast<T*>(A.out + row * A.ot + (x / (A.D / 4)) * A.oh) + 4 * (x % (A.D / 4));
+        const float z[4] = {0.f, 0.f, 0.f, 0.f};
+        st4_io(o, z);
+      }
+    }
+  }
+
+  const int range = range_of(blockIdx.x, A.G);
+  const Found f = find_range<R, KB>(A, range, sfound);
+  const long u0 = uniform(range * f.each), u1 = uniform(min(f.total, u0 + f.each));
+  Split* split = reinterpret_cast<Split*>(A.part + 2 * (size_t)A.G * A.slot) + range;
+  if (threadIdx.x == 0) split->parts = 0;
+  if (f.b < 0) return;
+  int b = f.b;
+  long local = u0 - f.unit;
+  Request q = f.q;
+  for (long u = u0; u < u1;) {
+    const Unit un = unit_of(q, local), at{uniform(un.head), uniform(un.tile), uniform(un.block)};
+    const int blocks = q.tile_blocks(at.tile), seg = (int)min((long)(blocks - at.block), u1 - u);
+    const int slot = 2 * range + (u > u0 ? 1 : 0);
+    if (at.block == 0 && seg < blocks && threadIdx.x == 0)  // the tile goes on in the next ranges
+      *split = {(int)((u + blocks - 1) / f.each) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile, at.head};
+    const Part part{seg == blocks ? nullptr : A.part + (size_t)slot * A.slot, at.tile, at.head};
+    if (MIXED && q.tile_rows == kWideRows) {
+      uint16_t* pa = reinterpret_cast<uint16_t*>(sa);
+      if constexpr (MIXED)
+        wide_tile<DT, PAD, WHOLE>(q, b, part, at.block, seg, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
+                                  reinterpret_cast<uint16_t*>(sc), sd, sbad);
+    } else {
+      stream_tile<T, DT, NQ, PAD, WHOLE>(q, b, part, at.block, seg, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
+      __syncthreads();
+    }
+    u += seg;
+    local += seg;
+    while (u < u1 && local >= q.cost) {  // the next request with rows
+      if (++b >= A.B) return;
+      local -= q.cost;
+      q = uniform(request<R, KB>(A, b));
+    }
+  }
+}
+
+// The tiles that more than one range holds: their parts joined, one workgroup per range. Bound by latency (few rows)
+// or memory (wide tiles): the maxima and sums of all parts are read at once, the results as many at a time as the
+// registers hold.
+template <int DT>
+constexpr int join_threads() { return DT == 64 ? 256 : 512; }
+
+template <class T, int DT, int ROWS, bool WIDE>
+__device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, const float* first, const float* next, float (*sm)[kWideRows],
+                                          float (*sl)[kWideRows]) {
+  constexpr int NT = join_threads<DT>(), NG = NT / ROWS, NE = ROWS * DT / 4 / NT;
+  static_assert(NG >= 1 && NE >= 1, "");
+  // part p's slot: the range that the tile begins in holds part 0, the others follow two slots apart
+  const int parts = q.parts, tile = q.tile, h = q.head;
+  auto part = [&](int p) { return p ? next + (size_t)(p - 1) * 2 * A.slot : first; };
+  const int tid = threadIdx.x, row = tid % ROWS, grp = tid / ROWS;
+  const int live = min(ROWS, (q.rows - tile * ROWS + 31) / 32 * 32);  // rows that the parts hold
+  {
+    float m = kNegInf, l = 0.f;
+#pragma unroll 4
+    for (int p = grp; p < (row < live ? parts : 0); p += NG) {
+      const float* s = part(p) + ROWS * DT + row;
+      const float pm = s[0], pl = s[ROWS], mn = fmaxf(m, pm), base = base_of(mn);
+      l = l * __builtin_amdgcn_exp2f(m - base) + pl * __builtin_amdgcn_exp2f(pm - base);
+      m = mn;
+    }
+    sm[grp][row] = m;
+    sl[grp][row] = l;
+  }
+  __syncthreads();
+  if (grp == 0) {
+    float m = kNegInf, l = 0.f;
+    for (int i = 0; i < NG; ++i) m = fmaxf(m, sm[i][row]);
+    const float base = base_of(m);
+    for (int i = 0; i < NG; ++i) l += sl[i][row] * __builtin_amdgcn_exp2f(sm[i][row] - base);
+    sm[0][row] = base;
+    sl[0][row] = l > 0.f || l != l ? 1.0f / l : 0.f;
+  }
+  __syncthreads();
+  f32x4 acc[NE];
+  int er[NE];
+  float eb[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int x = tid + i * NT;
+    er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
+    eb[i] = sm[0][er[i]];
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr int U = NE >= 8 ? 1 : 8 / NE;
+  for (int p0 = 0; p0 < parts; p0 += U) {
+    f32x4 v[U][NE];
+    float pm[U][NE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* s = part(min(p0 + u, parts - 1));
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        if (WIDE && er[i] >= live) continue;
+        v[u][i] = reinterpret_cast<const f32x4*>(s)[tid + i * NT];
+        pm[u][i] = s[ROWS * DT + er[i]];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (p0 + u < parts && !(WIDE && er[i] >= live)) acc[i] += v[u][i] * __builtin_amdgcn_exp2f(pm[u][i] - eb[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int x = tid + i * NT, r = tile * ROWS + er[i], t = r / A.g, ln = x % 64, v = x / 64 % (DT / 8);
+    const int d = WIDE ? 32 * (v / 4) + 8 * (v % 4) + 4 * (ln / 32) : x % (DT / 4) * 4;
+    if (r >= q.rows || d >= A.D) continue;
+    const long token = q.s0 + t;
+    const int head = h * A.g + (r - t * A.g);
+    const float inv = sl[0][er[i]];
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = acc[i][j] * inv;
+    if (A.gate) {
+      Raw4<T> gt;
+      gt.load(reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + d);
+      float gf[4];
+      gt.get(gf);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] *= sigmoidf_(gf[j]);
+    }
+    st4_io(reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d, y);
+  }
+}
+
+template <class T, int DT, int NQ, bool MIXED>
+__global__ __launch_bounds__(join_threads<DT>()) void k_attention_join(AttnArgs A) {
+  constexpr int R = 16 * NQ, NT = join_threads<DT>();
+  __shared__ float sm[NT / R][kWideRows], sl[NT / R][kWideRows];
+  GDN_POISON_LDS(sm, sl);
+  const Split q = reinterpret_cast<const Split*>(A.part + 2 * (size_t)A.G * A.slot)[blockIdx.x];
+  if (q.parts < 2) return;
+  const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (blockIdx.x + 1)) * A.slot;
+  if constexpr (MIXED) {
+    if (q.tile_rows == kWideRows) {
+      join_tile<T, DT, kWideRows, true>(A, q, first, next, sm, sl);
+      return;
+    }
+  }
+  join_tile<T, DT, R, false>(A, q, first, next, sm, sl);
+}
+
+}  // namespace
+}  // namespace gdn

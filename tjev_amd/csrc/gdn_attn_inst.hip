@@ -1,0 +1,47 @@
+// One unit of paged attention: the kernels of one type (GDN_T: bf16 or f32) and head dims up to GDN_D.
+#include "gdn_attention.h"
+
+namespace gdn {
+namespace {
+
+template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
+hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
+  A.G = r.G;
+  A.slot = r.slot;
+  A.wide = MIXED ? 16 * NQ : 0x7fffffff;
+  hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);
+  hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED>), dim3(r.G), dim3(join_threads<DT>()), 0, st, A);
+  return hipGetLastError();
+}
+
+template <class T, int DT, int NQ>
+hipError_t dispatch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
+  auto with = [&](auto pad, auto whole) {
+    if constexpr (sizeof(T) == 2)
+      if (r.mixed) return launch<T, DT, NQ, pad.value, whole.value, true>(r, A, st);
+    return launch<T, DT, NQ, pad.value, whole.value, false>(r, A, st);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  const bool pad = A.D != DT, whole = A.page % 16 == 0;
+  return pad ? whole ? with(yes, yes) : with(yes, no) : whole ? with(no, yes) : with(no, no);
+}
+
+// bf16: more than 16 rows of a request take the wide tiles. fp32 streams all, up to as many rows as the registers hold.
+template <class T, int DT>
+hipError_t by_rows(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
+  if constexpr (sizeof(T) == 4)
+    if (r.nq > 1) return dispatch<T, DT, DT == 256 ? 2 : 4>(r, A, st);
+  return dispatch<T, DT, 1>(r, A, st);
+}
+
+using bf16 = uint16_t;
+using f32 = float;
+
+}  // namespace
+
+#define GDN_NAME_(t, d) attention_##t##_##d
+#define GDN_NAME(t, d) GDN_NAME_(t, d)
+hipError_t GDN_NAME(GDN_T, GDN_D)(const AttnPlan& r, AttnArgs& A, hipStream_t st) { return by_rows<GDN_T, GDN_D>(r, A, st); }
+
+}  // namespace gdn

@@ -14,16 +14,45 @@ struct Batch {
   long N;                    // rows of q
   int B, M, page, pages;     // requests, table width, page size, pages of the cache
   int Hk, g;                 // key heads, query heads to each
+  int wide;                  // requests of more packed rows take wide tiles
+  uint32_t page_mul;         // k / page = the high word of k page_mul, shifted right by page_shift (k < 2^31)
+  int page_shift;
   const int32_t *table, *starts, *lengths;
 };
 
+// With 2^(L-1) < page <= 2^L and page_mul = ceil(2^(31+L) / page) < 2^32 the product is off by less than k page <=
+// 2^(31+L): the quotient is exact. (A page of one token: page_shift -1, k itself.)
+__host__ __device__ __forceinline__ void set_page(Batch& A, int page) {
+  int L = 0;
+  while ((1l << L) < page) ++L;
+  A.page = page;
+  A.page_mul = (uint32_t)(((1ul << (31 + L)) + page - 1) / page);
+  A.page_shift = L - 1;
+}
+__host__ __device__ __forceinline__ int page_of(const Batch& A, int key) {
+  return A.page_shift < 0 ? key : (int)(((uint64_t)(uint32_t)key * A.page_mul) >> 32 >> A.page_shift);
+}
+
 // The packed rows of a request and key head are its new tokens' query heads of that key head: row r
-// is token r / g, head r % g; R of them are a tile. A unit of work is a tile's next KB keys.
+// is token r / g, head r % g. Requests of more than `wide` rows are worked on in tiles of kWideRows, the others
+// in tiles of R. A unit of work is a tile's next KB keys, in the order key head, tile, keys.
+constexpr int kWideRows = 128;
+
 struct Request {
-  int s0, rows, tiles, blocks;  // first row of q; packed rows; tiles of them; key blocks
-  int keys;                     // keys that the table's row has pages for
-  long first;                   // position of the first new token
-  long cost;                    // units
+  int s0, rows, tiles, tile_rows;  // first row of q; packed rows; tiles of them
+  int keys;                        // keys that the table's row has pages for
+  int blocks;                      // units of every tile, or 0: tile t has (y + t) / g of them
+  long y, g;
+  long first;                      // position of the first new token
+  long per_head, cost;             // units of a key head, of the request
+
+  // sum of (0 .. x - 1) / g
+  __host__ __device__ __forceinline__ long below(long x) const {
+    const long q = x / g;
+    return g * (q * (q - 1) / 2) + q * (x - q * g);
+  }
+  __host__ __device__ __forceinline__ int tile_blocks(int t) const { return blocks ? blocks : (int)((y + t) / g); }
+  __host__ __device__ __forceinline__ long before_tile(int t) const { return blocks ? (long)t * blocks : below(y + t) - below(y); }
 };
 
 template <int R, int KB>
@@ -34,12 +63,48 @@ __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   const long cap = (long)A.M * A.page, keys = len < 0 ? 0 : len < cap ? len : cap;
   q.s0 = (int)s0;
   q.rows = (int)(s1 - s0) * A.g;
-  q.tiles = (q.rows + R - 1) / R;
+  const bool wide = q.rows > A.wide;
+  q.tile_rows = wide ? kWideRows : R;
+  q.tiles = (q.rows + q.tile_rows - 1) / q.tile_rows;
   q.keys = (int)keys;
-  q.blocks = keys ? (int)((keys + KB - 1) / KB) : 1;  // a row without keys is written too
   q.first = len - (e - a);
-  q.cost = (long)q.tiles * A.Hk * q.blocks;
+  q.g = A.g;
+  q.y = 0;
+  q.blocks = keys ? (int)((keys + KB - 1) / KB) : 1;  // a row without keys is written too
+  if (wide && q.first >= 0 && keys == len) {
+    // Tile t's last row may attend to first + (kWideRows (t + 1) - 1) / g + 1 keys, which are
+    // floor((first g + kWideRows (t + 1) - 1) / (KB g)) + 1 blocks, and with KB = kWideRows floor((y + t) / g)
+    static_assert(KB == kWideRows || KB < kWideRows, "");
+    if (KB == kWideRows) {
+      q.blocks = 0;
+      q.y = (q.first * q.g + KB * q.g - 1) / KB + 1;
+    }
+  }
+  q.per_head = q.before_tile(q.tiles);
+  q.cost = q.per_head * A.Hk;
   return q;
+}
+
+// a unit of the request: its key head, tile and key block
+struct Unit {
+  int head, tile, block;
+};
+__host__ __device__ __forceinline__ Unit unit_of(const Request& q, long local) {
+  Unit u;
+  u.head = (int)(local / q.per_head);
+  local -= (long)u.head * q.per_head;
+  if (q.blocks) {
+    u.tile = (int)(local / q.blocks);
+  } else {
+    int lo = 0, hi = q.tiles;  // the last tile that begins at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (q.before_tile(mid) <= local) lo = mid; else hi = mid;
+    }
+    u.tile = lo;
+  }
+  u.block = (int)(local - q.before_tile(u.tile));
+  return u;
 }
 
 // keys that the packed row may attend to: those up to its token's own, of the request's
@@ -55,9 +120,42 @@ struct Place {
   bool good;
 };
 __host__ __device__ __forceinline__ Place place_of(const Batch& A, const int32_t* row, int key, int keys) {
-  const int k = key < keys ? key : keys - 1, i = k / A.page, p = row[i];
+  const int k = key < keys ? key : keys - 1, i = page_of(A, k), p = row[i];
   const bool good = p >= 0 && p < A.pages;
   return {good ? p : 0, k - i * A.page, good};
 }
+
+// The paged attention's arguments, and how its rows are shared out
+struct AttnArgs : Batch {
+  int D, fill;
+  float c;                          // scale * log2(e)
+  const char *q, *k, *v, *gate;
+  char* out;
+  long qt, qh, gt, gh, ot, oh;      // bytes: token and head of q, gate, out
+  long kp, ks, kh, vp, vs, vh;      // bytes: page, slot and head of the caches
+  float* part;                      // the workgroups' unfinished rows, slots of `slot` floats
+  long slot;
+  int G;                            // workgroups
+};
+
+constexpr int kSplitBytes = 32;  // of the workspace, per range: the tile that goes on behind it
+
+struct AttnPlan {
+  int nq;            // streamed tiles of 16 nq rows
+  bool mixed;        // wide tiles too
+  int G;             // ranges
+  long slot;         // floats of a workspace slot
+  size_t bytes;      // workspace
+};
+
+// One unit of gdn_attn_inst.hip: attention in bf16 (bf = true) or fp32, head dims up to d
+#define GDN_ATTENTION(t, d) hipError_t attention_##t##_##d(const AttnPlan& r, AttnArgs& A, hipStream_t st);
+GDN_ATTENTION(bf16, 64)
+GDN_ATTENTION(bf16, 128)
+GDN_ATTENTION(bf16, 256)
+GDN_ATTENTION(f32, 64)
+GDN_ATTENTION(f32, 128)
+GDN_ATTENTION(f32, 256)
+#undef GDN_ATTENTION
 
 }  // namespace gdn
