@@ -30,15 +30,15 @@ static void walk(const gdn::Batch& A) {
     long sum = 0;  // every unit once, in order, and at least one to a tile
     for (int t = 0; t < q.tiles; ++t) {
       check(q.before_tile(t) == sum && q.tile_blocks(t) >= 1, "units before a tile");
-      sum += q.tile_blocks(t);
+      sum += q.extra + q.tile_blocks(t);
     }
     check(sum == q.per_head, "units of a head");
     long at = 0;
     for (int h = 0; h < A.Hk && q.cost < 3000; ++h)
       for (int t = 0; t < q.tiles; ++t)
-        for (int k = 0; k < q.tile_blocks(t); ++k, ++at) {
+        for (int k = 0; k < q.extra + q.tile_blocks(t); ++k, ++at) {
           const gdn::Unit u = gdn::unit_of(q, at);
-          check(u.head == h && u.tile == t && u.block == k, "a unit's place");
+          check(u.head == h && u.tile == t && u.at == k, "a unit's place");
         }
     if (!q.rows) continue;
     const int hi = gdn::row_limit(q, q.rows - 1, A.g);

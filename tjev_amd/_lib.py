@@ -274,6 +274,14 @@ def current_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+def one_gpu(what: str, devices) -> None:
+    """Raises unless all of a call's tensors (their device indices, -1: none) are on one GPU."""
+    if min(devices) < 0:
+        raise RuntimeError(f"{what} runs on the GPU (HIP); got a CPU tensor")
+    if len(set(devices)) > 1:
+        raise ValueError(f"{what}: tensors on GPUs {sorted(set(devices))}")
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one: a launch goes to the current device, whatever stream it names.
     Nothing is entered where it is current already (1 us of a small call)."""

@@ -31,8 +31,9 @@ __device__ __forceinline__ long uniform(long v) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ Request uniform(const Request& q) {
-  return {uniform(q.s0), uniform(q.rows), uniform(q.tiles), uniform(q.tile_rows), uniform(q.keys), uniform(q.blocks), uniform(q.y),
-          uniform(q.g), uniform(q.first), uniform(q.per_head), uniform(q.cost)};
+  return {uniform(q.s0), uniform(q.rows), uniform(q.tiles), uniform(q.tile_rows), uniform(q.keys), uniform(q.extra), uniform(q.blocks), uniform(q.y),
+          uniform(q.g), __builtin_bit_cast(double, uniform(__builtin_bit_cast(long, q.inv_g))), uniform(q.first), uniform(q.per_head),
+          uniform(q.cost)};
 }
 
 // The kernel's arguments read anew: what a tile needs of them is then held for the tile only, and not (spilled)
@@ -313,26 +314,36 @@ template <class T, int DT, bool PAD>
 __device__ __forceinline__ void store_row(const AttnArgs& A, const f32x4 (&o)[Shape<T, DT>::VH][Shape<T, DT>::VE], float l, long token,
                                           int head) {
   using S = Shape<T, DT>;
+  using G = std::conditional_t<S::VE == 8, Raw8<T>, Raw4<T>>;
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+  const int d0 = 4 * (lane() / 16) * S::VE;
+  const T* gp = reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + d0;
+  T* op = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d0;
+  G gate[S::VH][4];  // all loaded before the first is used
+  if (A.gate)
+#pragma unroll
+    for (int h = 0; h < S::VH; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!PAD || d0 + (h * 16 + r) * S::VE < A.D) gate[h][r].load(gp + (h * 16 + r) * S::VE);
 #pragma unroll
   for (int h = 0; h < S::VH; ++h)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int d = h * 16 * S::VE + (4 * (lane() / 16) + r) * S::VE;
-      if (PAD && d >= A.D) continue;
+      if (PAD && d0 + (h * 16 + r) * S::VE >= A.D) continue;
       float x[S::VE];
 #pragma unroll
       for (int e = 0; e < S::VE; ++e) x[e] = o[h][e][r] * inv;
       if (A.gate) {
-        const T* gp = reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + d;
+        float gv[S::VE];
+        gate[h][r].get(gv);
 #pragma unroll
-        for (int e = 0; e < S::VE; ++e) x[e] *= sigmoidf_(ldf(gp + e));
+        for (int e = 0; e < S::VE; ++e) x[e] *= sigmoid_io<T>(gv[e]);
       }
-      T* op = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d;
       if constexpr (S::VE == 8) {
-        st8_io(op, x);
+        st8_io(op + (h * 16 + r) * S::VE, x);
       } else {
-        st4_io(op, x);
+        st4_io(op + (h * 16 + r) * S::VE, x);
       }
     }
 }
@@ -354,6 +365,10 @@ struct Split {
   int parts, first, s0, rows, tile_rows, tile, head, pad;
 };
 static_assert(sizeof(Split) == kSplitBytes, "the workspace's last part");
+
+__device__ __forceinline__ Split* split_of(const AttnArgs& A, int range) {
+  return reinterpret_cast<Split*>(A.part + 2 * (size_t)A.G * A.slot) + range;
+}
 
 // the workgroup's i-th range: consecutive ranges stay on one XCD (its L2 holds the keys that they share)
 __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block : (block % 8) * (G / 8) + block / 8; }
@@ -628,7 +643,7 @@ template <int DT>
 struct Wide {
   static constexpr int TK = DT == 256 ? 32 : 64;  // keys per buffer
   static constexpr int NS = TK / 32, CPR = DT / 8, RW = TK / 4, RI = 64 / CPR, NI = RW / RI;
-  static constexpr int QL = DT == 256 ? 2 : 0;  // fragments of a wave's queries kept in LDS: what the registers cannot hold
+  static constexpr int QL = DT == 256 ? 3 : 0;  // fragments of a wave's queries kept in LDS: what the registers cannot hold
   static constexpr int SPAN = CPR >= 16 ? 256 : 128;  // bytes within which the pieces of a row are exchanged
   // the place of piece c of row r: c ^ swz(r)
   static constexpr __device__ __forceinline__ int swz(int r) {
@@ -735,26 +750,6 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   const bool flip = A.c < 0.f;  // the scale's sign goes into q, which is exact
   const float c = flip ? -A.c : A.c;
 
-  bf16x8 qf[KQ - QL];
-  {
-  const int lq = lane_anew();
-  bool live;
-  long token;
-  int head;
-  place(lq, live, token, head);
-#pragma unroll
-  for (int i = 0; i < KQ; ++i) {
-    const int e = i * 16 + lq / 32 * 8;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (live && !(PAD && e >= A.D)) v = *reinterpret_cast<const uint4*>(A.q + token * A.qt + head * A.qh + e * 2);
-    if (flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-    if (i < KQ - QL) {
-      qf[i] = __builtin_bit_cast(bf16x8, v);
-    } else {
-      sq[(w * QL + i - (KQ - QL)) * 64 + lq] = v;  // read by this lane alone
-    }
-  }
-  }
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -773,6 +768,31 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     __syncthreads();
   }
 
+  int entry = 0;
+  if (k_first < k_end) {  // the first keys are on their way while the queries are read
+    tile.issue(k_first, tile.look(k_first), 0, sk0, sv0);
+    entry = tile.look(k_first + TK);
+  }
+  bf16x8 qf[KQ - QL];
+  {
+  const int lq = lane_anew();
+  bool live;
+  long token;
+  int head;
+  place(lq, live, token, head);
+#pragma unroll
+  for (int i = 0; i < KQ; ++i) {
+    const int e = i * 16 + lq / 32 * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);  // a row past the last reads row 0's: its results go nowhere
+    if (!(PAD && e >= A.D)) v = *reinterpret_cast<const uint4*>(A.q + token * A.qt + head * A.qh + e * 2);
+    if (flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+    if (i < KQ - QL) {
+      qf[i] = __builtin_bit_cast(bf16x8, v);
+    } else {
+      sq[(w * QL + i - (KQ - QL)) * 64 + lq] = v;  // read by this lane alone
+    }
+  }
+  }
   // The lane's byte addresses in a buffer: its row of K's fragments, and of V's transposing reads. A piece's place is
   // then one exclusive or with a constant away (the buffers' rows are aligned to their length).
   static_assert(DT >= 64, "rows of 8 pieces and more");
@@ -830,7 +850,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       for (int x = 0; x < 16; ++x) s[n][x] = 0.f;
     // Fragments are read AHEAD products before their own: left to itself the compiler reads them all first, which
     // runs it out of registers
-    constexpr int AHEAD = NS == 1 ? 3 : 2;
+    constexpr int AHEAD = 2;
     bf16x8 kf[AHEAD][NS];
     auto read_k = [&](int i) {
 #pragma unroll
@@ -840,6 +860,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     };
 #pragma unroll
     for (int i = 0; i < AHEAD - 1; ++i) read_k(i);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < KQ; ++i) {
       if (i + AHEAD - 1 < KQ) read_k(i + AHEAD - 1);
@@ -848,6 +869,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD][n], qi, s[n], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (k0 + TK > lo_w) {
       const int left = lim - k0 - 4 * (lane_anew() / 32);
 #pragma unroll
@@ -906,6 +928,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         for (int j = 0; j < 2; ++j) vf[d % 2][n][j] = v_frag(sv, vl, d, n, j);
     };
     read_v(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       if (d + 1 < ND) read_v(d + 1);
@@ -915,6 +938,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         for (int j = 0; j < 2; ++j) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d % 2][n][j], p[n][j], o[d], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   // a buffer's loads are waited for and its readers of the step before joined by the one barrier of a step
@@ -922,20 +946,16 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
   };
-  if (k_first < k_end) {
-    tile.issue(k_first, tile.look(k_first), 0, sk0, sv0);
-    int entry = tile.look(k_first + TK);
-    for (int k0 = k_first; k0 < k_end; k0 += 2 * TK) {
-      ready();
-      if (k0 + TK < k_end) tile.issue(k0 + TK, entry, 1, sk1, sv1);
-      entry = tile.look(k0 + 2 * TK);
-      compute(k0, 0, sk0, sv0);
-      if (k0 + TK >= k_end) break;
-      ready();
-      if (k0 + 2 * TK < k_end) tile.issue(k0 + 2 * TK, entry, 0, sk0, sv0);
-      entry = tile.look(k0 + 3 * TK);
-      compute(k0 + TK, 1, sk1, sv1);
-    }
+  for (int k0 = k_first; k0 < k_end; k0 += 2 * TK) {
+    ready();
+    if (k0 + TK < k_end) tile.issue(k0 + TK, entry, 1, sk1, sv1);
+    entry = tile.look(k0 + 2 * TK);
+    compute(k0, 0, sk0, sv0);
+    if (k0 + TK >= k_end) break;
+    ready();
+    if (k0 + 2 * TK < k_end) tile.issue(k0 + 2 * TK, entry, 0, sk0, sv0);
+    entry = tile.look(k0 + 3 * TK);
+    compute(k0 + TK, 1, sk1, sv1);
   }
   const int ln = lane_anew(), r32 = ln % 32, hf = ln / 32;
   if (special) {  // the whole workgroup: counted per row (add_special), the values brought once more
@@ -975,33 +995,61 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     }
   }
   l += __shfl_xor(l, 32);
-  // the lane's results: row r32, values 32 d + 8 x + 4 hf .. + 3
+  // The lane's results: row r32, values 32 d + 8 x + 4 hf .. + 3. Finished rows are turned in the wave's own buffer (its
+  // pieces of four exchanged by the row), so that gate and result move as 16-byte pieces of whole rows, all gates
+  // of a turn on their way at once: taken as they lie, a lane's 8-byte pieces of the gate cost a memory round trip each
+  // (a 4096-token prompt, 32 heads of 256 with a gate: 722 us).
   if (!part.p) {
-    bool live;
-    long token;
-    int head;
-    place(ln, live, token, head);
-    if (live) {
+    __syncthreads();  // the last buffers' readers
+    if (rows_w) {
+      constexpr int HD = DT == 64 ? 64 : 128, LPR = HD / 8, NI = 32 * LPR / 64;  // columns of a turn; lanes of a row
+      float* sx = reinterpret_cast<float*>(w == 0 ? sk0 : w == 1 ? sv0 : w == 2 ? sk1 : sv1);
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-      const char* gp = A.gate ? A.gate + token * A.gt + head * A.gh : nullptr;
-      char* op = A.out + token * A.ot + head * A.oh;
+      const int c8 = (ln % LPR) * 8;
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
+      for (int p = 0; p < DT / HD; ++p) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int e = 32 * d + 8 * x + 4 * hf;
-          if (PAD && e >= A.D) continue;
-          float y[4];
+        for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = o[d][4 * x + i] * inv;
-          if (gp) {
-            Raw4<T> gt;
-            gt.load(reinterpret_cast<const T*>(gp) + e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] *= sigmoidf_(gt.elem(i));
+          for (int x = 0; x < 4; ++x) {
+            const f32x16& v = o[p * (HD / 32) + d];
+            *reinterpret_cast<f32x4*>(sx + r32 * HD + (((8 * d + 2 * x + hf) ^ r32) & (HD / 4 - 1)) * 4) =
+                f32x4{v[4 * x] * inv, v[4 * x + 1] * inv, v[4 * x + 2] * inv, v[4 * x + 3] * inv};
           }
-          st4_io(reinterpret_cast<T*>(op) + e, y);
+        __builtin_amdgcn_wave_barrier();
+        Raw8<T> gate[NI];
+        T* op[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int r = i * (64 / LPR) + ln / LPR, row = row0 + w * 32 + r, t = row / A.g, e = p * HD + c8;
+          op[i] = nullptr;
+          if (row < q.rows && !(PAD && e >= A.D)) {
+            const long token = q.s0 + t;
+            const int head = h * A.g + (row - t * A.g);
+            op[i] = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + e;
+            if (A.gate) gate[i].load(reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + e);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int r = i * (64 / LPR) + ln / LPR;
+          float y[8];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(sx + r * HD + (((c8 / 4 + x) ^ r) & (HD / 4 - 1)) * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[4 * x + j] = v[j];
+          }
+          if (A.gate && op[i]) {
+            float gv[8];
+            gate[i].get(gv);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= sigmoid_io<T>(gv[j]);
+          }
+          if (op[i]) st8_io(op[i], y);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   } else if (rows_w) {
     f32x4* po = reinterpret_cast<f32x4*>(part.p) + w * (ND * 4) * 64;
@@ -1014,7 +1062,6 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       part.p[kWideRows * DT + kWideRows + w * 32 + r32] = l;
     }
   }
-  __syncthreads();
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -1051,38 +1098,80 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
     }
   }
 
-  const int range = range_of(blockIdx.x, A.G);
-  const Found f = find_range<R, KB>(A, range, sfound);
-  const long u0 = uniform(range * f.each), u1 = uniform(min(f.total, u0 + f.each));
-  Split* split = reinterpret_cast<Split*>(A.part + 2 * (size_t)A.G * A.slot) + range;
-  if (threadIdx.x == 0) split->parts = 0;
-  if (f.b < 0) return;
-  int b = f.b;
-  long local = u0 - f.unit;
-  Request q = f.q;
-  for (long u = u0; u < u1;) {
-    const Unit un = unit_of(q, local), at{uniform(un.head), uniform(un.tile), uniform(un.block)};
-    const int blocks = q.tile_blocks(at.tile), seg = (int)min((long)(blocks - at.block), u1 - u);
-    const int slot = 2 * range + (u > u0 ? 1 : 0);
-    if (at.block == 0 && seg < blocks && threadIdx.x == 0)  // the tile goes on in the next ranges
-      *split = {(int)((u + blocks - 1) / f.each) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile, at.head};
-    const Part part{seg == blocks ? nullptr : A.part + (size_t)slot * A.slot, at.tile, at.head};
-    if (MIXED && q.tile_rows == kWideRows) {
-      uint16_t* pa = reinterpret_cast<uint16_t*>(sa);
-      if constexpr (MIXED)
-        wide_tile<DT, PAD, WHOLE>(q, b, part, at.block, seg, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
-                                  reinterpret_cast<uint16_t*>(sc), sd, sbad);
-    } else {
-      stream_tile<T, DT, NQ, PAD, WHOLE>(q, b, part, at.block, seg, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
+  // Where the range stands. In LDS while a tile is worked on: held in registers it would be spilled there.
+  __shared__ struct {
+    Request q;
+    long u, u1, local, each;
+    Unit at;
+    int b, range, begun;
+  } st;
+  {
+    const int range = range_of(blockIdx.x, A.G);
+    const Found f = find_range<R, KB>(A, range, sfound);
+    if (threadIdx.x == 0) split_of(A, range)->parts = 0;
+    if (f.b < 0) return;
+    if (threadIdx.x == 0) {
+      const long u0 = range * f.each;
+      st.q = f.q;
+      st.u = u0;
+      st.u1 = min(f.total, u0 + f.each);
+      st.local = u0 - f.unit;
+      st.each = f.each;
+      st.at = unit_of(f.q, u0 - f.unit);
+      st.b = f.b;
+      st.range = range;
+      st.begun = 0;
+    }
+    __syncthreads();
+  }
+  while (true) {
+    {
+      const Request q = uniform(st.q);
+      const Unit at{uniform(st.at.head), uniform(st.at.tile), uniform(st.at.at)};
+      const int b = uniform(st.b), range = uniform(st.range), begun = uniform(st.begun);
+      const long u = uniform(st.u), u1 = uniform(st.u1);
+      const int blocks = q.tile_blocks(at.tile), seg = (int)min((long)(q.extra + blocks - at.at), u1 - u);
+      const int k0 = max(0, at.at - q.extra), keys = max(0, at.at + seg - q.extra) - k0;  // blocks of keys
+      const int slot = 2 * range + begun;
+      const Part part{keys == blocks ? nullptr : A.part + (size_t)slot * A.slot, at.tile, at.head};
       __syncthreads();
+      if (threadIdx.x == 0) {
+        if (keys > 0 && k0 == 0 && keys < blocks)  // the tile goes on in the next ranges
+          *split_of(A, range) = {(int)((u - at.at + q.extra + blocks - 1) / st.each) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile,
+                                 at.head};
+        // the next tile, the next head's first, or the next request's with rows
+        long local = st.local + seg;
+        st.u = u + seg;
+        st.begun = 1;
+        if (local < q.cost) {
+          st.at = at.tile + 1 < q.tiles ? Unit{at.head, at.tile + 1, 0} : Unit{at.head + 1, 0, 0};
+        } else if (u + seg < u1) {
+          Request n = q;
+          int nb = b;
+          while (local >= n.cost && ++nb < A.B) {
+            local -= n.cost;
+            n = request<R, KB>(A, nb);
+          }
+          if (nb >= A.B) st.u = u1;
+          st.q = n;
+          st.b = nb;
+          st.at = {0, 0, 0};
+        }
+        st.local = local;
+      }
+      if (keys > 0) {
+        if (MIXED && q.tile_rows == kWideRows) {
+          uint16_t* pa = reinterpret_cast<uint16_t*>(sa);
+          if constexpr (MIXED)
+            wide_tile<DT, PAD, WHOLE>(q, b, part, k0, keys, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
+                                      reinterpret_cast<uint16_t*>(sc), sd, sbad);
+        } else {
+          stream_tile<T, DT, NQ, PAD, WHOLE>(q, b, part, k0, keys, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
+        }
+      }
     }
-    u += seg;
-    local += seg;
-    while (u < u1 && local >= q.cost) {  // the next request with rows
-      if (++b >= A.B) return;
-      local -= q.cost;
-      q = uniform(request<R, KB>(A, b));
-    }
+    __syncthreads();
+    if (uniform(st.u) >= uniform(st.u1)) break;
   }
 }
 
@@ -1171,7 +1260,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
       float gf[4];
       gt.get(gf);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] *= sigmoidf_(gf[j]);
+      for (int j = 0; j < 4; ++j) y[j] *= sigmoid_io<T>(gf[j]);
     }
     st4_io(reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d, y);
   }
@@ -1182,7 +1271,7 @@ __global__ __launch_bounds__(join_threads<DT>()) void k_attention_join(AttnArgs 
   constexpr int R = 16 * NQ, NT = join_threads<DT>();
   __shared__ float sm[NT / R][kWideRows], sl[NT / R][kWideRows];
   GDN_POISON_LDS(sm, sl);
-  const Split q = reinterpret_cast<const Split*>(A.part + 2 * (size_t)A.G * A.slot)[blockIdx.x];
+  const Split q = *split_of(A, blockIdx.x);
   if (q.parts < 2) return;
   const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (blockIdx.x + 1)) * A.slot;
   if constexpr (MIXED) {

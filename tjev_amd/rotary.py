@@ -12,6 +12,7 @@ HIP library, or on a CPU tensor, the operator raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -23,36 +24,59 @@ _POSITION_BITS = {torch.int32: 32, torch.int64: 64}
 _FREQ_BITS = {torch.float32: 32, torch.float64: 64}
 
 
-@_lib.by_value
-def _options(half: int, dim: int, axes: int, sections: str, interleaved: bool):
-    """The sections as the library takes them, checked (``sections``: their text, kept by value)."""
-    secs = [half] if sections == "None" else [int(s) for s in sections.split()]
+@functools.lru_cache(maxsize=256)
+def _checked(q_shape, q_dtype, k_shape, k_dtype, p_shape, p_dtype, f_shape, f_dtype, sections, interleaved: bool, devices):
+    """The checks of a call, kept by its shapes, types and options: the number of axes."""
+    if q_dtype not in _DTYPES:
+        raise ValueError(f"rotary_axes takes float32 or bfloat16 tensors, not {q_dtype}")
+    if len(q_shape) < 3 or len(f_shape) != 1:
+        raise ValueError(f"q is [..., T, heads, dim] and inv_freq [pairs], not {tuple(q_shape)} and {tuple(f_shape)}")
+    if k_shape is not None and (len(k_shape) != len(q_shape) or k_shape[:-2] != q_shape[:-2] or k_shape[-1] != q_shape[-1]
+                                or k_dtype != q_dtype):
+        raise ValueError(f"k {tuple(k_shape)} {k_dtype} does not go with q {tuple(q_shape)} {q_dtype}")
+    lead, half, dim = q_shape[:-2], f_shape[0], q_shape[-1]
+    if sections is None and p_shape == lead:
+        p_shape = (1, *p_shape)
+    if p_shape[1:] != lead or len(p_shape) != len(lead) + 1:
+        raise ValueError(f"positions {tuple(p_shape)} are not one of {tuple(lead)} per axis")
+    if p_dtype not in _POSITION_BITS or f_dtype not in _FREQ_BITS:
+        raise ValueError(f"positions are int32 or int64 and frequencies float32 or float64, not {p_dtype} and {f_dtype}")
+    secs = [half] if sections is None else list(sections)
     if not 0 < 2 * half <= dim or dim % 2:
         raise ValueError(f"{half} frequencies turn {2 * half} lanes of heads of {dim}")
     if not 1 <= len(secs) <= _lib.MAX_AXES:
         raise ValueError(f"1 to {_lib.MAX_AXES} position axes, not {len(secs)}")
     if min(secs) < 0 or sum(secs) != half:
         raise ValueError(f"sections {secs} do not add up to {half} pairs")
-    if axes != len(secs):
-        raise ValueError(f"positions of {axes} axes for {len(secs)} sections")
+    if p_shape[0] != len(secs):
+        raise ValueError(f"positions of {p_shape[0]} axes for {len(secs)} sections")
     if interleaved and any(n and a + len(secs) * (n - 1) >= half for a, n in enumerate(secs) if a):
         raise ValueError(f"interleaved sections {secs}: an axis runs out of the {half} pairs")
-    return (ctypes.c_int32 * _lib.MAX_AXES)(*secs)
+    _lib.one_gpu("rotary_axes", devices)
+    return len(secs)
 
 
-def _launch(q, k, positions, inv_freq, sections, interleaved: bool, adjacent: bool, inverse: bool):
+@functools.lru_cache(maxsize=256)
+def _params(q_shape, q_stride, dtype, k_shape, k_stride, half, axes, sections, interleaved, adjacent, inverse, p_dtype, f_dtype):
+    """The library's view of a call (a reference to the struct; never changed): q [B, T, Hq, D], k [B, T, Hk, D] or None."""
+    batch, length, heads, dim = q_shape
+    return ctypes.byref(_lib.RotaryParams(
+        batch, length, heads, 0 if k_shape is None else k_shape[2], dim, 2 * half, axes, (ctypes.c_int32 * _lib.MAX_AXES)(*sections),
+        interleaved, adjacent, inverse, _DTYPES[dtype], _POSITION_BITS[p_dtype], _FREQ_BITS[f_dtype], 0, q_stride[:3],
+        (0, 0, 0) if k_shape is None else k_stride[:3]))
+
+
+def _launch(q, k, positions, inv_freq, axes, sections, interleaved: bool, adjacent: bool, inverse: bool):
     """The library's call: q [B, T, Hq, D], k [B, T, Hk, D] or None (the last dim contiguous)."""
-    batch, length, heads, dim = q.shape
-    k_heads = 0 if k is None else k.shape[2]
-    p = _lib.RotaryParams(batch, length, heads, k_heads, dim, 2 * inv_freq.shape[0], positions.shape[0], sections,
-                          interleaved, adjacent, inverse, _DTYPES[q.dtype], _POSITION_BITS[positions.dtype],
-                          _FREQ_BITS[inv_freq.dtype], 0, q.stride()[:3], (0, 0, 0) if k is None else k.stride()[:3])
-    q_out = torch.empty((batch, length, heads, dim), dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty((batch, length, k_heads, dim), dtype=q.dtype, device=q.device)
-    with _lib.on_device(q.device):
+    dev = q.device
+    p = _params(q.shape, q.stride(), q.dtype, None if k is None else k.shape, None if k is None else k.stride(), inv_freq.shape[0],
+                axes, sections, interleaved, adjacent, inverse, positions.dtype, inv_freq.dtype)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    k_out = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    with _lib.on_device(dev):
         _lib.check_status(_lib.load().tjev_gdn_rotary(
-            ctypes.byref(p), _lib.current_stream(q.device), q.data_ptr(), None if k is None else k.data_ptr(),
-            positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(), None if k is None else k_out.data_ptr()))
+            p, _lib.current_stream(dev), q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+            q_out.data_ptr(), None if k is None else k_out.data_ptr()))
     return q_out, k_out
 
 
@@ -63,10 +87,10 @@ def _rows(x):
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, interleaved, adjacent):
-        ctx.options = (sections, interleaved, adjacent)
+    def forward(ctx, q, k, positions, inv_freq, *options):
+        ctx.options = options
         ctx.save_for_backward(positions, inv_freq)
-        return _launch(q, k, positions, inv_freq, *ctx.options, False)
+        return _launch(q, k, positions, inv_freq, *options, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -75,7 +99,7 @@ class _Rotary(torch.autograd.Function):
         if not ctx.needs_input_grad[1]:
             d_k = None
         d_q, d_k = _launch(_rows(d_q), None if d_k is None else _rows(d_k), positions, inv_freq, *ctx.options, True)
-        return d_q, d_k, None, None, None, None, None
+        return d_q, d_k, None, None, None, None, None, None
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections=None,
@@ -88,30 +112,18 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     turn with axis 0 and so on, or (``interleaved``) pair i with axis i mod A while i < A * sections[i mod A] and with
     axis 0 from there. A pair is lanes i and i + R/2, or 2i and 2i + 1 (``adjacent``). q and k may be views
     with any strides whose last dim is contiguous; others are copied."""
-    if q.dtype not in _DTYPES:
-        raise ValueError(f"rotary_axes takes float32 or bfloat16 tensors, not {q.dtype}")
-    if q.dim() < 3 or inv_freq.dim() != 1:
-        raise ValueError(f"q is [..., T, heads, dim] and inv_freq [pairs], not {tuple(q.shape)} and {tuple(inv_freq.shape)}")
-    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-    lead = q.shape[:-2]
-    if sections is None and positions.shape == lead:
-        positions = positions[None]
-    if positions.shape[1:] != lead or positions.dim() != len(lead) + 1:
-        raise ValueError(f"positions {tuple(positions.shape)} are not one of {tuple(lead)} per axis")
-    if positions.dtype not in _POSITION_BITS or inv_freq.dtype not in _FREQ_BITS:
-        raise ValueError(f"positions are int32 or int64 and frequencies float32 or float64, not {positions.dtype} and {inv_freq.dtype}")
-    secs = _options(inv_freq.shape[0], q.shape[-1], positions.shape[0],
-                    "None" if sections is None else " ".join([str(int(s)) for s in sections]), bool(interleaved))
-    for t in (q, k, positions, inv_freq):
-        if t is not None and not t.is_cuda:
-            raise RuntimeError("rotary_axes runs on the GPU (HIP); got a CPU tensor")
-        if t is not None and t.device != q.device:
-            raise ValueError(f"tensors on {q.device} and {t.device}")
-    batch = math.prod(lead[:-1])
-    q4 = _rows(q if q.dim() == 4 else q.reshape(batch, *q.shape[-3:]))
-    k4 = None if k is None else _rows(k if k.dim() == 4 else k.reshape(batch, *k.shape[-3:]))
-    args = (q4, k4, positions.contiguous(), inv_freq.contiguous(), secs, bool(interleaved), bool(adjacent))
+    secs = None if sections is None else tuple([int(n) for n in sections])
+    interleaved, adjacent = bool(interleaved), bool(adjacent)
+    axes = _checked(q.shape, q.dtype, None if k is None else k.shape, None if k is None else k.dtype, positions.shape, positions.dtype,
+                    inv_freq.shape, inv_freq.dtype, secs, interleaved,
+                    (q.get_device(), positions.get_device(), inv_freq.get_device(), q.get_device() if k is None else k.get_device()))
+    q4, k4 = q, k
+    if q.dim() != 4:
+        batch = math.prod(q.shape[:-3])
+        q4 = q.reshape(batch, *q.shape[-3:])
+        k4 = None if k is None else k.reshape(batch, *k.shape[-3:])
+    args = (_rows(q4), None if k is None else _rows(k4), positions.contiguous(), inv_freq.contiguous(), axes,
+            (inv_freq.shape[0],) if secs is None else secs, interleaved, adjacent)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         q4, k4 = _Rotary.apply(*args)
     else:
