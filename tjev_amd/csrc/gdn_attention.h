@@ -1065,6 +1065,23 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
 }
 
 // ---------------------------------------------------------------- the kernel
+// the rows of no request, shared out to the workgroups
+template <class T>
+__device__ __forceinline__ void clear_rest(const AttnArgs& A) {
+  const long b0 = A.starts[0], b1 = A.starts[A.B];
+  const long lo = b0 < 0 ? 0 : b0 > A.N ? A.N : b0, hi = b1 < lo ? lo : b1 > A.N ? A.N : b1;
+  const long rest = lo + (A.N - hi);
+  const int heads = A.Hk * A.g;
+  for (long i = blockIdx.x; i < rest; i += gridDim.x) {
+    const long row = i < lo ? i : hi + (i - lo);
+    for (int x = threadIdx.x; x < heads * (A.D / 4); x += kThreads) {
+      T* o = reinterpret_cast<T*>(A.out + row * A.ot + (x / (A.D / 4)) * A.oh) + 4 * (x % (A.D / 4));
+      const float z[4] = {0.f, 0.f, 0.f, 0.f};
+      st4_io(o, z);
+    }
+  }
+}
+
 // MIXED: the batch may hold requests of more than A.wide packed rows, which take the wide tiles.
 template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
 __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
@@ -1083,21 +1100,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
   __shared__ __align__(16) uint4 sd[MIXED && Wide<DT>::QL ? 4 * Wide<DT>::QL * 64 : 1];
   GDN_POISON_LDS(sfound, sm, sl, sbad, sa, sb, sc, sd);
 
-  if (A.fill) {  // rows of no request
-    const long b0 = A.starts[0], b1 = A.starts[A.B];
-    const long lo = b0 < 0 ? 0 : b0 > A.N ? A.N : b0, hi = b1 < lo ? lo : b1 > A.N ? A.N : b1;
-    const long rest = lo + (A.N - hi);
-    const int heads = A.Hk * A.g;
-    for (long i = blockIdx.x; i < rest; i += gridDim.x) {
-      const long row = i < lo ? i : hi + (i - lo);
-      for (int x = threadIdx.x; x < heads * (A.D / 4); x += kThreads) {
-        T* o = reinterpret_cast<T*>(A.out + row * A.ot + (x / (A.D / 4)) * A.oh) + 4 * (x % (A.D / 4));
-        const float z[4] = {0.f, 0.f, 0.f, 0.f};
-        st4_io(o, z);
-      }
-    }
-  }
-
   // Where the range stands. In LDS while a tile is worked on: held in registers it would be spilled there.
   __shared__ struct {
     Request q;
@@ -1109,6 +1111,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
     const int range = range_of(blockIdx.x, A.G);
     const Found f = find_range<R, KB>(A, range, sfound);
     if (threadIdx.x == 0) split_of(A, range)->parts = 0;
+    if (A.fill) clear_rest<T>(A);
     if (f.b < 0) return;
     if (threadIdx.x == 0) {
       const long u0 = range * f.each;
@@ -1178,13 +1181,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 // The tiles that more than one range holds: their parts joined, one workgroup per range. Bound by latency (few rows)
 // or memory (wide tiles): the maxima and sums of all parts are read at once, the results as many at a time as the
 // registers hold.
-template <int DT>
-constexpr int join_threads() { return DT == 64 ? 256 : 512; }
+// Few tiles have many parts each (one request of 16000 tokens, 4 key heads: 126): SLICED spreads a tile's results over
+// gridDim.y workgroups and its parts over two halves of each, 16 at a time; gridDim.x is then the most tiles there can
+// be, and a workgroup finds its one among the ranges' notes.
+constexpr int kSlice = 128;  // results of four per workgroup
+template <int DT, bool SLICED>
+constexpr int join_threads() { return DT == 64 || SLICED ? 256 : 512; }
+template <int DT, int ROWS>
+constexpr int join_slices() { return ROWS * DT / 4 / kSlice; }
 
-template <class T, int DT, int ROWS, bool WIDE>
+template <class T, int DT, int ROWS, bool WIDE, bool SLICED>
 __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, const float* first, const float* next, float (*sm)[kWideRows],
                                           float (*sl)[kWideRows]) {
-  constexpr int NT = join_threads<DT>(), NG = NT / ROWS, NE = ROWS * DT / 4 / NT;
+  constexpr int NT = join_threads<DT, SLICED>(), NG = NT / ROWS;
+  constexpr int PG = SLICED ? NT / kSlice : 1, NE = SLICED ? 1 : ROWS * DT / 4 / NT;  // groups of parts; results of a thread
   static_assert(NG >= 1 && NE >= 1, "");
   // part p's slot: the range that the tile begins in holds part 0, the others follow two slots apart
   const int parts = q.parts, tile = q.tile, h = q.head;
@@ -1218,13 +1228,14 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   float eb[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int x = tid + i * NT;
+    const int x = SLICED ? blockIdx.y * kSlice + tid % kSlice : tid + i * NT;
     er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
     eb[i] = sm[0][er[i]];
     acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   constexpr int U = NE >= 8 ? 1 : 8 / NE;
-  for (int p0 = 0; p0 < parts; p0 += U) {
+  const int pg = SLICED ? tid / kSlice : 0;
+  for (int p0 = pg * U; p0 < parts; p0 += PG * U) {
     f32x4 v[U][NE];
     float pm[U][NE];
 #pragma unroll
@@ -1233,7 +1244,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
 #pragma unroll
       for (int i = 0; i < NE; ++i) {
         if (WIDE && er[i] >= live) continue;
-        v[u][i] = reinterpret_cast<const f32x4*>(s)[tid + i * NT];
+        v[u][i] = reinterpret_cast<const f32x4*>(s)[SLICED ? blockIdx.y * kSlice + tid % kSlice : tid + i * NT];
         pm[u][i] = s[ROWS * DT + er[i]];
       }
     }
@@ -1243,9 +1254,17 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
       for (int i = 0; i < NE; ++i)
         if (p0 + u < parts && !(WIDE && er[i] >= live)) acc[i] += v[u][i] * __builtin_amdgcn_exp2f(pm[u][i] - eb[i]);
   }
+  if constexpr (SLICED) {
+    __shared__ __align__(16) f32x4 sacc[(PG - 1) * kSlice];
+    if (pg) sacc[(pg - 1) * kSlice + tid % kSlice] = acc[0];
+    __syncthreads();
+    if (pg) return;
+#pragma unroll
+    for (int i = 0; i < PG - 1; ++i) acc[0] += sacc[i * kSlice + tid];
+  }
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int x = tid + i * NT, r = tile * ROWS + er[i], t = r / A.g, ln = x % 64, v = x / 64 % (DT / 8);
+    const int x = SLICED ? blockIdx.y * kSlice + tid : tid + i * NT, r = tile * ROWS + er[i], t = r / A.g, ln = x % 64, v = x / 64 % (DT / 8);
     const int d = WIDE ? 32 * (v / 4) + 8 * (v % 4) + 4 * (ln / 32) : x % (DT / 4) * 4;
     if (r >= q.rows || d >= A.D) continue;
     const long token = q.s0 + t;
@@ -1266,21 +1285,46 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   }
 }
 
-template <class T, int DT, int NQ, bool MIXED>
-__global__ __launch_bounds__(join_threads<DT>()) void k_attention_join(AttnArgs A) {
-  constexpr int R = 16 * NQ, NT = join_threads<DT>();
+template <class T, int DT, int NQ, bool MIXED, bool SLICED>
+__global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join(AttnArgs A) {
+  constexpr int R = 16 * NQ, NT = join_threads<DT, SLICED>();
   __shared__ float sm[NT / R][kWideRows], sl[NT / R][kWideRows];
   GDN_POISON_LDS(sm, sl);
-  const Split q = *split_of(A, blockIdx.x);
+  int range = blockIdx.x;
+  if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note
+    __shared__ int scount[NT / 64], sfound;
+    GDN_POISON_LDS(scount, sfound);
+    const int run = (A.G + NT - 1) / NT, r0 = threadIdx.x * run;
+    int n = 0;
+    for (int r = r0; r < min(A.G, r0 + run); ++r) n += split_of(A, r)->parts > 1;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int t = __shfl_up(upto, d);
+      if (lane() >= d) upto += t;
+    }
+    if (lane() == 63) scount[wave()] = upto;
+    if (threadIdx.x == 0) sfound = -1;
+    __syncthreads();
+    for (int w = 0; w < wave(); ++w) upto += scount[w];
+    int k = upto - n;
+    for (int r = r0; r < min(A.G, r0 + run); ++r)
+      if (split_of(A, r)->parts > 1 && k++ == (int)blockIdx.x) sfound = r;
+    __syncthreads();
+    range = uniform(sfound);
+    if (range < 0) return;
+  }
+  const Split q = *split_of(A, range);
   if (q.parts < 2) return;
-  const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (blockIdx.x + 1)) * A.slot;
+  const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (range + 1)) * A.slot;
   if constexpr (MIXED) {
     if (q.tile_rows == kWideRows) {
-      join_tile<T, DT, kWideRows, true>(A, q, first, next, sm, sl);
+      join_tile<T, DT, kWideRows, true, SLICED>(A, q, first, next, sm, sl);
       return;
     }
   }
-  join_tile<T, DT, R, false>(A, q, first, next, sm, sl);
+  if (SLICED && (int)blockIdx.y >= join_slices<DT, R>()) return;
+  join_tile<T, DT, R, false, SLICED>(A, q, first, next, sm, sl);
 }
 
 }  // namespace

@@ -20,9 +20,13 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   r.nq = bf || mean <= 16 ? 1 : dt == 256 ? 2 : 4;
   r.mixed = bf && (p->tokens - p->requests + 1) * g > 16;
   const int kb = bf ? 128 : 64;
-  const long tiles = (rows / (16 * r.nq) + p->requests) * p->kv_heads;
-  const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb;
+  // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
+  const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + p->requests) * p->kv_heads;
+  const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb + kWideExtra;
   r.G = tiles >= kRanges || blocks * tiles >= kRanges ? kRanges : (int)(blocks * tiles);
+  // so few tiles that a workgroup each would leave most CUs idle, and take parts by the dozen
+  r.sliced = tiles <= (r.mixed ? 16 : 64);
+  r.tiles = (int)(tiles < (1l << 30) ? tiles : 1l << 30);
   r.slot = (long)(r.mixed ? kWideRows : 16 * r.nq) * (dt + 2);
   r.bytes = (size_t)r.G * (2 * r.slot * sizeof(float) + kSplitBytes);
   return r;

@@ -10,7 +10,12 @@ hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   A.slot = r.slot;
   A.wide = MIXED ? 16 * NQ : 0x7fffffff;
   hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);
-  hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED>), dim3(r.G), dim3(join_threads<DT>()), 0, st, A);
+  constexpr int slices = join_slices<DT, MIXED ? kWideRows : 16 * NQ>();
+  if (r.sliced) {
+    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, true>), dim3(r.tiles, slices), dim3(join_threads<DT, true>()), 0, st, A);
+  } else {
+    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, false>), dim3(r.G), dim3(join_threads<DT, false>()), 0, st, A);
+  }
   return hipGetLastError();
 }
 

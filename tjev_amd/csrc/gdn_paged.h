@@ -158,6 +158,8 @@ constexpr int kSplitBytes = 32;  // of the workspace, per range: the tile that g
 struct AttnPlan {
   int nq;            // streamed tiles of 16 nq rows
   bool mixed;        // wide tiles too
+  bool sliced;       // few tiles: their parts joined by several workgroups each
+  int tiles;         // the most there can be, up to 2^30
   int G;             // ranges
   long slot;         // floats of a workspace slot
   size_t bytes;      // workspace
