@@ -66,6 +66,8 @@ int main() {
       const long top = 0x7fffffffl / page, n = i < 1000 ? i : top - (i - 1000);
       for (long k = n * page - 1; k <= n * page + 1; ++k)
         if (k >= 0 && k <= 0x7fffffffl) check(gdn::page_of(A, (int)k) == k / page, "a key's page");
+      const long high = (1l << 50) / page * page + i * page;  // slots of a long cache
+      for (long k = high - 1; k <= high + 1; ++k) check(gdn::div_by(page)(k) == k / page, "a slot's page");
     }
   }
   std::mt19937 rng(7);

@@ -32,7 +32,7 @@ __device__ __forceinline__ long uniform(long v) {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ Request uniform(const Request& q) {
   return {uniform(q.s0), uniform(q.rows), uniform(q.tiles), uniform(q.tile_rows), uniform(q.keys), uniform(q.extra), uniform(q.blocks), uniform(q.y),
-          uniform(q.g), __builtin_bit_cast(double, uniform(__builtin_bit_cast(long, q.inv_g))), uniform(q.first), uniform(q.per_head),
+          {__builtin_bit_cast(double, uniform(__builtin_bit_cast(long, q.by_g.inv))), uniform(q.by_g.d)}, uniform(q.first), uniform(q.per_head),
           uniform(q.cost)};
 }
 

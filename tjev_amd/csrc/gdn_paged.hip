@@ -8,12 +8,15 @@
 // token's request found by bisection. What bounds it is the launch and that chain (load, scan, bisection);
 // the bytes are few.
 //
-// Append: bound by memory, every vector of 16 bytes loaded and stored once, four in flight per lane.
+// Append: bound by memory, every vector of 16 bytes loaded and stored once, one at a time per lane and
+// enough waves to cover it: 16000 tokens of 8 key heads of 128 (131 MB) take 21.7 us (6.0 TB/s, part of it from the last
+// level cache). Two to eight vectors in flight per lane took 28 to 35 us (their addresses went to scratch memory).
 #include <hip/hip_runtime.h>
 
 #include "../../include/tjev_gdn.h"
 #include "gdn_device.h"
 #include "gdn_launch.h"
+#include "gdn_paged.h"
 
 namespace gdn {
 namespace {
@@ -21,7 +24,8 @@ namespace {
 constexpr int kThreads = 256;
 
 struct TableArgs {
-  int B, M, page;
+  int B, M;
+  Div page, width;
   long N, n_free;
   const int32_t *cached, *fresh, *table, *free, *taken;
   int32_t* table_out;
@@ -32,7 +36,7 @@ struct TableArgs {
 __device__ __forceinline__ int clamp_int(long v) { return (int)(v < 0 ? 0 : v > 0x7fffffffl ? 0x7fffffffl : v); }
 // pages of n tokens, at most the table's width
 __device__ __forceinline__ int pages_of(long n, const TableArgs& A) {
-  const long p = (n + A.page - 1) / A.page;
+  const long p = A.page(n + A.page.d - 1);
   return (int)(p < A.M ? p : A.M);
 }
 
@@ -86,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_tables(TableArgs A) {
   const long stride = (long)gridDim.x * kThreads, id = (long)blockIdx.x * kThreads + tid;
   const bool keep = A.table_out == A.table;
   for (long i = id; i < (long)A.B * A.M; i += stride) {
-    const int b = (int)(i / A.M), j = (int)(i - (long)b * A.M);
+    const int b = (int)A.width(i), j = (int)(i - (long)b * A.M);
     const long c = clamp_int(A.cached[b]), n = clamp_int(A.fresh[b]);
     const int e = pages_of(c, A), f = pages_of(c + n, A);
     if (j >= e && j < f) {
@@ -103,11 +107,11 @@ __global__ __launch_bounds__(kThreads) void k_paged_tables(TableArgs A) {
         const int mid = (lo + hi) / 2;
         if (sstart[mid] <= t) lo = mid; else hi = mid;
       }
-      const long c = clamp_int(A.cached[lo]), pos = c + (t - sstart[lo]), j = pos / A.page;
+      const long c = clamp_int(A.cached[lo]), pos = c + (t - sstart[lo]), j = A.page(pos);
       if (j < A.M) {
         const int e = pages_of(c, A);
         const long p = j < e ? A.table[(long)lo * A.M + j] : fresh_page(taken + spage[lo] + (j - e));
-        if (p >= 0) slot = p * A.page + (pos - j * A.page);
+        if (p >= 0) slot = p * A.page.d + (pos - j * A.page.d);
       }
     }
     A.slots[t] = slot;
@@ -116,7 +120,8 @@ __global__ __launch_bounds__(kThreads) void k_paged_tables(TableArgs A) {
 
 struct AppendArgs {
   long N, n_slots;
-  int page, per, half, chunks, tile;  // vectors of a token: of k and v, of each; of a head; tokens per workgroup
+  Div page;
+  int per, half, chunks, tile;  // vectors of a token: of k and v, of each; of a head; tokens per workgroup
   unsigned inv_per, inv_chunks;       // 2^32 / per, / chunks rounded up
   const void* src[2];
   void* dst[2];
@@ -132,29 +137,17 @@ template <class W>
 __global__ __launch_bounds__(kThreads) void k_paged_append(AppendArgs A) {
   const long t0 = (long)blockIdx.x * A.tile;
   const int count = (int)min((long)A.tile, A.N - t0) * A.per;
-  constexpr int U = 4;
-  for (int u0 = threadIdx.x; u0 < count; u0 += U * kThreads) {
-    W v[U];
-    char* to[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = u0 + i * kThreads;
-      to[i] = nullptr;
-      if (u < count) {
-        const int tok = divide(u, A.inv_per, A.per), r = u - tok * A.per, which = r >= A.half, x = which ? r - A.half : r;
-        const int h = divide(x, A.inv_chunks, A.chunks), c = x - h * A.chunks;
-        const long slot = A.slots[t0 + tok];
-        if (slot >= 0 && slot < A.n_slots) {
-          const long p = slot / A.page, o = slot - p * A.page;
-          to[i] = static_cast<char*>(A.dst[which]) + p * A.dp[which] + o * A.ds[which] + h * A.dh[which] + c * (long)sizeof(W);
-          v[i] = *reinterpret_cast<const W*>(static_cast<const char*>(A.src[which]) + (t0 + tok) * A.st[which] + h * A.sh[which] +
-                                             c * (long)sizeof(W));
-        }
-      }
+  for (int u = threadIdx.x; u < count; u += kThreads) {
+    const int tok = divide(u, A.inv_per, A.per), r = u - tok * A.per, which = r >= A.half, x = which ? r - A.half : r;
+    const int h = divide(x, A.inv_chunks, A.chunks), c = x - h * A.chunks;
+    // on its way while the slot is looked up
+    const W v = *reinterpret_cast<const W*>(static_cast<const char*>(A.src[which]) + (t0 + tok) * A.st[which] + h * A.sh[which] +
+                                            c * (long)sizeof(W));
+    const long slot = A.slots[t0 + tok];
+    if (slot >= 0 && slot < A.n_slots) {
+      const long p = A.page(slot), o = slot - p * A.page.d;
+      *reinterpret_cast<W*>(static_cast<char*>(A.dst[which]) + p * A.dp[which] + o * A.ds[which] + h * A.dh[which] + c * (long)sizeof(W)) = v;
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (to[i]) *reinterpret_cast<W*>(to[i]) = v[i];
   }
 }
 
@@ -176,7 +169,7 @@ int tjev_gdn_paged_tables(const tjev_gdn_paged_params* p, void* stream, const in
       !lengths || !taken_out)
     return fail(TJEV_GDN_EINVAL, "null tensor argument");
   if (taken == taken_out) return fail(TJEV_GDN_EINVAL, "taken_out must not alias taken (every workgroup reads it)");
-  const gdn::TableArgs A{p->requests, p->table_width, p->page_size, p->tokens, n_free, cached, new_tokens, block_table, free_pages,
+  const gdn::TableArgs A{p->requests, p->table_width, gdn::div_by(p->page_size), gdn::div_by(p->table_width), p->tokens, n_free, cached, new_tokens, block_table, free_pages,
                          taken, table_out, slots, starts, lengths, taken_out};
   const long work = (long)p->requests * p->table_width + p->tokens;
   const long blocks = (work + 2047) / 2048;
@@ -205,7 +198,7 @@ int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const vo
   gdn::AppendArgs A{};
   A.N = p->tokens;
   A.n_slots = (long)p->pages * p->page_size;
-  A.page = p->page_size;
+  A.page = gdn::div_by(p->page_size);
   A.slots = slots;
   const void* src[2] = {k, v};
   void* dst[2] = {k_cache, v_cache};
@@ -231,7 +224,7 @@ int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const vo
   A.half = A.per / 2;
   A.inv_per = (unsigned)(((1ul << 32) + per - 1) / per);
   A.inv_chunks = (unsigned)(((1ul << 32) + chunks - 1) / chunks);
-  A.tile = per >= 1024 ? 1 : (int)(1024 / per);
+  A.tile = per >= 512 ? 1 : (int)(512 / per);
   const unsigned blocks = (unsigned)((A.N + A.tile - 1) / A.tile);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(blocks), block(gdn::kThreads);
