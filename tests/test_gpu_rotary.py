@@ -119,6 +119,22 @@ def test_gradient_against_differences():
         assert abs(diff - float(g.view(-1)[i])) <= room
 
 
+def test_second_derivative():
+    """The gradient's own gradient is the forward turn."""
+    from tjev_amd import rotary_axes
+
+    gen = torch.Generator().manual_seed(6)
+    q, k, w = (torch.randn(1, 5, h, 32, generator=gen) for h in (2, 1, 2))
+    pos, inv = torch.randint(0, 100, (2, 1, 5), generator=gen), _freqs(12)
+    x, y, d = q.cuda().requires_grad_(True), k.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    print("rotary second derivative", flush=True)
+    a, b = rotary_axes(x, y, pos.cuda(), inv.cuda(), sections=(7, 5))
+    (g,) = torch.autograd.grad(a, x, d, create_graph=True)
+    _check(g.detach(), w, pos, inv, (7, 5), False, False, -1.0)
+    (h,) = torch.autograd.grad(g, d, q.cuda())
+    _check(h, q, pos, inv, (7, 5), False, False)
+
+
 def test_one_gradient_and_graph():
     """Only k needing one; a captured forward replayed on new values."""
     from tjev_amd import rotary_axes

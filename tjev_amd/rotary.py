@@ -86,20 +86,25 @@ def _rows(x):
 
 
 class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, *options):
-        ctx.options = options
-        ctx.save_for_backward(positions, inv_freq)
-        return _launch(q, k, positions, inv_freq, *options, False)
+    """The launch with its gradient, which is the turn the other way: the same Function again where the backward itself
+    is differentiated."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, q, k, positions, inv_freq, options, inverse: bool):
+        ctx.options, ctx.inverse = options, inverse
+        ctx.save_for_backward(positions, inv_freq)
+        return _launch(q, k, positions, inv_freq, *options, inverse)
+
+    @staticmethod
     def backward(ctx, d_q, d_k):
         positions, inv_freq = ctx.saved_tensors
-        if not ctx.needs_input_grad[1]:
-            d_k = None
-        d_q, d_k = _launch(_rows(d_q), None if d_k is None else _rows(d_k), positions, inv_freq, *ctx.options, True)
-        return d_q, d_k, None, None, None, None, None, None
+        d_q = _rows(d_q)
+        d_k = _rows(d_k) if ctx.needs_input_grad[1] else None
+        if torch.is_grad_enabled():
+            d_q, d_k = _Rotary.apply(d_q, d_k, positions, inv_freq, ctx.options, not ctx.inverse)
+        else:
+            d_q, d_k = _launch(d_q, d_k, positions, inv_freq, *ctx.options, not ctx.inverse)
+        return d_q, d_k, None, None, None, None
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections=None,
@@ -122,12 +127,12 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         batch = math.prod(q.shape[:-3])
         q4 = q.reshape(batch, *q.shape[-3:])
         k4 = None if k is None else k.reshape(batch, *k.shape[-3:])
-    args = (_rows(q4), None if k is None else _rows(k4), positions.contiguous(), inv_freq.contiguous(), axes,
-            (inv_freq.shape[0],) if secs is None else secs, interleaved, adjacent)
+    args = (_rows(q4), None if k is None else _rows(k4), positions.contiguous(), inv_freq.contiguous())
+    options = (axes, (inv_freq.shape[0],) if secs is None else secs, interleaved, adjacent)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q4, k4 = _Rotary.apply(*args)
+        q4, k4 = _Rotary.apply(*args, options, False)
     else:
-        q4, k4 = _launch(*args, False)
+        q4, k4 = _launch(*args, *options, False)
     if q.dim() == 4:
         return q4, k4
     return q4.reshape(q.shape), None if k is None else k4.reshape(k.shape)
