@@ -690,19 +690,31 @@ struct WideTile {
     if (ln == 0) sbad[buf][w] = (u32)bad;
     // a row's pieces are exchanged by swz(row): the lane's part of it, and below the part of i
     const u32 piece = (u32)(pos ^ W::swz(w * W::RW + rl)) << 4;
-    if (WHOLE || A.page % 8 == 0) {  // the rows of a load lie in one page: a scalar base
-      const int in = WHOLE ? 0 : lane_key(k0) - page_of(A, lane_key(k0)) * A.page;
-      const int in0 = WHOLE ? first_key(k0) - page_of(A, first_key(k0)) * A.page : 0;
+    if constexpr (WHOLE) {  // all rows lie in one page: a scalar base
+      const int key = first_key(k0);
+      const long p = __builtin_amdgcn_readfirstlane(page), in = uniform(key - page_of(A, key) * A.page);
+      const char *kb = kc + p * A.kp + in * A.ks, *vb = vc + p * A.vp + in * A.vs;
+      u32 kr = rl * (u32)A.ks, vr = rl * (u32)A.vs;
+#pragma unroll
+      for (int i = 0; i < W::NI; ++i, kb += W::RI * A.ks, vb += W::RI * A.vs) {
+        const u32 c = piece ^ (u32)(W::swz(i * W::RI) << 4);
+        if (!PAD || (int)c < 2 * A.D) {
+          u32 ko = kr + c, vo = vr + c;
+          asm volatile("" : "+v"(ko), "+v"(vo));  // 32 bits beside the scalar base, not 64 held for each row
+          load_to_lds(kb + ko, sk + (w * W::RW + i * W::RI) * DT);
+          load_to_lds(vb + vo, sv + (w * W::RW + i * W::RI) * DT);
+        }
+      }
+    } else if (A.page % 8 == 0) {  // the rows of a load do
+      const int in = lane_key(k0) - page_of(A, lane_key(k0)) * A.page;
 #pragma unroll
       for (int i = 0; i < W::NI; ++i) {
-        const long p = WHOLE ? __builtin_amdgcn_readfirstlane(page) : __builtin_amdgcn_readlane(page, i * W::RI);
-        const long n = WHOLE ? uniform(in0) + i * W::RI : __builtin_amdgcn_readlane(in, i * W::RI);
+        const long p = __builtin_amdgcn_readlane(page, i * W::RI), n = __builtin_amdgcn_readlane(in, i * W::RI);
         const u32 c = piece ^ (u32)(W::swz(i * W::RI) << 4);
-        // rows behind the last key: none may lie past its page
-        const u32 r = WHOLE ? rl : min(rl, (int)(A.page - 1 - n));
+        const u32 r = min(rl, (int)(A.page - 1 - n));  // rows behind the last key: none may lie past its page
         if (!PAD || (int)c < 2 * A.D) {
           u32 ko = r * (u32)A.ks + c, vo = r * (u32)A.vs + c;
-          asm volatile("" : "+v"(ko), "+v"(vo));  // 32 bits beside a scalar base, not 64 held for each row
+          asm volatile("" : "+v"(ko), "+v"(vo));
           load_to_lds(kc + p * A.kp + n * A.ks + ko, sk + (w * W::RW + i * W::RI) * DT);
           load_to_lds(vc + p * A.vp + n * A.vs + vo, sv + (w * W::RW + i * W::RI) * DT);
         }
@@ -802,6 +814,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     return r * DT * 2 + ((c ^ W::swz(r)) << 4) + 8 * (l & 1);
   };
 
+  int k_held = DT == 256 ? 0 : k_lane(lane_anew()), v_held = DT == 256 ? 0 : v_lane(lane_anew());
   // V's fragment: 32 values (d) by 16 keys, in the order of the weights' lanes
   auto v_frag = [&](const uint16_t* sv, int vl, int d, int n, int j) {
     i16x4 v[2];
@@ -828,8 +841,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
 #pragma unroll
     for (int i = 0; i < 4; ++i) any_bad |= sbad[buf][i];
     any_bad = __builtin_amdgcn_readfirstlane(any_bad);
-    if (k0 + TK > hi_g || any_bad) clear_unseen(k0, buf, sv);
-    if (k0 + TK > lo_g && lo_g < hi_g) {  // such values are left out here and counted at the end
+    const bool edge = k0 + TK > lo_g || any_bad;  // not all rows attend to all keys
+    if (edge && (k0 + TK > hi_g || any_bad)) clear_unseen(k0, buf, sv);
+    if (edge && k0 + TK > lo_g && lo_g < hi_g) {  // such values are left out here and counted at the end
       bool nf = false;
       for (int x = threadIdx.x; x < TK * W::CPR; x += kThreads) {
         uint4& v = reinterpret_cast<uint4*>(sv)[x];
@@ -840,9 +854,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       }
       special = __syncthreads_or(nf) || special;
     }
-    if (k0 >= hi_w) return;
-    // taken anew for each buffer: held across the loop, the addresses of all the reads do not fit the registers
-    const int la = lane_anew(), kl = k_lane(la), vl = v_lane(la);
+    if (k0 >= hi_w) return;  // a wave without rows too
+    // at head dim 256 taken anew for each buffer: what is held across the loop must fit the registers
+    const int la = lane_anew(), kl = DT == 256 ? k_lane(la) : k_held, vl = DT == 256 ? v_lane(la) : v_held;
     f32x16 s[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n)
@@ -870,14 +884,14 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
-    if (k0 + TK > lo_w) {
+    if (edge && k0 + TK > lo_w) {
       const int left = lim - k0 - 4 * (lane_anew() / 32);
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[n][x] = n * 32 + 8 * (x / 4) + x % 4 < left ? s[n][x] : kNegInf;
     }
-    if (any_bad) {
+    if (edge && any_bad) {
       const int hb = lane_anew() / 32;
 #pragma unroll
       for (int n = 0; n < NS; ++n)
@@ -915,8 +929,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         for (int x = 0; x < 4; ++x) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x], c, -base));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x + 1], c, -base));
-          l += p0 + p1;
-          pk[x] = pack2(p0, p1);  // rounded for the product, as V is: the sums stay in 32 bits
+          // rounded for the product, as V is; the sums stay in 32 bits, l's too: of the rounded weights
+          pk[x] = pack2(p0, p1);
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk[x]), bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
         }
         p[n][j] = __builtin_bit_cast(bf16x8, make_uint4(pk[0], pk[1], pk[2], pk[3]));
       }
