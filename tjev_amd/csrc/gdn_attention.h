@@ -182,6 +182,12 @@ __device__ __forceinline__ float rows_sum(float v) {
 // the base of the powers: 0 where a row has seen no key yet, so that its powers are 0 and not NaN
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
 
+// The weights are rounded to bf16 for their product with V, which is bf16; their sums, which stay in 32 bits, are of the
+// rounded ones, so that a row's weights still add up to one.
+__device__ __forceinline__ float sum_pair(u32 pair, float sum) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+}
+
 // out += P V for one step (KG groups of 16 keys). V [key group][r]: the lane's keys 4 (lane / 16) + r
 template <class T, int DT, int NQ>
 __device__ __forceinline__ void add_pv(const typename Shape<T, DT>::VVec (&v)[Shape<T, DT>::KG][4][Shape<T, DT>::VH],
@@ -191,7 +197,7 @@ __device__ __forceinline__ void add_pv(const typename Shape<T, DT>::VVec (&v)[Sh
   if constexpr (S::BF) {
     bf16x8 pb[NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)  // rounded to bf16 for the product, as V is: the sums stay in 32 bits
+    for (int n = 0; n < NQ; ++n)
       pb[n] = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[0][n][0], p[0][n][1]), pack2(p[0][n][2], p[0][n][3]),
                                                     pack2(p[1][n][0], p[1][n][1]), pack2(p[1][n][2], p[1][n][3])));
 #pragma unroll
@@ -530,10 +536,16 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
       for (int j = 0; j < KG; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[j][n][r] = __builtin_amdgcn_exp2f(s[j][n][r] - base);
-          l[n] += s[j][n][r];
+        for (int r = 0; r < 4; ++r) s[j][n][r] = __builtin_amdgcn_exp2f(s[j][n][r] - base);
+#pragma unroll
+      for (int j = 0; j < KG; ++j) {
+        if constexpr (S::BF) {
+          l[n] = sum_pair(pack2(s[j][n][0], s[j][n][1]), l[n]);
+          l[n] = sum_pair(pack2(s[j][n][2], s[j][n][3]), l[n]);
+        } else {
+          l[n] += (s[j][n][0] + s[j][n][1]) + (s[j][n][2] + s[j][n][3]);
         }
+      }
 #pragma unroll
       for (int x = 0; x < S::VH; ++x)
 #pragma unroll
@@ -929,9 +941,8 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         for (int x = 0; x < 4; ++x) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x], c, -base));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x + 1], c, -base));
-          // rounded for the product, as V is; the sums stay in 32 bits, l's too: of the rounded weights
           pk[x] = pack2(p0, p1);
-          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk[x]), bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
+          l = sum_pair(pk[x], l);
         }
         p[n][j] = __builtin_bit_cast(bf16x8, make_uint4(pk[0], pk[1], pk[2], pk[3]));
       }
