@@ -178,6 +178,20 @@ def test_bad_values_reach_only_their_rows(dtype, lens, dim):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lens,dim", [([(50, 1)], 64), ([(600, 3), (7, 1)], 128), ([(40, 40)], 256), ([(3000, 1)], 128)])
+def test_infinities_that_all_rows_attend_to(dtype, lens, dim):
+    """Infinities among the values of a request's first tokens come out as such: no weight is or has a part that is 0."""
+    case = batch(torch.Generator().manual_seed(16), lens, heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    for b in range(len(lens)):
+        page = int(case["block_table"][b, 0])
+        case["v_cache"][page, 0, 0, 3], case["v_cache"][page, 1, 1, 5] = math.inf, -math.inf
+    print(f"attention with infinities {dtype} {lens} dim={dim}", flush=True)
+    want, room = attention64(*(case[n] for n in ("q", "k_cache", "v_cache", "block_table", "starts", "lengths")))
+    assert bool((want[:, :2, 3] == math.inf).all()) and bool((want[:, 2:, 5] == -math.inf).all()) and bool((~torch.isnan(want)).all())
+    compare(_attend(case), want, room)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_layouts_and_views(dtype):
     """Caches with the heads before the places, or keys and values in one tensor; q beside its gate; a given out
     whose rows of no request stay; another scale; int64 lengths; starts that leave rows in front."""
@@ -234,6 +248,49 @@ def test_long_requests_over_many_workgroups(dtype, lens, heads, dim):
             room = room + (2.0 ** -8 if dtype == BF else 2.0 ** -24) * (want.abs() + room)
             compare(got[s0:s0 + n, h], want.cpu(), room.cpu())
     assert torch.equal(got, _attend(case))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("requests,lens,heads,kv_heads,dim", [
+    (700, lambda b: (b * 7 % 40, 0 if b % 5 == 3 else 1), 2, 1, 64),      # more requests than a workgroup reads at once
+    (300, lambda b: (b % 23, b % 4), 8, 2, 40), (40, lambda b: (600 - b, 1), 4, 2, 128),
+    (3, lambda b: (900 + b, 200), 8, 4, 128), (9, lambda b: (400, 1 + 60 * (b % 2)), 10, 5, 64),
+])
+def test_many_requests(dtype, requests, lens, heads, kv_heads, dim):
+    """Batches of many tiles, whose parts are joined a tile to a workgroup."""
+    print(f"attention of {requests} requests {dtype} heads={heads}/{kv_heads} dim={dim}", flush=True)
+    lens = [lens(b) for b in range(requests)]
+    case = batch(torch.Generator().manual_seed(14), lens, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, pad_rows=2)
+    got = _attend(case).cpu()
+    assert bool(torch.isfinite(got).all()) and bool((got[-2:] == 0).all())
+    # every 40th request against the plain form (its rows alone, as a batch of one)
+    for b in range(0, requests, max(1, requests // 40)):
+        s0, s1 = int(case["starts"][b]), int(case["starts"][b + 1])
+        if s1 == s0:
+            continue
+        rows = slice(max(s0, s1 - 3), s1) if requests > 3 else slice(s1 - 2, s1)
+        n = rows.stop - rows.start
+        want, room = attention64(case["q"][rows], case["k_cache"], case["v_cache"], case["block_table"][b:b + 1], torch.tensor([0, n]),
+                                 case["lengths"][b:b + 1])
+        compare(got[rows], want, room)
+
+
+def test_uninitialised_lds():
+    """The debug build whose kernels first fill their LDS with NaN: the same bits."""
+    from tjev_amd import _lib, paged_tables
+
+    for lens, dim, dtype in (("ragged", 64, BF), ("chunk", 128, BF), ("chunk", 256, BF), ("drafts", 200, BF), ("decode", 128, F32), ("ragged", 256, F32)):
+        case = batch(torch.Generator().manual_seed(15), LENS[lens], heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype, gate=True)
+        print(f"poisoned LDS {lens} dim={dim} {dtype}", flush=True)
+        want = _attend(case)
+        with _lib.library(_lib.LDS_POISON_PATH):
+            assert torch.equal(_attend(case), want)
+    i = torch.tensor([5, 0, 40], dtype=torch.int32, device="cuda")
+    args = (i, i.flip(0), torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4), torch.arange(9, dtype=torch.int32, device="cuda"))
+    want = paged_tables(*args, page_size=16, tokens=60)
+    with _lib.library(_lib.LDS_POISON_PATH):
+        for x, y in zip(paged_tables(*args, page_size=16, tokens=60), want):
+            assert torch.equal(x, y)
 
 
 def test_offsets_past_32_bits():

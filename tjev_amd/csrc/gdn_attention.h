@@ -182,8 +182,17 @@ __device__ __forceinline__ float rows_sum(float v) {
 // the base of the powers: 0 where a row has seen no key yet, so that its powers are 0 and not NaN
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
 
-// The weights are rounded to bf16 for their product with V, which is bf16; their sums, which stay in 32 bits, are of the
-// rounded ones, so that a row's weights still add up to one.
+// Streamed rows' weights meet V, which is bf16, as two bf16 terms each, hi the first 8 bits and lo the rest (rounded:
+// 2^-15 of the weight); the second product is free beside the loads. A weight's last bit is set first, so that lo is
+// never 0 and an infinity of V stays one.
+__device__ __forceinline__ Split2 split_weights(float a, float b) {
+  const u32 x = __float_as_uint(a) | 1u, y = __float_as_uint(b) | 1u;
+  return {__builtin_amdgcn_perm(y, x, 0x07060302u),
+          pack2(__uint_as_float(x) - __uint_as_float(x & 0xffff0000u), __uint_as_float(y) - __uint_as_float(y & 0xffff0000u))};
+}
+
+// The wide tiles, bound by their products, round the weights to bf16; their sums, which stay in 32 bits, are of the rounded
+// ones, so that a row's weights still add up to one.
 __device__ __forceinline__ float sum_pair(u32 pair, float sum) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
 }
@@ -195,11 +204,14 @@ __device__ __forceinline__ void add_pv(const typename Shape<T, DT>::VVec (&v)[Sh
                                        f32x4 (&o)[NQ][Shape<T, DT>::VH][Shape<T, DT>::VE]) {
   using S = Shape<T, DT>;
   if constexpr (S::BF) {
-    bf16x8 pb[NQ];
+    bf16x8 hi[NQ], lo[NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-      pb[n] = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[0][n][0], p[0][n][1]), pack2(p[0][n][2], p[0][n][3]),
-                                                    pack2(p[1][n][0], p[1][n][1]), pack2(p[1][n][2], p[1][n][3])));
+    for (int n = 0; n < NQ; ++n) {
+      const Split2 a = split_weights(p[0][n][0], p[0][n][1]), b = split_weights(p[0][n][2], p[0][n][3]);
+      const Split2 c = split_weights(p[1][n][0], p[1][n][1]), d = split_weights(p[1][n][2], p[1][n][3]);
+      hi[n] = __builtin_bit_cast(bf16x8, make_uint4(a.hi, b.hi, c.hi, d.hi));
+      lo[n] = __builtin_bit_cast(bf16x8, make_uint4(a.lo, b.lo, c.lo, d.lo));
+    }
 #pragma unroll
     for (int h = 0; h < S::VH; ++h)
 #pragma unroll
@@ -211,7 +223,10 @@ __device__ __forceinline__ void add_pv(const typename Shape<T, DT>::VVec (&v)[Sh
           w[i] = __builtin_amdgcn_perm(word(v[i / 2][2 * (i % 2) + 1][h], e / 2), word(v[i / 2][2 * (i % 2)][h], e / 2), sel);
         const bf16x8 a = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) o[n][h][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[n], o[n][h][e], 0, 0, 0);
+        for (int n = 0; n < NQ; ++n) {
+          o[n][h][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo[n], o[n][h][e], 0, 0, 0);
+          o[n][h][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi[n], o[n][h][e], 0, 0, 0);
+        }
       }
   } else {
 #pragma unroll
@@ -538,14 +553,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[j][n][r] = __builtin_amdgcn_exp2f(s[j][n][r] - base);
 #pragma unroll
-      for (int j = 0; j < KG; ++j) {
-        if constexpr (S::BF) {
-          l[n] = sum_pair(pack2(s[j][n][0], s[j][n][1]), l[n]);
-          l[n] = sum_pair(pack2(s[j][n][2], s[j][n][3]), l[n]);
-        } else {
-          l[n] += (s[j][n][0] + s[j][n][1]) + (s[j][n][2] + s[j][n][3]);
-        }
-      }
+      for (int j = 0; j < KG; ++j) l[n] += (s[j][n][0] + s[j][n][1]) + (s[j][n][2] + s[j][n][3]);
 #pragma unroll
       for (int x = 0; x < S::VH; ++x)
 #pragma unroll
@@ -1124,8 +1132,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
   __shared__ __align__(16) uint4 sb[NB];
   __shared__ __align__(16) uint4 sc[MIXED ? BUF : 1];
   __shared__ __align__(16) uint4 sd[MIXED && Wide<DT>::QL ? 4 * Wide<DT>::QL * 64 : 1];
-  GDN_POISON_LDS(sfound, sm, sl, sbad, sa, sb, sc, sd);
-
   // Where the range stands. In LDS while a tile is worked on: held in registers it would be spilled there.
   __shared__ struct {
     Request q;
@@ -1133,6 +1139,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
     Unit at;
     int b, range, begun;
   } st;
+  GDN_POISON_LDS(sfound, sm, sl, sbad, sa, sb, sc, sd, st);
+
   {
     const int range = range_of(blockIdx.x, A.G);
     const Found f = find_range<R, KB>(A, range, sfound);
@@ -1282,6 +1290,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   }
   if constexpr (SLICED) {
     __shared__ __align__(16) f32x4 sacc[(PG - 1) * kSlice];
+    GDN_POISON_LDS(sacc);
     if (pg) sacc[(pg - 1) * kSlice + tid % kSlice] = acc[0];
     __syncthreads();
     if (pg) return;

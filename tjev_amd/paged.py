@@ -77,7 +77,7 @@ def _tables_params(t_shape, t_stride, t_dtype, lengths, list_shapes, int_dtypes,
         if dt not in (torch.int32, torch.int64):
             raise ValueError(f"lengths, pages and taken are int32 or int64, not {dt}")
     _lib.one_gpu("paged_tables", devices)
-    if inplace and width > 1 and (t_stride[1] != 1 or (requests > 1 and t_stride[0] != width)):
+    if inplace and ((width > 1 and t_stride[1] != 1) or (requests > 1 and t_stride[0] != width)):
         raise ValueError("inplace: the block table must be contiguous (a copy would leave the caller's unchanged)")
     return ctypes.byref(_lib.PagedParams(tokens=tokens, requests=requests, table_width=width, page_size=page_size))
 
@@ -194,11 +194,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q [N, heads, dim] (heads: groups of kv_heads; dim in multiples of 8 up to 256): rows starts[b] ..
     starts[b + 1] - 1 are the last tokens of request b, whose keys are ``lengths[b]`` in all, in the pages of row b of
     ``block_table`` [B, M] int32. Each attends to the keys up to its own, softmax(scale q k^T) v with scale
-    dim^-1/2 by default, in 32 bits (bf16: the weights rounded to bf16 for their product with v); a row without
-    keys is 0. ``gate`` [N, heads, dim] multiplies the result by its
-    sigmoid. Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
-    q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not). What the
-    cache holds elsewhere (NaN too) does not matter."""
+    dim^-1/2 by default, in 32 bits; a row without keys is 0. (In bf16 the weights of a request with more than 16
+    tokens times query heads per key head are rounded to bf16 for their product with v.) ``gate`` [N, heads, dim]
+    multiplies the result by its sigmoid. Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
+    q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
+    none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
     q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.contiguous() for x in (q, gate))
     lib = _lib.load()
     p, need = _attention_params(
