@@ -80,7 +80,7 @@ int main() {
     gdn::set_page(A, pages[pick(0, 7)]);
     A.pages = pick(1, 12);
     A.Hk = pick(1, 4);
-    A.g = pick(1, 20);
+    A.g = it % 7 ? pick(1, 20) : pick(1, 300);
     A.N = pick(0, it % 5 ? 40 : 150);
     A.wide = it % 2 ? 1 << 30 : pick(0, 64);
     std::vector<int32_t> table(A.B * A.M), starts(A.B + 1), lengths(A.B);

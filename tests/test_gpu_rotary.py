@@ -163,3 +163,36 @@ def test_one_gradient_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, call())
+
+
+def test_captured_gradient():
+    """Forward and gradient captured into a graph, replayed on new values beside eager calls."""
+    from tjev_amd import rotary_axes
+
+    gen = torch.Generator().manual_seed(7)
+    q, k = (torch.randn(2, 40, h, 64, generator=gen).to(BF).cuda().requires_grad_(True) for h in (4, 2))
+    dq, dk = torch.randn(2, 40, 4, 64, generator=gen).to(BF).cuda(), torch.randn(2, 40, 2, 64, generator=gen).to(BF).cuda()
+    pos, inv = torch.randint(0, 1000, (3, 2, 40), generator=gen).cuda(), _freqs(32).cuda()
+
+    def step():
+        a, b = rotary_axes(q, k, pos, inv, sections=(12, 10, 10), interleaved=True)
+        return [a.detach(), b.detach(), *torch.autograd.grad((a, b), (q, k), (dq, dk))]
+
+    print("rotary gradient captured", flush=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            q.mul_(-1.5)
+            dq.mul_(1.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, step()):
+            assert torch.equal(x, y)

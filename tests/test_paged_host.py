@@ -97,6 +97,17 @@ def test_tables_refusals(bad, match):
         paged_tables(**a)
 
 
+@pytest.mark.parametrize("table", [torch.zeros(2, 6, dtype=torch.int32)[:, ::2], torch.zeros(3, 2, dtype=torch.int32).t(),
+                                   torch.zeros(2, 3, dtype=torch.int32)[:, :1], torch.zeros(2, 5, dtype=torch.int32)[:, :3]])
+def test_tables_refuse_to_copy_a_table_changed_in_place(monkeypatch, table):
+    from tjev_amd import _lib, paged_tables
+
+    monkeypatch.setattr(_lib, "one_gpu", lambda what, devices: None)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="contiguous"):
+        paged_tables(i, i, table, i, page_size=16, tokens=4, inplace=True)
+
+
 @pytest.mark.parametrize("bad,match", [
     (dict(v=torch.zeros(3, 2, 32)), "alike"),
     (dict(k=torch.zeros(3, 2, 64, dtype=BF), v=torch.zeros(3, 2, 64, dtype=BF)), "cache's type"),

@@ -169,8 +169,8 @@ int tjev_gdn_paged_tables(const tjev_gdn_paged_params* p, void* stream, const in
       !lengths || !taken_out)
     return fail(TJEV_GDN_EINVAL, "null tensor argument");
   if (taken == taken_out) return fail(TJEV_GDN_EINVAL, "taken_out must not alias taken (every workgroup reads it)");
-  const gdn::TableArgs A{p->requests, p->table_width, gdn::div_by(p->page_size), gdn::div_by(p->table_width), p->tokens, n_free, cached, new_tokens, block_table, free_pages,
-                         taken, table_out, slots, starts, lengths, taken_out};
+  const gdn::TableArgs A{p->requests, p->table_width, gdn::div_by(p->page_size), gdn::div_by(p->table_width), p->tokens, n_free,
+                         cached, new_tokens, block_table, free_pages, taken, table_out, slots, starts, lengths, taken_out};
   const long work = (long)p->requests * p->table_width + p->tokens;
   const long blocks = (work + 2047) / 2048;
   const dim3 grid((unsigned)(blocks < 1024 ? blocks : 1024)), block(gdn::kThreads);
@@ -225,9 +225,10 @@ int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const vo
   A.inv_per = (unsigned)(((1ul << 32) + per - 1) / per);
   A.inv_chunks = (unsigned)(((1ul << 32) + chunks - 1) / chunks);
   A.tile = per >= 512 ? 1 : (int)(512 / per);
-  const unsigned blocks = (unsigned)((A.N + A.tile - 1) / A.tile);
+  const long blocks = (A.N + A.tile - 1) / A.tile;
+  if (blocks >= (1l << 32) / gdn::kThreads) return fail(TJEV_GDN_EINVAL, "problem too large");  // a launch's threads
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(blocks), block(gdn::kThreads);
+  const dim3 grid((unsigned)blocks), block(gdn::kThreads);
   if (w == 16) {
     hipLaunchKernelGGL((gdn::k_paged_append<uint4>), grid, block, 0, st, A);
   } else if (w == 4) {

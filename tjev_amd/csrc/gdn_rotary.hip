@@ -233,7 +233,7 @@ extern "C" int tjev_gdn_rotary(const tjev_gdn_rotary_params* p, void* stream, co
   const long fill = 262144 / (tokens * A.slots) + 1;
   A.groups = (int)(fill < total ? fill : total);
   const long blocks = (tokens * A.slots * A.groups + gdn::kThreads - 1) / gdn::kThreads;
-  if (blocks >= (1l << 31)) return fail(TJEV_GDN_EINVAL, "problem too large");
+  if (blocks >= (1l << 32) / gdn::kThreads) return fail(TJEV_GDN_EINVAL, "problem too large");  // a launch's threads
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == TJEV_GDN_BF16) {
     wide ? gdn::launch<uint16_t, 8>(A, p->adjacent, (unsigned)blocks, st) : gdn::launch<uint16_t, 1>(A, p->adjacent, (unsigned)blocks, st);
