@@ -100,7 +100,7 @@ def paged_tables(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Ten
     dev, requests = block_table.device, block_table.shape[0]
     cached, new, free_pages, table = _int32(cached), _int32(new), _int32(free_pages), block_table.contiguous()
     taken = None if taken is None else _int32(taken)
-    table_out = table if inplace else torch.empty(table.shape, dtype=torch.int32, device=dev)
+    table_out = table if inplace else torch.empty_like(table)
     slots = torch.empty(int(tokens), dtype=torch.int64, device=dev)
     starts, lengths, taken_out = torch.empty(2 * requests + 2, dtype=torch.int32, device=dev).split((requests + 1, requests, 1))
     with _lib.on_device(dev):
@@ -208,7 +208,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         (q.get_device(), k_cache.get_device(), v_cache.get_device(), block_table.get_device(), starts.get_device(), lengths.get_device(),
          _device(gate, q), _device(out, q)))
     starts, lengths, block_table, dev = _int32(starts), _int32(lengths), block_table.contiguous(), q.device
-    y = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         _lib.check_status(lib.tjev_gdn_paged_attention(

@@ -58,7 +58,12 @@ def _checked(q_shape, q_dtype, k_shape, k_dtype, p_shape, p_dtype, f_shape, f_dt
 
 @functools.lru_cache(maxsize=256)
 def _params(q_shape, q_stride, dtype, k_shape, k_stride, half, axes, sections, interleaved, adjacent, inverse, p_dtype, f_dtype):
-    """The library's view of a call (a reference to the struct; never changed): q [B, T, Hq, D], k [B, T, Hk, D] or None."""
+    """The library's view of a call (a reference to the struct; never changed): q [B, T, Hq, D], k [B, T, Hk, D] or None;
+    [T, Hq, D] is a batch of one."""
+    if len(q_shape) == 3:
+        q_shape, q_stride = (1, *q_shape), (0, *q_stride)
+        if k_shape is not None:
+            k_shape, k_stride = (1, *k_shape), (0, *k_stride)
     batch, length, heads, dim = q_shape
     return ctypes.byref(_lib.RotaryParams(
         batch, length, heads, 0 if k_shape is None else k_shape[2], dim, 2 * half, axes, (ctypes.c_int32 * _lib.MAX_AXES)(*sections),
@@ -67,12 +72,12 @@ def _params(q_shape, q_stride, dtype, k_shape, k_stride, half, axes, sections, i
 
 
 def _launch(q, k, positions, inv_freq, axes, sections, interleaved: bool, adjacent: bool, inverse: bool):
-    """The library's call: q [B, T, Hq, D], k [B, T, Hk, D] or None (the last dim contiguous)."""
+    """The library's call: q [B, T, Hq, D] or [T, Hq, D], k alike or None (the last dim contiguous)."""
     dev = q.device
     p = _params(q.shape, q.stride(), q.dtype, None if k is None else k.shape, None if k is None else k.stride(), inv_freq.shape[0],
                 axes, sections, interleaved, adjacent, inverse, positions.dtype, inv_freq.dtype)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     with _lib.on_device(dev):
         _lib.check_status(_lib.load().tjev_gdn_rotary(
             p, _lib.current_stream(dev), q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
@@ -123,7 +128,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
                     inv_freq.shape, inv_freq.dtype, secs, interleaved,
                     (q.get_device(), positions.get_device(), inv_freq.get_device(), q.get_device() if k is None else k.get_device()))
     q4, k4 = q, k
-    if q.dim() != 4:
+    if q.dim() > 4:
         batch = math.prod(q.shape[:-3])
         q4 = q.reshape(batch, *q.shape[-3:])
         k4 = None if k is None else k.reshape(batch, *k.shape[-3:])
@@ -133,6 +138,6 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         q4, k4 = _Rotary.apply(*args, options, False)
     else:
         q4, k4 = _launch(*args, *options, False)
-    if q.dim() == 4:
+    if q.dim() <= 4:
         return q4, k4
     return q4.reshape(q.shape), None if k is None else k4.reshape(k.shape)
