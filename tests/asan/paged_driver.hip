@@ -22,9 +22,9 @@ static void walk(const gdn::Batch& A) {
     check(q.rows == 0 || (q.s0 >= 0 && q.s0 + (q.rows - 1) / A.g < A.N), "rows");
     check((long)q.tiles * q.tile_rows >= q.rows, "tiles");
     for (int r = 0; r < q.rows; ++r) {
-      const int lim = gdn::row_limit(q, r, A.g);
+      const int lim = gdn::row_limit(A, q, r);
       check(lim >= 0 && lim <= q.keys, "limit");
-      check(r == 0 || lim >= gdn::row_limit(q, r - 1, A.g), "limits grow with the rows");
+      check(r == 0 || lim >= gdn::row_limit(A, q, r - 1), "limits grow with the rows");
       check((long)q.tile_blocks(r / q.tile_rows) * KB >= lim, "a tile's units hold its keys");
     }
     long sum = 0;  // every unit once, in order, and at least one to a tile
@@ -41,7 +41,7 @@ static void walk(const gdn::Batch& A) {
           check(u.head == h && u.tile == t && u.at == k, "a unit's place");
         }
     if (!q.rows) continue;
-    const int hi = gdn::row_limit(q, q.rows - 1, A.g);
+    const int hi = gdn::row_limit(A, q, q.rows - 1);
     for (int k0 = 0; k0 < hi; k0 += 32)  // a wave's steps (those of 16 keys are among them)
       for (int j = 0; j < 32; j += 16) {
         const int key0 = k0 + j;
@@ -80,7 +80,7 @@ int main() {
     gdn::set_page(A, pages[pick(0, 7)]);
     A.pages = pick(1, 12);
     A.Hk = pick(1, 4);
-    A.g = it % 7 ? pick(1, 20) : pick(1, 300);
+    gdn::set_group(A, it % 7 ? pick(1, 20) : pick(1, 300));
     A.N = pick(0, it % 5 ? 40 : 150);
     A.wide = it % 2 ? 1 << 30 : pick(0, 64);
     std::vector<int32_t> table(A.B * A.M), starts(A.B + 1), lengths(A.B);

@@ -30,10 +30,21 @@ __device__ __forceinline__ long uniform(long v) {
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// one lane's value, held once
+__device__ __forceinline__ int of_lane(int v, int from) { return __builtin_amdgcn_readlane(v, from); }
+__device__ __forceinline__ long of_lane(long v, int from) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, from), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), from);
+  return (long)((uint64_t)hi << 32 | lo);
+}
+// a request made of the values that f takes from q's
+template <class F>
+__device__ __forceinline__ Request each_of(const Request& q, F f) {
+  return {f(q.s0), f(q.rows), f(q.tiles), f(q.tile_rows), f(q.keys), f(q.extra), f(q.blocks), f(q.y),
+          {__builtin_bit_cast(double, f(__builtin_bit_cast(long, q.by_g.inv))), f(q.by_g.d)}, f(q.first), f(q.per_head), f(q.cost)};
+}
 __device__ __forceinline__ Request uniform(const Request& q) {
-  return {uniform(q.s0), uniform(q.rows), uniform(q.tiles), uniform(q.tile_rows), uniform(q.keys), uniform(q.extra), uniform(q.blocks), uniform(q.y),
-          {__builtin_bit_cast(double, uniform(__builtin_bit_cast(long, q.by_g.inv))), uniform(q.by_g.d)}, uniform(q.first), uniform(q.per_head),
-          uniform(q.cost)};
+  return each_of(q, [](auto v) { return uniform(v); });
 }
 
 // The kernel's arguments read anew: what a tile needs of them is then held for the tile only, and not (spilled)
@@ -52,13 +63,28 @@ __device__ __forceinline__ int lane_anew() {
   return l;
 }
 
+// the lane's value moved by a row shift (or broadcast) within the wave, 0 where none comes
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long moved(long v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)v >> 32), CTRL, ROWS, 0xf, true);
+  return (long)((uint64_t)hi << 32 | lo);
+}
+// inclusive running sum over the wave's lanes: within rows of 16, then each row's last to the row behind it, then
+// the first half's last to the second (no LDS: a step is a few cycles, a shuffle's a hundred)
+__device__ __forceinline__ long scan_wave(long v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
 // inclusive running sum over the workgroup's threads (in order); total: the sum of all
 __device__ __forceinline__ long scan_block(long v, long* swave, long& total) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const long t = __shfl_up(v, d);
-    if (lane() >= d) v += t;
-  }
+  v = scan_wave(v);
   __syncthreads();
   if (lane() == 63) swave[wave()] = v;
   __syncthreads();
@@ -85,46 +111,43 @@ struct FoundLds {
   Request q;
 };
 
-// Up to kThreads requests are read and summed once, more of them in turns, twice.
+// Up to 64 requests are read and summed by each wave for itself, more of them by the workgroup, in turns, twice.
 template <int R, int KB>
 __device__ __forceinline__ Found find_range(const AttnArgs& A, int range, FoundLds& f) {
   const int tid = threadIdx.x;
-  const bool once = A.B <= kThreads;
   Found r;
-  Request q{};
-  long units = 0, sum = 0;  // the thread's inclusive sum, the batch's
-  auto load = [&](int b) {
-    q = Request{};
-    if (b < A.B) q = request<R, KB>(A, b);
-  };
-  if (tid == 0) f.b = -1;
-  if (once) {
-    load(tid);
-    units = scan_block(q.cost, f.swave, sum);
-  } else {
-    long mine = 0;
-    for (int b0 = 0; b0 < A.B; b0 += kThreads) {
-      load(b0 + tid);
-      mine += q.cost;
+  auto load = [&](int b) { return b < A.B ? request<R, KB>(A, b) : Request{}; };
+  if (A.B <= 64) {
+    const Request q = load(lane());
+    const long upto = scan_wave(q.cost);
+    r.total = of_lane(upto, 63);
+    r.each = r.total ? A.by_G(r.total + A.G - 1) : 1;
+    const long place = range * r.each;
+    const uint64_t here = __ballot(place >= upto - q.cost && place < upto);
+    r.b = here ? __builtin_ctzll(here) : -1;
+    if (here) {
+      r.q = each_of(q, [&](auto v) { return of_lane(v, r.b); });
+      r.unit = of_lane(upto, r.b) - r.q.cost;
     }
-    scan_block(mine, f.swave, sum);
+    return r;
   }
+  if (tid == 0) f.b = -1;
+  long mine = 0, sum = 0;
+  for (int b0 = 0; b0 < A.B; b0 += kThreads) mine += load(b0 + tid).cost;
+  scan_block(mine, f.swave, sum);
   r.total = sum;
-  r.each = sum ? (sum + A.G - 1) / A.G : 1;
+  r.each = sum ? A.by_G(sum + A.G - 1) : 1;
   const long place = range * r.each;
-  long before = 0;
-  for (int b0 = 0; b0 < A.B; b0 += kThreads) {
-    if (!once) {
-      load(b0 + tid);
-      units = scan_block(q.cost, f.swave, sum) + before;
-      before += sum;
-    }
-    if (place >= units - q.cost && place < units) {
+  long before = 0;  // the turns' sum
+  for (int b0 = 0; b0 < A.B && before <= place; b0 += kThreads) {
+    const Request q = load(b0 + tid);
+    const long upto = scan_block(q.cost, f.swave, sum) + before;
+    before += sum;
+    if (place >= upto - q.cost && place < upto) {
       f.b = b0 + tid;
       f.q = q;
-      f.unit = units - q.cost;
+      f.unit = upto - q.cost;
     }
-    if (!once && before > place) break;
   }
   __syncthreads();
   r.b = uniform(f.b);
@@ -419,7 +442,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
     const int n = x / S::KS, i = x - n * S::KS, row = row0 + n * 16 + r16, e = (4 * i + g4) * E;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (row < q.rows && !(PAD && e >= A.D)) {
-      const int t = row / A.g;
+      const int t = A.by_g(row);
       v = *reinterpret_cast<const uint4*>(A.q + (long)(q.s0 + t) * A.qt + (h * A.g + (row - t * A.g)) * A.qh + e * (int)sizeof(T));
     }
     sq[x * 64 + ln] = v;
@@ -430,7 +453,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int row = row0 + n * 16 + r16;
-    lim[n] = row < q.rows ? row_limit(q, row, A.g) : 0;
+    lim[n] = row < q.rows ? row_limit(A, q, row) : 0;
     m[n] = kNegInf;
     l[n] = 0.f;
 #pragma unroll
@@ -438,7 +461,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
       for (int e = 0; e < S::VE; ++e) o[n][x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int lo_lim = uniform(row_limit(q, row0, A.g)), hi_lim = uniform(row_limit(q, min(row0 + R, q.rows) - 1, A.g));
+  const int lo_lim = uniform(row_limit(A, q, row0)), hi_lim = uniform(row_limit(A, q, min(row0 + R, q.rows) - 1));
   const int32_t* table = A.table + (long)b * A.M;
   const char *kc = A.k + h * A.kh, *vc = A.v + h * A.vh;
   __syncthreads();
@@ -621,7 +644,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
     if (!part.p) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        const int row = row0 + n * 16 + r16, t = row / A.g;
+        const int row = row0 + n * 16 + r16, t = A.by_g(row);
         if (row < q.rows) store_row<T, DT, PAD>(A, o[n], lj[n], q.s0 + t, h * A.g + (row - t * A.g));
       }
     } else {
@@ -764,7 +787,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   const int w = __builtin_amdgcn_readfirstlane(wave()), h = part.head, row0 = part.tile * kWideRows;
   // the lane's row: its token and head, the byte offset of its values (a row past the last: row 0's)
   auto place = [&](int l, bool& live, long& token, int& head) {
-    const int row = row0 + w * 32 + l % 32, t = row / A.g;
+    const int row = row0 + w * 32 + l % 32, t = A.by_g(row);
     live = row < q.rows;
     token = q.s0 + (live ? t : 0);
     head = h * A.g + (live ? row - t * A.g : 0);
@@ -772,13 +795,13 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   int lim;
   {
     const int row = row0 + w * 32 + lane_anew() % 32;
-    lim = row < q.rows ? row_limit(q, row, A.g) : 0;
+    lim = row < q.rows ? row_limit(A, q, row) : 0;
   }
   // limits of the wave's and of the workgroup's first and last rows
   const int wr = row0 + w * 32;
   const bool rows_w = wr < q.rows;  // a wave without rows only helps to bring K and V
-  const int lo_w = uniform(rows_w ? row_limit(q, wr, A.g) : 0), hi_w = uniform(rows_w ? row_limit(q, min(wr + 32, q.rows) - 1, A.g) : 0);
-  const int lo_g = uniform(row_limit(q, row0, A.g)), hi_g = uniform(row_limit(q, min(row0 + kWideRows, q.rows) - 1, A.g));
+  const int lo_w = uniform(rows_w ? row_limit(A, q, wr) : 0), hi_w = uniform(rows_w ? row_limit(A, q, min(wr + 32, q.rows) - 1) : 0);
+  const int lo_g = uniform(row_limit(A, q, row0)), hi_g = uniform(row_limit(A, q, min(row0 + kWideRows, q.rows) - 1));
   const bool flip = A.c < 0.f;  // the scale's sign goes into q, which is exact
   const float c = flip ? -A.c : A.c;
 
@@ -1055,7 +1078,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         T* op[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          const int r = i * (64 / LPR) + ln / LPR, row = row0 + w * 32 + r, t = row / A.g, e = p * HD + c8;
+          const int r = i * (64 / LPR) + ln / LPR, row = row0 + w * 32 + r, t = A.by_g(row), e = p * HD + c8;
           op[i] = nullptr;
           if (row < q.rows && !(PAD && e >= A.D)) {
             const long token = q.s0 + t;
@@ -1174,7 +1197,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
       __syncthreads();
       if (threadIdx.x == 0) {
         if (keys > 0 && k0 == 0 && keys < blocks)  // the tile goes on in the next ranges
-          *split_of(A, range) = {(int)((u - at.at + q.extra + blocks - 1) / st.each) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile,
+          *split_of(A, range) = {(int)div_by(st.each)(u - at.at + q.extra + blocks - 1) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile,
                                  at.head};
         // the next tile, the next head's first, or the next request's with rows
         long local = st.local + seg;
@@ -1299,7 +1322,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   }
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int x = SLICED ? blockIdx.y * kSlice + tid : tid + i * NT, r = tile * ROWS + er[i], t = r / A.g, ln = x % 64, v = x / 64 % (DT / 8);
+    const int x = SLICED ? blockIdx.y * kSlice + tid : tid + i * NT, r = tile * ROWS + er[i], t = A.by_g(r), ln = x % 64, v = x / 64 % (DT / 8);
     const int d = WIDE ? 32 * (v / 4) + 8 * (v % 4) + 4 * (ln / 32) : x % (DT / 4) * 4;
     if (r >= q.rows || d >= A.D) continue;
     const long token = q.s0 + t;

@@ -81,7 +81,7 @@ int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const
   gdn::set_page(A, p->page_size);
   A.pages = p->pages;
   A.Hk = p->kv_heads;
-  A.g = p->heads / p->kv_heads;
+  gdn::set_group(A, p->heads / p->kv_heads);
   A.D = p->dim;
   A.fill = p->fill;
   // a scale of 0 as the smallest number, so that a masked score stays at minus infinity

@@ -7,6 +7,7 @@ namespace {
 template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
 hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   A.G = r.G;
+  A.by_G = div_by(r.G);
   A.slot = r.slot;
   A.wide = MIXED ? 16 * NQ : 0x7fffffff;
   hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);

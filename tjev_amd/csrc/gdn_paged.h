@@ -21,29 +21,42 @@ struct Div {
 };
 inline __host__ __device__ Div div_by(long d) { return {1.0 / (double)d, d}; }
 
+// The same for 0 <= x < 2^31: the high word of x mul, shifted right. With 2^(L-1) < d <= 2^L and mul = ceil(2^(31+L) / d) <
+// 2^32 the product is off by less than x d <= 2^(31+L): the quotient is exact. (d = 1: shift -1, x itself.)
+struct Div32 {
+  uint32_t mul;
+  int shift;
+  __host__ __device__ __forceinline__ int operator()(int x) const {
+    return shift < 0 ? x : (int)(((uint64_t)(uint32_t)x * mul) >> 32 >> shift);
+  }
+};
+inline __host__ __device__ Div32 div32_by(int d) {
+  int L = 0;
+  while ((1l << L) < d) ++L;
+  return {(uint32_t)(((1ul << (31 + L)) + d - 1) / d), L - 1};
+}
+
 // The batch as the caller describes it
 struct Batch {
   long N;                    // rows of q
   int B, M, page, pages;     // requests, table width, page size, pages of the cache
   int Hk, g;                 // key heads, query heads to each
   int wide;                  // requests of more packed rows take wide tiles
-  uint32_t page_mul;         // k / page = the high word of k page_mul, shifted right by page_shift (k < 2^31)
-  int page_shift;
+  Div32 by_page, by_g;       // a key's page, a packed row's token
+  Div by_g_long;
   const int32_t *table, *starts, *lengths;
 };
 
-// With 2^(L-1) < page <= 2^L and page_mul = ceil(2^(31+L) / page) < 2^32 the product is off by less than k page <=
-// 2^(31+L): the quotient is exact. (A page of one token: page_shift -1, k itself.)
 __host__ __device__ __forceinline__ void set_page(Batch& A, int page) {
-  int L = 0;
-  while ((1l << L) < page) ++L;
   A.page = page;
-  A.page_mul = (uint32_t)(((1ul << (31 + L)) + page - 1) / page);
-  A.page_shift = L - 1;
+  A.by_page = div32_by(page);
 }
-__host__ __device__ __forceinline__ int page_of(const Batch& A, int key) {
-  return A.page_shift < 0 ? key : (int)(((uint64_t)(uint32_t)key * A.page_mul) >> 32 >> A.page_shift);
+__host__ __device__ __forceinline__ void set_group(Batch& A, int g) {
+  A.g = g;
+  A.by_g = div32_by(g);
+  A.by_g_long = div_by(g);
 }
+__host__ __device__ __forceinline__ int page_of(const Batch& A, int key) { return A.by_page(key); }
 
 // The packed rows of a request and key head are its new tokens' query heads of that key head: row r
 // is token r / g, head r % g. Requests of more than `wide` rows are worked on in tiles of kWideRows, the others
@@ -85,10 +98,10 @@ __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   const bool wide = q.rows > A.wide;
   q.tile_rows = wide ? kWideRows : R;
   q.extra = wide ? kWideExtra : kExtra;
-  q.tiles = (q.rows + q.tile_rows - 1) / q.tile_rows;
+  q.tiles = wide ? (q.rows + kWideRows - 1) / kWideRows : (q.rows + R - 1) / R;
   q.keys = (int)keys;
   q.first = len - (e - a);
-  q.by_g = div_by(A.g);
+  q.by_g = A.by_g_long;
   q.y = 0;
   q.blocks = keys ? (int)((keys + KB - 1) / KB) : 1;  // a row without keys is written too
   if (wide && q.first >= 0 && keys == len) {
@@ -111,10 +124,10 @@ struct Unit {
 };
 __host__ __device__ __forceinline__ Unit unit_of(const Request& q, long local) {
   Unit u;
-  u.head = (int)(local / q.per_head);
+  u.head = (int)div_by(q.per_head)(local);  // (a division of 64-bit integers is 150 instructions)
   local -= (long)u.head * q.per_head;
   if (q.blocks) {
-    u.tile = (int)(local / (q.blocks + q.extra));
+    u.tile = (int)div_by(q.blocks + q.extra)(local);
   } else {
     int lo = 0, hi = q.tiles;  // the last tile that begins at or before it
     while (hi - lo > 1) {
@@ -128,8 +141,8 @@ __host__ __device__ __forceinline__ Unit unit_of(const Request& q, long local) {
 }
 
 // keys that the packed row may attend to: those up to its token's own, of the request's
-__host__ __device__ __forceinline__ int row_limit(const Request& q, int row, int g) {
-  const long last = q.first + row / g + 1;
+__host__ __device__ __forceinline__ int row_limit(const Batch& A, const Request& q, int row) {
+  const long last = q.first + A.by_g(row) + 1;
   return last < 0 ? 0 : last < q.keys ? (int)last : q.keys;
 }
 
@@ -155,7 +168,8 @@ struct AttnArgs : Batch {
   long kp, ks, kh, vp, vs, vh;      // bytes: page, slot and head of the caches
   float* part;                      // the workgroups' unfinished rows, slots of `slot` floats
   long slot;
-  int G;                            // workgroups
+  int G;                            // workgroups, and the division by them
+  Div by_G;
 };
 
 constexpr int kSplitBytes = 32;  // of the workspace, per range: the tile that goes on behind it
