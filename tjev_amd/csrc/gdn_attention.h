@@ -1258,6 +1258,32 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   auto part = [&](int p) { return p ? next + (size_t)(p - 1) * 2 * A.slot : first; };
   const int tid = threadIdx.x, row = tid % ROWS, grp = tid / ROWS;
   const int live = min(ROWS, (q.rows - tile * ROWS + 31) / 32 * 32);  // rows that the parts hold
+  const int x0 = SLICED ? blockIdx.y * kSlice + tid % kSlice : tid;  // the thread's first result of four, others NT apart
+  f32x4 acc[NE];
+  int er[NE];  // their rows
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int x = x0 + i * NT;
+    er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr int U = NE >= 8 ? 1 : 8 / NE;
+  const int pg = SLICED ? tid / kSlice : 0;
+  f32x4 v[U][NE];
+  float pm[U][NE];
+  auto fetch = [&](int p0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* s = part(min(p0 + u, parts - 1));
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        if (WIDE && er[i] >= live) continue;
+        v[u][i] = reinterpret_cast<const f32x4*>(s)[x0 + i * NT];
+        pm[u][i] = s[ROWS * DT + er[i]];
+      }
+    }
+  };
+  fetch(pg * U);  // on their way while the maxima are read
   {
     float m = kNegInf, l = 0.f;
 #pragma unroll 4
@@ -1280,31 +1306,11 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
     sl[0][row] = l > 0.f || l != l ? 1.0f / l : 0.f;
   }
   __syncthreads();
-  f32x4 acc[NE];
-  int er[NE];
   float eb[NE];
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int x = SLICED ? blockIdx.y * kSlice + tid % kSlice : tid + i * NT;
-    er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
-    eb[i] = sm[0][er[i]];
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  constexpr int U = NE >= 8 ? 1 : 8 / NE;
-  const int pg = SLICED ? tid / kSlice : 0;
+  for (int i = 0; i < NE; ++i) eb[i] = sm[0][er[i]];
   for (int p0 = pg * U; p0 < parts; p0 += PG * U) {
-    f32x4 v[U][NE];
-    float pm[U][NE];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float* s = part(min(p0 + u, parts - 1));
-#pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        if (WIDE && er[i] >= live) continue;
-        v[u][i] = reinterpret_cast<const f32x4*>(s)[SLICED ? blockIdx.y * kSlice + tid % kSlice : tid + i * NT];
-        pm[u][i] = s[ROWS * DT + er[i]];
-      }
-    }
+    if (p0 != pg * U) fetch(p0);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -1322,7 +1328,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   }
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int x = SLICED ? blockIdx.y * kSlice + tid : tid + i * NT, r = tile * ROWS + er[i], t = A.by_g(r), ln = x % 64, v = x / 64 % (DT / 8);
+    const int x = x0 + i * NT, r = tile * ROWS + er[i], t = A.by_g(r), ln = x % 64, v = x / 64 % (DT / 8);
     const int d = WIDE ? 32 * (v / 4) + 8 * (v % 4) + 4 * (ln / 32) : x % (DT / 4) * 4;
     if (r >= q.rows || d >= A.D) continue;
     const long token = q.s0 + t;
@@ -1349,12 +1355,21 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
   __shared__ float sm[NT / R][kWideRows], sl[NT / R][kWideRows];
   GDN_POISON_LDS(sm, sl);
   int range = blockIdx.x;
-  if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note
+  Split q;
+  if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note, all read at once
     __shared__ int scount[NT / 64], sfound;
-    GDN_POISON_LDS(scount, sfound);
-    const int run = (A.G + NT - 1) / NT, r0 = threadIdx.x * run;
+    __shared__ Split snote;
+    GDN_POISON_LDS(scount, sfound, snote);
+    constexpr int RUN = kMostRanges / NT;
+    Split note[RUN];
     int n = 0;
-    for (int r = r0; r < min(A.G, r0 + run); ++r) n += split_of(A, r)->parts > 1;
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      note[i].parts = 0;
+      if (i * NT + (int)threadIdx.x < A.G) note[i] = *split_of(A, i * NT + threadIdx.x);
+    }
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) n += note[i].parts > 1;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -1366,14 +1381,20 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
     __syncthreads();
     for (int w = 0; w < wave(); ++w) upto += scount[w];
     int k = upto - n;
-    for (int r = r0; r < min(A.G, r0 + run); ++r)
-      if (split_of(A, r)->parts > 1 && k++ == (int)blockIdx.x) sfound = r;
+#pragma unroll
+    for (int i = 0; i < RUN; ++i)
+      if (note[i].parts > 1 && k++ == (int)blockIdx.x) {
+        sfound = i * NT + threadIdx.x;
+        snote = note[i];
+      }
     __syncthreads();
     range = uniform(sfound);
     if (range < 0) return;
+    q = snote;
+  } else {
+    q = *split_of(A, range);
+    if (q.parts < 2) return;
   }
-  const Split q = *split_of(A, range);
-  if (q.parts < 2) return;
   const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (range + 1)) * A.slot;
   if constexpr (MIXED) {
     if (q.tile_rows == kWideRows) {

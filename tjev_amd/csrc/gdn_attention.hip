@@ -12,7 +12,7 @@ namespace {
 // Workgroups of the attention kernel, all on the chip at once: two to a CU by their registers, three at head dims up to
 // 64 in bf16 (2048 new tokens over 30000, 16/4 heads of 64: 412 us with two, 362 with three; at 128, where the streaming
 // kernel alone would fit three times: 64 decoding requests 158 with two, 166 with three).
-int ranges_of(const tjev_gdn_paged_params* p) { return p->dtype == TJEV_GDN_BF16 && p->dim <= 64 ? 768 : 512; }
+int ranges_of(const tjev_gdn_paged_params* p) { return p->dtype == TJEV_GDN_BF16 && p->dim <= 64 ? kMostRanges : 512; }
 
 // What the host knows: the rows and requests of the call, not how they are shared out.
 AttnPlan plan_of(const tjev_gdn_paged_params* p) {

@@ -172,6 +172,7 @@ struct AttnArgs : Batch {
   Div by_G;
 };
 
+constexpr int kMostRanges = 768;
 constexpr int kSplitBytes = 32;  // of the workspace, per range: the tile that goes on behind it
 
 struct AttnPlan {
