@@ -437,16 +437,27 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
   const AttnArgs& A = arguments();
   const int w = __builtin_amdgcn_readfirstlane(wave()), ln = lane(), r16 = ln & 15, g4 = ln >> 4;
   const int row0 = part.tile * R, h = part.head;
-  // the queries, staged once for the four waves in the order of the fragments
-  for (int x = w; x < NQ * S::KS; x += 4) {
-    const int n = x / S::KS, i = x - n * S::KS, row = row0 + n * 16 + r16, e = (4 * i + g4) * E;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < q.rows && !(PAD && e >= A.D)) {
+  // The queries, staged once for the four waves in the order of the fragments: read first, stored (and waited for) when the
+  // first keys and values are on their way
+  constexpr int QN = (NQ * S::KS + 3) / 4;
+  uint4 qv[QN];
+#pragma unroll
+  for (int y = 0; y < QN; ++y) {
+    const int x = w + 4 * y, n = x / S::KS, i = x - n * S::KS, row = row0 + n * 16 + r16, e = (4 * i + g4) * E;
+    qv[y] = make_uint4(0, 0, 0, 0);
+    if (x < NQ * S::KS && row < q.rows && !(PAD && e >= A.D)) {
       const int t = A.by_g(row);
-      v = *reinterpret_cast<const uint4*>(A.q + (long)(q.s0 + t) * A.qt + (h * A.g + (row - t * A.g)) * A.qh + e * (int)sizeof(T));
+      qv[y] = *reinterpret_cast<const uint4*>(A.q + (long)(q.s0 + t) * A.qt + (h * A.g + (row - t * A.g)) * A.qh + e * (int)sizeof(T));
     }
-    sq[x * 64 + ln] = v;
   }
+  bool staged = false;
+  auto stage = [&]() {
+#pragma unroll
+    for (int y = 0; y < QN; ++y)
+      if (w + 4 * y < NQ * S::KS) sq[(w + 4 * y) * 64 + ln] = qv[y];
+    __syncthreads();
+    staged = true;
+  };
   int lim[NQ];  // the lane's row of each row tile: its last key + 1
   float m[NQ], l[NQ];
   f32x4 o[NQ][S::VH][S::VE];
@@ -464,7 +475,6 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
   const int lo_lim = uniform(row_limit(A, q, row0)), hi_lim = uniform(row_limit(A, q, min(row0 + R, q.rows) - 1));
   const int32_t* table = A.table + (long)b * A.M;
   const char *kc = A.k + h * A.kh, *vc = A.v + h * A.vh;
-  __syncthreads();
 
   for (int kb = kb0; kb < kb0 + seg; ++kb) {
     const int k0 = kb * KB + w * 16 * KG;
@@ -518,6 +528,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
         }
     }
     const bool bad_page = WHOLE ? !all_ok : __any(!all_ok);
+    if (!staged) stage();
 
     f32x4 s[KG][NQ];
 #pragma unroll
@@ -594,6 +605,8 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
     }
     add_pv<T, DT, NQ>(vf, s, o);
   }
+
+  if (!staged) stage();  // a wave without keys
 
   // the four waves' rows joined
 #pragma unroll
