@@ -353,43 +353,38 @@ __device__ __forceinline__ void add_special(VStep<T, DT>& v,
         }
 }
 
-// a row's 4 x VE consecutive results, divided by its sum, gated, rounded once and stored
+// VE consecutive results of a row in every 16 VE of them, divided by the row's sum, gated, rounded once and stored
 template <class T, int DT, bool PAD>
-__device__ __forceinline__ void store_row(const AttnArgs& A, const f32x4 (&o)[Shape<T, DT>::VH][Shape<T, DT>::VE], float l, long token,
-                                          int head) {
+__device__ __forceinline__ void store_row(const AttnArgs& A, const float (&o)[Shape<T, DT>::VH][Shape<T, DT>::VE], float l, long token,
+                                          int head, int d0) {
   using S = Shape<T, DT>;
   using G = std::conditional_t<S::VE == 8, Raw8<T>, Raw4<T>>;
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-  const int d0 = 4 * (lane() / 16) * S::VE;
   const T* gp = reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + d0;
   T* op = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + d0;
-  G gate[S::VH][4];  // all loaded before the first is used
+  G gate[S::VH];  // all loaded before the first is used
   if (A.gate)
 #pragma unroll
-    for (int h = 0; h < S::VH; ++h)
+    for (int x = 0; x < S::VH; ++x)
+      if (!PAD || d0 + x * 16 * S::VE < A.D) gate[x].load(gp + x * 16 * S::VE);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (!PAD || d0 + (h * 16 + r) * S::VE < A.D) gate[h][r].load(gp + (h * 16 + r) * S::VE);
+  for (int x = 0; x < S::VH; ++x) {
+    if (PAD && d0 + x * 16 * S::VE >= A.D) continue;
+    float y[S::VE];
 #pragma unroll
-  for (int h = 0; h < S::VH; ++h)
+    for (int e = 0; e < S::VE; ++e) y[e] = o[x][e] * inv;
+    if (A.gate) {
+      float gv[S::VE];
+      gate[x].get(gv);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (PAD && d0 + (h * 16 + r) * S::VE >= A.D) continue;
-      float x[S::VE];
-#pragma unroll
-      for (int e = 0; e < S::VE; ++e) x[e] = o[h][e][r] * inv;
-      if (A.gate) {
-        float gv[S::VE];
-        gate[h][r].get(gv);
-#pragma unroll
-        for (int e = 0; e < S::VE; ++e) x[e] *= sigmoid_io<T>(gv[e]);
-      }
-      if constexpr (S::VE == 8) {
-        st8_io(op + (h * 16 + r) * S::VE, x);
-      } else {
-        st4_io(op + (h * 16 + r) * S::VE, x);
-      }
+      for (int e = 0; e < S::VE; ++e) y[e] *= sigmoid_io<T>(gv[e]);
     }
+    if constexpr (S::VE == 8) {
+      st8_io(op + x * 16 * S::VE, y);
+    } else {
+      st4_io(op + x * 16 * S::VE, y);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- the workgroups' ranges
@@ -424,7 +419,7 @@ __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block
 template <class T, int DT, int NQ>
 struct StreamLds {
   static constexpr int NV = NQ * Shape<T, DT>::VH * Shape<T, DT>::VE;  // result registers of four
-  static constexpr int HALF = NV >= 32 ? NV / 2 : NV;                  // joined at a time
+  static constexpr int HALF = NV >= 32 ? NV / 2 : NV;                  // exchanged at a time
   static constexpr int Q = NQ * Shape<T, DT>::KS * 64, ACC = 2 * HALF * 64;  // pieces of 16 bytes
 };
 
@@ -608,76 +603,95 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 
   if (!staged) stage();  // a wave without keys
 
-  // the four waves' rows joined
+  // The four waves' rows joined: of a lane's four results of each register, wave w ends with the w-th. Waves two
+  // apart exchange halves (unscaled: their maxima are on their way too), then neighbours quarters, in the place
+  // that only they have read; all four waves then store. (The halves added by waves 0 and 1, and by wave 0 alone:
+  // five barriers instead of two, and one wave's stores.)
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     l[n] = rows_sum(l[n]);
     if (g4 == 0) sm[w][n * 16 + r16] = m[n], sl[w][n * 16 + r16] = l[n];
   }
-  __syncthreads();
-  float mj[NQ], lj[NQ];
+  const bool upper = w >> 1, odd = w & 1;
+  float mj[NQ], lj[NQ], own[NQ], other[NQ], res[NQ][S::VH][S::VE];
+  f32x4* const mine = sacc + w * (HALF / 2) * 64 + ln;
+  f32x4* const across = sacc + (w ^ 2) * (HALF / 2) * 64 + ln;
+  const f32x4* const beside = sacc + (w ^ 3) * (HALF / 2) * 64 + ln;
+  auto reg = [&](int v) -> f32x4& { return o[v / (S::VH * S::VE)][v / S::VE % S::VH][v % S::VE]; };
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    mj[n] = kNegInf;
+  for (int from = 0; from < NV; from += HALF) {
+    if (from) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mj[n] = fmaxf(mj[n], sm[i][n * 16 + r16]);
-    const float base = base_of(mj[n]);
-    lj[n] = 0.f;
+    for (int v = 0; v < HALF; v += 2) {
+      const f32x4 &x = reg(from + v), &y = reg(from + v + 1);
+      mine[v / 2 * 64] = upper ? f32x4{x[0], x[1], y[0], y[1]} : f32x4{x[2], x[3], y[2], y[3]};
+    }
+    __syncthreads();
+    if (!from)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lj[n] += sl[i][n * 16 + r16] * __builtin_amdgcn_exp2f(sm[i][n * 16 + r16] - base);
-    const float a = __builtin_amdgcn_exp2f(m[n] - base);
+      for (int n = 0; n < NQ; ++n) {
+        mj[n] = kNegInf;
 #pragma unroll
-    for (int x = 0; x < S::VH; ++x)
+        for (int i = 0; i < 4; ++i) mj[n] = fmaxf(mj[n], sm[i][n * 16 + r16]);
+        const float base = base_of(mj[n]);
+        lj[n] = 0.f;
 #pragma unroll
-      for (int e = 0; e < S::VE; ++e) o[n][x][e] *= a;
+        for (int i = 0; i < 4; ++i) lj[n] += sl[i][n * 16 + r16] * __builtin_amdgcn_exp2f(sm[i][n * 16 + r16] - base);
+        own[n] = __builtin_amdgcn_exp2f(m[n] - base);
+        other[n] = __builtin_amdgcn_exp2f(sm[w ^ 2][n * 16 + r16] - base);
+      }
+    float keep[HALF], send[HALF];
+#pragma unroll
+    for (int v = 0; v < HALF; v += 2) {
+      const f32x4 t = across[v / 2 * 64];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = (from + v + j / 2) / (S::VH * S::VE);
+        const f32x4& x = reg(from + v + j / 2);
+        const float y = (upper ? x[2 + j % 2] : x[j % 2]) * own[n] + t[j] * other[n];
+        if (j % 2 == 0) {
+          keep[v + j / 2] = y;
+        } else {
+          const float z = keep[v + j / 2];
+          keep[v + j / 2] = odd ? y : z;
+          send[v + j / 2] = odd ? z : y;
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < HALF; v += 4)
+      across[v / 4 * 64] = f32x4{send[v], send[v + 1], send[v + 2], send[v + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < HALF; v += 4) {
+      const f32x4 t = beside[v / 4 * 64];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = from + v + j;
+        res[at / (S::VH * S::VE)][at / S::VE % S::VH][at % S::VE] = keep[v + j] + t[j];
+      }
+    }
   }
-  auto each_reg = [&](int from, auto f) {  // registers from .. from + HALF - 1
+  const int d0 = (4 * g4 + w) * S::VE;
+  if (!part.p) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n) {
+      const int row = row0 + n * 16 + r16, t = A.by_g(row);
+      if (row < q.rows) store_row<T, DT, PAD>(A, res[n], lj[n], q.s0 + t, h * A.g + (row - t * A.g), d0);
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
 #pragma unroll
       for (int x = 0; x < S::VH; ++x)
 #pragma unroll
-        for (int e = 0; e < S::VE; ++e) {
-          const int v = (n * S::VH + x) * S::VE + e;
-          if (v >= from && v < from + HALF) f((v - from) * 64 + ln, o[n][x][e]);
-        }
-  };
-#pragma unroll
-  for (int from = 0; from < NV; from += HALF) {
-    if (w >= 2) each_reg(from, [&](int i, f32x4& x) { sacc[(w - 2) * HALF * 64 + i] = x; });
-    __syncthreads();
-    if (w < 2) each_reg(from, [&](int i, f32x4& x) { x += sacc[w * HALF * 64 + i]; });
-    __syncthreads();
-    if (w == 1) each_reg(from, [&](int i, f32x4& x) { sacc[i] = x; });
-    __syncthreads();
-    if (w == 0) each_reg(from, [&](int i, f32x4& x) { x += sacc[i]; });
-    __syncthreads();
-  }
-  if (w == 0) {
-    if (!part.p) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        const int row = row0 + n * 16 + r16, t = A.by_g(row);
-        if (row < q.rows) store_row<T, DT, PAD>(A, o[n], lj[n], q.s0 + t, h * A.g + (row - t * A.g));
+        for (int e = 0; e < S::VE; e += 4)  // rows of DT values
+          *reinterpret_cast<f32x4*>(part.p + (n * 16 + r16) * DT + d0 + x * 16 * S::VE + e) =
+              f32x4{res[n][x][e], res[n][x][e + 1], res[n][x][e + 2], res[n][x][e + 3]};
+      if (w == 0 && g4 == 0) {
+        part.p[R * DT + n * 16 + r16] = mj[n];
+        part.p[R * (DT + 1) + n * 16 + r16] = lj[n];
       }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int x = 0; x < S::VH; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {  // rows of DT values
-            float* po = part.p + (n * 16 + r16) * DT + (x * 16 + 4 * g4 + r) * S::VE;
-#pragma unroll
-            for (int e = 0; e < S::VE; e += 4)
-              *reinterpret_cast<f32x4*>(po + e) = f32x4{o[n][x][e][r], o[n][x][e + 1][r], o[n][x][e + 2][r], o[n][x][e + 3][r]};
-          }
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-        if (g4 == 0) {
-          part.p[R * DT + n * 16 + r16] = mj[n];
-          part.p[R * (DT + 1) + n * 16 + r16] = lj[n];
-        }
     }
   }
 }
