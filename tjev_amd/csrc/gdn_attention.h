@@ -193,15 +193,23 @@ __device__ __forceinline__ f32x4 dot_step(const uint4& k, const uint4& q, f32x4 
   }
 }
 
+// f of the lane's value and that of the lane 32 (or 16) away: exchanged within the registers (through LDS a shuffle waits
+// behind the fragments' reads)
+template <class F>
+__device__ __forceinline__ float with_far(float v, F f) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+template <class F>
+__device__ __forceinline__ float with_near(float v, F f) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 // max or sum over the four lanes that hold one row (lane % 16)
-__device__ __forceinline__ float rows_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float rows_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
+__device__ __forceinline__ float rows_max(float v) { return with_far(with_near(v, larger), larger); }
+__device__ __forceinline__ float rows_sum(float v) { return with_far(with_near(v, sum_of), sum_of); }
 // the base of the powers: 0 where a row has seen no key yet, so that its powers are 0 and not NaN
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
 
@@ -978,7 +986,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int x = 0; x < 16; ++x) t = fmaxf(t, s[n][x]);
-    t = fmaxf(t, __shfl_xor(t, 32)) * c;
+    t = with_far(t, larger) * c;
     if (__any(t > m + 8.f)) {
       const float mn = fmaxf(m, t), a = __builtin_amdgcn_exp2f(m - base_of(mn));
       m = mn;
@@ -1078,7 +1086,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       }
     }
   }
-  l += __shfl_xor(l, 32);
+  l = with_far(l, sum_of);
   // The lane's results: row r32, values 32 d + 8 x + 4 hf .. + 3. Finished rows are turned in the wave's own buffer (its
   // pieces of four exchanged by the row), so that gate and result move as 16-byte pieces of whole rows, all gates
   // of a turn on their way at once: taken as they lie, a lane's 8-byte pieces of the gate cost a memory round trip each
