@@ -915,24 +915,10 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   bool special = false;  // infinities or NaN where some rows attend and others do not
 
   auto compute = [&](int k0, int buf, uint16_t* sk, uint16_t* sv) {
-    u32 any_bad = 0;
+    const bool live = k0 < hi_w;  // a wave without rows, or whose rows end before, only helps
+    u32 any_bad = 0;  // read by now, looked at behind the scores
 #pragma unroll
     for (int i = 0; i < 4; ++i) any_bad |= sbad[buf][i];
-    any_bad = __builtin_amdgcn_readfirstlane(any_bad);
-    const bool edge = k0 + TK > lo_g || any_bad;  // not all rows attend to all keys
-    if (edge && (k0 + TK > hi_g || any_bad)) clear_unseen(k0, buf, sv);
-    if (edge && k0 + TK > lo_g && lo_g < hi_g) {  // such values are left out here and counted at the end
-      bool nf = false;
-      for (int x = threadIdx.x; x < TK * W::CPR; x += kThreads) {
-        uint4& v = reinterpret_cast<uint4*>(sv)[x];
-        if (not_finite<T>(v)) {
-          nf = true;
-          v = make_uint4(finite_of(v.x), finite_of(v.y), finite_of(v.z), finite_of(v.w));
-        }
-      }
-      special = __syncthreads_or(nf) || special;
-    }
-    if (k0 >= hi_w) return;  // a wave without rows too
     // at head dim 256 taken anew for each buffer: what is held across the loop must fit the registers
     const int la = lane_anew(), kl = DT == 256 ? k_lane(la) : k_held, vl = DT == 256 ? v_lane(la) : v_held;
     f32x16 s[NS];
@@ -950,18 +936,35 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         kf[i % AHEAD][n] = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(sk) + (kl ^ ((i * 32) & (W::SPAN - 1))) +
                                                             i * 32 / W::SPAN * W::SPAN + n * 32 * DT * 2);
     };
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < AHEAD - 1; ++i) read_k(i);
-    __builtin_amdgcn_s_setprio(1);
+      for (int i = 0; i < AHEAD - 1; ++i) read_k(i);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int i = 0; i < KQ; ++i) {
-      if (i + AHEAD - 1 < KQ) read_k(i + AHEAD - 1);
-      const bf16x8 qi = i < KQ - QL ? qf[i < KQ - QL ? i : 0] : __builtin_bit_cast(bf16x8, sq[(w * QL + i - (KQ - QL)) * 64 + la]);
+      for (int i = 0; i < KQ; ++i) {
+        if (i + AHEAD - 1 < KQ) read_k(i + AHEAD - 1);
+        const bf16x8 qi = i < KQ - QL ? qf[i < KQ - QL ? i : 0] : __builtin_bit_cast(bf16x8, sq[(w * QL + i - (KQ - QL)) * 64 + la]);
 #pragma unroll
-      for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD][n], qi, s[n], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < NS; ++n) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % AHEAD][n], qi, s[n], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_s_setprio(0);
+    any_bad = __builtin_amdgcn_readfirstlane(any_bad);
+    const bool edge = k0 + TK > lo_g || any_bad;  // not all rows attend to all keys
+    if (edge && (k0 + TK > hi_g || any_bad)) clear_unseen(k0, buf, sv);
+    if (edge && k0 + TK > lo_g && lo_g < hi_g) {  // such values are left out here and counted at the end
+      bool nf = false;
+      for (int x = threadIdx.x; x < TK * W::CPR; x += kThreads) {
+        uint4& v = reinterpret_cast<uint4*>(sv)[x];
+        if (not_finite<T>(v)) {
+          nf = true;
+          v = make_uint4(finite_of(v.x), finite_of(v.y), finite_of(v.z), finite_of(v.w));
+        }
+      }
+      special = __syncthreads_or(nf) || special;
+    }
+    if (!live) return;
     if (edge && k0 + TK > lo_w) {
       const int left = lim - k0 - 4 * (lane_anew() / 32);
 #pragma unroll
