@@ -984,6 +984,15 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
           for (int i = 0; i < 4; ++i) s[n][4 * x + i] = (word >> i) & 1 ? kNegInf : s[n][4 * x + i];
         }
     }
+    bf16x8 vf[2][NS][2];
+    auto read_v = [&](int d) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vf[d % 2][n][j] = v_frag(sv, vl, d, n, j);
+    };
+    read_v(0);  // on their way while the weights are computed
+    __builtin_amdgcn_sched_barrier(0);
     float t = kNegInf;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
@@ -1015,14 +1024,6 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         }
         p[n][j] = __builtin_bit_cast(bf16x8, make_uint4(pk[0], pk[1], pk[2], pk[3]));
       }
-    bf16x8 vf[2][NS][2];
-    auto read_v = [&](int d) {
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) vf[d % 2][n][j] = v_frag(sv, vl, d, n, j);
-    };
-    read_v(0);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
