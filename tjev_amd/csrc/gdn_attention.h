@@ -984,14 +984,12 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
           for (int i = 0; i < 4; ++i) s[n][4 * x + i] = (word >> i) & 1 ? kNegInf : s[n][4 * x + i];
         }
     }
-    bf16x8 vf[2][NS][2];
-    auto read_v = [&](int d) {
+    // V's fragments in the order of the products: all of a run of 16 keys, then the next run's
+    constexpr int F = 2 * NS, VA = 4;
+    bf16x8 vf[VA];
+    auto read_v = [&](int x) { vf[x % VA] = v_frag(sv, vl, x % ND, x / ND / 2, x / ND % 2); };
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) vf[d % 2][n][j] = v_frag(sv, vl, d, n, j);
-    };
-    read_v(0);  // on their way while the weights are computed
+    for (int x = 0; x < VA - 1; ++x) read_v(x);  // on their way while the weights are computed
     __builtin_amdgcn_sched_barrier(0);
     float t = kNegInf;
 #pragma unroll
@@ -1009,30 +1007,30 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
         for (int x = 0; x < 16; ++x) o[d][x] *= a;
     }
     const float base = base_of(m);
-    bf16x8 p[NS][2];
+    // the weights of a run of 16 keys are computed behind the products of the run before it, a pair at a time
+    u32 pk[2][4];
+    auto weights = [&](int f, int x) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[f / 2][8 * (f % 2) + 2 * x], c, -base));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[f / 2][8 * (f % 2) + 2 * x + 1], c, -base));
+      pk[f % 2][x] = pack2(p0, p1);
+      l = sum_pair(pk[f % 2][x], l);
+    };
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        u32 pk[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x], c, -base));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][8 * j + 2 * x + 1], c, -base));
-          pk[x] = pack2(p0, p1);
-          l = sum_pair(pk[x], l);
-        }
-        p[n][j] = __builtin_bit_cast(bf16x8, make_uint4(pk[0], pk[1], pk[2], pk[3]));
-      }
+    for (int x = 0; x < 4; ++x) weights(0, x);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      if (d + 1 < ND) read_v(d + 1);
+    for (int f = 0; f < F; ++f) {
+      const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pk[f % 2][0], pk[f % 2][1], pk[f % 2][2], pk[f % 2][3]));
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
+      for (int d = 0; d < ND; ++d) {
+        const int at = f * ND + d;
+        if (at + VA - 1 < F * ND) read_v(at + VA - 1);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[at % VA], pf, o[d], 0, 0, 0);
+        if (f + 1 < F)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d % 2][n][j], p[n][j], o[d], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int x = (4 * d + ND - 1) / ND; x < (4 * d + 4 + ND - 1) / ND; ++x) weights(f + 1, x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
   };
