@@ -927,8 +927,10 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
 #pragma unroll
       for (int x = 0; x < 16; ++x) s[n][x] = 0.f;
     // Fragments are read AHEAD products before their own: left to itself the compiler reads them all first, which
-    // runs it out of registers
-    constexpr int AHEAD = 2;
+    // Fragments are read AHEAD - 1 products before their own: left to itself the compiler reads them all first, which
+    // runs it out of registers. At head dim 256 a fragment has one product, not two, to hide the next one's read
+    // (2048 new tokens over 30000, 16/4 heads: 1192 us with 2, 1165 with 4, 1333 with 6, which spills).
+    constexpr int AHEAD = DT == 256 ? 4 : 2;
     bf16x8 kf[AHEAD][NS];
     auto read_k = [&](int i) {
 #pragma unroll
