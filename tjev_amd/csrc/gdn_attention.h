@@ -1297,28 +1297,35 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   auto part = [&](int p) { return p ? next + (size_t)(p - 1) * 2 * A.slot : first; };
   const int tid = threadIdx.x, row = tid % ROWS, grp = tid / ROWS;
   const int live = min(ROWS, (q.rows - tile * ROWS + 31) / 32 * 32);  // rows that the parts hold
-  const int x0 = SLICED ? blockIdx.y * kSlice + tid % kSlice : tid;  // the thread's first result of four, others NT apart
+  // The thread's results of four, as they lie in a part (place i). Those of a wide tile, whole: NE pieces of one row, the
+  // other half of each in the lane 32 on.
+  constexpr bool ROW = WIDE && !SLICED;
+  constexpr int NR = ROW ? 1 : NE;
+  static_assert(!ROW || (DT / 8 % NE == 0 && NE % 2 == 0), "a wave's pieces are of 32 rows");
+  const int x0 = SLICED ? blockIdx.y * kSlice + tid % kSlice : ROW ? wave() * NE * 64 + lane() : tid;
+  constexpr int STEP = ROW ? 64 : NT;
   f32x4 acc[NE];
-  int er[NE];  // their rows
+  int er[NR];  // their rows
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int x = x0 + i * NT;
+  for (int i = 0; i < NE; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int x = x0 + i * STEP;
     er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   constexpr int U = NE >= 8 ? 1 : 8 / NE;
   const int pg = SLICED ? tid / kSlice : 0;
   f32x4 v[U][NE];
-  float pm[U][NE];
+  float pm[U][NR];
   auto fetch = [&](int p0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float* s = part(min(p0 + u, parts - 1));
 #pragma unroll
       for (int i = 0; i < NE; ++i) {
-        if (WIDE && er[i] >= live) continue;
-        v[u][i] = reinterpret_cast<const f32x4*>(s)[x0 + i * NT];
-        pm[u][i] = s[ROWS * DT + er[i]];
+        if (WIDE && er[i % NR] >= live) continue;
+        v[u][i] = reinterpret_cast<const f32x4*>(s)[x0 + i * STEP];
+        if (i < NR) pm[u][i] = s[ROWS * DT + er[i]];
       }
     }
   };
@@ -1345,16 +1352,20 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
     sl[0][row] = l > 0.f || l != l ? 1.0f / l : 0.f;
   }
   __syncthreads();
-  float eb[NE];
+  float eb[NR];
 #pragma unroll
-  for (int i = 0; i < NE; ++i) eb[i] = sm[0][er[i]];
+  for (int i = 0; i < NR; ++i) eb[i] = sm[0][er[i]];
   for (int p0 = pg * U; p0 < parts; p0 += PG * U) {
     if (p0 != pg * U) fetch(p0);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      float a[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) a[i] = __builtin_amdgcn_exp2f(pm[u][i] - eb[i]);
 #pragma unroll
       for (int i = 0; i < NE; ++i)
-        if (p0 + u < parts && !(WIDE && er[i] >= live)) acc[i] += v[u][i] * __builtin_amdgcn_exp2f(pm[u][i] - eb[i]);
+        if (p0 + u < parts && !(WIDE && er[i % NR] >= live)) acc[i] += v[u][i] * a[i % NR];
+    }
   }
   if constexpr (SLICED) {
     __shared__ __align__(16) f32x4 sacc[(PG - 1) * kSlice];
@@ -1365,14 +1376,51 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
 #pragma unroll
     for (int i = 0; i < PG - 1; ++i) acc[0] += sacc[i * kSlice + tid];
   }
+  if constexpr (ROW) {
+    // halves exchanged: a lane has 8 values side by side of every second piece, which move as 16 bytes (8 at a time,
+    // the 2048 rows above took 63 us to join)
+    const int r = tile * ROWS + er[0], t = A.by_g(r);
+    const float inv = sl[0][er[0]];
+    const long token = q.s0 + t;
+    const int head = h * A.g + (r - t * A.g), v0 = wave() * NE % (DT / 8) + lane() / 32;
+    if (er[0] >= live) return;  // (both lanes of a row)
+    const T* gp = reinterpret_cast<const T*>(A.gate + token * A.gt + head * A.gh) + 8 * v0;
+    T* op = reinterpret_cast<T*>(A.out + token * A.ot + head * A.oh) + 8 * v0;
+    Raw8<T> gate[NE / 2];
+    const bool here = r < q.rows;
+#pragma unroll
+    for (int i = 0; i < NE; i += 2)
+      if (A.gate && here && 8 * (v0 + i) < A.D) gate[i / 2].load(gp + 8 * i);
+#pragma unroll
+    for (int i = 0; i < NE; i += 2) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float lo = acc[i][j], hi = acc[i + 1][j];
+        const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+        y[j] = __uint_as_float(z[0]) * inv;
+        y[4 + j] = __uint_as_float(z[1]) * inv;
+      }
+      if (here && 8 * (v0 + i) < A.D) {
+        if (A.gate) {
+          float gf[8];
+          gate[i / 2].get(gf);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] *= sigmoid_io<T>(gf[j]);
+        }
+        st8_io(op + 8 * i, y);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int x = x0 + i * NT, r = tile * ROWS + er[i], t = A.by_g(r), ln = x % 64, v = x / 64 % (DT / 8);
+    const int x = x0 + i * STEP, r = tile * ROWS + er[i % NR], t = A.by_g(r), ln = x % 64, v = x / 64 % (DT / 8);
     const int d = WIDE ? 32 * (v / 4) + 8 * (v % 4) + 4 * (ln / 32) : x % (DT / 4) * 4;
     if (r >= q.rows || d >= A.D) continue;
     const long token = q.s0 + t;
     const int head = h * A.g + (r - t * A.g);
-    const float inv = sl[0][er[i]];
+    const float inv = sl[0][er[i % NR]];
     float y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = acc[i][j] * inv;
@@ -1397,18 +1445,21 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
   Split q;
   if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note, all read at once
     __shared__ int scount[NT / 64], sfound;
-    __shared__ Split snote;
+    __shared__ __align__(16) uint4 snote[2];
     GDN_POISON_LDS(scount, sfound, snote);
     constexpr int RUN = kMostRanges / NT;
-    Split note[RUN];
+    uint4 note[RUN][2];
     int n = 0;
 #pragma unroll
     for (int i = 0; i < RUN; ++i) {
-      note[i].parts = 0;
-      if (i * NT + (int)threadIdx.x < A.G) note[i] = *split_of(A, i * NT + threadIdx.x);
+      const int r = i * NT + threadIdx.x;
+      const uint4* from = reinterpret_cast<const uint4*>(split_of(A, r < A.G ? r : 0));
+      note[i][0] = from[0];
+      note[i][1] = from[1];
+      if (r >= A.G) note[i][0].x = 0;
     }
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) n += note[i].parts > 1;
+    for (int i = 0; i < RUN; ++i) n += (int)note[i][0].x > 1;  // Split::parts
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -1422,14 +1473,15 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
     int k = upto - n;
 #pragma unroll
     for (int i = 0; i < RUN; ++i)
-      if (note[i].parts > 1 && k++ == (int)blockIdx.x) {
+      if ((int)note[i][0].x > 1 && k++ == (int)blockIdx.x) {
         sfound = i * NT + threadIdx.x;
-        snote = note[i];
+        snote[0] = note[i][0];
+        snote[1] = note[i][1];
       }
     __syncthreads();
     range = uniform(sfound);
     if (range < 0) return;
-    q = snote;
+    q = *reinterpret_cast<const Split*>(snote);
   } else {
     q = *split_of(A, range);
     if (q.parts < 2) return;
