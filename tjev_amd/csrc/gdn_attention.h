@@ -714,6 +714,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 // of the results is skipped otherwise (a softmax does not depend on its base; weights up to 2^8 have bf16's
 // relative precision like all others).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 
@@ -1445,21 +1446,21 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
   Split q;
   if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note, all read at once
     __shared__ int scount[NT / 64], sfound;
-    __shared__ __align__(16) uint4 snote[2];
+    __shared__ __align__(16) i32x4 snote[2];
     GDN_POISON_LDS(scount, sfound, snote);
     constexpr int RUN = kMostRanges / NT;
-    uint4 note[RUN][2];
+    i32x4 note[RUN][2];
     int n = 0;
 #pragma unroll
     for (int i = 0; i < RUN; ++i) {
       const int r = i * NT + threadIdx.x;
-      const uint4* from = reinterpret_cast<const uint4*>(split_of(A, r < A.G ? r : 0));
+      const i32x4* from = reinterpret_cast<const i32x4*>(split_of(A, r < A.G ? r : 0));
       note[i][0] = from[0];
       note[i][1] = from[1];
       if (r >= A.G) note[i][0].x = 0;
     }
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) n += (int)note[i][0].x > 1;  // Split::parts
+    for (int i = 0; i < RUN; ++i) n += note[i][0].x > 1;  // Split::parts
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -1473,7 +1474,7 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
     int k = upto - n;
 #pragma unroll
     for (int i = 0; i < RUN; ++i)
-      if ((int)note[i][0].x > 1 && k++ == (int)blockIdx.x) {
+      if (note[i][0].x > 1 && k++ == (int)blockIdx.x) {
         sfound = i * NT + threadIdx.x;
         snote[0] = note[i][0];
         snote[1] = note[i][1];
