@@ -83,6 +83,7 @@ int main() {
     gdn::set_group(A, it % 7 ? pick(1, 20) : pick(1, 300));
     A.N = pick(0, it % 5 ? 40 : 150);
     A.wide = it % 2 ? 1 << 30 : pick(0, 64);
+    A.wide_extra = pick(1, 3);
     std::vector<int32_t> table(A.B * A.M), starts(A.B + 1), lengths(A.B);
     const int kind = it % 3;  // as a scheduler writes them; with bad pages and lengths; anything
     int at = 0;

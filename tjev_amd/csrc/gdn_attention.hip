@@ -25,7 +25,7 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   const int kb = bf ? 128 : 64;
   // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
   const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + p->requests) * p->kv_heads;
-  const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb + kWideExtra;
+  const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb + kWideExtra + kGateExtra;
   const int most = ranges_of(p);
   r.G = tiles >= most || blocks * tiles >= most ? most : (int)(blocks * tiles);
   // so few tiles that a workgroup each would leave most CUs idle, and take parts by the dozen

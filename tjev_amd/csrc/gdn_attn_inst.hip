@@ -10,6 +10,7 @@ hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   A.by_G = div_by(r.G);
   A.slot = r.slot;
   A.wide = MIXED ? 16 * NQ : 0x7fffffff;
+  A.wide_extra = kWideExtra + (A.gate ? kGateExtra : 0);
   hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);
   constexpr int slices = join_slices<DT, MIXED ? kWideRows : 16 * NQ>();
   if (r.sliced) {

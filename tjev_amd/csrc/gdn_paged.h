@@ -41,7 +41,7 @@ struct Batch {
   long N;                    // rows of q
   int B, M, page, pages;     // requests, table width, page size, pages of the cache
   int Hk, g;                 // key heads, query heads to each
-  int wide;                  // requests of more packed rows take wide tiles
+  int wide, wide_extra;      // requests of more packed rows take wide tiles, which have so many units before their keys'
   Div32 by_page, by_g;       // a key's page, a packed row's token
   Div by_g_long;
   const int32_t *table, *starts, *lengths;
@@ -61,9 +61,12 @@ __host__ __device__ __forceinline__ int page_of(const Batch& A, int key) { retur
 // The packed rows of a request and key head are its new tokens' query heads of that key head: row r
 // is token r / g, head r % g. Requests of more than `wide` rows are worked on in tiles of kWideRows, the others
 // in tiles of R. A unit of work is a tile's next KB keys, in the order key head, tile, keys; before its keys a tile has
-// units for what it costs by itself (its queries, the first loads' latency, its results). Measured on a prompt of 4096
-// tokens, 32 heads of 256 and 4 key heads, whose first tiles have one block of keys: 592 us without them, see kWideExtra.
-constexpr int kWideRows = 128, kWideExtra = 2, kExtra = 1;
+// units for what it costs by itself (its queries, the first loads' latency, its results; a wide tile's gate). Measured with
+// 0, 1, 2, 3, 4 of them for a wide tile: a prompt of 4096 tokens, 32 heads of 256 and 4 key heads, whose first tiles
+// have one block of keys, without a gate -, 375, 337, 340, 341 us, with one 567, 447, 390, 354, 358; chunks of prompts
+// beside decoding requests (32/4 heads of 128, no gate) 106, 92.5, 87.3, 90.5, 94.2. For a streamed tile: 0 to 2 alike but for
+// ragged fp32 batches (22.2, 22.2, 24.4).
+constexpr int kWideRows = 128, kWideExtra = 2, kGateExtra = 1, kExtra = 1;
 
 struct Request {
   int s0, rows, tiles, tile_rows;  // first row of q; packed rows; tiles of them
@@ -97,7 +100,7 @@ __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   q.rows = (int)(s1 - s0) * A.g;
   const bool wide = q.rows > A.wide;
   q.tile_rows = wide ? kWideRows : R;
-  q.extra = wide ? kWideExtra : kExtra;
+  q.extra = wide ? A.wide_extra : kExtra;
   q.tiles = wide ? (q.rows + kWideRows - 1) / kWideRows : (q.rows + R - 1) / R;
   q.keys = (int)keys;
   q.first = len - (e - a);
