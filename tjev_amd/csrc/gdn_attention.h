@@ -2,6 +2,20 @@
 // that stand between the GDN layers), from one token per request to chunks of a prompt:
 //   o_r = sum_k p_rk v_k / sum_k p_rk,  p_rk = 2^(c q_r k_k - m_r),  c = scale log2(e),
 // one pass over the keys with the running maximum m_r and sum of each row in 32 bits.
+//
+// The query heads of a key head are rows of one tile beside its tokens, so a key is read once for all of them. Up to
+// 16 rows a request (decoding) are bound by memory, and their keys and values stream straight into registers
+// (stream_tile); more are bound by the products, and share tiles of 128 rows whose keys pass through LDS (wide_tile,
+// bf16). All tiles of a batch are cut into as many equal ranges of work as workgroups fit the chip (gdn_paged.h); a
+// tile that more than one range holds leaves its parts in the workspace for a second launch to join
+// (k_attention_join). Two launches whatever the lengths, which only the GPU knows.
+//
+// Measured, bf16, with a gate but for the first (floors: the cache and rows at 5.12 TB/s, the products at 1230 TFLOP/s, what a
+// large copy and a large library product reach on the same card):
+//   1 token over 4000, 16/4 heads of 256 (16 MB)                    16.7 us   floor   3.2   two launches' latency
+//   64 requests of up to 32768, 16/4 heads of 256 (1.57 GB)        300            307    memory, 5.2 TB/s
+//   2048 tokens over 30000, 16/4 heads of 256 (1.04 TFLOP)        1130            846    products, 921 TFLOP/s
+//   a prompt of 4096, 32/4 heads of 256 (0.27 TFLOP)               355            224    products, 774 TFLOP/s
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -422,7 +436,9 @@ __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block
 
 // ---------------------------------------------------------------- few rows: keys streamed
 // The four waves take steps of KG * 16 keys in turn, each with a running maximum, sum and result of its
-// own, joined in LDS at the end. Bound by memory: the keys and values are read once, straight into registers.
+// own, joined in LDS at the end. Bound by memory: the keys and values are read once, straight into registers (64 requests of
+// up to 32768 tokens, 16/4 heads of 256, 128, 64: 5.2, 5.1, 4.7 TB/s), or by latency: one token over 4000 takes 11 us, of
+// which its bytes are 3.
 // WHOLE: pages hold whole groups of 16 keys, whose page is then one value per wave.
 template <class T, int DT, int NQ>
 struct StreamLds {
@@ -709,7 +725,10 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 // 16-byte loads that do not touch registers; scores are again transposed (32 keys by 32 rows per MFMA), so that a
 // row's weights stay in its two lanes and are the second operand of out^T += V^T P^T as they come, V's
 // fragments by transposing LDS reads. The pieces of a row of K or V lie in LDS in an order that depends on the row
-// (swz), which spreads both kinds of read over the banks.
+// (swz), which spreads both kinds of read over the banks (no conflicts counted). Bound by the products and what
+// stands between them: 2048 tokens over 30000 at head dims 256, 128, 64 run at 921, 896, 755 TFLOP/s, the matrix
+// units busy for half of the cycles. The queries stay in registers (three fragments at 256 in LDS), the results too;
+// two workgroups to a CU cover each other's softmax and barriers.
 // The base of the powers follows the running maximum only when that has grown by more than 2^8: the rescaling
 // of the results is skipped otherwise (a softmax does not depend on its base; weights up to 2^8 have bf16's
 // relative precision like all others).
@@ -1095,7 +1114,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   // The lane's results: row r32, values 32 d + 8 x + 4 hf .. + 3. Finished rows are turned in the wave's own buffer (its
   // pieces of four exchanged by the row), so that gate and result move as 16-byte pieces of whole rows, all gates
   // of a turn on their way at once: taken as they lie, a lane's 8-byte pieces of the gate cost a memory round trip each
-  // (a 4096-token prompt, 32 heads of 256 with a gate: 722 us).
+  // (a 4096-token prompt, 32 heads of 256 with a gate: 722 us; turned, and with the ranges counting each tile, 397).
   if (!part.p) {
     __syncthreads();  // the last buffers' readers
     if (rows_w) {
@@ -1378,8 +1397,8 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
     for (int i = 0; i < PG - 1; ++i) acc[0] += sacc[i * kSlice + tid];
   }
   if constexpr (ROW) {
-    // halves exchanged: a lane has 8 values side by side of every second piece, which move as 16 bytes (8 at a time,
-    // the 2048 rows above took 63 us to join)
+    // halves exchanged: a lane has 8 values side by side of every second piece, which move as 16 bytes (2048 tokens over
+    // 30000, 135 MB of parts: 63 us with 8 bytes, 38 with 16)
     const int r = tile * ROWS + er[0], t = A.by_g(r);
     const float inv = sl[0][er[0]];
     const long token = q.s0 + t;
