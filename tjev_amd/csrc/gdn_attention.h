@@ -1333,7 +1333,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
     const int x = x0 + i * STEP;
     er[i] = WIDE ? x / (DT / 8 * 64) * 32 + x % 32 : x / (DT / 4);
   }
-  constexpr int U = NE >= 8 ? 1 : 8 / NE;
+  constexpr int U = SLICED ? 16 : NE >= 8 ? 1 : 8 / NE;
   const int pg = SLICED ? tid / kSlice : 0;
   f32x4 v[U][NE];
   float pm[U][NR];
@@ -1352,12 +1352,22 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   fetch(pg * U);  // on their way while the maxima are read
   {
     float m = kNegInf, l = 0.f;
-#pragma unroll 4
-    for (int p = grp; p < (row < live ? parts : 0); p += NG) {
-      const float* s = part(p) + ROWS * DT + row;
-      const float pm = s[0], pl = s[ROWS], mn = fmaxf(m, pm), base = base_of(mn);
-      l = l * __builtin_amdgcn_exp2f(m - base) + pl * __builtin_amdgcn_exp2f(pm - base);
-      m = mn;
+    constexpr int V = 8;  // parts at a time
+    for (int p0 = grp; p0 < (row < live ? parts : 0); p0 += V * NG) {
+      float pm[V], pl[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float* s = part(min(p0 + i * NG, parts - 1)) + ROWS * DT + row;
+        pm[i] = s[0];
+        pl[i] = s[ROWS];
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (p0 + i * NG < parts) {
+          const float mn = fmaxf(m, pm[i]), base = base_of(mn);
+          l = l * __builtin_amdgcn_exp2f(m - base) + pl[i] * __builtin_amdgcn_exp2f(pm[i] - base);
+          m = mn;
+        }
     }
     sm[grp][row] = m;
     sl[grp][row] = l;

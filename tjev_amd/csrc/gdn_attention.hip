@@ -20,7 +20,9 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   const int dt = p->dim <= 64 ? 64 : p->dim <= 128 ? 128 : 256;
   const long g = p->heads / p->kv_heads, rows = p->tokens * g, mean = (rows + p->requests - 1) / p->requests;
   AttnPlan r;
-  r.nq = bf || mean <= 16 ? 1 : dt == 256 ? 2 : 4;
+  // fp32 tiles of 32 rows where there are enough of them and registers to hold them (2 requests of 910 tokens after 858, 4/1
+  // heads of 128: 50.5 us, with 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6)
+  r.nq = bf || dt == 256 || mean <= 16 || rows / 32 * p->kv_heads < 128 ? 1 : 2;
   r.mixed = bf && (p->tokens - p->requests + 1) * g > 16;
   const int kb = bf ? 128 : 64;
   // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
