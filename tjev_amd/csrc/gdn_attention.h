@@ -443,8 +443,7 @@ __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block
 template <class T, int DT, int NQ>
 struct StreamLds {
   static constexpr int NV = NQ * Shape<T, DT>::VH * Shape<T, DT>::VE;  // result registers of four
-  static constexpr int HALF = NV >= 32 ? NV / 2 : NV;                  // exchanged at a time
-  static constexpr int Q = NQ * Shape<T, DT>::KS * 64, ACC = 2 * HALF * 64;  // pieces of 16 bytes
+  static constexpr int Q = NQ * Shape<T, DT>::KS * 64, ACC = 2 * NV * 64;  // pieces of 16 bytes
 };
 
 template <class T, int DT, int NQ, bool PAD, bool WHOLE>
@@ -452,7 +451,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
                                             f32x4* sacc, float (&sm)[4][16 * NQ], float (&sl)[4][16 * NQ]) {
   using S = Shape<T, DT>;
   constexpr int R = 16 * NQ, KB = S::KB, KG = S::KG, E = S::E;
-  constexpr int NV = StreamLds<T, DT, NQ>::NV, HALF = StreamLds<T, DT, NQ>::HALF;
+  constexpr int NV = StreamLds<T, DT, NQ>::NV;
   const AttnArgs& A = arguments();
   const int w = __builtin_amdgcn_readfirstlane(wave()), ln = lane(), r16 = ln & 15, g4 = ln >> 4;
   const int row0 = part.tile * R, h = part.head;
@@ -638,63 +637,54 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
   }
   const bool upper = w >> 1, odd = w & 1;
   float mj[NQ], lj[NQ], own[NQ], other[NQ], res[NQ][S::VH][S::VE];
-  f32x4* const mine = sacc + w * (HALF / 2) * 64 + ln;
-  f32x4* const across = sacc + (w ^ 2) * (HALF / 2) * 64 + ln;
-  const f32x4* const beside = sacc + (w ^ 3) * (HALF / 2) * 64 + ln;
+  f32x4* const mine = sacc + w * (NV / 2) * 64 + ln;
+  f32x4* const across = sacc + (w ^ 2) * (NV / 2) * 64 + ln;
+  const f32x4* const beside = sacc + (w ^ 3) * (NV / 2) * 64 + ln;
   auto reg = [&](int v) -> f32x4& { return o[v / (S::VH * S::VE)][v / S::VE % S::VH][v % S::VE]; };
 #pragma unroll
-  for (int from = 0; from < NV; from += HALF) {
-    if (from) __syncthreads();
+  for (int v = 0; v < NV; v += 2) {
+    const f32x4 &x = reg(v), &y = reg(v + 1);
+    mine[v / 2 * 64] = upper ? f32x4{x[0], x[1], y[0], y[1]} : f32x4{x[2], x[3], y[2], y[3]};
+  }
+  __syncthreads();
 #pragma unroll
-    for (int v = 0; v < HALF; v += 2) {
-      const f32x4 &x = reg(from + v), &y = reg(from + v + 1);
-      mine[v / 2 * 64] = upper ? f32x4{x[0], x[1], y[0], y[1]} : f32x4{x[2], x[3], y[2], y[3]};
-    }
-    __syncthreads();
-    if (!from)
+  for (int n = 0; n < NQ; ++n) {
+    mj[n] = kNegInf;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        mj[n] = kNegInf;
+    for (int i = 0; i < 4; ++i) mj[n] = fmaxf(mj[n], sm[i][n * 16 + r16]);
+    const float base = base_of(mj[n]);
+    lj[n] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mj[n] = fmaxf(mj[n], sm[i][n * 16 + r16]);
-        const float base = base_of(mj[n]);
-        lj[n] = 0.f;
+    for (int i = 0; i < 4; ++i) lj[n] += sl[i][n * 16 + r16] * __builtin_amdgcn_exp2f(sm[i][n * 16 + r16] - base);
+    own[n] = __builtin_amdgcn_exp2f(m[n] - base);
+    other[n] = __builtin_amdgcn_exp2f(sm[w ^ 2][n * 16 + r16] - base);
+  }
+  float keep[NV], send[NV];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lj[n] += sl[i][n * 16 + r16] * __builtin_amdgcn_exp2f(sm[i][n * 16 + r16] - base);
-        own[n] = __builtin_amdgcn_exp2f(m[n] - base);
-        other[n] = __builtin_amdgcn_exp2f(sm[w ^ 2][n * 16 + r16] - base);
-      }
-    float keep[HALF], send[HALF];
+  for (int v = 0; v < NV; v += 2) {
+    const f32x4 t = across[v / 2 * 64];
 #pragma unroll
-    for (int v = 0; v < HALF; v += 2) {
-      const f32x4 t = across[v / 2 * 64];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = (from + v + j / 2) / (S::VH * S::VE);
-        const f32x4& x = reg(from + v + j / 2);
-        const float y = (upper ? x[2 + j % 2] : x[j % 2]) * own[n] + t[j] * other[n];
-        if (j % 2 == 0) {
-          keep[v + j / 2] = y;
-        } else {
-          const float z = keep[v + j / 2];
-          keep[v + j / 2] = odd ? y : z;
-          send[v + j / 2] = odd ? z : y;
-        }
+    for (int j = 0; j < 4; ++j) {
+      const int n = (v + j / 2) / (S::VH * S::VE);
+      const f32x4& x = reg(v + j / 2);
+      const float y = (upper ? x[2 + j % 2] : x[j % 2]) * own[n] + t[j] * other[n];
+      if (j % 2 == 0) {
+        keep[v + j / 2] = y;
+      } else {
+        const float z = keep[v + j / 2];
+        keep[v + j / 2] = odd ? y : z;
+        send[v + j / 2] = odd ? z : y;
       }
     }
+  }
 #pragma unroll
-    for (int v = 0; v < HALF; v += 4)
-      across[v / 4 * 64] = f32x4{send[v], send[v + 1], send[v + 2], send[v + 3]};
-    __syncthreads();
+  for (int v = 0; v < NV; v += 4) across[v / 4 * 64] = f32x4{send[v], send[v + 1], send[v + 2], send[v + 3]};
+  __syncthreads();
 #pragma unroll
-    for (int v = 0; v < HALF; v += 4) {
-      const f32x4 t = beside[v / 4 * 64];
+  for (int v = 0; v < NV; v += 4) {
+    const f32x4 t = beside[v / 4 * 64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = from + v + j;
-        res[at / (S::VH * S::VE)][at / S::VE % S::VH][at % S::VE] = keep[v + j] + t[j];
-      }
-    }
+    for (int j = 0; j < 4; ++j) res[(v + j) / (S::VH * S::VE)][(v + j) / S::VE % S::VH][(v + j) % S::VE] = keep[v + j] + t[j];
   }
   const int d0 = (4 * g4 + w) * S::VE;
   if (!part.p) {
@@ -1298,7 +1288,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 // or memory (wide tiles): the maxima and sums of all parts are read at once, the results as many at a time as the
 // registers hold.
 // Few tiles have many parts each (one request of 16000 tokens, 4 key heads: 126): SLICED spreads a tile's results over
-// gridDim.y workgroups and its parts over two halves of each, 16 at a time; gridDim.x is then the most tiles there can
+// gridDim.y workgroups and its parts over two halves of each, 16 at a time in each; gridDim.x is then the most tiles there can
 // be, and a workgroup finds its one among the ranges' notes.
 constexpr int kSlice = 128;  // results of four per workgroup
 template <int DT, bool SLICED>
