@@ -10,12 +10,12 @@
 // tile that more than one range holds leaves its parts in the workspace for a second launch to join
 // (k_attention_join). Two launches whatever the lengths, which only the GPU knows.
 //
-// Measured, bf16, with a gate but for the first (floors: the cache and rows at 5.12 TB/s, the products at 1230 TFLOP/s, what a
+// Measured, bf16, with a gate but for the first, of several cards (floors: the cache and rows at 5.12 TB/s, the products at 1230 TFLOP/s, what a
 // large copy and a large library product reach on the same card):
-//   1 token over 4000, 16/4 heads of 256 (16 MB)                    16.7 us   floor   3.2   two launches' latency
+//   1 token over 4000, 16/4 heads of 256 (16 MB)                    16.5 us   floor   3.2   two launches' latency
 //   64 requests of up to 32768, 16/4 heads of 256 (1.57 GB)        300            307    memory, 5.2 TB/s
-//   2048 tokens over 30000, 16/4 heads of 256 (1.04 TFLOP)        1130            846    products, 921 TFLOP/s
-//   a prompt of 4096, 32/4 heads of 256 (0.27 TFLOP)               355            224    products, 774 TFLOP/s
+//   2048 tokens over 30000, 16/4 heads of 256 (1.04 TFLOP)        1100 to 1155    846    products, 900 to 945 TFLOP/s
+//   a prompt of 4096, 32/4 heads of 256 (0.27 TFLOP)               344 to 366     224    products, 750 to 800 TFLOP/s
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -716,8 +716,8 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 // row's weights stay in its two lanes and are the second operand of out^T += V^T P^T as they come, V's
 // fragments by transposing LDS reads. The pieces of a row of K or V lie in LDS in an order that depends on the row
 // (swz), which spreads both kinds of read over the banks (no conflicts counted). Bound by the products and what
-// stands between them: 2048 tokens over 30000 at head dims 256, 128, 64 run at 921, 896, 755 TFLOP/s, the matrix
-// units busy for half of the cycles. The queries stay in registers (three fragments at 256 in LDS), the results too;
+// stands between them: 2048 tokens over 30000 at head dims 256, 128, 64 run at 945, 944, 810 TFLOP/s (a
+// warmer card 873, 877, 739), the matrix units busy for half of the cycles. The queries stay in registers (three fragments at 256 in LDS), the results too;
 // two workgroups to a CU cover each other's softmax and barriers.
 // The base of the powers follows the running maximum only when that has grown by more than 2^8: the rescaling
 // of the results is skipped otherwise (a softmax does not depend on its base; weights up to 2^8 have bf16's
