@@ -375,9 +375,10 @@ int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const vo
  *   out = softmax(scale q k^T) v, times sigmoid(gate) when gate [tokens, heads, dim] is not null
  * with heads / kv_heads query heads to a key head. Keys without a page, or past the table's width, are left out; a row
  * without keys is 0. Rows of no request: see fill. What a cache holds in other places (NaN too) does not matter.
- * dim in multiples of 8 up to 256; q, gate, out and the caches 16-byte aligned, with strides that keep
+ * dim in multiples of 8 up to 256, table_width * page_size up to TJEV_GDN_MAX_KEYS; q, gate, out and the caches 16-byte aligned, with strides that keep
  * their rows so. The workspace (tjev_gdn_paged_workspace_bytes, 256-byte aligned) needs no
  * clearing; calls that may overlap need one each. */
+#define TJEV_GDN_MAX_KEYS (0x7fffffff - 4096)
 size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p);
 int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const void* q,
                              const void* k_cache, const void* v_cache, const int32_t* block_table,

@@ -319,6 +319,42 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads", [4, 24])
+def test_shared_pages(dtype, heads):
+    """Requests whose first pages are the same (a common prompt), one of them with a page twice, gate and rows broadcast."""
+    case = batch(torch.Generator().manual_seed(17), [(70, 3), (64, 9), (90, 1)], heads=heads, kv_heads=2, dim=64, page=16, dtype=dtype)
+    table = case["block_table"]
+    table[1, :3], table[2, 1:4], table[2, 4] = table[0, :3], table[0, 1:4], table[0, 1]
+    case["gate"] = torch.randn(1, 1, 64, generator=torch.Generator().manual_seed(18)).to(dtype).expand(13, heads, 64)
+    case["q"] = case["q"][:, :1].expand(13, heads, 64)
+    print(f"attention over shared pages {dtype} heads={heads}", flush=True)
+    want, room = attention64(*(case[n] for n in ("q", "k_cache", "v_cache", "block_table", "starts", "lengths")), gate=case["gate"])
+    compare(_attend(case), want, room)
+
+
+def test_as_many_keys_as_there_can_be():
+    """A table whose entries are all one page, up to the last key that the operator takes."""
+    from tjev_amd import paged_attention
+
+    page, width = 65536, 32767
+    gen = torch.Generator().manual_seed(19)
+    kc, vc = (torch.randn(1, page, 1, 8, generator=gen).to(BF).cuda() for _ in range(2))
+    q = torch.randn(1, 1, 8, generator=gen).to(BF).cuda()
+    table, starts = torch.zeros(1, width, dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    print(f"attention over {width * page} keys", flush=True)
+    got = paged_attention(q, kc, vc, table, starts, torch.tensor([width * page], dtype=torch.int32, device="cuda"))
+    k, v, x = kc[0, :, 0].double(), vc[0, :, 0].double(), q[0, 0].double()
+    w = torch.softmax(8 ** -0.5 * (k @ x), 0)
+    want, a = w @ v, w @ v.abs()
+    # sums of 2^31 numbers in 32 bits: a wave of a range adds fewer than 2^15 steps into one number, the weights' sum in
+    # two additions a step and the result in eight (two products of 32 keys, a rounding for every 8), each off
+    # by 2^-24 of it; the weights and the rounding as in attention64
+    delta = 16 * 2.0 ** -24 * 8 ** -0.5 * float((k.abs() @ x.abs()).max())
+    room = a * (4 * delta + 10 * (2 ** 15 + 64) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -8)
+    compare(got[0, 0], want.cpu(), (room + 2.0 ** -8 * (want.abs() + room)).cpu())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
 def test_scales(dtype, scale):
     case = batch(torch.Generator().manual_seed(13), [(60, 2), (30, 90), (9, 1)], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)

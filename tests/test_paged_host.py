@@ -222,6 +222,7 @@ def _paged_params(**kw):
     (dict(requests=0), 1, "positive"), (dict(page_size=0), 1, "positive"), (dict(pages=0), 1, "positive"), (dict(tokens=-1), 1, "negative"),
     (dict(heads=3), 1, "groups"), (dict(dtype=3), 1, "dtype"), (dict(dim=12), 2, "multiples of 8"), (dict(dim=264), 2, "multiples of 8"),
     (dict(scale=float("nan")), 1, "finite"), (dict(scale=float("inf")), 1, "finite"), (dict(table_width=1 << 28), 1, "too large"),
+    (dict(table_width=(1 << 20) - 1, page_size=2048), 1, "too large"),  # keys whose tiles end past the 32-bit numbers
     (dict(tokens=1 << 30), 1, "too large"), (dict(q_stride=(256, 60)), 1, "16-byte"), (dict(k_stride=(2044, 128, 64)), 1, "16-byte"),
 ])
 def test_attention_c_abi(bad, status, msg):

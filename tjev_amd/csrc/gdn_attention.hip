@@ -48,7 +48,8 @@ int validate(const tjev_gdn_paged_params* p) {
   if (p->dim < 8 || p->dim % 8 || p->dim > 256)
     return fail(TJEV_GDN_EUNSUPPORTED, "paged attention kernels hold head dims in multiples of 8 up to 256");
   if (!(p->scale - p->scale == 0.f)) return fail(TJEV_GDN_EINVAL, "scale must be finite");
-  if ((long)p->table_width * p->page_size >= (1l << 31) || p->tokens * p->heads >= (1l << 31) ||
+  // (keys are 32-bit numbers, and a tile looks some blocks past the last)
+  if ((long)p->table_width * p->page_size > TJEV_GDN_MAX_KEYS || p->tokens * p->heads >= (1l << 31) ||
       ((p->tokens * (p->heads / p->kv_heads)) / 16 + p->requests) * p->kv_heads >= (1l << 31) / 256)
     return fail(TJEV_GDN_EINVAL, "problem too large");
   return 0;

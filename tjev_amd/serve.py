@@ -8,7 +8,8 @@ Here the state is the megakernel's: the prefill returns the recurrent state afte
 last token (fp32 [B, H, Dk, Dv]) and the conv history (the last K-1 raw rows [B, K-1, W] in
 qkv's dtype, zero outside the last token's segment), and ``gdn_decode_step`` continues both
 (HF ``causal_conv1d_update`` for the conv). A decode step continues the segment the state
-belongs to; a new request starts from a fresh prefill.
+belongs to; a new request starts from a fresh prefill. The full-attention layers that stand between a
+model's GDN layers are served by ``rotary.py`` and ``paged.py``.
 """
 
 from __future__ import annotations
