@@ -5,7 +5,8 @@ them; its queries and keys are turned by their positions before they meet. ``rot
 the first 2 * len(inv_freq) lanes of every head of q and k in one launch: pair i by the angle
 positions[axis of i] * inv_freq[i], the angle taken in 64 bits and the turn in 32, rounded once. The
 axes divide the pairs by ``sections``. Differentiable in q and k (the gradient is the turn back and keeps
-neither of them); positions and frequencies take no gradient. There is no fallback: without the
+neither of them); positions and frequencies take no gradient. A gradient may be captured into a HIP graph when
+no eager graph of the same leaves is alive, as torch requires of any operator. There is no fallback: without the
 HIP library, or on a CPU tensor, the operator raises.
 """
 
