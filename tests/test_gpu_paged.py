@@ -135,6 +135,19 @@ def test_attention(dtype, heads, kv_heads, dim, page, lens):
     assert bool((got[-3:] == 0).all())
 
 
+@pytest.mark.parametrize("dtype,dim,page,heads,kv_heads,lens", [
+    (BF, 64, 16, 8, 1, [(31, 3), (0, 4), (200, 3), (77, 2)]), (BF, 40, 24, 8, 1, [(700, 4)]), (BF, 64, 10, 16, 2, [(31, 1), (5, 1), (64, 9)]),
+    (BF, 64, 64, 5, 1, [(3000, 5), (9, 5), (0, 5)]), (F32, 64, 16, 16, 8, [(130, 260)]), (F32, 96, 24, 16, 8, [(30, 200), (9, 65)]),
+])
+def test_tiles_of_32_rows(dtype, dim, page, heads, kv_heads, lens):
+    """Requests of 17 to 32 rows on average (bf16, head dims up to 64) and large fp32 batches."""
+    print(f"attention {dtype} heads={heads}/{kv_heads} dim={dim} page={page} {lens}", flush=True)
+    case = batch(torch.Generator().manual_seed(20), lens, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype, pad_rows=1, gate=True)
+    want, room = attention64(case["q"], case["k_cache"], case["v_cache"], case["block_table"], case["starts"], case["lengths"],
+                             gate=case["gate"])
+    compare(_attend(case), want, room)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("page", [16, 10])
 @pytest.mark.parametrize("heads", [4, 16])

@@ -4,7 +4,7 @@
 // one pass over the keys with the running maximum m_r and sum of each row in 32 bits.
 //
 // The query heads of a key head are rows of one tile beside its tokens, so a key is read once for all of them. Up to
-// 16 rows a request (decoding) are bound by memory, and their keys and values stream straight into registers
+// 16 or 32 rows a request (decoding) are bound by memory, and their keys and values stream straight into registers
 // (stream_tile); more are bound by the products, and share tiles of 128 rows whose keys pass through LDS (wide_tile,
 // bf16). All tiles of a batch are cut into as many equal ranges of work as workgroups fit the chip (gdn_paged.h); a
 // tile that more than one range holds leaves its parts in the workspace for a second launch to join

@@ -20,10 +20,13 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   const int dt = p->dim <= 64 ? 64 : p->dim <= 128 ? 128 : 256;
   const long g = p->heads / p->kv_heads, rows = p->tokens * g, mean = (rows + p->requests - 1) / p->requests;
   AttnPlan r;
-  // fp32 tiles of 32 rows where there are enough of them and registers to hold them (2 requests of 910 tokens after 858, 4/1
-  // heads of 128: 50.5 us, with 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6)
-  r.nq = bf || dt == 256 || mean <= 16 || rows / 32 * p->kv_heads < 128 ? 1 : 2;
-  r.mixed = bf && (p->tokens - p->requests + 1) * g > 16;
+  // Streamed tiles of 32 rows instead of 16 where the registers hold them without a loss. In bf16 at head dims up to 64 for
+  // requests of 17 to 32 on average, which would else take a tile of 128 (32 requests of 5 tokens over 8192, 32/8 heads of
+  // 64: 33.7 us, with that 39.0; one request 18.2, 21.8; at 128 the tile of 128 is the faster one, 63 against 69). In fp32
+  // up to 128 where there are enough of them (2 requests of 910 tokens after 858, 4/1 heads of 128: 50.5 us, with
+  // 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6).
+  r.nq = mean > 16 && (bf ? dt == 64 && mean <= 32 : dt <= 128 && rows / 32 * p->kv_heads >= 128) ? 2 : 1;
+  r.mixed = bf && (p->tokens - p->requests + 1) * g > 16 * r.nq;
   const int kb = bf ? 128 : 64;
   // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
   const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + p->requests) * p->kv_heads;

@@ -34,11 +34,11 @@ hipError_t dispatch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   return pad ? whole ? with(yes, yes) : with(yes, no) : whole ? with(no, yes) : with(no, no);
 }
 
-// bf16: more than 16 rows of a request take the wide tiles. fp32 streams all, in tiles of 16 or 32 rows (more are spilled:
-// 64 at head dim 128 and 32 at 256 take twice the time).
+// bf16: requests of more rows than a streamed tile has take the wide tiles. fp32 streams all. Streamed tiles have 16 rows or
+// 32 (more are spilled: in fp32 64 at head dim 128 and 32 at 256 take twice the time).
 template <class T, int DT>
 hipError_t by_rows(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
-  if constexpr (sizeof(T) == 4 && DT <= 128)
+  if constexpr (DT <= (sizeof(T) == 4 ? 128 : 64))
     if (r.nq > 1) return dispatch<T, DT, 2>(r, A, st);
   return dispatch<T, DT, 1>(r, A, st);
 }

@@ -194,8 +194,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q [N, heads, dim] (heads: groups of kv_heads; dim in multiples of 8 up to 256): rows starts[b] ..
     starts[b + 1] - 1 are the last tokens of request b, whose keys are ``lengths[b]`` in all, in the pages of row b of
     ``block_table`` [B, M] int32. Each attends to the keys up to its own, softmax(scale q k^T) v with scale
-    dim^-1/2 by default, in 32 bits; a row without keys is 0. (In bf16 the weights of a request with more than 16
-    tokens times query heads per key head are rounded to bf16 for their product with v.) ``gate`` [N, heads, dim]
+    dim^-1/2 by default, in 32 bits; a row without keys is 0. (In bf16 the weights of a request with more than 32
+    tokens times query heads per key head, or 16, are rounded to bf16 for their product with v.) ``gate`` [N, heads, dim]
     multiplies the result by its sigmoid. Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
