@@ -5,9 +5,9 @@ them; its queries and keys are turned by their positions before they meet. ``rot
 the first 2 * len(inv_freq) lanes of every head of q and k in one launch: pair i by the angle
 positions[axis of i] * inv_freq[i], the angle taken in 64 bits and the turn in 32, rounded once. The
 axes divide the pairs by ``sections``. Differentiable in q and k (the gradient is the turn back and keeps
-neither of them); positions and frequencies take no gradient. A gradient may be captured into a HIP graph when
-no eager graph of the same leaves is alive, as torch requires of any operator. There is no fallback: without the
-HIP library, or on a CPU tensor, the operator raises.
+neither of them); positions and frequencies take no gradient, and forward-mode derivatives raise. A gradient
+may be captured into a HIP graph when no eager graph of the same leaves is alive, as torch requires of any
+operator. There is no fallback: without the HIP library, or on a CPU tensor, the operator raises.
 """
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -106,11 +107,16 @@ class _Rotary(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         d_q = _rows(d_q)
         d_k = _rows(d_k) if ctx.needs_input_grad[1] else None
-        if torch.is_grad_enabled():
-            d_q, d_k = _Rotary.apply(d_q, d_k, positions, inv_freq, ctx.options, not ctx.inverse)
-        else:
-            d_q, d_k = _launch(d_q, d_k, positions, inv_freq, *ctx.options, not ctx.inverse)
+        d_q, d_k = _turned(d_q, d_k, positions, inv_freq, ctx.options, not ctx.inverse)
         return d_q, d_k, None, None, None, None
+
+
+def _turned(q, k, positions, inv_freq, options, inverse: bool):
+    """The launch, through its Function where q or k may carry a derivative: a gradient, or (whatever the grad mode) a tangent,
+    which the Function refuses. Elsewhere without it, which is some us of host time."""
+    if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return _Rotary.apply(q, k, positions, inv_freq, options, inverse)
+    return _launch(q, k, positions, inv_freq, *options, inverse)
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections=None,
@@ -133,12 +139,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
         batch = math.prod(q.shape[:-3])
         q4 = q.reshape(batch, *q.shape[-3:])
         k4 = None if k is None else k.reshape(batch, *k.shape[-3:])
-    args = (_rows(q4), None if k is None else _rows(k4), positions.contiguous(), inv_freq.contiguous())
     options = (axes, (inv_freq.shape[0],) if secs is None else secs, interleaved, adjacent)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q4, k4 = _Rotary.apply(*args, options, False)
-    else:
-        q4, k4 = _launch(*args, *options, False)
+    q4, k4 = _turned(_rows(q4), None if k is None else _rows(k4), positions.contiguous(), inv_freq.contiguous(), options, False)
     if q.dim() <= 4:
         return q4, k4
     return q4.reshape(q.shape), None if k is None else k4.reshape(k.shape)
