@@ -26,14 +26,16 @@ class _Library:
 
 @pytest.fixture
 def library(monkeypatch):
-    from tjev_amd import _lib
+    from tjev_amd import _lib, paged, rotary
 
     lib = _Library()
     monkeypatch.setattr(_lib, "load", lambda: lib)
     monkeypatch.setattr(_lib, "one_gpu", lambda what, devices: None)
     monkeypatch.setattr(_lib, "current_stream", lambda device: 0)
     monkeypatch.setattr(_lib, "on_device", lambda device: contextlib.nullcontext())
-    return lib
+    yield lib
+    for kept in (paged._tables_params, paged._append_params, paged._attention_params, rotary._checked, rotary._params):
+        kept.cache_clear()  # checks that passed here alone
 
 
 def _rotary(q, k=None):
@@ -69,3 +71,57 @@ def test_rotary_within_a_dual_level(library):
         y, _ = _rotary(torch.randn(1, 3, 2, 16))
         assert forward_ad.unpack_dual(y).tangent is None
     assert [n for n, _ in library.calls] == ["tjev_gdn_rotary"]
+
+
+# ---------------------------------------------------------------- recorded calls
+def _calls():
+    """Each operator as a function of one tensor."""
+    from tjev_amd import paged_append, paged_attention, paged_tables
+
+    i = torch.zeros(2, dtype=torch.int32)
+    table, starts = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    cache = torch.zeros(4, 16, 2, 64)
+
+    def append(k):
+        paged_append(k, k, cache, cache, torch.zeros(3, dtype=torch.int64))
+        return cache + 0
+
+    return {"rotary_axes": (lambda q: _rotary(q)[0], torch.randn(1, 3, 2, 16)),
+            "paged_tables": (lambda t: paged_tables(i, i, t, i, page_size=16, tokens=4).slots, table),
+            "paged_append": (append, torch.randn(3, 2, 64)),
+            "paged_attention": (lambda q: paged_attention(q, cache, cache, table, starts, i), torch.randn(3, 4, 64))}
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("what", ["rotary_axes", "paged_tables", "paged_append", "paged_attention"])
+@pytest.mark.parametrize("record", ["jit", "make_fx", "pre_dispatch"])
+def test_recorded_calls_are_refused(library, what, record):
+    """A launch is no operator of torch's: a record of it would be of its uninitialised output."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f, x = _calls()[what]
+    with pytest.raises(RuntimeError, match=f"{what}.*recorded"):
+        torch.jit.trace(f, (x,), check_trace=False) if record == "jit" else make_fx(f, pre_dispatch=record == "pre_dispatch")(x)
+    assert not library.calls
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_a_recorded_rotary_gradient_is_refused(library):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    q = torch.randn(1, 3, 2, 16, requires_grad=True)
+    y, _ = _rotary(q)
+    with pytest.raises(RuntimeError, match="rotary_axes.*recorded"):
+        make_fx(lambda d: torch.autograd.grad(y, q, d)[0])(torch.ones_like(y))
+
+
+@pytest.mark.parametrize("what", ["rotary_axes", "paged_tables", "paged_append", "paged_attention"])
+def test_modes_that_only_look_on(library, what):
+    """A dispatch mode that records nothing (a FLOP counter) lets the calls through."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    f, x = _calls()[what]
+    library.tjev_gdn_paged_workspace_bytes = lambda p: 256
+    with FlopCounterMode(display=False):
+        f(x)
+    assert len(library.calls) == 1

@@ -13,6 +13,7 @@ import functools
 from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
+from torch._ops import _len_torch_dispatch_stack_pre_dispatch
 
 LIB_PATH = Path(__file__).resolve().parent / "libtjev_gdn.so"
 # the debug build whose kernels first fill their LDS with NaN (python -m tjev_amd.build --lds-poison)
@@ -280,6 +281,18 @@ def one_gpu(what: str, devices) -> None:
         raise RuntimeError(f"{what} runs on the GPU (HIP); got a CPU tensor")
     if len(set(devices)) > 1:
         raise ValueError(f"{what}: tensors on GPUs {sorted(set(devices))}")
+
+
+def not_recorded(what: str) -> None:
+    """Raises where torch records the calls of its operators to run them again (jit tracing, make_fx): a launch by address is none
+    of them, and the record would hold its output uninitialised. (torch.compile leaves these calls out of its graphs, and
+    runs them as they are.)"""
+    if (torch.jit.is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None
+            or _len_torch_dispatch_stack_pre_dispatch() > 0):
+        raise RuntimeError(f"{what} is a launch of the HIP library and cannot be recorded (jit tracing, make_fx)")
+
+
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 def on_device(device: torch.device):

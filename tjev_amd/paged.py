@@ -12,7 +12,7 @@ A step of a batch, with what every layer shares first:
 Caches are [pages, page_size, kv_heads, dim] with any strides whose last dim is contiguous (another order
 of the dims, or keys and values in one tensor, are views of this). Token t of a request lies in page
 block_table[request, t // page_size] at place t % page_size; its slot is page * page_size + place. A
-table entry that is no page of the cache (-1) holds no keys. Every call runs on torch's current stream of the tensors'
+table entry that is no page of the cache (-1) holds no keys. Recorded calls (jit tracing, make_fx) raise. Every call runs on torch's current stream of the tensors'
 device; workspaces come from torch's allocator, so calls on several streams, and captured graphs,
 have their own.
 """
@@ -91,6 +91,7 @@ def paged_tables(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Ten
     ``inplace`` the taken ones are written into ``block_table`` and all others left. ``tokens``: the size of the
     slot map; slots behind the last request's tokens, and of tokens without a page (past the free list or the
     table's width), are -1. Unused requests have both lengths 0; up to 8192 requests."""
+    _lib.not_recorded("paged_tables")
     p = _tables_params(
         block_table.shape, block_table.stride(), block_table.dtype, (cached.shape, new.shape),
         (free_pages.shape, 1 if taken is None else taken.numel()),
@@ -134,6 +135,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     """Writes the new tokens' k and v [N, kv_heads, dim] (any strides with a contiguous last dim) into the
     slots [N] of the caches, in place. Slots outside the cache (-1) are skipped. The slots of one call are
     distinct: of two tokens with one slot, either's values or parts of both remain."""
+    _lib.not_recorded("paged_append")
     k, v = (x if x.dim() != 3 or x.stride(-1) == 1 else x.contiguous() for x in (k, v))
     p = _append_params(
         k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
@@ -199,6 +201,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     multiplies the result by its sigmoid. Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
+    _lib.not_recorded("paged_attention")
     q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.contiguous() for x in (q, gate))
     lib = _lib.load()
     p, need = _attention_params(

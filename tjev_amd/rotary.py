@@ -5,7 +5,8 @@ them; its queries and keys are turned by their positions before they meet. ``rot
 the first 2 * len(inv_freq) lanes of every head of q and k in one launch: pair i by the angle
 positions[axis of i] * inv_freq[i], the angle taken in 64 bits and the turn in 32, rounded once. The
 axes divide the pairs by ``sections``. Differentiable in q and k (the gradient is the turn back and keeps
-neither of them); positions and frequencies take no gradient, and forward-mode derivatives raise. A gradient
+neither of them); positions and frequencies take no gradient. Forward-mode derivatives raise, as do recorded calls
+(jit tracing, make_fx). A gradient
 may be captured into a HIP graph when no eager graph of the same leaves is alive, as torch requires of any
 operator. There is no fallback: without the HIP library, or on a CPU tensor, the operator raises.
 """
@@ -75,6 +76,7 @@ def _params(q_shape, q_stride, dtype, k_shape, k_stride, half, axes, sections, i
 
 def _launch(q, k, positions, inv_freq, axes, sections, interleaved: bool, adjacent: bool, inverse: bool):
     """The library's call: q [B, T, Hq, D] or [T, Hq, D], k alike or None (the last dim contiguous)."""
+    _lib.not_recorded("rotary_axes")
     dev = q.device
     p = _params(q.shape, q.stride(), q.dtype, None if k is None else k.shape, None if k is None else k.stride(), inv_freq.shape[0],
                 axes, sections, interleaved, adjacent, inverse, positions.dtype, inv_freq.dtype)
