@@ -125,3 +125,31 @@ def test_modes_that_only_look_on(library, what):
     with FlopCounterMode(display=False):
         f(x)
     assert len(library.calls) == 1
+
+
+# ---------------------------------------------------------------- views
+def _attend(**kw):
+    from tjev_amd import paged_attention
+
+    n = kw["q"].shape[0]
+    cache = torch.zeros(4, 16, 2, 64, dtype=kw["q"].dtype)
+    a = dict(k_cache=cache, v_cache=cache, block_table=torch.zeros(1, 3, dtype=torch.int32), starts=torch.tensor([0, n], dtype=torch.int32),
+             lengths=torch.tensor([n], dtype=torch.int32))
+    return paged_attention(**{**a, **kw})
+
+
+Q, GATE, OUT = 2, 8, 9  # places in the library's call
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 2])
+@pytest.mark.parametrize("which", ["q", "gate"])
+def test_rows_off_16_bytes_are_copied(library, dtype, n, which):
+    """One row of a wider tensor is contiguous, and no less a row off 16 bytes."""
+    x = {"q": torch.zeros(n, 4, 64, dtype=dtype), "gate": torch.zeros(n, 4, 64, dtype=dtype)}
+    x[which] = torch.zeros(n, 3 + 4 * 64, dtype=dtype)[:, 3:].view(n, 4, 64)
+    assert x[which].data_ptr() % 16 and (n > 1 or x[which].is_contiguous())
+    _attend(**x)
+    (_, args), = [c for c in library.calls if c[0] == "tjev_gdn_paged_attention"]
+    at, other = (Q, "gate") if which == "q" else (GATE, "q")
+    assert args[at] % 16 == 0 and args[at] != x[which].data_ptr() and args[Q + GATE - at] == x[other].data_ptr()

@@ -202,7 +202,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
     _lib.not_recorded("paged_attention")
-    q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.contiguous() for x in (q, gate))
+    # (contiguous() would leave a contiguous view that starts off 16 bytes where it is)
+    q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, gate))
     lib = _lib.load()
     p, need = _attention_params(
         lib, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,
