@@ -153,3 +153,18 @@ def test_rows_off_16_bytes_are_copied(library, dtype, n, which):
     (_, args), = [c for c in library.calls if c[0] == "tjev_gdn_paged_attention"]
     at, other = (Q, "gate") if which == "q" else (GATE, "q")
     assert args[at] % 16 == 0 and args[at] != x[which].data_ptr() and args[Q + GATE - at] == x[other].data_ptr()
+
+
+@pytest.mark.parametrize("which", ["q", "gate", "out", "k_cache", "v_cache"])
+def test_strides_of_one_row_do_not_matter(library, which):
+    """Where a dim has one place its stride is no row's distance: such a view is neither copied nor refused."""
+    x = {n: torch.zeros(1, 4, 64) for n in ("q", "gate", "out")}
+    x.update({n: torch.zeros(4, 16, 1, 64) for n in ("k_cache", "v_cache")})
+    old = x[which]
+    x[which] = old.as_strided(old.shape, tuple(s if n > 1 else 1003 for n, s in zip(old.shape, old.stride())))
+    _attend(**x)
+    (_, args), = [c for c in library.calls if c[0] == "tjev_gdn_paged_attention"]
+    p = args[0]._obj
+    assert [args[i] for i in (Q, 3, 4, GATE, OUT)] == [x[n].data_ptr() for n in ("q", "k_cache", "v_cache", "gate", "out")]
+    for s in (p.q_stride, p.gate_stride, p.out_stride, p.k_stride, p.v_stride):
+        assert all(v % 4 == 0 for v in s)

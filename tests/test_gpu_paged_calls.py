@@ -32,3 +32,20 @@ def test_rows_off_16_bytes(dtype, n):
         off[x].copy_(case[x])
     print(f"attention of rows off 16 bytes {dtype} n={n}", flush=True)
     compare(_attend(case, **off), want, room)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strides_of_one_row(dtype):
+    """One token into a row of a wider tensor, over a cache of one key head whose heads' stride is no multiple of 16 bytes."""
+    case = batch(torch.Generator().manual_seed(22), [(70, 1)], heads=4, kv_heads=1, dim=64, page=16, dtype=dtype)
+    want, room = attention64(*(case[x] for x in NAMES))
+    wide = torch.full((1, 1003), 7.0, dtype=dtype, device="cuda")
+    out = wide[:, 8:264].view(1, 4, 64)
+    caches = {}
+    for x in ("k_cache", "v_cache"):
+        c = case[x].cuda()
+        caches[x] = c.as_strided(c.shape, (*c.stride()[:2], 1003, 1))
+    print(f"attention into one row {dtype}", flush=True)
+    assert _attend(case, out=out, **caches) is out
+    compare(out, want, room)
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 264:] == 7).all())

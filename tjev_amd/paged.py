@@ -178,9 +178,15 @@ def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_d
         raise ValueError("out's last dim must be contiguous, and none expanded")
     _lib.one_gpu("paged_attention", devices)
     p = _lib.PagedParams(tokens, requests, t_shape[1], kc_shape[0], kc_shape[1], heads, kv_heads, dim, _DTYPES[q_dtype], int(out is None),
-                         dim ** -0.5 if scale is None else scale, q_stride[:2], (0, 0) if gate is None else gate[1][:2],
-                         (heads * dim, dim) if out is None else out[1][:2], kc_stride[:3], vc_stride[:3])
+                         dim ** -0.5 if scale is None else scale, _strides(q_shape, q_stride),
+                         (0, 0) if gate is None else _strides(*gate[:2]), (heads * dim, dim) if out is None else _strides(*out[:2]),
+                         _strides(kc_shape, kc_stride), _strides(vc_shape, vc_stride))
     return ctypes.byref(p), lib.tjev_gdn_paged_workspace_bytes(ctypes.byref(p))
+
+
+def _strides(shape, stride):
+    """The strides of all dims but the last, 0 where a dim has one place: no distance between rows, which may be any number."""
+    return tuple(s if n > 1 else 0 for n, s in zip(shape[:-1], stride))
 
 
 def _like(x: torch.Tensor | None):
@@ -224,4 +230,4 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def _aligned(x: torch.Tensor) -> bool:
     """Whether the rows of x [N, heads, dim] start on 16 bytes."""
     s, e = x.stride(), 16 // x.element_size()
-    return s[2] == 1 and s[0] % e == 0 and s[1] % e == 0 and x.data_ptr() % 16 == 0
+    return s[2] == 1 and (s[0] % e == 0 or x.shape[0] == 1) and (s[1] % e == 0 or x.shape[1] == 1) and x.data_ptr() % 16 == 0
