@@ -168,3 +168,41 @@ def test_strides_of_one_row_do_not_matter(library, which):
     assert [args[i] for i in (Q, 3, 4, GATE, OUT)] == [x[n].data_ptr() for n in ("q", "k_cache", "v_cache", "gate", "out")]
     for s in (p.q_stride, p.gate_stride, p.out_stride, p.k_stride, p.v_stride):
         assert all(v % 4 == 0 for v in s)
+
+
+# ---------------------------------------------------------------- gradients that there are none of
+@pytest.mark.parametrize("which", ["q", "gate", "out", "k_cache", "v_cache"])
+def test_attention_refuses_to_lose_a_gradient(library, which):
+    x = {n: torch.zeros(2, 4, 64) for n in ("q", "gate", "out")}
+    x.update({n: torch.zeros(4, 16, 2, 64) for n in ("k_cache", "v_cache")})
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match="paged_attention has no gradient"):
+            _attend(**{**x, which: forward_ad.make_dual(x[which], torch.ones_like(x[which]))})
+    x[which].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="paged_attention has no gradient"):
+        _attend(**x)
+    assert not [c for c in library.calls if c[0] == "tjev_gdn_paged_attention"]
+    with torch.no_grad():
+        _attend(**x)
+    x[which] = x[which].detach()
+    _attend(**x)
+    assert len([c for c in library.calls if c[0] == "tjev_gdn_paged_attention"]) == 2
+
+
+@pytest.mark.parametrize("which", ["k", "v", "k_cache", "v_cache"])
+def test_append_refuses_to_lose_a_gradient(library, which):
+    from tjev_amd import paged_append
+
+    x = {n: torch.zeros(3, 2, 64) for n in ("k", "v")}
+    x.update({n: torch.zeros(4, 16, 2, 64) for n in ("k_cache", "v_cache")})
+    slots = torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match="paged_append has no gradient"):
+            paged_append(**{**x, which: forward_ad.make_dual(x[which], torch.ones_like(x[which]))}, slots=slots)
+    x[which].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="paged_append has no gradient"):
+        paged_append(**x, slots=slots)
+    assert not library.calls
+    with torch.no_grad():
+        paged_append(**x, slots=slots)
+    assert len(library.calls) == 1

@@ -14,6 +14,7 @@ from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 from torch._ops import _len_torch_dispatch_stack_pre_dispatch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libtjev_gdn.so"
 # the debug build whose kernels first fill their LDS with NaN (python -m tjev_amd.build --lds-poison)
@@ -293,6 +294,19 @@ def not_recorded(what: str) -> None:
 
 
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def inference_only(what: str, *tensors) -> None:
+    """Raises where one of the tensors (or None) carries a derivative, which ``what`` would lose: it requires a gradient while
+    gradients are recorded, or has a tangent."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or with detached tensors")
+    if forward_ad._current_level >= 0:
+        for x in tensors:
+            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+                raise RuntimeError(f"{what} has no gradient: call it with tensors without tangents")
 
 
 def on_device(device: torch.device):

@@ -1,6 +1,7 @@
 """The paged key/value cache and its attention on MI355X: the full-attention layers that stand between the
 GDN layers of a served hybrid decoder, beside ``gdn_prefill`` and ``gdn_decode_step`` (serve.py). Inference
-only (no autograd), through the HIP library; nothing here waits for the GPU or reads a length on the host.
+only, through the HIP library: there is no gradient, and tensors that carry one raise outside
+torch.no_grad(). Nothing here waits for the GPU or reads a length on the host.
 
 A step of a batch, with what every layer shares first:
 
@@ -12,9 +13,9 @@ A step of a batch, with what every layer shares first:
 Caches are [pages, page_size, kv_heads, dim] with any strides whose last dim is contiguous (another order
 of the dims, or keys and values in one tensor, are views of this). Token t of a request lies in page
 block_table[request, t // page_size] at place t % page_size; its slot is page * page_size + place. A
-table entry that is no page of the cache (-1) holds no keys. Recorded calls (jit tracing, make_fx) raise. Every call runs on torch's current stream of the tensors'
-device; workspaces come from torch's allocator, so calls on several streams, and captured graphs,
-have their own.
+table entry that is no page of the cache (-1) holds no keys. Every call runs on torch's current stream of the
+tensors' device; workspaces come from torch's allocator, so calls on several streams, and captured
+graphs, have their own. Calls recorded by jit tracing or make_fx raise.
 """
 
 from __future__ import annotations
@@ -136,6 +137,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     slots [N] of the caches, in place. Slots outside the cache (-1) are skipped. The slots of one call are
     distinct: of two tokens with one slot, either's values or parts of both remain."""
     _lib.not_recorded("paged_append")
+    _lib.inference_only("paged_append", k, v, k_cache, v_cache)
     k, v = (x if x.dim() != 3 or x.stride(-1) == 1 else x.contiguous() for x in (k, v))
     p = _append_params(
         k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
@@ -208,6 +210,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
     _lib.not_recorded("paged_attention")
+    _lib.inference_only("paged_attention", q, k_cache, v_cache, gate, out)
     # (contiguous() would leave a contiguous view that starts off 16 bytes where it is)
     q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, gate))
     lib = _lib.load()
