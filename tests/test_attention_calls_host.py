@@ -206,3 +206,36 @@ def test_append_refuses_to_lose_a_gradient(library, which):
     with torch.no_grad():
         paged_append(**x, slots=slots)
     assert len(library.calls) == 1
+
+
+# ---------------------------------------------------------------- sizes past 32 bits
+FAR = 2 ** 32 + 16
+
+
+def test_tables_refuse_pages_past_32_bits(library):
+    from tjev_amd import paged_tables
+
+    i, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32)
+    for kw in (dict(page_size=FAR), dict(page_size=2 ** 31), dict(block_table=torch.zeros(1, 1, dtype=torch.int32).expand(2, FAR))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged_tables(**{**dict(cached=i, new=i, block_table=table, free_pages=i, page_size=16, tokens=4), **kw})
+    assert not library.calls
+
+
+@pytest.mark.parametrize("shape", [(FAR, 16, 2, 64), (4, FAR, 2, 64)])
+def test_caches_past_32_bits_are_refused(library, shape):
+    from tjev_amd import paged
+
+    cache = torch.zeros(1, 1, 1, 64).expand(shape)
+    with pytest.raises(ValueError, match="2\\^31"):
+        _attend(q=torch.zeros(1, 4, 64), k_cache=cache, v_cache=cache)
+    # (no tensor of this size: a call's checks take the shape alone)
+    like = lambda s: (s, (1 << 40, 128, 64, 1), torch.float32)  # noqa: E731
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged._append_params(*(2 * ((3, 2, 64), (128, 64, 1), torch.float32)), *like(shape), *like(shape), (3,), torch.int64, (0,))
+    assert not [c for c in library.calls if c[0] != "tjev_gdn_paged_workspace_bytes"]
+
+
+def test_table_widths_past_32_bits_are_refused(library):
+    with pytest.raises(ValueError, match="2\\^31"):
+        _attend(q=torch.zeros(1, 4, 64), block_table=torch.zeros(1, 1, dtype=torch.int32).expand(1, FAR))

@@ -51,12 +51,19 @@ def _device(x: torch.Tensor | None, like: torch.Tensor) -> int:
     return like.get_device() if x is None else x.get_device()
 
 
+def _check_sizes(*sizes: int) -> None:
+    """The library's sizes are 32-bit numbers: a larger one would arrive as its low half."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"tables, pages and page sizes of less than 2^31, not {max(sizes)}")
+
+
 def _check_caches(k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, heads: int, dim: int) -> None:
     if len(k_shape) != 4 or k_shape[2:] != (heads, dim) or v_shape != k_shape or v_dtype != k_dtype:
         raise ValueError(f"caches [pages, page_size, {heads}, {dim}] of one type, not {tuple(k_shape)} {k_dtype} and {tuple(v_shape)} "
                          f"{v_dtype}")
     if dim > 1 and (k_stride[-1] != 1 or v_stride[-1] != 1):
         raise ValueError("the caches' last dim must be contiguous (a copy would leave the caller's cache unchanged)")
+    _check_sizes(*k_shape[:2])
 
 
 # The checks and parameters of a call depend on its shapes, strides, types and options alone, and are kept by
@@ -69,6 +76,7 @@ def _tables_params(t_shape, t_stride, t_dtype, lengths, list_shapes, int_dtypes,
     if not 1 <= requests <= _lib.MAX_REQUESTS or width < 1 or page_size < 1 or tokens < 0:
         raise ValueError(f"1 to {_lib.MAX_REQUESTS} requests of pages of at least one token, not {requests} of {width} pages of "
                          f"{page_size}, and {tokens} tokens")
+    _check_sizes(width, page_size)
     if lengths != ((requests,), (requests,)):
         raise ValueError(f"lengths {tuple(map(tuple, lengths))} of {requests} requests")
     free_shape, taken_size = list_shapes
@@ -166,6 +174,7 @@ def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_d
     if dim % 8 or not 8 <= dim <= 256:
         raise ValueError(f"head dims in multiples of 8 up to 256, not {dim}")
     requests = t_shape[0]
+    _check_sizes(*t_shape)
     if requests < 1 or t_shape[1] < 1 or kc_shape[0] < 1 or kc_shape[1] < 1:
         raise ValueError(f"a block table {tuple(t_shape)} or a cache {tuple(kc_shape)} without pages")
     if s_shape != (requests + 1,) or l_shape != (requests,):
