@@ -1244,35 +1244,25 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
       const int slot = 2 * range + begun;
       const Part part{keys == blocks ? nullptr : A.part + (size_t)slot * A.slot, at.tile, at.head};
       __syncthreads();
-      if (uniform(wave()) == 0) {
-        if (threadIdx.x == 0 && keys > 0 && k0 == 0 && keys < blocks)  // the tile goes on in the next ranges
+      if (threadIdx.x == 0) {
+        if (keys > 0 && k0 == 0 && keys < blocks)  // the tile goes on in the next ranges
           *split_of(A, range) = {(int)div_by(st.each)(u - at.at + q.extra + blocks - 1) - range + 1, slot, q.s0, q.rows, q.tile_rows, at.tile,
                                  at.head};
-        // the next tile, the next head's first, or the next request's with rows: looked for among 64 at once, as thousands
-        // that bring nothing may lie between two (3 requests of one token over 80000, a thousand unused ones between them:
-        // 60 us; looked at one by one 418)
-        const long local = uniform(st.local) + seg;
-        const bool more = local < q.cost;
-        int nb = b;
-        if (!more && u + seg < u1) {
-          for (++nb; nb < A.B; nb += 64) {
-            const Request next = nb + lane() < A.B ? request<R, KB>(A, nb + lane()) : Request{};
-            const uint64_t here = __ballot(next.cost > 0);
-            if (here) {
-              const int first = __builtin_ctzll(here);
-              if (lane() == first) st.q = next;
-              nb += first;
-              break;
-            }
-          }
+        // the next tile, the next head's first, or the next request's (if that brings none, the next one's with rows is looked
+        // for behind this tile)
+        long local = st.local + seg;
+        st.u = u + seg;
+        st.begun = 1;
+        if (local < q.cost) {
+          st.at = at.tile + 1 < q.tiles ? Unit{at.head, at.tile + 1, 0} : Unit{at.head + 1, 0, 0};
+        } else if (u + seg < u1) {
+          const Request n = b + 1 < A.B ? request<R, KB>(A, b + 1) : Request{};
+          local = 0;
+          st.q = n;
+          st.b = b + 1;
+          st.at = {0, 0, 0};
         }
-        if (threadIdx.x == 0) {
-          st.begun = 1;
-          st.u = nb < A.B ? u + seg : u1;
-          st.local = more ? local : 0;
-          st.b = nb;
-          st.at = !more ? Unit{0, 0, 0} : at.tile + 1 < q.tiles ? Unit{at.head, at.tile + 1, 0} : Unit{at.head + 1, 0, 0};
-        }
+        st.local = local;
       }
       if (keys > 0) {
         if (MIXED && q.tile_rows == kWideRows) {
@@ -1287,6 +1277,27 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
     }
     __syncthreads();
     if (uniform(st.u) >= uniform(st.u1)) break;
+    if (uniform(st.q.cost) == 0) {  // 64 at once: thousands that bring nothing may lie between two requests
+      if (uniform(wave()) == 0) {
+        int b = uniform(st.b) + 1;
+        for (; b < A.B; b += 64) {
+          const Request n = b + lane() < A.B ? request<R, KB>(A, b + lane()) : Request{};
+          const uint64_t here = __ballot(n.cost > 0);
+          if (here) {
+            const int first = __builtin_ctzll(here);
+            if (lane() == first) st.q = n;
+            b += first;
+            break;
+          }
+        }
+        if (threadIdx.x == 0) {
+          st.b = b;
+          if (b >= A.B) st.u = st.u1;
+        }
+      }
+      __syncthreads();
+      if (uniform(st.u) >= uniform(st.u1)) break;
+    }
   }
 }
 
