@@ -342,6 +342,7 @@ typedef struct tjev_gdn_paged_params {
   int64_t q_stride[2], gate_stride[2], out_stride[2]; /* elements: token, head */
   int64_t k_stride[3], v_stride[3]; /* elements: the caches' page, slot and head (attention, append) */
   int64_t k_new_stride[2], v_new_stride[2];           /* append: k's and v's token and head */
+  int64_t max_new;                  /* attention: the most new tokens of one request, 0: not known (see below) */
 } tjev_gdn_paged_params;
 
 /* Block tables and slot maps of a step: request b holds cached[b] tokens and brings new_tokens[b]
@@ -375,8 +376,9 @@ int tjev_gdn_paged_append(const tjev_gdn_paged_params* p, void* stream, const vo
  *   out = softmax(scale q k^T) v, times sigmoid(gate) when gate [tokens, heads, dim] is not null
  * with heads / kv_heads query heads to a key head. Keys without a page, or past the table's width, are left out; a row
  * without keys is 0. Rows of no request: see fill. What a cache holds in other places (NaN too) does not matter.
- * dim in multiples of 8 up to 256, table_width * page_size up to TJEV_GDN_MAX_KEYS; q, gate, out and the caches 16-byte aligned, with strides that keep
- * their rows so. The workspace (tjev_gdn_paged_workspace_bytes, 256-byte aligned) needs no
+ * dim in multiples of 8 up to 256, table_width * page_size up to TJEV_GDN_MAX_KEYS; q, gate, out and the caches 16-byte
+ * aligned, with strides that keep their rows so. max_new chooses kernels and nothing else: with 0 the requests are taken to
+ * bring a token each (those that no token is left for excepted). The workspace (tjev_gdn_paged_workspace_bytes, 256-byte aligned) needs no
  * clearing; calls that may overlap need one each. */
 #define TJEV_GDN_MAX_KEYS (0x7fffffff - 4096)
 size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p);

@@ -239,3 +239,36 @@ def test_caches_past_32_bits_are_refused(library, shape):
 def test_table_widths_past_32_bits_are_refused(library):
     with pytest.raises(ValueError, match="2\\^31"):
         _attend(q=torch.zeros(1, 4, 64), block_table=torch.zeros(1, 1, dtype=torch.int32).expand(1, FAR))
+
+
+# ---------------------------------------------------------------- the kernels chosen by what one request may bring
+def _workspace(**kw):
+    """Bytes of a bf16 call's workspace: tiles of 128 rows have eight times the places of those of 16."""
+    import ctypes
+
+    from tjev_amd import _lib
+
+    p = dict(tokens=64, requests=64, table_width=4096, pages=64, page_size=16, heads=16, kv_heads=4, dim=256, dtype=_lib.BF16, scale=1.0)
+    return _lib.load().tjev_gdn_paged_workspace_bytes(ctypes.byref(_lib.PagedParams(**{**p, **kw})))
+
+
+def test_unused_requests_do_not_count():
+    """More rows per token than a streamed tile holds: no batch is of streamed tiles, whatever places its table has."""
+    kw = dict(tokens=40, heads=20, kv_heads=1, dim=128)
+    assert _workspace(**kw, requests=64) == _workspace(**kw, requests=40) > _workspace(**{**kw, "heads": 8}, requests=40)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(256, 16, 4), (128, 32, 4), (64, 16, 4)])
+def test_the_most_new_tokens_choose(dim, heads, kv_heads):
+    kw = dict(dim=dim, heads=heads, kv_heads=kv_heads)
+    wide = _workspace(**kw, requests=1)
+    for requests in (2, 64, 256):
+        assert _workspace(**kw, requests=requests, max_new=64) == _workspace(**kw, requests=requests, max_new=10 ** 6) == wide
+        assert _workspace(**kw, requests=requests, max_new=1) < wide
+    assert _workspace(**kw, max_new=-1) == 0
+
+
+@pytest.mark.parametrize("max_new", [0, -1, 2 ** 31])
+def test_the_most_new_tokens_are_a_number_of_tokens(library, max_new):
+    with pytest.raises(ValueError, match="max_new"):
+        _attend(q=torch.zeros(1, 4, 64), max_new=max_new)

@@ -88,3 +88,31 @@ def test_gaps_of_unused_requests(new):
     near, far = (_us(c) for c in cases)
     print(f"{near:.1f} us side by side, {far:.1f} us apart", flush=True)
     assert far < 2 * near
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,lens,requests", [
+    (8, 2, 64, [(700, 6), (0, 1), (90, 40)], 60), (16, 4, 256, [(3000, 64)], 64), (40, 2, 128, [(50, 1), (600, 1)], 9),
+    (8, 1, 64, [(900, 3), (40, 1)], 300), (6, 3, 40, [(2000, 90), (5, 9)], 200), (4, 4, 200, [(77, 50), (1, 1)], 120),
+])
+def test_unused_requests_and_the_most_new_tokens(dtype, heads, kv_heads, dim, lens, requests):
+    """More places than tokens, and bounds on a request's tokens: the true one, none, and (which costs time alone) wrong ones."""
+    case = batch(torch.Generator().manual_seed(24), lens, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, gate=True)
+    want, room = attention64(*(case[x] for x in NAMES), gate=case["gate"])
+    case = _with_idle(case, [b * (requests - 1) // max(1, len(lens) - 1) for b in range(len(lens))], requests)
+    most = max(n for _, n in lens)
+    for max_new in (None, most, 1, 5, 10 ** 6):
+        print(f"attention {dtype} {heads}/{kv_heads} of {dim} {lens} in {requests} places, max_new={max_new}", flush=True)
+        compare(_attend(case, max_new=max_new), want, room)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 4, 256), (32, 4, 128), (32, 8, 64)])
+def test_a_prompt_among_unused_requests(heads, kv_heads, dim):
+    """64 tokens over 30000 in one of 256 places of a table, with their bound: less than 1.5 times their time alone in it (74 and
+    83 us at head dim 256; streamed, 283)."""
+    case = batch(torch.Generator().manual_seed(25), [(30000, 64)], heads=heads, kv_heads=kv_heads, dim=dim, page=64, extra_pages=0)
+    alone, among = ({n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in c.items()} for c in (case, _with_idle(case, [128], 256)))
+    print(f"attention of one prompt {heads}/{kv_heads} of {dim}", flush=True)
+    alone, among = _us(alone), _us(dict(among, max_new=64))
+    print(f"{alone:.1f} us alone, {among:.1f} us among unused requests", flush=True)
+    assert among < 1.5 * alone

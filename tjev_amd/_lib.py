@@ -105,7 +105,7 @@ class PagedParams(ctypes.Structure):
                 ("scale", ctypes.c_float),
                 *((n, ctypes.c_int64 * 2) for n in ("q_stride", "gate_stride", "out_stride")),
                 *((n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride")),
-                *((n, ctypes.c_int64 * 2) for n in ("k_new_stride", "v_new_stride"))]
+                *((n, ctypes.c_int64 * 2) for n in ("k_new_stride", "v_new_stride")), ("max_new", ctypes.c_int64)]
 
 
 class Merge(ctypes.Structure):

@@ -1307,16 +1307,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 // Few tiles have many parts each (one request of 16000 tokens, 4 key heads: 126): SLICED spreads a tile's results over
 // gridDim.y workgroups and its parts over two halves of each, 16 at a time in each; gridDim.x is then the most tiles there can
 // be, and a workgroup finds its one among the ranges' notes.
+// Tiles of which the host does not know whether they are few (a table's unused places count as one each): the ranges' notes are
+// counted, and each tile has an equal share of the workgroups where that is kShare or more (64 tokens over 30000 in one of
+// 64 places, 16/4 heads of 256: 81 us, with one workgroup per range 136; with a share of 4 or more, which decoding requests'
+// tiles have too, those of 20 requests take 66 us instead of 54).
 constexpr int kSlice = 128;  // results of four per workgroup
-template <int DT, bool SLICED>
-constexpr int join_threads() { return DT == 64 || SLICED ? 256 : 512; }
+constexpr int kShare = 32;
+template <int DT, Join J>
+constexpr int join_threads() { return DT == 64 || J == kJoinSliced ? 256 : 512; }
 template <int DT, int ROWS>
 constexpr int join_slices() { return ROWS * DT / 4 / kSlice; }
 
-template <class T, int DT, int ROWS, bool WIDE, bool SLICED>
-__device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, const float* first, const float* next, float (*sm)[kWideRows],
-                                          float (*sl)[kWideRows]) {
-  constexpr int NT = join_threads<DT, SLICED>(), NG = NT / ROWS;
+template <class T, int DT, int ROWS, bool WIDE, bool SLICED, int NT>
+__device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, const float* first, const float* next, int slice,
+                                          float (*sm)[kWideRows], float (*sl)[kWideRows]) {
+  constexpr int NG = NT / ROWS;
   constexpr int PG = SLICED ? NT / kSlice : 1, NE = SLICED ? 1 : ROWS * DT / 4 / NT;  // groups of parts; results of a thread
   static_assert(NG >= 1 && NE >= 1, "");
   // part p's slot: the range that the tile begins in holds part 0, the others follow two slots apart
@@ -1329,7 +1334,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   constexpr bool ROW = WIDE && !SLICED;
   constexpr int NR = ROW ? 1 : NE;
   static_assert(!ROW || (DT / 8 % NE == 0 && NE % 2 == 0), "a wave's pieces are of 32 rows");
-  const int x0 = SLICED ? blockIdx.y * kSlice + tid % kSlice : ROW ? wave() * NE * 64 + lane() : tid;
+  const int x0 = SLICED ? slice * kSlice + tid % kSlice : ROW ? wave() * NE * 64 + lane() : tid;
   constexpr int STEP = ROW ? 64 : NT;
   f32x4 acc[NE];
   int er[NR];  // their rows
@@ -1473,18 +1478,26 @@ __device__ __forceinline__ void join_tile(const AttnArgs& A, const Split& q, con
   }
 }
 
-template <class T, int DT, int NQ, bool MIXED, bool SLICED>
-__global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join(AttnArgs A) {
-  constexpr int R = 16 * NQ, NT = join_threads<DT, SLICED>();
+template <class T, int DT, int NQ, bool MIXED, Join J>
+__global__ __launch_bounds__((join_threads<DT, J>())) void k_attention_join(AttnArgs A) {
+  constexpr int R = 16 * NQ, NT = join_threads<DT, J>(), RUN = (kMostRanges + NT - 1) / NT;
   __shared__ float sm[NT / R][kWideRows], sl[NT / R][kWideRows];
   GDN_POISON_LDS(sm, sl);
   int range = blockIdx.x;
-  Split q;
-  if constexpr (SLICED) {  // the blockIdx.x-th of the ranges that left a note, all read at once
+  auto join = [&](const Split& q, auto sliced, int slice) {
+    const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (range + 1)) * A.slot;
+    if constexpr (MIXED) {
+      if (q.tile_rows == kWideRows) {
+        join_tile<T, DT, kWideRows, true, sliced.value, NT>(A, q, first, next, slice, sm, sl);
+        return;
+      }
+    }
+    if (!sliced.value || slice < join_slices<DT, R>()) join_tile<T, DT, R, false, sliced.value, NT>(A, q, first, next, slice, sm, sl);
+  };
+  if constexpr (J == kJoinSliced) {  // the blockIdx.x-th of the ranges that left a note, all read at once
     __shared__ int scount[NT / 64], sfound;
     __shared__ __align__(16) i32x4 snote[2];
     GDN_POISON_LDS(scount, sfound, snote);
-    constexpr int RUN = kMostRanges / NT;
     i32x4 note[RUN][2];
     int n = 0;
 #pragma unroll
@@ -1518,20 +1531,48 @@ __global__ __launch_bounds__((join_threads<DT, SLICED>())) void k_attention_join
     __syncthreads();
     range = uniform(sfound);
     if (range < 0) return;
-    q = *reinterpret_cast<const Split*>(snote);
-  } else {
-    q = *split_of(A, range);
-    if (q.parts < 2) return;
-  }
-  const float *first = A.part + (size_t)q.first * A.slot, *next = A.part + (size_t)(2 * (range + 1)) * A.slot;
-  if constexpr (MIXED) {
-    if (q.tile_rows == kWideRows) {
-      join_tile<T, DT, kWideRows, true, SLICED>(A, q, first, next, sm, sl);
+    join(*reinterpret_cast<const Split*>(snote), std::true_type{}, blockIdx.y);
+  } else if constexpr (J == kJoinCounted) {  // the ranges that left a note, in order, and how many workgroups each may have
+    __shared__ int scount[RUN][NT / 64], swhere[kMostRanges];
+    GDN_POISON_LDS(scount, swhere);
+    uint64_t noted[RUN];
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      const int r = i * NT + threadIdx.x;
+      const int parts = split_of(A, r < A.G ? r : 0)->parts;
+      noted[i] = __ballot(r < A.G && parts > 1);
+      if (lane() == 0) scount[i][wave()] = __builtin_popcountll(noted[i]);
+    }
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < RUN; ++i)
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) {
+        if (w == wave() && (noted[i] >> lane() & 1)) swhere[n + __builtin_popcountll(noted[i] & ((1ull << lane()) - 1))] = i * NT + threadIdx.x;
+        n += scount[i][w];
+      }
+    __syncthreads();
+    n = uniform(n);
+    const int share = n ? A.G / n : 0;
+    const int k = share >= kShare ? (int)blockIdx.x / share : (int)blockIdx.x;
+    if (k >= n) return;
+    range = uniform(swhere[k]);
+    const Split q = *split_of(A, range);
+    if (share < kShare) {
+      join(q, std::false_type{}, 0);
       return;
     }
+    const int slices = MIXED && q.tile_rows == kWideRows ? join_slices<DT, kWideRows>() : join_slices<DT, R>();
+    for (int slice = (int)blockIdx.x % share; slice < slices; slice += share) {
+      join(q, std::true_type{}, slice);
+      __syncthreads();
+    }
+  } else {
+    const Split q = *split_of(A, range);
+    if (q.parts < 2) return;
+    join(q, std::false_type{}, 0);
   }
-  if (SLICED && (int)blockIdx.y >= join_slices<DT, R>()) return;
-  join_tile<T, DT, R, false, SLICED>(A, q, first, next, sm, sl);
 }
 
 }  // namespace

@@ -2,6 +2,8 @@
 // gdn_attention.h, their units in gdn_attn_inst.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/tjev_gdn.h"
 #include "gdn_launch.h"
 #include "gdn_paged.h"
@@ -18,23 +20,31 @@ int ranges_of(const tjev_gdn_paged_params* p) { return p->dtype == TJEV_GDN_BF16
 AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   const bool bf = p->dtype == TJEV_GDN_BF16;
   const int dt = p->dim <= 64 ? 64 : p->dim <= 128 ? 128 : 256;
-  const long g = p->heads / p->kv_heads, rows = p->tokens * g, mean = (rows + p->requests - 1) / p->requests;
+  const long g = p->heads / p->kv_heads, rows = p->tokens * g;
+  // Requests that bring a token, at most: a table may have places for many more. The most rows of one request: the caller's
+  // bound, or what is left when the others bring one token each (a batch with fewer tokens than that would bring is taken for
+  // decoding requests alone, which the streaming kernel serves 1 to 3% faster at head dims up to 128, 5 to 15% at 256; the
+  // bound tells 64 tokens of one request of 64 from them: over 30000, 16/4 heads of 256, 81 us instead of 283).
+  const long active = std::max<long>(1, std::min<long>(p->tokens, p->requests)), mean = (rows + active - 1) / active;
+  const long top = (p->max_new ? std::min<long>(p->max_new, p->tokens) : p->tokens - active + 1) * g;
   AttnPlan r;
   // Streamed tiles of 32 rows instead of 16 where the registers hold them without a loss. In bf16 at head dims up to 64 for
-  // requests of 17 to 32 on average, which would else take a tile of 128 (32 requests of 5 tokens over 8192, 32/8 heads of
-  // 64: 33.7 us, with that 39.0; one request 18.2, 21.8; at 128 the tile of 128 is the faster one, 63 against 69). In fp32
-  // up to 128 where there are enough of them (2 requests of 910 tokens after 858, 4/1 heads of 128: 50.5 us, with
-  // 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6).
-  r.nq = mean > 16 && (bf ? dt == 64 && mean <= 32 : dt <= 128 && rows / 32 * p->kv_heads >= 128) ? 2 : 1;
-  r.mixed = bf && (p->tokens - p->requests + 1) * g > 16 * r.nq;
+  // requests of 17 to 32 on average (or at most, where the caller says so), which would else take a tile of 128 (32 requests of
+  // 5 tokens over 8192, 32/8 heads of 64: 33.7 us, with that 39.0; one request 18.2, 21.8; at 128 the tile of 128 is the
+  // faster one, 63 against 69). In fp32 up to 128 where there are enough of them (2 requests of 910 tokens after 858, 4/1 heads
+  // of 128: 50.5 us, with 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6).
+  auto few = [](long n) { return n > 16 && n <= 32; };
+  r.nq = (bf ? dt == 64 && (few(mean) || (p->max_new && few(top))) : mean > 16 && dt <= 128 && rows / 32 * p->kv_heads >= 128) ? 2 : 1;
+  r.mixed = bf && top > 16 * r.nq;
   const int kb = bf ? 128 : 64;
   // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
-  const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + p->requests) * p->kv_heads;
+  const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + active) * p->kv_heads;
   const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb + kWideExtra + kGateExtra;
   const int most = ranges_of(p);
   r.G = tiles >= most || blocks * tiles >= most ? most : (int)(blocks * tiles);
-  // so few tiles that a workgroup each would leave most CUs idle, and take parts by the dozen
-  r.sliced = tiles <= (r.mixed ? 16 : 64);
+  // so few tiles that a workgroup each would leave most CUs idle, and take parts by the dozen; or rows for so few, in a batch
+  // whose other requests may bring none
+  r.join = tiles <= (r.mixed ? 16 : 64) ? kJoinSliced : r.mixed && p->max_new && rows / kWideRows * p->kv_heads <= 16 ? kJoinCounted : kJoinRanges;
   r.tiles = (int)(tiles < (1l << 30) ? tiles : 1l << 30);
   r.slot = (long)(r.mixed ? kWideRows : 16 * r.nq) * (dt + 2);
   r.bytes = (size_t)r.G * (2 * r.slot * sizeof(float) + kSplitBytes);
@@ -43,8 +53,8 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
 
 int validate(const tjev_gdn_paged_params* p) {
   if (!p) return fail(TJEV_GDN_EINVAL, "null params");
-  if (p->requests < 1 || p->table_width < 1 || p->pages < 1 || p->page_size < 1 || p->tokens < 0)
-    return fail(TJEV_GDN_EINVAL, "requests, table_width, pages and page_size must be positive, tokens not negative");
+  if (p->requests < 1 || p->table_width < 1 || p->pages < 1 || p->page_size < 1 || p->tokens < 0 || p->max_new < 0)
+    return fail(TJEV_GDN_EINVAL, "requests, table_width, pages and page_size must be positive, tokens and max_new not negative");
   if (p->kv_heads < 1 || p->heads < 1 || p->heads % p->kv_heads)
     return fail(TJEV_GDN_EINVAL, "the query heads must be groups of the key heads");
   if ((p->dtype | 1) != 1) return fail(TJEV_GDN_EINVAL, "dtype must be TJEV_GDN_F32 or TJEV_GDN_BF16");

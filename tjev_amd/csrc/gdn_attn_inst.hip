@@ -13,10 +13,13 @@ hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   A.wide_extra = kWideExtra + (A.gate ? kGateExtra : 0);
   hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);
   constexpr int slices = join_slices<DT, MIXED ? kWideRows : 16 * NQ>();
-  if (r.sliced) {
-    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, true>), dim3(r.tiles, slices), dim3(join_threads<DT, true>()), 0, st, A);
+  if (r.join == kJoinSliced) {
+    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, kJoinSliced>), dim3(r.tiles, slices), dim3(join_threads<DT, kJoinSliced>()), 0, st, A);
+  } else if (MIXED && r.join == kJoinCounted) {
+    if constexpr (MIXED)
+      hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, kJoinCounted>), dim3(r.G), dim3(join_threads<DT, kJoinCounted>()), 0, st, A);
   } else {
-    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, false>), dim3(r.G), dim3(join_threads<DT, false>()), 0, st, A);
+    hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, kJoinRanges>), dim3(r.G), dim3(join_threads<DT, kJoinRanges>()), 0, st, A);
   }
   return hipGetLastError();
 }

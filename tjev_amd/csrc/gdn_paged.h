@@ -178,10 +178,13 @@ struct AttnArgs : Batch {
 constexpr int kMostRanges = 768;
 constexpr int kSplitBytes = 32;  // of the workspace, per range: the tile that goes on behind it
 
+// How the parts of tiles are joined: a workgroup per range, several per tile, or as many as there are for the tiles found
+enum Join : int { kJoinRanges, kJoinSliced, kJoinCounted };
+
 struct AttnPlan {
   int nq;            // streamed tiles of 16 nq rows
   bool mixed;        // wide tiles too
-  bool sliced;       // few tiles: their parts joined by several workgroups each
+  Join join;
   int tiles;         // the most there can be, up to 2^30
   int G;             // ranges
   long slot;         // floats of a workspace slot

@@ -159,7 +159,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 
 @functools.lru_cache(maxsize=256)
 def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_dtype, vc_shape, vc_stride, vc_dtype, t_shape, t_dtype,
-                      s_shape, s_dtype, l_shape, l_dtype, gate, out, scale, devices):
+                      s_shape, s_dtype, l_shape, l_dtype, gate, out, scale, max_new, devices):
     """The library's view of a call (a reference to the struct; never changed) and its workspace. gate and out: their
     (shape, stride, dtype), or None."""
     if len(q_shape) != 3 or q_dtype not in _DTYPES or kc_dtype != q_dtype:
@@ -187,11 +187,13 @@ def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_d
             raise ValueError(f"{name} {tuple(t[0])} {t[2]} is not like q {tuple(q_shape)} {q_dtype}")
     if out is not None and (out[1][-1] != 1 or any(s == 0 and n > 1 for s, n in zip(out[1], out[0]))):
         raise ValueError("out's last dim must be contiguous, and none expanded")
+    if max_new is not None and not 1 <= max_new < 1 << 31:
+        raise ValueError(f"max_new is a number of tokens, not {max_new}")
     _lib.one_gpu("paged_attention", devices)
     p = _lib.PagedParams(tokens, requests, t_shape[1], kc_shape[0], kc_shape[1], heads, kv_heads, dim, _DTYPES[q_dtype], int(out is None),
                          dim ** -0.5 if scale is None else scale, _strides(q_shape, q_stride),
                          (0, 0) if gate is None else _strides(*gate[:2]), (heads * dim, dim) if out is None else _strides(*out[:2]),
-                         _strides(kc_shape, kc_stride), _strides(vc_shape, vc_stride))
+                         _strides(kc_shape, kc_stride), _strides(vc_shape, vc_stride), max_new=max_new or 0)
     return ctypes.byref(p), lib.tjev_gdn_paged_workspace_bytes(ctypes.byref(p))
 
 
@@ -206,16 +208,21 @@ def _like(x: torch.Tensor | None):
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     starts: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
-                    gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    gate: torch.Tensor | None = None, out: torch.Tensor | None = None, max_new: int | None = None) -> torch.Tensor:
     """Causal attention of the batch's new tokens over the paged cache, which holds their own keys and
     values already: one token per request, chunks of prompts, or both in one call.
 
     q [N, heads, dim] (heads: groups of kv_heads; dim in multiples of 8 up to 256): rows starts[b] ..
     starts[b + 1] - 1 are the last tokens of request b, whose keys are ``lengths[b]`` in all, in the pages of row b of
     ``block_table`` [B, M] int32. Each attends to the keys up to its own, softmax(scale q k^T) v with scale
-    dim^-1/2 by default, in 32 bits; a row without keys is 0. (In bf16 the weights of a request with more than 32
-    tokens times query heads per key head, or 16, are rounded to bf16 for their product with v.) ``gate`` [N, heads, dim]
-    multiplies the result by its sigmoid. Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
+    dim^-1/2 by default, in 32 bits; a row without keys is 0. ``gate`` [N, heads, dim] multiplies the result by its sigmoid.
+    Rows of no request (a padded batch) come back 0, or, with ``out`` given, are left as they were.
+    ``max_new``: the most new tokens of one request, where the caller knows; it chooses kernels and no row's keys. By default
+    every request is taken to bring one token at least, so a batch whose table has unused places, and whose tokens are no more
+    than its places, is served as decoding requests: right, but a prompt in it takes up to four times as long.
+    (In bf16 the kernel for many rows rounds the weights to bf16 for their product with v. It takes the requests of more than 16
+    tokens times query heads per key head, 32 at head dims up to 64 where the average or max_new is 17 to 32 of them, of
+    batches that may hold one by max_new or the default.)
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
     _lib.not_recorded("paged_attention")
@@ -226,7 +233,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     p, need = _attention_params(
         lib, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,
         block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, _like(gate), _like(out),
-        None if scale is None else float(scale),
+        None if scale is None else float(scale), None if max_new is None else int(max_new),
         (q.get_device(), k_cache.get_device(), v_cache.get_device(), block_table.get_device(), starts.get_device(), lengths.get_device(),
          _device(gate, q), _device(out, q)))
     starts, lengths, block_table, dev = _int32(starts), _int32(lengths), block_table.contiguous(), q.device
