@@ -1,7 +1,9 @@
-"""The paged cache's operators (tjev_amd.paged) called in ways that a served batch comes to: views off 16 bytes, against their
-plain 64-bit forms (tests/paged_cases.py)."""
+"""The paged cache's operators (tjev_amd.paged) called in ways that a served batch comes to: views off 16 bytes, tables with
+unused places, several streams, workspaces that hold anything; against their plain 64-bit forms (tests/paged_cases.py)."""
 
 from __future__ import annotations
+
+import ctypes
 
 import pytest
 import torch
@@ -116,3 +118,103 @@ def test_a_prompt_among_unused_requests(heads, kv_heads, dim):
     alone, among = _us(alone), _us(dict(among, max_new=64))
     print(f"{alone:.1f} us alone, {among:.1f} us among unused requests", flush=True)
     assert among < 1.5 * alone
+
+
+# tiles of few rows and of many, whose parts are joined by several workgroups each, by one, and by as many as there are
+SPLIT = {
+    "streamed, few": ([(9000, 1)], 8, 2, 128, None, 0), "streamed, many": ([(900, 1)] * 70, 8, 2, 128, None, 0),
+    "wide, few": ([(3000, 64)], 16, 4, 256, None, 0), "wide, many": ([(1500, 70)] * 6, 16, 4, 128, None, 0),
+    "wide, counted": ([(3000, 64)], 16, 4, 256, 64, 64), "wide, counted, many": ([(700, 1)] * 40 + [(2000, 64)], 16, 4, 64, 64, 0),
+}
+
+
+def _split(kind, dtype=BF):
+    lens, heads, kv_heads, dim, max_new, requests = SPLIT[kind]
+    case = batch(torch.Generator().manual_seed(26), lens, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, gate=True)
+    if requests:
+        case = _with_idle(case, [requests // 2], requests)
+    return {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in dict(case, max_new=max_new).items()}
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("kind", sorted(SPLIT))
+def test_poisoned_workspace(monkeypatch, dtype, kind):
+    """The poison mode, and a workspace and an output that hold anything: the same bits."""
+    case = _split(kind, dtype)
+    print(f"poisoned workspace: {kind} {dtype}", flush=True)
+    want = _attend(case)
+    assert bool(torch.isfinite(want).all())
+    monkeypatch.setenv("TJEV_GDN_POISON", "1")
+    assert torch.equal(_attend(case), want)
+    monkeypatch.delenv("TJEV_GDN_POISON")
+    empty = torch.empty
+
+    def filled(*args, **kw):
+        x = empty(*args, **kw)
+        return x.fill_(0xFF) if x.dtype == torch.uint8 else x  # the workspace: NaN, and notes of -1 parts
+
+    monkeypatch.setattr(torch, "empty", filled)
+    out = torch.full_like(want, float("nan"))
+    assert torch.equal(_attend(case, out=out), want)
+
+
+def test_poison_reaches_the_workspace(monkeypatch):
+    """All of it but the ranges' notes, which are numbers."""
+    from tjev_amd import _lib, paged
+
+    case = _split("streamed, few")
+    lib, held = _lib.load(), {}
+    real = paged._attention_params
+
+    def keep(*args):
+        held["p"], held["need"] = real(*args)
+        return held["p"], held["need"]
+
+    monkeypatch.setattr(paged, "_attention_params", keep)
+    want = _attend(case)
+    ws, out = torch.zeros(held["need"], dtype=torch.uint8, device="cuda"), torch.empty_like(want)
+    monkeypatch.setenv("TJEV_GDN_POISON", "1")
+    print("poison in the workspace", flush=True)
+    _lib.check_status(lib.tjev_gdn_paged_attention(
+        held["p"], ctypes.c_void_p(_lib.current_stream(ws.device)), *(case[n].data_ptr() for n in NAMES), case["gate"].data_ptr(),
+        out.data_ptr(), ws.data_ptr(), held["need"]))
+    assert torch.equal(out, want)
+    # ranges of two places of 16 rows (results, maximum, sum) and a note; places that no part went to are left NaN
+    place, note = 16 * (128 + 2) * 4, 32
+    notes = held["need"] // (2 * place + note) * note
+    assert bool(torch.isnan(ws[:-notes].view(torch.float32)).any()) and not bool((ws[-notes:].view(torch.int32) == 0x7FC00000).any())
+
+
+@pytest.mark.parametrize("kinds", [("streamed, few", "wide, few"), ("wide, many", "wide, counted"), ("streamed, many", "streamed, many")])
+def test_two_calls_at_once(kinds):
+    """Calls queued on two streams without a wait between them, and graphs replayed on both at once: a workspace of its own each."""
+    cases = [_split(k) for k in kinds]
+    want = [_attend(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    print(f"two calls at once: {kinds}", flush=True)
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(12):
+        for s, c, g in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                g.append(_attend(c))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(x, w) for x in g)
+    graphs = []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ys = [_attend(c) for _ in range(3)]
+        graphs.append((graph, ys))
+    for _ in range(3):
+        for _, ys in graphs:
+            for y in ys:
+                y.zero_()
+        torch.cuda.synchronize()
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for w, (_, ys) in zip(want, graphs):
+            assert all(torch.equal(y, w) for y in ys)

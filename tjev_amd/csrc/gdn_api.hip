@@ -313,7 +313,7 @@ void prof_mark(void*, int kernel, int end, hipStream_t st) {
 const gdn::Timer g_timer{prof_mark, nullptr};
 
 // ---- the poison debug mode: with TJEV_GDN_POISON=1 in the environment, every forward fills its
-// workspace and residual buffer, and every backward its workspace, with NaN on the stream before
+// workspace and residual buffer, every backward its workspace, and paged attention its parts, with NaN on the stream before
 // its kernels run, so a read of memory the kernels did not write reaches the outputs (the
 // reference's interpret mode poisons uninitialised scratch the same way)
 __global__ void k_poison(uint32_t* p, size_t n) {
@@ -362,6 +362,7 @@ int run_v2(const tjev_gdn_params* p, void* stream, gdn::GdnArgs& A, int backward
 namespace gdn {
 int fail(int status, const char* msg) { return ::fail(status, msg); }
 const Timer* active_timer() { return g_prof.on ? &g_timer : nullptr; }
+int poison_workspace(void* ptr, size_t bytes, void* stream) { return poison_on() ? poison(ptr, bytes, stream) : 0; }
 }  // namespace gdn
 
 extern "C" {

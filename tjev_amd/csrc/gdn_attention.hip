@@ -123,6 +123,8 @@ int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const
   if (any % 16) return fail(TJEV_GDN_EINVAL, "q, gate, out and the caches must be 16-byte aligned, with strides that keep their rows so");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const gdn::AttnPlan plan = gdn::plan_of(p);
+  // (the parts: the ranges' notes behind them, which say how many there are, are never NaN)
+  if (int s = gdn::poison_workspace(workspace, plan.bytes - (size_t)plan.G * gdn::kSplitBytes, stream)) return s;
   using gdn::AttnArgs;
   hipError_t (*const unit[2][3])(const gdn::AttnPlan&, AttnArgs&, hipStream_t) = {
       {gdn::attention_f32_64, gdn::attention_f32_128, gdn::attention_f32_256},

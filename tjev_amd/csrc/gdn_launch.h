@@ -35,6 +35,8 @@ struct ShapeTable {
 // for tjev_gdn_last_error(), and the timing hook while profiling is on (else null).
 int fail(int status, const char* msg);
 const Timer* active_timer();
+// in the poison debug mode (TJEV_GDN_POISON=1): NaN into a workspace, before the kernels that use it. A status code.
+int poison_workspace(void* ptr, size_t bytes, void* stream);
 
 #define GDN_SHAPE(c, d) const ShapeTable* table_##c##_##d();
 #include "gdn_shapes.def"
