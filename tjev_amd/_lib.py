@@ -287,26 +287,30 @@ def one_gpu(what: str, devices) -> None:
 def not_recorded(what: str) -> None:
     """Raises where torch records the calls of its operators to run them again (jit tracing, make_fx): a launch by address is none
     of them, and the record would hold its output uninitialised. (torch.compile leaves these calls out of its graphs, and
-    runs them as they are.)"""
-    if (torch.jit.is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None
-            or _len_torch_dispatch_stack_pre_dispatch() > 0):
-        raise RuntimeError(f"{what} is a launch of the HIP library and cannot be recorded (jit tracing, make_fx)")
+    runs them as they are.) make_fx puts a mode on one of torch's stacks; which it is is asked only where there is one."""
+    if _is_tracing() or _dispatch_modes() or _function_modes():
+        if (_is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+                or _len_torch_dispatch_stack_pre_dispatch() > 0):
+            raise RuntimeError(f"{what} is a launch of the HIP library and cannot be recorded (jit tracing, make_fx)")
 
 
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _dispatch_modes, _function_modes = (
+    torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack)
 
 
 def inference_only(what: str, *tensors) -> None:
     """Raises where one of the tensors (or None) carries a derivative, which ``what`` would lose: it requires a gradient while
-    gradients are recorded, or has a tangent."""
-    if torch.is_grad_enabled():
-        for x in tensors:
-            if x is not None and x.requires_grad:
-                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or with detached tensors")
-    if forward_ad._current_level >= 0:
-        for x in tensors:
-            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
-                raise RuntimeError(f"{what} has no gradient: call it with tensors without tangents")
+    gradients are recorded, or has a tangent. Asked only where one may (the operators look at requires_grad and
+    ``dual_level`` themselves, which is a third of this call's time)."""
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or with detached tensors")
+    if dual_level() and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it with tensors without tangents")
+
+
+def dual_level() -> bool:
+    """Whether tensors may have tangents."""
+    return forward_ad._current_level >= 0
 
 
 def on_device(device: torch.device):

@@ -145,8 +145,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     slots [N] of the caches, in place. Slots outside the cache (-1) are skipped. The slots of one call are
     distinct: of two tokens with one slot, either's values or parts of both remain."""
     _lib.not_recorded("paged_append")
-    _lib.inference_only("paged_append", k, v, k_cache, v_cache)
-    k, v = (x if x.dim() != 3 or x.stride(-1) == 1 else x.contiguous() for x in (k, v))
+    if _lib.dual_level() or (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad
+                                                          or v_cache.requires_grad)):
+        _lib.inference_only("paged_append", k, v, k_cache, v_cache)
+    if k.dim() == 3 and k.stride(-1) != 1:
+        k = k.contiguous()
+    if v.dim() == 3 and v.stride(-1) != 1:
+        v = v.contiguous()
     p = _append_params(
         k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
         v_cache.stride(), v_cache.dtype, slots.shape, slots.dtype,
@@ -226,9 +231,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
     _lib.not_recorded("paged_attention")
-    _lib.inference_only("paged_attention", q, k_cache, v_cache, gate, out)
+    if _lib.dual_level() or (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (
+            gate is not None and gate.requires_grad) or (out is not None and out.requires_grad))):
+        _lib.inference_only("paged_attention", q, k_cache, v_cache, gate, out)
     # (contiguous() would leave a contiguous view that starts off 16 bytes where it is)
-    q, gate = (x if x is None or x.dim() != 3 or _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, gate))
+    if q.dim() == 3 and not _aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if gate is not None and gate.dim() == 3 and not _aligned(gate):
+        gate = gate.clone(memory_format=torch.contiguous_format)
     lib = _lib.load()
     p, need = _attention_params(
         lib, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,

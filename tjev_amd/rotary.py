@@ -18,7 +18,6 @@ import functools
 import math
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -116,7 +115,7 @@ class _Rotary(torch.autograd.Function):
 def _turned(q, k, positions, inv_freq, options, inverse: bool):
     """The launch, through its Function where q or k may carry a derivative: a gradient, or (whatever the grad mode) a tangent,
     which the Function refuses. Elsewhere without it, which is some us of host time."""
-    if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+    if _lib.dual_level() or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
         return _Rotary.apply(q, k, positions, inv_freq, options, inverse)
     return _launch(q, k, positions, inv_freq, *options, inverse)
 
