@@ -1278,6 +1278,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
     __syncthreads();
     if (uniform(st.u) >= uniform(st.u1)) break;
     if (uniform(st.q.cost) == 0) {  // 64 at once: thousands that bring nothing may lie between two requests
+      __syncthreads();  // all waves have seen it
       if (uniform(wave()) == 0) {
         int b = uniform(st.b) + 1;
         for (; b < A.B; b += 64) {
