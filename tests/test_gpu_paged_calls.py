@@ -93,6 +93,21 @@ def test_gaps_of_unused_requests(new):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(32, 2, 200, 1), (8, 2, 64, 16), (16, 4, 256, 16)])
+def test_unused_requests_between_others(dtype, heads, kv_heads, dim, page):
+    """Every second to fifth request unused, and ranges that go on behind them: right, and the same bits every time."""
+    lens = [((b * 37) % 340, 0 if b % 5 in (0, 3) or b % 7 == 2 else 1 + (b * b) % 9) for b in range(90)]
+    case = batch(torch.Generator().manual_seed(27), lens, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype)
+    print(f"attention between unused requests {dtype} {heads}/{kv_heads} of {dim} page={page}", flush=True)
+    want, room = attention64(*(case[x] for x in NAMES))
+    case = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in case.items()}
+    got = _attend(case)
+    compare(got, want, room)
+    for _ in range(50):
+        assert torch.equal(_attend(case), got)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("heads,kv_heads,dim,lens,requests", [
     (8, 2, 64, [(700, 6), (0, 1), (90, 40)], 60), (16, 4, 256, [(3000, 64)], 64), (40, 2, 128, [(50, 1), (600, 1)], 9),
     (8, 1, 64, [(900, 3), (40, 1)], 300), (6, 3, 40, [(2000, 90), (5, 9)], 200), (4, 4, 200, [(77, 50), (1, 1)], 120),
