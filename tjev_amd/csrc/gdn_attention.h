@@ -10,12 +10,13 @@
 // tile that more than one range holds leaves its parts in the workspace for a second launch to join
 // (k_attention_join). Two launches whatever the lengths, which only the GPU knows.
 //
-// Measured, bf16, with a gate but for the first, of several cards (floors: the cache and rows at 5.12 TB/s, the products at 1230 TFLOP/s, what a
-// large copy and a large library product reach on the same card):
-//   1 token over 4000, 16/4 heads of 256 (16 MB)                    16.5 us   floor   3.2   two launches' latency
-//   64 requests of up to 32768, 16/4 heads of 256 (1.57 GB)        300            307    memory, 5.2 TB/s
-//   2048 tokens over 30000, 16/4 heads of 256 (1.04 TFLOP)        1100 to 1155    846    products, 900 to 945 TFLOP/s
-//   a prompt of 4096, 32/4 heads of 256 (0.27 TFLOP)               344 to 366     224    products, 750 to 800 TFLOP/s
+// Measured, bf16, with a gate but for the first, of several cards (beside the time that the cache and rows take at 5.12 TB/s, or the
+// products at 1230 TFLOP/s: what a large copy and a large library product reach on the same card):
+//   1 token over 4000, 16/4 heads of 256 (16 MB)                    16.5 us     3.2   two launches' latency
+//   64 requests of up to 32768, 16/4 heads of 256 (1.57 GB)        300        307     memory, 5.2 TB/s
+//   2048 tokens over 30000, 16/4 heads of 256 (1.04 TFLOP)        1100 to 1155  846   products, 900 to 945 TFLOP/s
+//   a prompt of 4096, 32/4 heads of 256 (0.27 TFLOP)               344 to 366 224     products, 750 to 800 TFLOP/s, and the 1024
+//                                                                                   tiles' starts and ends beside them
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,7 +34,7 @@ constexpr int kThreads = 256;
 constexpr float kNegInf = -__builtin_inff();
 
 // ---------------------------------------------------------------- the stream's plan
-// All units of a batch (gdn_paged.h) in a line (request, tile, key head, keys) are cut into G equal ranges, one
+// All units of a batch (gdn_paged.h) in a line (request, key head, tile, keys) are cut into G equal ranges, one
 // per workgroup, so that requests of very different lengths keep every CU busy to the end, whatever
 // the host knows of them.
 
@@ -936,10 +937,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
     for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int x = 0; x < 16; ++x) s[n][x] = 0.f;
-    // Fragments are read AHEAD products before their own: left to itself the compiler reads them all first, which
     // Fragments are read AHEAD - 1 products before their own: left to itself the compiler reads them all first, which
     // runs it out of registers. At head dim 256 a fragment has one product, not two, to hide the next one's read
-    // (2048 new tokens over 30000, 16/4 heads: 1192 us with 2, 1165 with 4, 1333 with 6, which spills).
+    // (2048 new tokens over 30000, 16/4 heads: 1192 us with AHEAD = 2, 1165 with 4, 1333 with 6, which spills).
     constexpr int AHEAD = DT == 256 ? 4 : 2;
     bf16x8 kf[AHEAD][NS];
     auto read_k = [&](int i) {
@@ -1305,13 +1305,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 // The tiles that more than one range holds: their parts joined, one workgroup per range. Bound by latency (few rows)
 // or memory (wide tiles): the maxima and sums of all parts are read at once, the results as many at a time as the
 // registers hold.
-// Few tiles have many parts each (one request of 16000 tokens, 4 key heads: 126): SLICED spreads a tile's results over
+// Few tiles have many parts each (one request of 16000 tokens, 4 key heads: 126): kJoinSliced spreads a tile's results over
 // gridDim.y workgroups and its parts over two halves of each, 16 at a time in each; gridDim.x is then the most tiles there can
 // be, and a workgroup finds its one among the ranges' notes.
-// Tiles of which the host does not know whether they are few (a table's unused places count as one each): the ranges' notes are
-// counted, and each tile has an equal share of the workgroups where that is kShare or more (64 tokens over 30000 in one of
-// 64 places, 16/4 heads of 256: 81 us, with one workgroup per range 136; with a share of 4 or more, which decoding requests'
-// tiles have too, those of 20 requests take 66 us instead of 54).
+// Tiles of which the host does not know whether they are few (a table's unused places count as one each): the ranges' notes
+// are counted (kJoinCounted), and each tile has an equal share of the workgroups where that is kShare or more (64 tokens over
+// 30000 in one of 64 places, 16/4 heads of 256: 81 us, with one workgroup per range 136; with a share of 4 or more, which
+// decoding requests' tiles have too, those of 20 requests take 66 us instead of 54).
 constexpr int kSlice = 128;  // results of four per workgroup
 constexpr int kShare = 32;
 template <int DT, Join J>
