@@ -387,6 +387,91 @@ int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const
                              const int32_t* starts, const int32_t* lengths, const void* gate,
                              void* out, void* workspace, size_t workspace_bytes);
 
+/* The same for trees of new tokens (drafts): a row attends to all keys before its request's new tokens and, of those, to the
+ * ones named by its bits: bit j % 64 of ancestors[row, j / 64] (int64 [tokens, words]; see tjev_gdn_draft_tree) is the request's new token j,
+ * whose key stands at lengths[b] - (starts[b + 1] - starts[b]) + j. A row may name any of them, or none; tokens from 64 words on cannot
+ * be named. All else as above, the workspace too. */
+int tjev_gdn_paged_tree_attention(const tjev_gdn_paged_params* p, void* stream, const void* q,
+                                  const void* k_cache, const void* v_cache,
+                                  const int32_t* block_table, const int32_t* starts,
+                                  const int32_t* lengths, const int64_t* ancestors, int32_t words,
+                                  const void* gate, void* out, void* workspace,
+                                  size_t workspace_bytes);
+
+/* ---- Drafted tokens (no counterpart in the megakernel) ----
+ *
+ * A request's new tokens are a tree: parents[starts[b] + i] is the number within the request of token i's parent, less than i;
+ * anything else: none (the request's cached tokens are all that stands before it). Token 0, the root, is the one that the
+ * last step sampled. Of each request the first max_new tokens are looked at. */
+typedef struct tjev_gdn_draft_params {
+  int64_t tokens;                       /* rows of the batch */
+  int64_t max_new;                      /* the most tokens of a request */
+  int64_t target_stride, draft_stride;  /* verification: elements from row to row */
+  int32_t requests, vocab, dtype;       /* verification: tjev_gdn_dtype of the probabilities */
+  int32_t reserved;
+} tjev_gdn_draft_params;
+
+/* ancestors [tokens, ceil(max_new / 64)] int64: bit j % 64 of word j / 64 of row i is set for its request's token j = i and its
+ * ancestors; positions [tokens] int32: the request's cached tokens (lengths[b] - its new ones, 0 if that is negative) + how many
+ * ancestors there are. 0 in rows of no request and of tokens from max_new on. */
+int tjev_gdn_draft_tree(const tjev_gdn_draft_params* p, void* stream, const int32_t* parents,
+                        const int32_t* starts, const int32_t* lengths, int64_t* ancestors,
+                        int32_t* positions);
+
+/* Which drafted tokens are kept, and one token more. target [tokens, vocab]: row i is the target model's distribution behind token i;
+ * tokens [tokens] (of the roots: not read); uniforms [tokens] in [0, 1). From the root on, the children c of the node r reached are
+ * looked at in order; c is accepted if uniforms[c] * (1 - target[r] of the siblings before it, each token once) < target[r, x_c]; with
+ * draft [tokens, vocab] (row c: the distribution that token c was drawn from; parents must be null) if uniforms[c] * draft[c, x_c] <
+ * target[r, x_c]. parents null: chains (i - 1). Behind the last accepted token one is drawn: the first v whose running sum of the
+ * weights is over uniforms[root] times their whole, in 64 bits; the weights are target[r] with 0 for its rejected children's tokens, or
+ * max(target[r] - draft[c], 0) for the rejected child c; target[r] itself where that leaves nothing; -1 where that has nothing either.
+ * Probabilities that are no positive finite number count as 0, tokens outside 0 .. vocab - 1 are not accepted.
+ *   tokens_out [requests, max_new] int32   the accepted tokens, then the drawn one; -1 behind
+ *   path       [requests, max_new] int32   the numbers of the kept tokens, the root first; -1 behind
+ *   kept       [requests] int32            how many (of both; 0 for a request without tokens)
+ * The workspace (256-byte aligned) needs no clearing. */
+size_t tjev_gdn_verify_workspace_bytes(const tjev_gdn_draft_params* p);
+int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const int32_t* tokens,
+                           const int32_t* parents, const int32_t* starts, const float* uniforms,
+                           const void* target, const void* draft, int32_t* tokens_out,
+                           int32_t* path, int32_t* kept, void* workspace, size_t workspace_bytes);
+
+/* ---- Who holds the cache's pages ---- k_caches and v_caches: host arrays of `layers` addresses (0: the tables alone), caches of
+ * the same layout, as in tjev_gdn_paged_params. */
+typedef struct tjev_gdn_pages_params {
+  int64_t max_new, n_free;
+  int32_t requests, new_requests, table_width, pages, page_size;
+  int32_t kv_heads, dim, dtype, layers;
+  int32_t reserved;
+  int64_t k_stride[3], v_stride[3]; /* elements: page, slot, head */
+} tjev_gdn_pages_params;
+
+/* The kept ones of each request's new tokens (lengths[b] in all, its new ones starts[b + 1] - starts[b]) move to the front of
+ * them: number path[b, j] (int32 [requests, max_new], growing with j) becomes number j, j < kept[b]. lengths_out [requests] = lengths -
+ * the new ones + kept. Numbers that are less than j or no new token, and places without a page, are left out. */
+int tjev_gdn_paged_compact(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches,
+                           void* const* v_caches, const int32_t* block_table, const int32_t* starts,
+                           const int32_t* lengths, const int32_t* path, const int32_t* kept,
+                           int32_t* lengths_out);
+
+/* New places of the table go on from old ones: place i (of new_requests) with the first keep[i] tokens (null: all) of place
+ * sources[i] (anything but 0 .. requests - 1: it is unused). shared [pages] counts who holds a page beside its first holder. The
+ * pages are shared, but a last page with room has one holder: the first new place that would write on in it where all its holders
+ * would; each other one takes a page from the free list, and the tokens are copied in every cache. Pages that are held no more go
+ * back on the list, in the old table's order, in front of index taken[0] (those that find no room there are lost), and are the first that copies
+ * take. Writes
+ *   table_out  [new_requests, table_width]  -1 behind a place's pages, and for a copy that finds the list at its end
+ *   lengths_out [new_requests], free_out [n_free], shared_out [pages]
+ *   taken_out  [1]  more than n_free means a shortage
+ * aliasing none of the inputs. The workspace (256-byte aligned) needs no clearing. */
+size_t tjev_gdn_fork_workspace_bytes(const tjev_gdn_pages_params* p);
+int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches,
+                        void* const* v_caches, const int32_t* block_table, const int32_t* lengths,
+                        const int32_t* sources, const int32_t* keep, const int32_t* free_pages,
+                        const int32_t* taken, const int32_t* shared, int32_t* table_out,
+                        int32_t* lengths_out, int32_t* free_out, int32_t* taken_out,
+                        int32_t* shared_out, void* workspace, size_t workspace_bytes);
+
 /* Per-kernel timing (no counterpart in the reference, whose kernels are timed by xprof):
  * between tjev_gdn_profile_begin() and tjev_gdn_profile_end(), every launch of the megakernel
  * and norm calls is bracketed by a hipEvent pair on the call's stream. _end synchronizes those events

@@ -54,6 +54,13 @@ EXPORTS = (
     "tjev_gdn_paged_append",
     "tjev_gdn_paged_workspace_bytes",
     "tjev_gdn_paged_attention",
+    "tjev_gdn_paged_tree_attention",
+    "tjev_gdn_draft_tree",
+    "tjev_gdn_verify_workspace_bytes",
+    "tjev_gdn_verify_drafts",
+    "tjev_gdn_paged_compact",
+    "tjev_gdn_fork_workspace_bytes",
+    "tjev_gdn_paged_fork",
     "tjev_gdn_profile_begin",
     "tjev_gdn_profile_end",
     "tjev_gdn_kernel_name",
@@ -106,6 +113,22 @@ class PagedParams(ctypes.Structure):
                 *((n, ctypes.c_int64 * 2) for n in ("q_stride", "gate_stride", "out_stride")),
                 *((n, ctypes.c_int64 * 3) for n in ("k_stride", "v_stride")),
                 *((n, ctypes.c_int64 * 2) for n in ("k_new_stride", "v_new_stride")), ("max_new", ctypes.c_int64)]
+
+
+class DraftParams(ctypes.Structure):
+    """tjev_gdn_draft_params"""
+
+    _fields_ = [*((n, ctypes.c_int64) for n in ("tokens", "max_new", "target_stride", "draft_stride")),
+                *((n, ctypes.c_int32) for n in ("requests", "vocab", "dtype", "reserved"))]
+
+
+class PagesParams(ctypes.Structure):
+    """tjev_gdn_pages_params"""
+
+    _fields_ = [*((n, ctypes.c_int64) for n in ("max_new", "n_free")),
+                *((n, ctypes.c_int32) for n in ("requests", "new_requests", "table_width", "pages", "page_size", "kv_heads", "dim", "dtype",
+                                                "layers", "reserved")),
+                ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)]
 
 
 class Merge(ctypes.Structure):
@@ -220,6 +243,21 @@ def open_library(path: Path) -> ctypes.CDLL:
     lib.tjev_gdn_paged_workspace_bytes.restype = sz
     lib.tjev_gdn_paged_attention.argtypes = [gpp, vp] + [vp] * 9 + [sz]
     lib.tjev_gdn_paged_attention.restype = i32
+    lib.tjev_gdn_paged_tree_attention.argtypes = [gpp, vp] + [vp] * 7 + [ctypes.c_int32] + [vp] * 3 + [sz]
+    lib.tjev_gdn_paged_tree_attention.restype = i32
+    dpp, hpp = ctypes.POINTER(DraftParams), ctypes.POINTER(PagesParams)
+    lib.tjev_gdn_draft_tree.argtypes = [dpp, vp] + [vp] * 5
+    lib.tjev_gdn_draft_tree.restype = i32
+    lib.tjev_gdn_verify_workspace_bytes.argtypes = [dpp]
+    lib.tjev_gdn_verify_workspace_bytes.restype = sz
+    lib.tjev_gdn_verify_drafts.argtypes = [dpp, vp] + [vp] * 10 + [sz]
+    lib.tjev_gdn_verify_drafts.restype = i32
+    lib.tjev_gdn_paged_compact.argtypes = [hpp, vp] + [vp] * 8
+    lib.tjev_gdn_paged_compact.restype = i32
+    lib.tjev_gdn_fork_workspace_bytes.argtypes = [hpp]
+    lib.tjev_gdn_fork_workspace_bytes.restype = sz
+    lib.tjev_gdn_paged_fork.argtypes = [hpp, vp] + [vp] * 15 + [sz]
+    lib.tjev_gdn_paged_fork.restype = i32
     lib.tjev_gdn_profile_begin.argtypes = []
     lib.tjev_gdn_profile_begin.restype = i32
     lib.tjev_gdn_profile_end.argtypes = [ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int), i32]

@@ -127,11 +127,11 @@ struct FoundLds {
 };
 
 // Up to 64 requests are read and summed by each wave for itself, more of them by the workgroup, in turns, twice.
-template <int R, int KB>
+template <int R, int KB, bool TREE>
 __device__ __forceinline__ Found find_range(const AttnArgs& A, int range, FoundLds& f) {
   const int tid = threadIdx.x;
   Found r;
-  auto load = [&](int b) { return b < A.B ? request<R, KB>(A, b) : Request{}; };
+  auto load = [&](int b) { return b < A.B ? request<R, KB, TREE>(A, b) : Request{}; };
   if (A.B <= 64) {
     const Request q = load(lane());
     const long upto = scan_wave(q.cost);
@@ -435,6 +435,29 @@ __device__ __forceinline__ Split* split_of(const AttnArgs& A, int range) {
 // the workgroup's i-th range: consecutive ranges stay on one XCD (its L2 holds the keys that they share)
 __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block : (block % 8) * (G / 8) + block / 8; }
 
+// ---------------------------------------------------------------- a tree's rows
+// TREE: a row attends to all keys before the request's new tokens, and of those to the ones that its bits name. Which of the
+// 64 keys from k0 on that is; rows behind the request's last attend to none.
+__device__ __forceinline__ uint64_t tree_keys(const AttnArgs& A, const Request& q, int row, int k0) {
+  if (row >= q.rows) return 0;
+  const uint64_t* bits = A.tree + (long)(q.s0 + A.by_g(row)) * A.words;
+  const long at = k0 - q.first;  // of the first of them among the new tokens
+  uint64_t s;
+  if (at <= -64) {
+    s = ~0ull;
+  } else if (at < 0) {
+    s = ((1ull << -at) - 1) | bits[0] << -at;
+  } else {
+    const long i = at >> 6;
+    const int sh = at & 63;
+    s = (i < A.words ? bits[i] >> sh : 0) | (sh && i + 1 < A.words ? bits[i + 1] << (64 - sh) : 0);
+  }
+  const int left = q.keys - k0;
+  return left >= 64 ? s : left > 0 ? s & ((1ull << left) - 1) : 0;
+}
+// the keys that all rows attend to
+__device__ __forceinline__ int tree_first(const Request& q) { return q.first < 0 ? 0 : q.first < q.keys ? (int)q.first : q.keys; }
+
 // ---------------------------------------------------------------- few rows: keys streamed
 // The four waves take steps of KG * 16 keys in turn, each with a running maximum, sum and result of its
 // own, joined in LDS at the end. Bound by memory: the keys and values are read once, straight into registers (64 requests of
@@ -447,7 +470,7 @@ struct StreamLds {
   static constexpr int Q = NQ * Shape<T, DT>::KS * 64, ACC = 2 * NV * 64;  // pieces of 16 bytes
 };
 
-template <class T, int DT, int NQ, bool PAD, bool WHOLE>
+template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool TREE>
 __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part& part, int kb0, int seg, uint4* sq,
                                             f32x4* sacc, float (&sm)[4][16 * NQ], float (&sl)[4][16 * NQ]) {
   using S = Shape<T, DT>;
@@ -491,7 +514,8 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
       for (int e = 0; e < S::VE; ++e) o[n][x][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int lo_lim = uniform(row_limit(A, q, row0)), hi_lim = uniform(row_limit(A, q, min(row0 + R, q.rows) - 1));
+  const int lo_lim = uniform(TREE ? tree_first(q) : row_limit(A, q, row0));
+  const int hi_lim = uniform(TREE ? q.keys : row_limit(A, q, min(row0 + R, q.rows) - 1));
   const int32_t* table = A.table + (long)b * A.M;
   const char *kc = A.k + h * A.kh, *vc = A.v + h * A.vh;
 
@@ -568,14 +592,21 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
       for (int n = 0; n < NQ; ++n) s[j][n] *= A.c;
     const bool masked = k0 + 16 * KG > lo_lim || bad_page;
     bool careful = false;
+    uint64_t sees[NQ];  // TREE: which of the step's keys the lane's rows attend to
     if (masked) {
+      if constexpr (TREE)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) sees[n] = tree_keys(A, q, row0 + n * 16 + r16, k0) >> (4 * g4);
 #pragma unroll
       for (int j = 0; j < KG; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = k0 + 16 * j + 4 * g4 + r;
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) s[j][n][r] = key < lim[n] && ok[j][r] ? s[j][n][r] : kNegInf;
+          for (int n = 0; n < NQ; ++n) {
+            const bool on = TREE ? (bool)(sees[n] >> (16 * j + r) & 1) : key < lim[n];
+            s[j][n][r] = on && ok[j][r] ? s[j][n][r] : kNegInf;
+          }
           // what no row attends to must not meet its zero weight: 0 * NaN
           if (key >= hi_lim || !ok[j][r])
 #pragma unroll
@@ -619,7 +650,7 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) on[j][r][n] = k0 + 16 * j + 4 * g4 + r < lim[n];
+          for (int n = 0; n < NQ; ++n) on[j][r][n] = TREE ? (bool)(sees[n] >> (16 * j + r) & 1) : k0 + 16 * j + 4 * g4 + r < lim[n];
       add_special<T, DT, NQ>(vf, on, o);
     }
     add_pv<T, DT, NQ>(vf, s, o);
@@ -823,7 +854,7 @@ struct WideTile {
   }
 };
 
-template <int DT, bool PAD, bool WHOLE>
+template <int DT, bool PAD, bool WHOLE, bool TREE>
 __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& part, int kb0, int seg, uint16_t* sk0,
                                           uint16_t* sv0, uint16_t* sk1, uint16_t* sv1, uint4* sq, u32 (*sbad)[4]) {
   using W = Wide<DT>;
@@ -846,8 +877,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
   // limits of the wave's and of the workgroup's first and last rows
   const int wr = row0 + w * 32;
   const bool rows_w = wr < q.rows;  // a wave without rows only helps to bring K and V
-  const int lo_w = uniform(rows_w ? row_limit(A, q, wr) : 0), hi_w = uniform(rows_w ? row_limit(A, q, min(wr + 32, q.rows) - 1) : 0);
-  const int lo_g = uniform(row_limit(A, q, row0)), hi_g = uniform(row_limit(A, q, min(row0 + kWideRows, q.rows) - 1));
+  auto limit_of = [&](int row, bool last) { return TREE ? last ? q.keys : tree_first(q) : row_limit(A, q, row); };
+  const int lo_w = uniform(rows_w ? limit_of(wr, false) : 0), hi_w = uniform(rows_w ? limit_of(min(wr + 32, q.rows) - 1, true) : 0);
+  const int lo_g = uniform(limit_of(row0, false)), hi_g = uniform(limit_of(min(row0 + kWideRows, q.rows) - 1, true));
   const bool flip = A.c < 0.f;  // the scale's sign goes into q, which is exact
   const float c = flip ? -A.c : A.c;
 
@@ -977,7 +1009,14 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       special = __syncthreads_or(nf) || special;
     }
     if (!live) return;
-    if (edge && k0 + TK > lo_w) {
+    if (TREE && edge && k0 + TK > lo_w) {
+      const int lt = lane_anew();
+      const uint64_t sees = tree_keys(A, q, row0 + w * 32 + lt % 32, k0) >> (4 * (lt / 32));
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[n][x] = sees >> (n * 32 + 8 * (x / 4) + x % 4) & 1 ? s[n][x] : kNegInf;
+    } else if (edge && k0 + TK > lo_w) {
       const int left = lim - k0 - 4 * (lane_anew() / 32);
 #pragma unroll
       for (int n = 0; n < NS; ++n)
@@ -1071,6 +1110,7 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
       tile.issue(k0, tile.look(k0), 0, sk0, sv0);
       ready();
       clear_unseen(k0, 0, sv0);
+      const uint64_t sees = TREE ? tree_keys(A, q, row0 + w * 32 + r32, k0) : 0;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         f32x16 o1;
@@ -1084,8 +1124,9 @@ __device__ __forceinline__ void wide_tile(const Request& q, int b, const Part& p
             u32 on[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int key = k0 + n * 32 + 16 * j + (x / 2) * 8 + 4 * hf + 2 * (x % 2);
-              on[x] = (key < lim ? 0x3f80u : 0u) | (key + 1 < lim ? 0x3f800000u : 0u);
+              const int at = n * 32 + 16 * j + (x / 2) * 8 + 4 * hf + 2 * (x % 2), key = k0 + at;
+              const bool lo = TREE ? (bool)(sees >> at & 1) : key < lim, hi = TREE ? (bool)(sees >> at & 2) : key + 1 < lim;
+              on[x] = (lo ? 0x3f80u : 0u) | (hi ? 0x3f800000u : 0u);
             }
             o1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(bf16x8, make_uint4(marks_of(v.x), marks_of(v.y), marks_of(v.z), marks_of(v.w))),
@@ -1188,8 +1229,8 @@ __device__ __forceinline__ void clear_rest(const AttnArgs& A) {
   }
 }
 
-// MIXED: the batch may hold requests of more than A.wide packed rows, which take the wide tiles.
-template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
+// MIXED: the batch may hold requests of more than A.wide packed rows, which take the wide tiles. TREE: see tree_keys.
+template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
   using S = Shape<T, DT>;
   using L = StreamLds<T, DT, NQ>;
@@ -1215,7 +1256,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 
   {
     const int range = range_of(blockIdx.x, A.G);
-    const Found f = find_range<R, KB>(A, range, sfound);
+    const Found f = find_range<R, KB, TREE>(A, range, sfound);
     if (threadIdx.x == 0) split_of(A, range)->parts = 0;
     if (A.fill) clear_rest<T>(A);
     if (f.b < 0) return;
@@ -1256,7 +1297,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
         if (local < q.cost) {
           st.at = at.tile + 1 < q.tiles ? Unit{at.head, at.tile + 1, 0} : Unit{at.head + 1, 0, 0};
         } else if (u + seg < u1) {
-          const Request n = b + 1 < A.B ? request<R, KB>(A, b + 1) : Request{};
+          const Request n = b + 1 < A.B ? request<R, KB, TREE>(A, b + 1) : Request{};
           local = 0;
           st.q = n;
           st.b = b + 1;
@@ -1268,10 +1309,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
         if (MIXED && q.tile_rows == kWideRows) {
           uint16_t* pa = reinterpret_cast<uint16_t*>(sa);
           if constexpr (MIXED)
-            wide_tile<DT, PAD, WHOLE>(q, b, part, k0, keys, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
+            wide_tile<DT, PAD, WHOLE, TREE>(q, b, part, k0, keys, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
                                       reinterpret_cast<uint16_t*>(sc), sd, sbad);
         } else {
-          stream_tile<T, DT, NQ, PAD, WHOLE>(q, b, part, k0, keys, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
+          stream_tile<T, DT, NQ, PAD, WHOLE, TREE>(q, b, part, k0, keys, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
         }
       }
     }
@@ -1282,7 +1323,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
       if (uniform(wave()) == 0) {
         int b = uniform(st.b) + 1;
         for (; b < A.B; b += 64) {
-          const Request n = b + lane() < A.B ? request<R, KB>(A, b + lane()) : Request{};
+          const Request n = b + lane() < A.B ? request<R, KB, TREE>(A, b + lane()) : Request{};
           const uint64_t here = __ballot(n.cost > 0);
           if (here) {
             const int first = __builtin_ctzll(here);

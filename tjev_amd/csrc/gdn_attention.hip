@@ -71,33 +71,29 @@ int validate(const tjev_gdn_paged_params* p) {
 }  // namespace
 }  // namespace gdn
 
-extern "C" {
+namespace gdn {
+namespace {
 
-size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p) {
-  if (gdn::validate(p)) return 0;
-  return gdn::plan_of(p).bytes;
-}
-
-int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const void* k_cache, const void* v_cache,
-                             const int32_t* block_table, const int32_t* starts, const int32_t* lengths, const void* gate, void* out,
-                             void* workspace, size_t workspace_bytes) {
-  using gdn::fail;
-  if (int s = gdn::validate(p)) return s;
+// Both entries; ancestors: the tree's bits, or null for causal rows.
+int attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const void* k_cache, const void* v_cache,
+              const int32_t* block_table, const int32_t* starts, const int32_t* lengths, const uint64_t* ancestors, int words,
+              const void* gate, void* out, void* workspace, size_t workspace_bytes) {
+  if (int s = validate(p)) return s;
   if (!p->tokens) return 0;
   if (!q || !k_cache || !v_cache || !block_table || !starts || !lengths || !out) return fail(TJEV_GDN_EINVAL, "null tensor argument");
-  const size_t need = tjev_gdn_paged_workspace_bytes(p);
+  const size_t need = plan_of(p).bytes;
   if (!workspace || workspace_bytes < need)
     return fail(TJEV_GDN_EWORKSPACE, "paged attention needs a workspace of tjev_gdn_paged_workspace_bytes");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TJEV_GDN_EINVAL, "the workspace must be 256-byte aligned");
   const long e = p->dtype == TJEV_GDN_BF16 ? 2 : 4;
-  gdn::AttnArgs A{};
+  AttnArgs A{};
   A.N = p->tokens;
   A.B = p->requests;
   A.M = p->table_width;
-  gdn::set_page(A, p->page_size);
+  set_page(A, p->page_size);
   A.pages = p->pages;
   A.Hk = p->kv_heads;
-  gdn::set_group(A, p->heads / p->kv_heads);
+  set_group(A, p->heads / p->kv_heads);
   A.D = p->dim;
   A.fill = p->fill;
   // a scale of 0 as the smallest number, so that a masked score stays at minus infinity
@@ -122,15 +118,43 @@ int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const
   if (A.ks > (1l << 26) || A.vs > (1l << 26)) return fail(TJEV_GDN_EUNSUPPORTED, "cache slots more than 64 MB apart");
   if (any % 16) return fail(TJEV_GDN_EINVAL, "q, gate, out and the caches must be 16-byte aligned, with strides that keep their rows so");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const gdn::AttnPlan plan = gdn::plan_of(p);
+  const AttnPlan plan = plan_of(p);
   // (the parts: the ranges' notes behind them, which say how many there are, are never NaN)
-  if (int s = gdn::poison_workspace(workspace, plan.bytes - (size_t)plan.G * gdn::kSplitBytes, stream)) return s;
-  using gdn::AttnArgs;
-  hipError_t (*const unit[2][3])(const gdn::AttnPlan&, AttnArgs&, hipStream_t) = {
-      {gdn::attention_f32_64, gdn::attention_f32_128, gdn::attention_f32_256},
-      {gdn::attention_bf16_64, gdn::attention_bf16_128, gdn::attention_bf16_256}};
-  const hipError_t err = unit[p->dtype == TJEV_GDN_BF16][p->dim <= 64 ? 0 : p->dim <= 128 ? 1 : 2](plan, A, st);
+  if (int s = poison_workspace(workspace, plan.bytes - (size_t)plan.G * kSplitBytes, stream)) return s;
+  A.tree = ancestors;
+  A.words = words;
+  hipError_t (*const unit[2][2][3])(const AttnPlan&, AttnArgs&, hipStream_t) = {
+      {{attention_f32_64, attention_f32_128, attention_f32_256}, {attention_bf16_64, attention_bf16_128, attention_bf16_256}},
+      {{attention_tree_f32_64, attention_tree_f32_128, attention_tree_f32_256},
+       {attention_tree_bf16_64, attention_tree_bf16_128, attention_tree_bf16_256}}};
+  const hipError_t err = unit[ancestors != nullptr][p->dtype == TJEV_GDN_BF16][p->dim <= 64 ? 0 : p->dim <= 128 ? 1 : 2](plan, A, st);
   return err == hipSuccess ? 0 : fail(TJEV_GDN_EHIP, hipGetErrorString(err));
+}
+
+}  // namespace
+}  // namespace gdn
+
+extern "C" {
+
+size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p) {
+  if (gdn::validate(p)) return 0;
+  return gdn::plan_of(p).bytes;
+}
+
+int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const void* k_cache, const void* v_cache,
+                             const int32_t* block_table, const int32_t* starts, const int32_t* lengths, const void* gate, void* out,
+                             void* workspace, size_t workspace_bytes) {
+  return gdn::attention(p, stream, q, k_cache, v_cache, block_table, starts, lengths, nullptr, 0, gate, out, workspace, workspace_bytes);
+}
+
+int tjev_gdn_paged_tree_attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const void* k_cache,
+                                  const void* v_cache, const int32_t* block_table, const int32_t* starts, const int32_t* lengths,
+                                  const int64_t* ancestors, int32_t words, const void* gate, void* out, void* workspace,
+                                  size_t workspace_bytes) {
+  if (p && p->tokens && !ancestors) return gdn::fail(TJEV_GDN_EINVAL, "null tensor argument");
+  if (words < 1) return gdn::fail(TJEV_GDN_EINVAL, "ancestors have a word of 64 tokens at least");
+  return gdn::attention(p, stream, q, k_cache, v_cache, block_table, starts, lengths, reinterpret_cast<const uint64_t*>(ancestors), words,
+                        gate, out, workspace, workspace_bytes);
 }
 
 }  // extern "C"

@@ -1,8 +1,15 @@
-// One unit of paged attention: the kernels of one type (GDN_T: bf16 or f32) and head dims up to GDN_D.
+// One unit of paged attention: the kernels of one type (GDN_T: bf16 or f32) and head dims up to GDN_D, with GDN_TREE those for
+// trees of new tokens.
 #include "gdn_attention.h"
 
 namespace gdn {
 namespace {
+
+#ifdef GDN_TREE
+constexpr bool kTree = true;
+#else
+constexpr bool kTree = false;
+#endif
 
 template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED>
 hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
@@ -11,7 +18,7 @@ hipError_t launch(const AttnPlan& r, AttnArgs& A, hipStream_t st) {
   A.slot = r.slot;
   A.wide = MIXED ? 16 * NQ : 0x7fffffff;
   A.wide_extra = kWideExtra + (A.gate ? kGateExtra : 0);
-  hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED>), dim3(r.G), dim3(kThreads), 0, st, A);
+  hipLaunchKernelGGL((k_attention<T, DT, NQ, PAD, WHOLE, MIXED, kTree>), dim3(r.G), dim3(kThreads), 0, st, A);
   constexpr int slices = join_slices<DT, MIXED ? kWideRows : 16 * NQ>();
   if (r.join == kJoinSliced) {
     hipLaunchKernelGGL((k_attention_join<T, DT, NQ, MIXED, kJoinSliced>), dim3(r.tiles, slices), dim3(join_threads<DT, kJoinSliced>()), 0, st, A);
@@ -51,7 +58,11 @@ using f32 = float;
 
 }  // namespace
 
+#ifdef GDN_TREE
+#define GDN_NAME_(t, d) attention_tree_##t##_##d
+#else
 #define GDN_NAME_(t, d) attention_##t##_##d
+#endif
 #define GDN_NAME(t, d) GDN_NAME_(t, d)
 hipError_t GDN_NAME(GDN_T, GDN_D)(const AttnPlan& r, AttnArgs& A, hipStream_t st) { return by_rows<GDN_T, GDN_D>(r, A, st); }
 

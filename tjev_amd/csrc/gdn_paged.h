@@ -90,7 +90,8 @@ struct Request {
   }
 };
 
-template <int R, int KB>
+// TREE: a tree's rows may attend to any of the request's new tokens, so every tile has all of its keys.
+template <int R, int KB, bool TREE = false>
 __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   Request q;
   const long n = A.N, a = A.starts[b], e = A.starts[b + 1], len = A.lengths[b];
@@ -107,7 +108,7 @@ __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   q.by_g = A.by_g_long;
   q.y = 0;
   q.blocks = keys ? (int)((keys + KB - 1) / KB) : 1;  // a row without keys is written too
-  if (wide && q.first >= 0 && keys == len) {
+  if (!TREE && wide && q.first >= 0 && keys == len) {
     // Tile t's last row may attend to first + (kWideRows (t + 1) - 1) / g + 1 keys, which are
     // floor((first g + kWideRows (t + 1) - 1) / (KB g)) + 1 blocks, and with KB = kWideRows floor((y + t) / g)
     static_assert(KB == kWideRows || KB < kWideRows, "");
@@ -173,6 +174,8 @@ struct AttnArgs : Batch {
   long slot;
   int G;                            // workgroups, and the division by them
   Div by_G;
+  const uint64_t* tree;             // trees: which of its request's new tokens each of them attends to, `words` of 64 bits
+  long words;
 };
 
 constexpr int kMostRanges = 768;
@@ -191,8 +194,10 @@ struct AttnPlan {
   size_t bytes;      // workspace
 };
 
-// One unit of gdn_attn_inst.hip: attention in bf16 (bf = true) or fp32, head dims up to d
-#define GDN_ATTENTION(t, d) hipError_t attention_##t##_##d(const AttnPlan& r, AttnArgs& A, hipStream_t st);
+// One unit of gdn_attn_inst.hip each: attention in bf16 or fp32, head dims up to d, and the same of trees
+#define GDN_ATTENTION(t, d)                                                        \
+  hipError_t attention_##t##_##d(const AttnPlan& r, AttnArgs& A, hipStream_t st); \
+  hipError_t attention_tree_##t##_##d(const AttnPlan& r, AttnArgs& A, hipStream_t st);
 GDN_ATTENTION(bf16, 64)
 GDN_ATTENTION(bf16, 128)
 GDN_ATTENTION(bf16, 256)

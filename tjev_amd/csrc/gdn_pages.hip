@@ -1,0 +1,465 @@
+// Who holds the pages of the paged key/value cache, for gfx950: the accepted ones of drafted tokens moved to their places
+// (compaction), and requests that go on from others' pages, shortened, several times or not at all (forks).
+//
+// Compaction: token path[j] of a request's new ones becomes its j-th, path growing, so path[j] >= j and a place is read
+// before it is written when the moves run in order. A workgroup moves some columns of 16 bytes of all tokens of one request, of
+// one cache: a round of tokens is loaded, then (behind a barrier) stored. Bound by latency: lengths, path, table, keys, each
+// behind the other; the bytes are few.
+//
+// Forks: place i of the new table holds the first pages of place sources[i] of the old one. What changes is counted per page
+// with atomics on whole numbers (sums, minima: their order does not matter): `shared`, how many hold a page beside the first
+// one, and of the last pages that are not full how many go on writing there. Pages that nobody holds go back on the free list
+// in the order of the old table, copies of last pages are taken from it in the order of the new one.
+#include <hip/hip_runtime.h>
+
+#include "../../include/tjev_gdn.h"
+#include "gdn_device.h"
+#include "gdn_launch.h"
+#include "gdn_paged.h"
+
+namespace gdn {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kLayers = 16;  // of a launch
+
+struct Caches {
+  char *k[kLayers], *v[kLayers];
+  long kp, ks, kh, vp, vs, vh;  // bytes: page, slot and head
+  int chunks, per;              // vectors of a head, of a token
+  int cols;                     // of them, a workgroup's
+  int groups;                   // of columns
+  // where a vector of a slot lies
+  __device__ __forceinline__ char* at(int layer, bool values, long page, long in, int col, int bytes) const {
+    const int h = col / chunks, c = col - h * chunks;
+    return values ? v[layer] + page * vp + in * vs + h * vh + (long)c * bytes : k[layer] + page * kp + in * ks + h * kh + (long)c * bytes;
+  }
+};
+
+// ---------------------------------------------------------------- compaction
+struct CompactArgs {
+  Caches c;
+  int B, M, pages, layers;
+  long most;
+  Div page;
+  const int32_t *table, *starts, *lengths, *path, *kept;
+  int32_t* lengths_out;  // null: not this launch's
+};
+
+template <class W>
+__global__ __launch_bounds__(kThreads) void k_paged_compact(CompactArgs A) {
+  constexpr int UN = 8;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const long n = max(0l, (long)A.starts[b + 1] - A.starts[b]), len = A.lengths[b], first = len - n;
+  const long count = min(min((long)max(A.kept[b], 0), A.most), n);
+  if (A.lengths_out && blockIdx.y == 0 && tid == 0) A.lengths_out[b] = (int)max(0l, first + count);
+  if (!A.layers || first < 0) return;
+  const int32_t* path = A.path + b * A.most;
+  const int group = blockIdx.y % A.c.groups, cache = blockIdx.y / A.c.groups, layer = cache / 2;
+  const bool values = cache % 2;
+  const int cols = A.c.cols, step = kThreads / cols, mine = tid / cols, col = group * cols + tid % cols;
+  // a token's place, or null
+  auto place = [&](long t) -> char* {
+    const long j = A.page(t);
+    const int p = j < A.M ? A.table[(long)b * A.M + j] : -1;
+    return p >= 0 && p < A.pages ? A.c.at(layer, values, p, t - j * A.page.d, col, sizeof(W)) : nullptr;
+  };
+  for (long j0 = 0; j0 < count; j0 += UN * step) {
+    W x[UN];
+    char* to[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const long j = j0 + i * step + mine;
+      to[i] = nullptr;
+      if (mine < step && col < A.c.per && j < count) {
+        const long f = path[j];
+        if (f > j && f < n) {
+          const char* from = place(first + f);
+          to[i] = from ? place(first + j) : nullptr;
+          if (to[i]) x[i] = *reinterpret_cast<const W*>(from);
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): read by all before it is written by any
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (to[i]) *reinterpret_cast<W*>(to[i]) = x[i];
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- forks
+struct ForkArgs {
+  int B, B2, M, pages;  // places of the old and the new table
+  long n_free;
+  Div page;
+  const int32_t *table, *lengths, *sources, *keep, *free, *taken, *shared;  // keep: null for all
+  int32_t *table_out, *lengths_out, *free_out, *taken_out, *shared_out;
+  // of each page: the new places that write on in it, and the first of them; the first of the old table's entries that leave it
+  int32_t *writers, *writer, *entry;
+  int32_t *freed, *copied;  // of each old place, the pages given back; of each new one, whether it takes a copy of its last page
+  int32_t* where;           // and where that stands on the free list, or -1
+};
+
+__device__ __forceinline__ int fork_pages(const ForkArgs& A, long n) {
+  const long p = A.page(n + A.page.d - 1);
+  return (int)(p < A.M ? p : A.M);
+}
+__device__ __forceinline__ bool is_page(const ForkArgs& A, int p) { return p >= 0 && p < A.pages; }
+
+// What a place of the new table goes on with
+struct Going {
+  int source, pages, last;  // last: the page that it writes on in, or -1
+  long keep;
+};
+__device__ __forceinline__ Going going(const ForkArgs& A, int i) {
+  Going g{-1, 0, -1, 0};
+  if (i >= A.B2) return g;
+  const int s = A.sources[i];
+  if (s < 0 || s >= A.B) return g;
+  g.source = s;
+  const long len = max(A.lengths[s], 0);
+  g.keep = A.keep ? min((long)max(A.keep[i], 0), len) : len;
+  g.pages = fork_pages(A, g.keep);
+  const long j = A.page(g.keep);
+  if (g.keep > j * A.page.d && j < A.M) {
+    const int p = A.table[(long)s * A.M + j];
+    if (is_page(A, p)) g.last = p;
+  }
+  return g;
+}
+
+// the first new place that goes on from old place b, or B2; by a workgroup
+__device__ __forceinline__ int heir_of(const ForkArgs& A, int b, int* sheir) {
+  int mine = A.B2;
+  for (int i = threadIdx.x; i < A.B2; i += kThreads)
+    if (A.sources[i] == b) mine = min(mine, i);
+  __syncthreads();
+  if (threadIdx.x == 0) *sheir = A.B2;
+  __syncthreads();
+  if (mine < A.B2) atomicMin(sheir, mine);
+  __syncthreads();
+  return *sheir;
+}
+
+__global__ __launch_bounds__(kThreads) void k_fork_init(ForkArgs A) {
+  const long stride = (long)gridDim.x * kThreads, id = (long)blockIdx.x * kThreads + threadIdx.x;
+  for (long i = id; i < A.pages; i += stride) {
+    A.shared_out[i] = A.shared[i];
+    A.writers[i] = 0;
+    A.writer[i] = A.entry[i] = 0x7fffffff;
+  }
+  for (long i = id; i < A.n_free; i += stride) A.free_out[i] = A.free[i];
+}
+
+// A workgroup per place: what the old place of that number loses, and what the new one takes on. The first new place that goes on
+// from an old one keeps what it has, and nothing is counted for that.
+__global__ __launch_bounds__(kThreads) void k_fork_count(ForkArgs A) {
+  __shared__ int sheir;
+  GDN_POISON_LDS(sheir);
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r < A.B) {
+    const int heir = heir_of(A, r, &sheir);
+    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
+    for (int j = kept + tid; j < held; j += kThreads) {
+      const int p = A.table[(long)r * A.M + j];
+      if (!is_page(A, p)) continue;
+      atomicSub(&A.shared_out[p], 1);
+      atomicMin(&A.entry[p], r * A.M + j);
+    }
+  }
+  const Going g = going(A, r);
+  if (g.source < 0) return;
+  if (heir_of(A, g.source, &sheir) != r)
+    for (int j = tid; j < g.pages; j += kThreads) {
+      const int p = A.table[(long)g.source * A.M + j];
+      if (is_page(A, p)) atomicAdd(&A.shared_out[p], 1);
+    }
+  if (tid == 0 && g.last >= 0) {
+    atomicAdd(&A.writers[g.last], 1);
+    atomicMin(&A.writer[g.last], r);
+  }
+}
+
+// whether the old table's entry gives its page back
+__device__ __forceinline__ bool gives_back(const ForkArgs& A, int r, int j, int& p) {
+  p = A.table[(long)r * A.M + j];
+  return is_page(A, p) && A.entry[p] == r * A.M + j && A.shared_out[p] == -1;
+}
+
+__global__ __launch_bounds__(kThreads) void k_fork_decide(ForkArgs A) {
+  __shared__ int sheir, scount;
+  GDN_POISON_LDS(sheir, scount);
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r < A.B) {
+    const int heir = heir_of(A, r, &sheir);
+    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
+    if (tid == 0) scount = 0;
+    __syncthreads();
+    int n = 0, p;
+    for (int j = kept + tid; j < held; j += kThreads) n += gives_back(A, r, j, p);
+    if (n) atomicAdd(&scount, n);
+    __syncthreads();
+    if (tid == 0) A.freed[r] = scount;
+  }
+  if (r < A.B2 && tid == 0) {
+    const Going g = going(A, r);
+    // a last page with room has one holder: the first of those that write on in it, if all of its holders do
+    A.copied[r] = g.last >= 0 && !(A.shared_out[g.last] + 1 == A.writers[g.last] && A.writer[g.last] == r);
+  }
+}
+
+// sums of freed before place r, of copied before it, and of all freed
+struct Sums {
+  int freed, copied, all_freed, all_copied;
+};
+__device__ __forceinline__ Sums sums_before(const ForkArgs& A, int r, int (*ssum)[4]) {
+  int v[4] = {0, 0, 0, 0};
+  for (int b = threadIdx.x; b < A.B; b += kThreads) {
+    const int n = A.freed[b];
+    v[2] += n;
+    if (b < r) v[0] += n;
+  }
+  for (int i = threadIdx.x; i < A.B2; i += kThreads) {
+    const int n = A.copied[i] != 0;
+    v[3] += n;
+    if (i < r) v[1] += n;
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) v[x] += __shfl_xor(v[x], d);
+    if (lane() == 0) ssum[wave()][x] = v[x];
+  }
+  __syncthreads();
+  Sums s{0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    s.freed += ssum[w][0];
+    s.copied += ssum[w][1];
+    s.all_freed += ssum[w][2];
+    s.all_copied += ssum[w][3];
+  }
+  return s;
+}
+
+__global__ __launch_bounds__(kThreads) void k_fork_tables(ForkArgs A) {
+  __shared__ int sheir, ssum[kThreads / 64][4], srank[kThreads / 64];
+  GDN_POISON_LDS(sheir, ssum, srank);
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const Sums s = sums_before(A, r, ssum);
+  const long had = min((long)max(A.taken[0], 0), A.n_free);
+  const long back = min((long)s.all_freed, had);  // what the list has room for
+  if (r == 0 && tid == 0) A.taken_out[0] = (int)min(had - back + s.all_copied, 0x7fffffffl);
+  if (r < A.B) {
+    const int heir = heir_of(A, r, &sheir);
+    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
+    long rank = s.freed;
+    for (int j0 = kept; j0 < held; j0 += kThreads) {
+      const int j = j0 + tid;
+      int p = -1;
+      const bool gone = j < held && gives_back(A, r, j, p);
+      const uint64_t mask = __ballot(gone);
+      if (lane() == 0) srank[wave()] = __builtin_popcountll(mask);
+      __syncthreads();
+      long at = rank + __builtin_popcountll(mask & ((1ull << lane()) - 1));
+#pragma unroll
+      for (int w = 0; w < kThreads / 64; ++w) {
+        if (w < wave()) at += srank[w];
+        rank += srank[w];
+      }
+      if (gone) {
+        A.shared_out[p] = 0;  // (read by this entry alone from here on)
+        if (at < back) A.free_out[had - back + at] = p;
+      }
+      __syncthreads();
+    }
+  }
+  if (r >= A.B2) return;
+  const Going g = going(A, r);
+  const bool copy = A.copied[r] != 0;
+  for (int j = tid; j < A.M; j += kThreads)
+    A.table_out[(long)r * A.M + j] = j < g.pages ? A.table[(long)g.source * A.M + j] : -1;
+  if (tid == 0) {
+    A.lengths_out[r] = (int)g.keep;
+    A.where[r] = copy ? (int)min(had - back + s.copied, 0x7fffffffl) : -1;
+    if (copy) atomicSub(&A.shared_out[g.last], 1);  // others hold it on: it is not given back
+  }
+}
+
+struct ForkCopyArgs {
+  Caches c;
+  ForkArgs f;
+  int layers;
+  bool first;  // of the launches: it writes the table
+};
+
+// The copies: a workgroup per new place, cache and group of columns. The free list is whole by now: a copy may take a page that
+// was given back (which no copy is made of: what writers leave is held by others).
+template <class W>
+__global__ __launch_bounds__(kThreads) void k_fork_copy(ForkCopyArgs A) {
+  const ForkArgs& F = A.f;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r >= F.B2) return;
+  const int at = F.where[r];
+  if (at < 0) return;
+  const Going g = going(F, r);
+  const int got = at < F.n_free ? F.free_out[at] : -1;
+  const long j = F.page(g.keep);
+  if (A.first && blockIdx.y == 0 && tid == 0) {
+    F.table_out[(long)r * F.M + j] = is_page(F, got) ? got : -1;
+    if (is_page(F, got)) F.shared_out[got] = 0;
+  }
+  if (!A.layers || !is_page(F, got)) return;
+  const int group = blockIdx.y % A.c.groups, cache = blockIdx.y / A.c.groups, layer = cache / 2;
+  const bool values = cache % 2;
+  const int cols = A.c.cols, step = kThreads / cols, mine = tid / cols, col = group * cols + tid % cols;
+  if (mine >= step || col >= A.c.per) return;
+  const int count = (int)(g.keep - j * F.page.d);
+  for (int t0 = mine; t0 < count; t0 += 4 * step) {
+    W x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t0 + i * step < count) x[i] = *reinterpret_cast<const W*>(A.c.at(layer, values, g.last, t0 + i * step, col, sizeof(W)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t0 + i * step < count) *reinterpret_cast<W*>(A.c.at(layer, values, got, t0 + i * step, col, sizeof(W))) = x[i];
+  }
+}
+
+int check(const tjev_gdn_pages_params* p, void* const* k, void* const* v, bool caches) {
+  if (!p) return fail(TJEV_GDN_EINVAL, "null params");
+  if (p->requests < 1 || p->table_width < 1 || p->page_size < 1 || p->pages < 1 || p->layers < 0)
+    return fail(TJEV_GDN_EINVAL, "requests, table_width, pages and page_size must be positive, layers not negative");
+  if (p->requests > TJEV_GDN_MAX_REQUESTS || p->new_requests > TJEV_GDN_MAX_REQUESTS)
+    return fail(TJEV_GDN_EUNSUPPORTED, "block tables of up to 8192 requests");
+  if (!caches || !p->layers) return 0;
+  if ((p->dtype | 1) != 1) return fail(TJEV_GDN_EINVAL, "dtype must be TJEV_GDN_F32 or TJEV_GDN_BF16");
+  if (p->kv_heads < 1 || p->dim < 1) return fail(TJEV_GDN_EINVAL, "kv_heads and dim must be positive");
+  if ((long)p->kv_heads * p->dim >= (1l << 24)) return fail(TJEV_GDN_EUNSUPPORTED, "kv_heads * dim too large");
+  if (!k || !v) return fail(TJEV_GDN_EINVAL, "null tensor argument");
+  for (int l = 0; l < p->layers; ++l)
+    if (!k[l] || !v[l]) return fail(TJEV_GDN_EINVAL, "null tensor argument");
+  return 0;
+}
+
+// The caches' addresses are given launch by launch; the width of a vector (16 bytes where every address and stride allows it), and
+// how a token's are shared out
+int fill(Caches& c, const tjev_gdn_pages_params* p, void* const* k, void* const* v) {
+  const int bytes = p->dtype == TJEV_GDN_BF16 ? 2 : 4;
+  c.kp = p->k_stride[0] * bytes, c.ks = p->k_stride[1] * bytes, c.kh = p->k_stride[2] * bytes;
+  c.vp = p->v_stride[0] * bytes, c.vs = p->v_stride[1] * bytes, c.vh = p->v_stride[2] * bytes;
+  long any = (long)p->dim * bytes | c.kp | c.ks | c.kh | c.vp | c.vs | c.vh;
+  for (int l = 0; l < p->layers; ++l) any |= (long)reinterpret_cast<uintptr_t>(k[l]) | (long)reinterpret_cast<uintptr_t>(v[l]);
+  if (any % bytes) return 0;
+  const int w = any % 16 == 0 ? 16 : bytes;
+  c.chunks = p->dim * bytes / w;
+  c.per = c.chunks * p->kv_heads;
+  c.cols = c.per < kThreads ? c.per : kThreads;
+  c.groups = (c.per + c.cols - 1) / c.cols;
+  return w;
+}
+
+// launch(W, caches of the launch, layers of the launch, whether it is the first) for every kLayers layers, once at least
+template <class F>
+int by_layers(const tjev_gdn_pages_params* p, void* const* k, void* const* v, F launch) {
+  Caches c{};
+  c.groups = c.cols = 1;
+  int w = 16;
+  if (p->layers && !(w = fill(c, p, k, v))) return fail(TJEV_GDN_EINVAL, "the caches must be aligned to their elements");
+  if (2l * kLayers * c.groups > 65535) return fail(TJEV_GDN_EUNSUPPORTED, "kv_heads * dim too large");
+  for (int l0 = 0; l0 == 0 || l0 < p->layers; l0 += kLayers) {
+    const int n = p->layers - l0 < kLayers ? p->layers - l0 : kLayers;
+    for (int l = 0; l < n; ++l) c.k[l] = static_cast<char*>(k[l0 + l]), c.v[l] = static_cast<char*>(v[l0 + l]);
+    if (w == 16) {
+      launch(uint4{}, c, n, l0 == 0);
+    } else if (w == 4) {
+      launch(uint32_t{}, c, n, l0 == 0);
+    } else {
+      launch(uint16_t{}, c, n, l0 == 0);
+    }
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : fail(TJEV_GDN_EHIP, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace gdn
+
+extern "C" {
+
+int tjev_gdn_paged_compact(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches, void* const* v_caches,
+                           const int32_t* block_table, const int32_t* starts, const int32_t* lengths, const int32_t* path,
+                           const int32_t* kept, int32_t* lengths_out) {
+  using gdn::fail;
+  if (int s = gdn::check(p, k_caches, v_caches, true)) return s;
+  if (p->max_new < 1) return fail(TJEV_GDN_EINVAL, "max_new must be positive");
+  if (p->max_new >= (1l << 31)) return fail(TJEV_GDN_EINVAL, "problem too large");
+  if (!block_table || !starts || !lengths || !path || !kept || !lengths_out) return fail(TJEV_GDN_EINVAL, "null tensor argument");
+  if (lengths_out == lengths) return fail(TJEV_GDN_EINVAL, "lengths_out must not alias lengths (every workgroup reads it)");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  gdn::CompactArgs A{};
+  A.B = p->requests, A.M = p->table_width, A.pages = p->pages, A.most = p->max_new;
+  A.page = gdn::div_by(p->page_size);
+  A.table = block_table, A.starts = starts, A.lengths = lengths, A.path = path, A.kept = kept;
+  return gdn::by_layers(p, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
+    A.c = c;
+    A.layers = layers;
+    A.lengths_out = first ? lengths_out : nullptr;
+    const int y = 2 * layers * c.groups;
+    hipLaunchKernelGGL((gdn::k_paged_compact<decltype(w)>), dim3(A.B, y ? y : 1), dim3(gdn::kThreads), 0, st, A);
+  });
+}
+
+size_t tjev_gdn_fork_workspace_bytes(const tjev_gdn_pages_params* p) {
+  if (gdn::check(p, nullptr, nullptr, false) || p->new_requests < 1) return 0;
+  return sizeof(int32_t) * (3 * (size_t)p->pages + p->requests + 2 * (size_t)p->new_requests);
+}
+
+int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches, void* const* v_caches,
+                        const int32_t* block_table, const int32_t* lengths, const int32_t* sources, const int32_t* keep,
+                        const int32_t* free_pages, const int32_t* taken, const int32_t* shared, int32_t* table_out, int32_t* lengths_out,
+                        int32_t* free_out, int32_t* taken_out, int32_t* shared_out, void* workspace, size_t workspace_bytes) {
+  using gdn::fail;
+  if (int s = gdn::check(p, k_caches, v_caches, true)) return s;
+  if (p->new_requests < 1 || p->n_free < 0) return fail(TJEV_GDN_EINVAL, "new_requests must be positive, n_free not negative");
+  if (p->n_free >= (1l << 31) || (long)p->requests * p->table_width >= (1l << 31) || (long)p->new_requests * p->table_width >= (1l << 31))
+    return fail(TJEV_GDN_EINVAL, "problem too large");
+  if (!block_table || !lengths || !sources || !taken || !shared || !table_out || !lengths_out || !taken_out || !shared_out ||
+      (p->n_free && (!free_pages || !free_out)))
+    return fail(TJEV_GDN_EINVAL, "null tensor argument");
+  if (table_out == block_table || lengths_out == lengths || (p->n_free && free_out == free_pages) || taken_out == taken || shared_out == shared)
+    return fail(TJEV_GDN_EINVAL, "the outputs must not alias the inputs");
+  const size_t need = tjev_gdn_fork_workspace_bytes(p);
+  if (!workspace || workspace_bytes < need) return fail(TJEV_GDN_EWORKSPACE, "forks need a workspace of tjev_gdn_fork_workspace_bytes");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TJEV_GDN_EINVAL, "the workspace must be 256-byte aligned");
+  if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
+  int32_t* ws = static_cast<int32_t*>(workspace);
+  gdn::ForkCopyArgs C{};
+  gdn::ForkArgs& A = C.f;
+  A = {p->requests, p->new_requests, p->table_width, p->pages, p->n_free, gdn::div_by(p->page_size), block_table, lengths, sources, keep,
+       free_pages, taken, shared, table_out, lengths_out, free_out, taken_out, shared_out};
+  A.writers = ws;
+  A.writer = A.writers + p->pages;
+  A.entry = A.writer + p->pages;
+  A.freed = A.entry + p->pages;
+  A.copied = A.freed + p->requests;
+  A.where = A.copied + p->new_requests;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const long most = p->pages > p->n_free ? p->pages : p->n_free, blocks = (most + gdn::kThreads - 1) / gdn::kThreads;
+  const dim3 places((unsigned)(A.B > A.B2 ? A.B : A.B2)), block(gdn::kThreads);
+  hipLaunchKernelGGL(gdn::k_fork_init, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), block, 0, st, A);
+  hipLaunchKernelGGL(gdn::k_fork_count, places, block, 0, st, A);
+  hipLaunchKernelGGL(gdn::k_fork_decide, places, block, 0, st, A);
+  hipLaunchKernelGGL(gdn::k_fork_tables, places, block, 0, st, A);
+  return gdn::by_layers(p, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
+    C.c = c;
+    C.layers = layers;
+    C.first = first;
+    const int y = 2 * layers * c.groups;
+    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1), block, 0, st, C);
+  });
+}
+
+}  // extern "C"

@@ -10,6 +10,11 @@ A step of a batch, with what every layer shares first:
     paged_append(k, v, k_cache, v_cache, t.slots)
     out = paged_attention(q, k_cache, v_cache, t.block_table, t.starts, t.lengths, gate=gate)
 
+With trees of drafted tokens (drafts.py: their ancestors and positions, their verification) attention is
+``paged_tree_attention``; ``paged_compact`` moves the accepted ones to their places in all layers, and
+``paged_fork`` says which requests go on, with how much of what they hold: sharing pages, copying last ones and giving back what
+nobody holds.
+
 Caches are [pages, page_size, kv_heads, dim] with any strides whose last dim is contiguous (another order
 of the dims, or keys and values in one tensor, are views of this). Token t of a request lies in page
 block_table[request, t // page_size] at place t % page_size; its slot is page * page_size + place. A
@@ -45,6 +50,11 @@ class PagedTables(NamedTuple):
 
 def _int32(x: torch.Tensor) -> torch.Tensor:
     return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
+def _int32_near(x: torch.Tensor) -> torch.Tensor:
+    """_int32 of numbers that may be anything: those past 32 bits become the last of them, not their low half."""
+    return _int32(x.clamp(-(1 << 31), (1 << 31) - 1) if x.dtype == torch.int64 else x)
 
 
 def _device(x: torch.Tensor | None, like: torch.Tensor) -> int:
@@ -164,7 +174,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 
 @functools.lru_cache(maxsize=256)
 def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_dtype, vc_shape, vc_stride, vc_dtype, t_shape, t_dtype,
-                      s_shape, s_dtype, l_shape, l_dtype, gate, out, scale, max_new, devices):
+                      s_shape, s_dtype, l_shape, l_dtype, gate, out, scale, max_new, devices, what):
     """The library's view of a call (a reference to the struct; never changed) and its workspace. gate and out: their
     (shape, stride, dtype), or None."""
     if len(q_shape) != 3 or q_dtype not in _DTYPES or kc_dtype != q_dtype:
@@ -194,7 +204,7 @@ def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_d
         raise ValueError("out's last dim must be contiguous, and none expanded")
     if max_new is not None and not 1 <= max_new < 1 << 31:
         raise ValueError(f"max_new is a number of tokens, not {max_new}")
-    _lib.one_gpu("paged_attention", devices)
+    _lib.one_gpu(what, devices)
     p = _lib.PagedParams(tokens, requests, t_shape[1], kc_shape[0], kc_shape[1], heads, kv_heads, dim, _DTYPES[q_dtype], int(out is None),
                          dim ** -0.5 if scale is None else scale, _strides(q_shape, q_stride),
                          (0, 0) if gate is None else _strides(*gate[:2]), (heads * dim, dim) if out is None else _strides(*out[:2]),
@@ -209,6 +219,43 @@ def _strides(shape, stride):
 
 def _like(x: torch.Tensor | None):
     return None if x is None else (x.shape, x.stride(), x.dtype)
+
+
+def _attend(what: str, q, k_cache, v_cache, block_table, starts, lengths, ancestors, scale, gate, out, max_new) -> torch.Tensor:
+    """paged_attention, and with ancestors paged_tree_attention."""
+    _lib.not_recorded(what)
+    if _lib.dual_level() or (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (
+            gate is not None and gate.requires_grad) or (out is not None and out.requires_grad))):
+        _lib.inference_only(what, q, k_cache, v_cache, gate, out)
+    # (contiguous() would leave a contiguous view that starts off 16 bytes where it is)
+    if q.dim() == 3 and not _aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if gate is not None and gate.dim() == 3 and not _aligned(gate):
+        gate = gate.clone(memory_format=torch.contiguous_format)
+    lib = _lib.load()
+    p, need = _attention_params(
+        lib, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,
+        block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, _like(gate), _like(out),
+        None if scale is None else float(scale), None if max_new is None else int(max_new),
+        (q.get_device(), k_cache.get_device(), v_cache.get_device(), block_table.get_device(), starts.get_device(), lengths.get_device(),
+         _device(gate, q), _device(out, q), _device(ancestors, q)), what)
+    starts, lengths, block_table, dev = _int32(starts), _int32(lengths), block_table.contiguous(), q.device
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    gate_at = None if gate is None else gate.data_ptr()
+    with _lib.on_device(dev):
+        stream = _lib.current_stream(dev)
+        if ancestors is None:
+            status = lib.tjev_gdn_paged_attention(
+                p, stream, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
+                lengths.data_ptr(), gate_at, y.data_ptr(), ws.data_ptr(), need)
+        else:
+            ancestors = ancestors.contiguous()
+            status = lib.tjev_gdn_paged_tree_attention(
+                p, stream, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
+                lengths.data_ptr(), ancestors.data_ptr(), ancestors.shape[1], gate_at, y.data_ptr(), ws.data_ptr(), need)
+        _lib.check_status(status)
+    return y
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -230,33 +277,184 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     batches that may hold one by max_new or the default.)
     q, gate and out may be views whose rows start on 16 bytes (q and gate are copied where they do not); out is
     none of the inputs. What the cache holds elsewhere (NaN too) does not matter."""
-    _lib.not_recorded("paged_attention")
-    if _lib.dual_level() or (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or (
-            gate is not None and gate.requires_grad) or (out is not None and out.requires_grad))):
-        _lib.inference_only("paged_attention", q, k_cache, v_cache, gate, out)
-    # (contiguous() would leave a contiguous view that starts off 16 bytes where it is)
-    if q.dim() == 3 and not _aligned(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    if gate is not None and gate.dim() == 3 and not _aligned(gate):
-        gate = gate.clone(memory_format=torch.contiguous_format)
-    lib = _lib.load()
-    p, need = _attention_params(
-        lib, q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape, v_cache.stride(), v_cache.dtype,
-        block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, _like(gate), _like(out),
-        None if scale is None else float(scale), None if max_new is None else int(max_new),
-        (q.get_device(), k_cache.get_device(), v_cache.get_device(), block_table.get_device(), starts.get_device(), lengths.get_device(),
-         _device(gate, q), _device(out, q)))
-    starts, lengths, block_table, dev = _int32(starts), _int32(lengths), block_table.contiguous(), q.device
-    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        _lib.check_status(lib.tjev_gdn_paged_attention(
-            p, _lib.current_stream(dev), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), starts.data_ptr(),
-            lengths.data_ptr(), None if gate is None else gate.data_ptr(), y.data_ptr(), ws.data_ptr(), need))
-    return y
+    return _attend("paged_attention", q, k_cache, v_cache, block_table, starts, lengths, None, scale, gate, out, max_new)
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                         starts: torch.Tensor, lengths: torch.Tensor, ancestors: torch.Tensor, *, scale: float | None = None,
+                         gate: torch.Tensor | None = None, out: torch.Tensor | None = None, max_new: int | None = None) -> torch.Tensor:
+    """``paged_attention`` of trees of new tokens: each attends to all keys before its request's new tokens and, of those, to the
+    ones that its row of ``ancestors`` [N, W] int64 names (bit j % 64 of word j / 64: the request's j-th), in whatever order they
+    stand; as ``draft_tree`` makes them these are its ancestors and itself. A row may name any of them, or none (one that then
+    has no keys is 0); a request's tokens from 64 W on cannot be named. ``max_new``: the most new tokens of one request; it
+    chooses kernels and no row's keys. All else as for ``paged_attention``."""
+    if ancestors.dim() != 2 or ancestors.shape[0] != q.shape[0] or ancestors.shape[1] < 1 or ancestors.dtype != torch.int64:
+        raise ValueError(f"ancestors are [{q.shape[0]}, words] int64, not {tuple(ancestors.shape)} {ancestors.dtype}")
+    _check_sizes(ancestors.shape[1])
+    return _attend("paged_tree_attention", q, k_cache, v_cache, block_table, starts, lengths, ancestors, scale, gate, out, max_new)
 
 
 def _aligned(x: torch.Tensor) -> bool:
     """Whether the rows of x [N, heads, dim] start on 16 bytes."""
     s, e = x.stride(), 16 // x.element_size()
     return s[2] == 1 and (s[0] % e == 0 or x.shape[0] == 1) and (s[1] % e == 0 or x.shape[1] == 1) and x.data_ptr() % 16 == 0
+
+
+# ---------------------------------------------------------------- who holds the pages
+class Forked(NamedTuple):
+    """What paged_fork leaves: the block table [B', M] int32 and lengths [B'] int32 of the places that go on, the free list [F], the
+    pages taken of it [1] (more than there are: a shortage) and how many hold each page beside its first holder [pages], int32."""
+
+    block_table: torch.Tensor
+    lengths: torch.Tensor
+    free_pages: torch.Tensor
+    taken: torch.Tensor
+    shared: torch.Tensor
+
+
+def _layer(pair) -> tuple:
+    k, v = pair
+    return k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k.get_device(), v.get_device()
+
+
+@functools.lru_cache(maxsize=256)
+def _caches_params(what: str, like, layers: int, page_size, pages: int | None):
+    """The caches' part of a call's parameters, from the first layer's (None: there are no layers)."""
+    if like is None:
+        return dict(pages=1 if pages is None else pages, page_size=1 if page_size is None else page_size, layers=0)
+    k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype = like[:6]
+    if len(k_shape) != 4 or k_dtype not in _DTYPES:
+        raise ValueError(f"caches are [pages, page_size, heads, dim], float32 or bfloat16, not {tuple(k_shape)} {k_dtype}")
+    _check_caches(k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, k_shape[2], k_shape[3])
+    if min(k_shape) < 1:
+        raise ValueError(f"caches {tuple(k_shape)} without pages, heads or values")
+    if page_size not in (None, k_shape[1]) or pages not in (None, k_shape[0]):
+        raise ValueError(f"{what}: {pages} pages of {page_size} tokens, and caches {tuple(k_shape)}")
+    if any(s == 0 and n > 1 for strides in (k_stride, v_stride) for s, n in zip(strides, k_shape)):
+        raise ValueError("an expanded cache cannot be written")
+    return dict(pages=k_shape[0], page_size=k_shape[1], kv_heads=k_shape[2], dim=k_shape[3], dtype=_DTYPES[k_dtype], layers=layers,
+                k_stride=k_stride[:3], v_stride=v_stride[:3])
+
+
+def _layers(what: str, caches, page_size, pages):
+    """The layers' caches as the library takes them: their part of the parameters, their addresses, their devices."""
+    pairs = [tuple(pair) for pair in caches]
+    like = None
+    for pair in pairs:
+        if len(pair) != 2:
+            raise ValueError(f"{what} takes pairs of caches, k and v of every layer")
+        if like is None:
+            like = _layer(pair)
+        elif _layer(pair) != like:
+            raise ValueError(f"the layers' caches are alike in shape, strides, type and device: {like} and {_layer(pair)}")
+    flat = [x for pair in pairs for x in pair]
+    if any(x.requires_grad for x in flat) or _lib.dual_level():
+        _lib.inference_only(what, *flat)
+    n = len(pairs)
+    ks, vs = ((ctypes.c_void_p * max(1, n))(*(pair[i].data_ptr() for pair in pairs)) for i in (0, 1))
+    return _caches_params(what, like, n, page_size, pages), ks, vs, () if like is None else like[6:]
+
+
+@functools.lru_cache(maxsize=256)
+def _check_compact(t_shape, t_dtype, s_shape, s_dtype, l_shape, l_dtype, p_shape, p_dtype, k_shape, k_dtype, devices) -> None:
+    if len(t_shape) != 2 or t_dtype != torch.int32 or not 1 <= t_shape[0] <= _lib.MAX_REQUESTS or t_shape[1] < 1:
+        raise ValueError(f"block_table is [requests, pages] int32 of 1 to {_lib.MAX_REQUESTS} requests, not {tuple(t_shape)} {t_dtype}")
+    requests = t_shape[0]
+    _check_sizes(t_shape[1])
+    if s_shape != (requests + 1,) or l_shape != (requests,) or k_shape != (requests,):
+        raise ValueError(f"starts {tuple(s_shape)}, lengths {tuple(l_shape)} and kept {tuple(k_shape)} of {requests} requests")
+    if len(p_shape) != 2 or p_shape[0] != requests or p_shape[1] < 1:
+        raise ValueError(f"path is [{requests}, max_new], not {tuple(p_shape)}")
+    _check_sizes(p_shape[1])
+    for dt in (s_dtype, l_dtype, p_dtype, k_dtype):
+        if dt not in (torch.int32, torch.int64):
+            raise ValueError(f"starts, lengths, path and kept are int32 or int64, not {dt}")
+    _lib.one_gpu("paged_compact", devices)
+
+
+def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor,
+                  kept: torch.Tensor) -> torch.Tensor:
+    """Moves the kept ones of every request's new tokens to the front of them, in all layers' caches at once, in place, and
+    returns the lengths that are left [B] int32: token path[b, j] becomes the j-th, j < kept[b], as ``verify_drafts`` names them.
+
+    ``caches``: the (k_cache, v_cache) of every layer, alike in shape and strides (none: the lengths alone). ``starts`` and
+    ``lengths`` are the step's, with the new tokens. A request's numbers in ``path`` [B, max_new] grow; those that are less than their
+    place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct. What
+    stands behind a request's kept tokens is left as it was."""
+    _lib.not_recorded("paged_compact")
+    params, ks, vs, devices = _layers("paged_compact", caches, None, None)
+    _check_compact(block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, path.shape, path.dtype,
+                   kept.shape, kept.dtype, (block_table.get_device(), starts.get_device(), lengths.get_device(), path.get_device(),
+                                            kept.get_device(), *devices))
+    dev = block_table.device
+    table, starts, lengths, path, kept = block_table.contiguous(), _int32(starts), _int32(lengths), _int32_near(path), _int32_near(kept)
+    out = torch.empty(table.shape[0], dtype=torch.int32, device=dev)
+    p = _lib.PagesParams(max_new=path.shape[1], requests=table.shape[0], table_width=table.shape[1], **params)
+    with _lib.on_device(dev):
+        _lib.check_status(_lib.load().tjev_gdn_paged_compact(
+            ctypes.byref(p), _lib.current_stream(dev), ks, vs, table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), path.data_ptr(),
+            kept.data_ptr(), out.data_ptr()))
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _check_fork(t_shape, t_dtype, l_shape, l_dtype, s_shape, s_dtype, keep, f_shape, f_dtype, taken, sh_shape, sh_dtype, page_size: int,
+                devices) -> None:
+    if len(t_shape) != 2 or t_dtype != torch.int32 or not 1 <= t_shape[0] <= _lib.MAX_REQUESTS or t_shape[1] < 1:
+        raise ValueError(f"block_table is [requests, pages] int32 of 1 to {_lib.MAX_REQUESTS} requests, not {tuple(t_shape)} {t_dtype}")
+    if page_size < 1:
+        raise ValueError(f"pages of at least one token, not {page_size}")
+    if l_shape != (t_shape[0],):
+        raise ValueError(f"lengths {tuple(l_shape)} of {t_shape[0]} requests")
+    if len(s_shape) != 1 or not 1 <= s_shape[0] <= _lib.MAX_REQUESTS or keep not in (None, (s_shape, keep and keep[1])):
+        raise ValueError(f"sources and keep are [new requests] of 1 to {_lib.MAX_REQUESTS}, not {tuple(s_shape)} and {keep and tuple(keep[0])}")
+    if len(f_shape) != 1 or len(sh_shape) != 1 or sh_shape[0] < 1 or taken[0] != 1:
+        raise ValueError("free_pages is a list of pages, taken one number, and shared a number for every page")
+    for dt in (l_dtype, s_dtype, f_dtype, taken[1], sh_dtype, *(() if keep is None else (keep[1],))):
+        if dt not in (torch.int32, torch.int64):
+            raise ValueError(f"lengths, sources, keep, pages and their numbers are int32 or int64, not {dt}")
+    _check_sizes(t_shape[0] * t_shape[1], s_shape[0] * t_shape[1], f_shape[0], sh_shape[0], page_size)
+    _lib.one_gpu("paged_fork", devices)
+
+
+def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources: torch.Tensor, keep: torch.Tensor | None,
+               free_pages: torch.Tensor, taken: torch.Tensor, shared: torch.Tensor, *, page_size: int) -> Forked:
+    """Which requests go on, with what: place i of the new table with the first ``keep[i]`` tokens (None: all) of place
+    ``sources[i]`` [B'] of ``block_table`` [B, M] (-1: it is unused). That is a batch's samples or beams (a source several times),
+    a roll back behind rejected drafts (``keep`` shorter), requests that end (no place goes on from them) and a table made dense, all at
+    once, on the GPU. ``lengths`` [B] are those that the places have pages for: after a step the step's own (``PagedTables.lengths``), not what
+    was kept of it, or the pages of the rest would be nobody's.
+
+    ``shared`` [pages]: how many hold each page beside its first holder (0 in the beginning). Places share pages; but a last page with room
+    in it, where the next tokens go, has one holder: the first place that goes on in it where nobody holds it otherwise, and for each
+    other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides;
+    those may be none). Pages that nobody holds any more come back in front of index ``taken`` of ``free_pages`` [F], in the
+    table's order, and are the first to be taken again; the list needs room for them there, as it has where all of them were
+    taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
+
+    Nothing given is changed but the caches: the new table, lengths, list, ``taken`` and ``shared`` come back."""
+    _lib.not_recorded("paged_fork")
+    page_size = int(page_size)
+    params, ks, vs, devices = _layers("paged_fork", caches, page_size, shared.shape[0] if shared.dim() == 1 else None)
+    _check_fork(block_table.shape, block_table.dtype, lengths.shape, lengths.dtype, sources.shape, sources.dtype,
+                None if keep is None else (keep.shape, keep.dtype), free_pages.shape, free_pages.dtype, (taken.numel(), taken.dtype),
+                shared.shape, shared.dtype, page_size,
+                (block_table.get_device(), lengths.get_device(), sources.get_device(), _device(keep, lengths), free_pages.get_device(),
+                 taken.get_device(), shared.get_device(), *devices))
+    lib, dev = _lib.load(), block_table.device
+    table, lengths, sources, free, taken, shared = (block_table.contiguous(), _int32(lengths), _int32_near(sources), _int32(free_pages),
+                                                    _int32(taken), _int32(shared))
+    keep = None if keep is None else _int32_near(keep)
+    requests, width, new, n_free, pages = *table.shape, sources.shape[0], free.shape[0], shared.shape[0]
+    table_out = torch.empty((new, width), dtype=torch.int32, device=dev)
+    free_out, shared_out, lengths_out, taken_out = torch.empty(n_free + pages + new + 1, dtype=torch.int32, device=dev).split(
+        (n_free, pages, new, 1))
+    p = _lib.PagesParams(n_free=n_free, requests=requests, new_requests=new, table_width=width, **params)
+    need = lib.tjev_gdn_fork_workspace_bytes(ctypes.byref(p))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        _lib.check_status(lib.tjev_gdn_paged_fork(
+            ctypes.byref(p), _lib.current_stream(dev), ks, vs, table.data_ptr(), lengths.data_ptr(), sources.data_ptr(),
+            None if keep is None else keep.data_ptr(), free.data_ptr(), taken.data_ptr(), shared.data_ptr(), table_out.data_ptr(),
+            lengths_out.data_ptr(), free_out.data_ptr(), taken_out.data_ptr(), shared_out.data_ptr(), ws.data_ptr(), need))
+    return Forked(table_out, lengths_out, free_out, taken_out, shared_out)
