@@ -24,6 +24,14 @@ def library(monkeypatch):
     from tjev_amd import _lib, drafts, paged
 
     lib = _Library()
+    lib.addresses = []
+
+    def compact(p, stream, ks, vs, *rest):
+        lib.calls.append(("tjev_gdn_paged_compact", (p, stream, ks, vs, *rest)))
+        lib.addresses = [list((ctypes.c_uint64 * p._obj.layers).from_address(a)) for a in (ks, vs)]
+        return 0
+
+    lib.tjev_gdn_paged_compact = compact
     lib.tjev_gdn_verify_workspace_bytes = lambda p: 256
     lib.tjev_gdn_fork_workspace_bytes = lambda p: 256
     lib.tjev_gdn_paged_workspace_bytes = lambda p: 256
@@ -32,7 +40,7 @@ def library(monkeypatch):
     monkeypatch.setattr(_lib, "current_stream", lambda device: 0)
     monkeypatch.setattr(_lib, "on_device", lambda device: contextlib.nullcontext())
     yield lib
-    for kept in (paged._attention_params, paged._caches_params, paged._check_compact, paged._check_fork, drafts._tree_params,
+    for kept in (paged._attention_params, paged._compact_params, paged._fork_params, drafts._tree_params,
                  drafts._verify_params):
         kept.cache_clear()  # checks that passed here alone
 
@@ -189,7 +197,7 @@ def test_layers_reach_the_library(library):
     (_, args), = library.calls
     p = args[0]._obj
     assert p.layers == 20 and list(p.k_stride) == [2048, 64, 1024] and (p.pages, p.page_size, p.kv_heads, p.dim) == (4, 16, 2, 64)
-    assert list(args[2]) == [k.data_ptr() for k, _ in pairs] and list(args[3]) == [v.data_ptr() for _, v in pairs]
+    assert library.addresses == [[k.data_ptr() for k, _ in pairs], [v.data_ptr() for _, v in pairs]]
     library.calls.clear()
     _call("paged_fork", caches=[])
     p = library.calls[0][1][0]._obj

@@ -14,7 +14,8 @@
 // as the first v whose running sum of w is over u_root times the whole. Every emitted token is then distributed as the
 // target's. The sums and products are taken in 64 bits: a choice among 100000 tokens must not depend on the order of a sum.
 // The rows that the last tokens are drawn from are read by as many workgroups as there are slices of kSlice
-// numbers (k_verify_sums; each finds the request's walk by itself), and the one slice that holds the token once more (k_verify_draw).
+// numbers (k_verify_sums; each finds the request's walk by itself), and the one slice that holds the token once more (k_verify_draw,
+// which loads what it needs to find it at once).
 #include <hip/hip_runtime.h>
 
 #include "../../include/tjev_gdn.h"
@@ -94,17 +95,20 @@ __global__ __launch_bounds__(64) void k_draft_tree(TreeArgs A) {
 }
 
 // ---------------------------------------------------------------- verification
-constexpr int kSlice = 4096;
+constexpr int kSlice = 4096, kPart = kSlice / (kThreads / 64);  // numbers of a workgroup, of a wave
 
 struct VerifyArgs {
   long N, most, pt, qt;  // tokens; the most of a request; elements from row to row
-  int B, V, slices;
+  int B, V, slices, parts;
   const int32_t *tokens, *parents, *starts;
   const float* u;
   const char *p, *q;     // q: null for chosen tokens
   int32_t *out, *path, *kept;
-  double* sums;          // [B, slices]
-  int* ends;             // [B, 2]: the row that the walk ends in, q's row or -1
+  // for the second launch: where each walk ends, the parts' sums; of each slice whether it has rejected tokens, and those as bits
+  struct WalkEnd* ends;
+  double* sums;
+  int32_t* marked;
+  uint32_t* bits;
   // the number of token i's parent within the request
   __device__ __forceinline__ int up(const Rows& r, long i) const { return parents ? parents[r.s0 + i] : (int)i - 1; }
 };
@@ -115,19 +119,26 @@ __device__ __forceinline__ float number(const char* base, long at) {
   return reinterpret_cast<const float*>(base)[at];
 }
 // what is no positive number counts as 0
-__device__ __forceinline__ float clean(float x) { return x > 0.f && x < __builtin_inff() ? x : 0.f; }
+__device__ __forceinline__ float clean(float x) { return __builtin_amdgcn_classf(x, 0x180) ? x : 0.f; }  // positive, finite
 
-// The walk of a request, by one wave: the node it ends in, and the child whose draft distribution is taken off (or -1).
-// write: its path, accepted tokens and their number too.
+// What the second launch needs of a request: the rows that its token is drawn from (q's: -1 for none; p's: -1 for a request
+// without tokens), its number, and the place for the token
+struct WalkEnd {
+  long prow, qrow, out;
+  double u;
+};
+
+// The walk of a request, by one wave: the node it ends in, the child whose draft distribution is taken off (or -1), and how many
+// tokens it has. write: its path, accepted tokens and their number too.
 struct End {
-  long node, off;
+  long node, off, count;
 };
 template <class T, bool CHOSEN>
 __device__ __forceinline__ End walk(const VerifyArgs& A, int b, const Rows& r, bool write) {
   const int ln = lane();
   const long n = min(r.n, A.most);
   int32_t *path = A.path + b * A.most, *out = A.out + b * A.most;
-  End end{0, -1};
+  End end{0, -1, 0};
   long count = 1;
   if (write && ln == 0 && n > 0) path[0] = 0;
   if constexpr (!CHOSEN) {
@@ -197,85 +208,107 @@ __device__ __forceinline__ End walk(const VerifyArgs& A, int b, const Rows& r, b
     for (long j = count + ln; j < A.most; j += 64) path[j] = out[j] = -1;
     if (ln == 0) A.kept[b] = (int)count;
   }
+  end.count = count;
   return end;
 }
 
-// The rejected ones of chosen tokens in the slice from v0 on, as bits: all children of the node that the walk ended in.
-__device__ __forceinline__ void reject(const VerifyArgs& A, const Rows& r, long node, long v0, uint32_t* sbits) {
-  for (int i = threadIdx.x; i < kSlice / 32; i += kThreads) sbits[i] = 0;
-  __syncthreads();
+// The rejected ones of chosen tokens in the slice from v0 on, as bits: all children of the node that the walk ended in. Whether there
+// are any.
+__device__ __forceinline__ bool reject(const VerifyArgs& A, const Rows& r, long node, long v0, uint32_t* sbits) {
   const long n = min(r.n, A.most);
+  bool any = false;
   for (long i = node + 1 + threadIdx.x; i < n; i += kThreads) {
     const long x = A.up(r, i) == node ? A.tokens[r.s0 + i] - v0 : -1;
-    if (x >= 0 && x < kSlice) atomicOr(&sbits[x / 32], 1u << (x % 32));
+    if (x >= 0 && x < kSlice) {
+      atomicOr(&sbits[x / 32], 1u << (x % 32));
+      any = true;
+    }
   }
-  __syncthreads();
+  return __syncthreads_or(any);
 }
 
 // 16 bytes that start on an element
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) Piece {
-  T x[16 / sizeof(T)];
+  uint64_t lo, hi;
 };
 
-// the weights of the E numbers from v on; behind the row's end 0
-template <class T, bool CHOSEN, int E>
-__device__ __forceinline__ void weights(const VerifyArgs& A, const char* prow, const char* qrow, long v, const uint32_t* sbits, long v0,
-                                        double (&w)[E]) {
-  static_assert(E * sizeof(T) == 16, "");
-  float p[E], q[E];
-  if (v + E <= A.V) {
-    const Piece<T> a = *reinterpret_cast<const Piece<T>*>(prow + v * sizeof(T));
-    const Piece<T> c = qrow ? *reinterpret_cast<const Piece<T>*>(qrow + v * sizeof(T)) : Piece<T>{};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if constexpr (sizeof(T) == 2) {
-        p[e] = bf2f(a.x[e]);
-        q[e] = bf2f(c.x[e]);
-      } else {
-        p[e] = a.x[e];
-        q[e] = c.x[e];
-      }
+// The E numbers of a row from v on, 0 behind its end: the row's last piece, moved down, without a branch to each number
+template <class T, int E>
+__device__ __forceinline__ void numbers(const VerifyArgs& A, const char* row, long v, float (&x)[E]) {
+  constexpr int BITS = 8 * sizeof(T);
+  static_assert(E * BITS == 128, "");
+  uint64_t lo = 0, hi = 0;
+  if (A.V >= E) {
+    const long at = min(v, (long)A.V - E);
+    const Piece<T> a = *reinterpret_cast<const Piece<T>*>(row + at * (long)sizeof(T));
+    lo = a.lo, hi = a.hi;
+    if (v > at) {
+      const int n = (int)min((v - at) * BITS, 128l);
+      lo = n < 64 ? lo >> n | hi << (64 - n) : n < 128 ? hi >> (n - 64) : 0;
+      hi = n < 64 ? hi >> n : 0;
     }
   } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      p[e] = v + e < A.V ? number<T>(prow, v + e) : 0.f;
-      q[e] = qrow && v + e < A.V ? number<T>(qrow, v + e) : 0.f;
+    for (int e = 0; e < A.V; ++e) {
+      const uint64_t y = v + e < A.V ? reinterpret_cast<const std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>*>(row)[v + e] : 0;
+      (e * BITS < 64 ? lo : hi) |= y << (e * BITS % 64);
     }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const double x = (double)clean(p[e]) - (double)clean(q[e]);
-    w[e] = x > 0.0 ? x : 0.0;
-    if (CHOSEN && sbits && (sbits[(v - v0 + e) / 32] >> ((v - v0 + e) % 32) & 1)) w[e] = 0.0;
+    const uint32_t y = (uint32_t)((e * BITS < 64 ? lo : hi) >> (e * BITS % 64));
+    x[e] = clean(__uint_as_float(sizeof(T) == 2 ? y << 16 : y));
   }
 }
 
-__device__ __forceinline__ double sum_wave(double v) {
+// the weights of the E numbers from v on; sbits: the rejected tokens from v0 on, or null
+template <class T, bool CHOSEN, int E>
+__device__ __forceinline__ void weights(const VerifyArgs& A, const char* prow, const char* qrow, long v, const uint32_t* sbits, long v0,
+                                        double (&w)[E]) {
+  float p[E];
+  numbers<T>(A, prow, v, p);
+  if constexpr (CHOSEN) {
+    static_assert(32 % E == 0, "E numbers lie in one word: v is a multiple of E");
+    const uint32_t off = sbits && v < A.V ? sbits[(v - v0) / 32] >> ((v - v0) % 32) : 0;
 #pragma unroll
-  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+    for (int e = 0; e < E; ++e) w[e] = off >> e & 1 ? 0.f : p[e];
+  } else if (qrow) {
+    float q[E];
+    numbers<T>(A, qrow, v, q);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const double x = (double)p[e] - (double)q[e];
+      w[e] = x > 0.0 ? x : 0.0;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = p[e];
+  }
+}
+
+// the lane's number moved by a row shift (or broadcast) within the wave, 0 where none comes
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// running sum over the wave's lanes: within rows of 16, then each row's last to the row behind it, then the first half's last to the
+// second
+__device__ __forceinline__ double scan_wave(double v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ double sum_block(double v, double* swave) {
-  v = sum_wave(v);
-  __syncthreads();
-  if (lane() == 0) swave[wave()] = v;
-  __syncthreads();
-  double s = 0.0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) s += swave[w];
-  return s;
-}
-// running sum over the workgroup's threads, the whole, and what stands before the thread: the sum of the thread before it, bit by bit
+// running sum over the workgroup's threads, the whole, and what stands before the thread: the sum of the thread before it
 __device__ __forceinline__ double scan_block(double v, double* swave, double& total, double& until) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double t = __shfl_up(v, d);
-    if (lane() >= d) v += t;
-  }
-  until = __shfl_up(v, 1);
-  if (lane() == 0) until = 0.0;
+  v = scan_wave(v);
+  until = moved<0x138, 0xf>(v);  // the lane before, 0 in the first
   __syncthreads();
   if (lane() == 63) swave[wave()] = v;
   __syncthreads();
@@ -290,138 +323,275 @@ __device__ __forceinline__ double scan_block(double v, double* swave, double& to
   return v + before;
 }
 
+// The first of a wave's lanes whose running sum is over the goal, or (over: false) the last with a weight, or -1
+__device__ __forceinline__ int pick_lane(double mine, double upto, double goal, bool& over) {
+  const uint64_t some = __ballot(mine > 0.0), first = __ballot(mine > 0.0 && upto > goal);
+  over = first != 0;
+  return first ? __builtin_ctzll(first) : some ? 63 - __builtin_clzll(some) : -1;
+}
+// The same among the workgroup's waves: the first of all in `found`, the last in `last`. (One lane of a wave adds to each: left to
+// the compiler, an atomic of many lanes on one address is a loop over them.)
+__device__ __forceinline__ void note(double mine, double upto, double goal, int at, int& found, int& last) {
+  const uint64_t some = __ballot(mine > 0.0), first = __ballot(mine > 0.0 && upto > goal);
+  if (some && lane() == 63 - __builtin_clzll(some)) atomicMax(&last, at);
+  if (first && lane() == __builtin_ctzll(first)) atomicMin(&found, at);
+}
+// The same of numbers in a row, of which one is positive; run: the sum before them, then the sum before the one picked
+template <int N>
+__device__ __forceinline__ int pick(const double (&x)[N], double goal, bool over, double& run) {
+  int found = 0;
+  bool done = false;
+  double sum = run;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (x[i] > 0.0 && !done) {
+      found = i;
+      run = sum;
+      done = over && sum + x[i] > goal;
+    }
+    sum += x[i];
+  }
+  return found;
+}
+
+// The sum of a part of the row, by one wave, in its last lane
 template <class T, bool CHOSEN>
-__device__ __forceinline__ double slice_sum(const VerifyArgs& A, const char* prow, const char* qrow, long v0, const uint32_t* sbits,
-                                            double* swave) {
-  constexpr int E = 16 / sizeof(T), RUNS = kSlice / (kThreads * E);
+__device__ __forceinline__ double part_sum(const VerifyArgs& A, const char* prow, const char* qrow, long from, const uint32_t* sbits, long v0) {
+  constexpr int E = 16 / sizeof(T), RUNS = kPart / (64 * E);
   double s = 0.0;
 #pragma unroll
   for (int i = 0; i < RUNS; ++i) {
     double w[E];
-    weights<T, CHOSEN, E>(A, prow, qrow, v0 + (i * kThreads + threadIdx.x) * E, sbits, v0, w);
+    weights<T, CHOSEN, E>(A, prow, qrow, from + (i * 64 + lane()) * E, sbits, v0, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) s += w[e];
   }
-  return sum_block(s, swave);
+  return scan_wave(s);
 }
 
 template <class T, bool CHOSEN>
 __global__ __launch_bounds__(kThreads) void k_verify_sums(VerifyArgs A) {
-  __shared__ double swave[kThreads / 64];
   __shared__ uint32_t sbits[kSlice / 32];
   __shared__ long send[2];
-  GDN_POISON_LDS(swave, sbits, send);
+  GDN_POISON_LDS(sbits, send);
   const int b = blockIdx.y, slice = blockIdx.x;
   const Rows r = rows_of(A.starts, b, A.N);
+  if (CHOSEN)
+    for (int i = threadIdx.x; i < kSlice / 32; i += kThreads) sbits[i] = 0;
   if (uniform(wave()) == 0) {
     const End e = walk<T, CHOSEN>(A, b, r, slice == 0);
     if (lane() == 0) {
       send[0] = e.node;
       send[1] = e.off;
-      if (slice == 0) A.ends[2 * b] = (int)e.node, A.ends[2 * b + 1] = (int)send[1];
+      if (slice == 0)
+        A.ends[b] = {r.n ? r.s0 + e.node : -1, e.off >= 0 ? r.s0 + e.off : -1, b * A.most + e.count - 1, r.n ? (double)A.u[r.s0] : 0.0};
     }
   }
   __syncthreads();
   if (!r.n) return;
-  const long node = send[0], off = send[1], v0 = (long)slice * kSlice;
-  if (CHOSEN) reject(A, r, node, v0, sbits);
+  const long node = send[0], off = send[1], v0 = (long)slice * kSlice, at = (long)b * A.slices + slice;
+  bool any = false;
+  if (CHOSEN) {
+    any = reject(A, r, node, v0, sbits);
+    if (threadIdx.x == 0) A.marked[at] = any;
+    if (any)
+      for (int i = threadIdx.x; i < kSlice / 32; i += kThreads) A.bits[at * (kSlice / 32) + i] = sbits[i];
+  }
   const char* prow = A.p + (r.s0 + node) * A.pt * (long)sizeof(T);
   const char* qrow = off >= 0 ? A.q + (r.s0 + off) * A.qt * (long)sizeof(T) : nullptr;
-  const double s = slice_sum<T, CHOSEN>(A, prow, qrow, v0, sbits, swave);
-  if (threadIdx.x == 0) A.sums[(long)b * A.slices + slice] = s;
+  const int part = slice * (kSlice / kPart) + uniform(wave());
+  if ((long)part * kPart >= A.V) return;
+  const double s = part_sum<T, CHOSEN>(A, prow, qrow, (long)part * kPart, any ? sbits : nullptr, v0);
+  if (lane() == 63) A.sums[(long)b * A.parts + part] = s;
 }
 
-// The first v whose running sum is over u times the whole: the slice by the slices' sums, then the place in it. Where rounding
+// The first v whose running sum is over u times the whole: the part by the parts' sums, then the place in it. Where rounding
 // leaves none (or u is 1 or more), the last token with a weight; a row without any gives -1.
 template <class T, bool CHOSEN>
 __global__ __launch_bounds__(kThreads) void k_verify_draw(VerifyArgs A) {
-  constexpr int E = 16 / sizeof(T), PER = kSlice / kThreads;
-  __shared__ double swave[kThreads / 64];
-  __shared__ uint32_t sbits[kSlice / 32];
-  __shared__ double sbefore;
+  constexpr int E = 16 / sizeof(T);
+  static_assert(kPart % E == 0 && kPart / E <= kThreads, "a part is one load of the workgroup's");
+  __shared__ double swave[kThreads / 64], sbefore;
   __shared__ int sfound, slast;
-  GDN_POISON_LDS(swave, sbits, sbefore, sfound, slast);
+  GDN_POISON_LDS(swave, sbefore, sfound, slast);
   const int b = blockIdx.x, tid = threadIdx.x;
-  const Rows r = rows_of(A.starts, b, A.N);
-  if (!r.n) return;
-  const long node = A.ends[2 * b], off = A.ends[2 * b + 1];
-  const char* prow = A.p + (r.s0 + node) * A.pt * (long)sizeof(T);
-  const char* qrow = off >= 0 ? A.q + (r.s0 + off) * A.qt * (long)sizeof(T) : nullptr;
-  double* sums = A.sums + (long)b * A.slices;
+  const WalkEnd end = A.ends[b];
+  double* sums = A.sums + (long)b * A.parts;
+  double mine = tid < A.parts ? sums[tid] : 0.0;  // on its way with the end
+  if (end.prow < 0) return;
+  const char* prow = A.p + end.prow * A.pt * (long)sizeof(T);
+  const char* qrow = end.qrow >= 0 ? A.q + end.qrow * A.qt * (long)sizeof(T) : nullptr;
+  int32_t* out = A.out + end.out;
+  if (tid == 0) sfound = 0x7fffffff, slast = -1;
   bool rest = CHOSEN || qrow;  // something is taken off the row
-  double total = 0.0;
-  for (int turn = 0; turn < 2; ++turn) {
-    double mine = 0.0;
-    for (int s = tid; s < A.slices; s += kThreads) mine += sums[s];
-    total = sum_block(mine, swave);
+  double total, goal;
+  while (true) {
+    // the first part over the goal, kThreads of them at a time (their whole first, where there are more)
+    double before = 0.0, until, upto;
+    if (A.parts > kThreads) {
+      for (int s = tid + kThreads; s < A.parts; s += kThreads) mine += sums[s];
+      scan_block(mine, swave, total, until);
+      goal = end.u > 0.0 ? end.u * total : 0.0;
+    }
+    for (int s0 = 0; s0 < A.parts; s0 += kThreads) {
+      const int s = s0 + tid;
+      if (A.parts > kThreads) mine = s < A.parts ? sums[s] : 0.0;
+      double all;
+      upto = before + scan_block(mine, swave, all, until);
+      if (A.parts <= kThreads) {
+        total = all;
+        goal = end.u > 0.0 ? end.u * total : 0.0;
+      }
+      note(mine, upto, goal, s, sfound, slast);
+      __syncthreads();
+      if (sfound == s) sbefore = before + until;
+      if (sfound != 0x7fffffff) break;
+      before += all;
+    }
     if (total > 0.0 || !rest) break;
-    // nothing is left: from the row itself, whose slices are summed here
+    // nothing is left: from the row itself, whose parts are summed here
     rest = false;
     qrow = nullptr;
-    for (int s = 0; s < A.slices; ++s) {
-      const double x = slice_sum<T, false>(A, prow, nullptr, (long)s * kSlice, nullptr, swave);
-      if (tid == 0) sums[s] = x;
+    for (int s = uniform(wave()); s < A.parts; s += kThreads / 64) {
+      const double x = part_sum<T, false>(A, prow, nullptr, (long)s * kPart, nullptr, 0);
+      if (lane() == 63) sums[s] = x;
     }
-    __threadfence_block();
     __syncthreads();
+    mine = tid < A.parts ? sums[tid] : 0.0;
   }
-  if (tid == 0) sfound = -1, slast = -1;
   __syncthreads();
-  const double u = A.u[r.s0], goal = u > 0.0 ? u * total : 0.0;
-  double before = 0.0;  // of the turns
-  for (int s0 = 0; s0 < A.slices; s0 += kThreads) {
-    const int s = s0 + tid;
-    const double v = s < A.slices ? sums[s] : 0.0;
-    double all, until;
-    const double upto = before + scan_block(v, swave, all, until);
-    until += before;
-    if (v > 0.0) atomicMax(&slast, s);
-    if (until <= goal && upto > goal) sfound = s, sbefore = until;  // one thread's
-
-    before += all;
-    __syncthreads();
-    if (sfound >= 0) break;
-  }
-  const int slice = sfound >= 0 ? sfound : slast;
-  const double start = sfound >= 0 ? sbefore : -1.0;
-  __syncthreads();
-  int32_t* out = A.out + b * A.most + A.kept[b] - 1;
-  if (slice < 0) {
+  bool over = sfound != 0x7fffffff;
+  const int part = uniform(over ? sfound : slast);
+  const double start = sbefore;
+  if (part < 0) {
     if (tid == 0) *out = -1;
     return;
   }
-  const long v0 = (long)slice * kSlice;
-  const uint32_t* bits = CHOSEN && rest ? sbits : nullptr;
-  if (CHOSEN && rest) reject(A, r, node, v0, sbits);
+  __syncthreads();
   if (tid == 0) sfound = 0x7fffffff, slast = -1;
-  double w[PER], sum = 0.0;
-  int last = -1;
+  // the numbers of the part, E to a thread, and whether the rejected ones are among them
+  const long v = (long)part * kPart + tid * E, at = (long)b * A.slices + part / (kSlice / kPart);
+  double x[E] = {};
+  if (tid < kPart / E) weights<T, false, E>(A, prow, qrow, v, nullptr, 0, x);
+  if (CHOSEN && rest && A.marked[at] && tid < kPart / E) {
+    const uint32_t off = A.bits[at * (kSlice / 32) + v % kSlice / 32] >> (v % 32);
 #pragma unroll
-  for (int i = 0; i < PER; i += E) {
-    double x[E];
-    weights<T, CHOSEN, E>(A, prow, qrow, v0 + tid * PER + i, bits, v0, x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      w[i + e] = x[e];
-      sum += x[e];
-      if (x[e] > 0.0) last = i + e;
-    }
+    for (int e = 0; e < E; ++e)
+      if (off >> e & 1) x[e] = 0.0;
   }
-  double all, until;
-  const double upto = scan_block(sum, swave, all, until);
-  if (last >= 0) atomicMax(&slast, tid * PER + last);
-  if (start >= 0.0 && start + upto > goal) {
-    double run = start + until;
-    int at = -1;
+  mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      run += w[i];
-      if (at < 0 && w[i] > 0.0 && run > goal) at = i;
-    }
-    if (at >= 0) atomicMin(&sfound, tid * PER + at);
+  for (int e = 0; e < E; ++e) mine += x[e];
+  double all, until;
+  const double upto = start + scan_block(mine, swave, all, until);
+  note(mine, upto, over ? goal : __builtin_inf(), tid, sfound, slast);
+  __syncthreads();
+  over = sfound != 0x7fffffff;
+  if (tid == (over ? sfound : slast)) {
+    double run = start + until;
+    *out = (int)v + pick(x, goal, over, run);
+  }
+}
+
+// Vocabularies of up to kOneRow: the walk and both passes over the row in one launch, a request to a workgroup of kOne threads.
+constexpr int kOne = 1024, kOneRow = 1 << 16;
+
+template <class T, bool CHOSEN>
+__global__ __launch_bounds__(kOne) void k_verify_one(VerifyArgs A) {
+  constexpr int E = 16 / sizeof(T), NW = kOne / 64, TURNS = kOneRow / (kOne * E), AT_ONCE = 16 / E;
+  __shared__ double sturn[TURNS][kOne];  // the threads' sums of each turn
+  __shared__ uint32_t sbits[CHOSEN ? kOneRow / 32 : 1];
+  __shared__ double ssum[NW];
+  __shared__ long send[3];
+  __shared__ int smarked;
+  GDN_POISON_LDS(sturn, sbits, ssum, send, smarked);
+  const int b = blockIdx.x, tid = threadIdx.x, w = uniform(wave()), ln = lane();
+  const Rows r = rows_of(A.starts, b, A.N);
+  if (CHOSEN)
+    for (int i = tid; i < (A.V + 31) / 32; i += kOne) sbits[i] = 0;
+  if (tid == 0) smarked = 0;
+  if (w == 0) {
+    const End e = walk<T, CHOSEN>(A, b, r, true);
+    if (ln == 0) send[0] = e.node, send[1] = e.off, send[2] = e.count;
   }
   __syncthreads();
-  if (tid == 0) *out = (int)v0 + (sfound != 0x7fffffff ? sfound : slast);
+  if (!r.n) return;
+  const long node = send[0], off = send[1];
+  const double u = A.u[r.s0];
+  if (CHOSEN) {
+    const long n = min(r.n, A.most);
+    for (long i = node + 1 + tid; i < n; i += kOne) {
+      const int x = A.up(r, i) == node ? A.tokens[r.s0 + i] : -1;
+      if (x >= 0 && x < A.V) {
+        atomicOr(&sbits[x / 32], 1u << (x % 32));
+        smarked = 1;
+      }
+    }
+    __syncthreads();
+  }
+  const char* prow = A.p + (r.s0 + node) * A.pt * (long)sizeof(T);
+  const char* qrow = off >= 0 ? A.q + (r.s0 + off) * A.qt * (long)sizeof(T) : nullptr;
+  int32_t* out = A.out + b * A.most + send[2] - 1;
+  const uint32_t* bits = CHOSEN && smarked ? sbits : nullptr;
+  // A wave has a part of the row to itself, `turns` times 64 E numbers side by side: its sum is one of 16
+  const int turns = (A.V + kOne * E - 1) / (kOne * E);
+  const long v0 = (long)w * turns * 64 * E + ln * E;
+  while (true) {
+    double mine = 0.0;
+    for (int t0 = 0; t0 < turns; t0 += AT_ONCE) {
+      double x[AT_ONCE][E];
+#pragma unroll
+      for (int t = 0; t < AT_ONCE; ++t)
+        if (t0 + t < turns) weights<T, CHOSEN, E>(A, prow, qrow, v0 + (t0 + t) * 64 * E, bits, 0, x[t]);
+#pragma unroll
+      for (int t = 0; t < AT_ONCE; ++t)
+        if (t0 + t < turns) {
+          double s = 0.0;
+#pragma unroll
+          for (int e = 0; e < E; ++e) s += x[t][e];
+          sturn[t0 + t][tid] = s;
+          mine += s;
+        }
+    }
+    mine = scan_wave(mine);
+    if (ln == 63) ssum[w] = mine;
+    __syncthreads();
+    // every wave sums the 16, and knows whether the token is its own
+    const double of = ln < NW ? ssum[ln] : 0.0;
+    double upto = scan_wave(of), until = moved<0x138, 0xf>(upto);
+    const double total = __shfl(upto, NW - 1), goal = u > 0.0 ? u * total : 0.0;
+    bool over;
+    const int at = pick_lane(of, upto, goal, over);
+    if (at < 0 && (bits || qrow)) {  // nothing is left: from the row itself
+      bits = nullptr;
+      qrow = nullptr;
+      __syncthreads();
+      continue;
+    }
+    if (at < 0 && tid == 0) *out = -1;
+    if (w != at) return;
+    double before = __shfl(until, at);
+    // the turn: the first that goes over the goal, or the last with a weight
+    int turn = -1;
+    double start = 0.0;
+    for (int t = 0; t < turns && (turn < 0 || !over || !(before > goal)); ++t) {
+      const double s = sturn[t][tid];
+      if (!__any(s > 0.0)) continue;
+      turn = t;
+      start = before;
+      before += __shfl(scan_wave(s), 63);
+    }
+    const long v = v0 + turn * 64 * E;
+    double x[E];
+    weights<T, CHOSEN, E>(A, prow, qrow, v, bits, 0, x);
+    mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += x[e];
+    upto = scan_wave(mine);
+    double run = start + moved<0x138, 0xf>(upto);
+    if (ln == pick_lane(mine, start + upto, over ? goal : __builtin_inf(), over)) *out = (int)v + pick(x, goal, over, run);
+    return;
+  }
 }
 
 int check(const tjev_gdn_draft_params* p) {
@@ -442,9 +612,19 @@ int check_verify(const tjev_gdn_draft_params* p) {
   return 0;
 }
 
-// the ends, on 256 bytes, then the slices' sums
 long slices_of(const tjev_gdn_draft_params* p) { return ((long)p->vocab + kSlice - 1) / kSlice; }
-size_t ends_bytes(const tjev_gdn_draft_params* p) { return ((size_t)p->requests * 2 * sizeof(int) + 255) / 256 * 256; }
+long parts_of(const tjev_gdn_draft_params* p) { return ((long)p->vocab + kPart - 1) / kPart; }
+// the workspace: the ends, the parts' sums, the slices' bits and marks
+size_t lay_out(const tjev_gdn_draft_params* p, VerifyArgs* A, char* ws) {
+  const size_t n = (size_t)p->requests * slices_of(p), sums = p->requests * parts_of(p), ends = p->requests * sizeof(WalkEnd);
+  if (A) {
+    A->ends = reinterpret_cast<WalkEnd*>(ws);
+    A->sums = reinterpret_cast<double*>(ws + ends);
+    A->bits = reinterpret_cast<uint32_t*>(A->sums + sums);
+    A->marked = reinterpret_cast<int32_t*>(A->bits + n * (kSlice / 32));
+  }
+  return ends + sums * sizeof(double) + n * (kSlice / 8 + sizeof(int32_t));
+}
 
 }  // namespace
 }  // namespace gdn
@@ -470,7 +650,7 @@ int tjev_gdn_draft_tree(const tjev_gdn_draft_params* p, void* stream, const int3
 
 size_t tjev_gdn_verify_workspace_bytes(const tjev_gdn_draft_params* p) {
   if (gdn::check_verify(p)) return 0;
-  return gdn::ends_bytes(p) + (size_t)p->requests * gdn::slices_of(p) * sizeof(double);
+  return gdn::lay_out(p, nullptr, nullptr);
 }
 
 int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const int32_t* tokens, const int32_t* parents,
@@ -490,10 +670,9 @@ int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const i
     return fail(TJEV_GDN_EINVAL, "the probabilities must be aligned to their elements");
   if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
   const long slices = gdn::slices_of(p);
-  char* ws = static_cast<char*>(workspace);
-  const gdn::VerifyArgs A{p->tokens, p->max_new, p->target_stride, p->draft_stride, p->requests, p->vocab, (int)slices, tokens, parents, starts,
-                          uniforms, static_cast<const char*>(target), static_cast<const char*>(draft), tokens_out, path, kept,
-                          reinterpret_cast<double*>(ws + gdn::ends_bytes(p)), reinterpret_cast<int*>(ws)};
+  gdn::VerifyArgs A{p->tokens, p->max_new, p->target_stride, p->draft_stride, p->requests, p->vocab, (int)slices, (int)gdn::parts_of(p), tokens, parents, starts,
+                    uniforms, static_cast<const char*>(target), static_cast<const char*>(draft), tokens_out, path, kept};
+  gdn::lay_out(p, &A, static_cast<char*>(workspace));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 sums((unsigned)slices, (unsigned)p->requests), draw((unsigned)p->requests), block(gdn::kThreads);
   auto launch = [&](auto type, auto chosen) {
@@ -501,7 +680,16 @@ int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const i
     hipLaunchKernelGGL((gdn::k_verify_sums<T, chosen.value>), sums, block, 0, st, A);
     hipLaunchKernelGGL((gdn::k_verify_draw<T, chosen.value>), draw, block, 0, st, A);
   };
-  if (e == 2) {
+  auto one = [&](auto type, auto chosen) {
+    hipLaunchKernelGGL((gdn::k_verify_one<decltype(type), chosen.value>), draw, dim3(gdn::kOne), 0, st, A);
+  };
+  if (p->vocab <= gdn::kOneRow) {
+    if (e == 2) {
+      draft ? one(uint16_t{}, std::false_type{}) : one(uint16_t{}, std::true_type{});
+    } else {
+      draft ? one(float{}, std::false_type{}) : one(float{}, std::true_type{});
+    }
+  } else if (e == 2) {
     draft ? launch(uint16_t{}, std::false_type{}) : launch(uint16_t{}, std::true_type{});
   } else {
     draft ? launch(float{}, std::false_type{}) : launch(float{}, std::true_type{});

@@ -12,6 +12,8 @@
 // in the order of the old table, copies of last pages are taken from it in the order of the new one.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/tjev_gdn.h"
 #include "gdn_device.h"
 #include "gdn_launch.h"
@@ -46,9 +48,16 @@ struct CompactArgs {
   int32_t* lengths_out;  // null: not this launch's
 };
 
+// a round's places: where a token is read and written, as page and slot (page -1: it is left out)
+struct Move {
+  int from, from_in, to, to_in;
+};
+
 template <class W>
 __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactArgs A) {
   constexpr int UN = 8;
+  __shared__ Move smove[kThreads];
+  GDN_POISON_LDS(smove);
   const int b = blockIdx.x, tid = threadIdx.x;
   const long n = max(0l, (long)A.starts[b + 1] - A.starts[b]), len = A.lengths[b], first = len - n;
   const long count = min(min((long)max(A.kept[b], 0), A.most), n);
@@ -58,48 +67,65 @@ __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactArgs A) {
   const int group = blockIdx.y % A.c.groups, cache = blockIdx.y / A.c.groups, layer = cache / 2;
   const bool values = cache % 2;
   const int cols = A.c.cols, step = kThreads / cols, mine = tid / cols, col = group * cols + tid % cols;
-  // a token's place, or null
-  auto place = [&](long t) -> char* {
-    const long j = A.page(t);
-    const int p = j < A.M ? A.table[(long)b * A.M + j] : -1;
-    return p >= 0 && p < A.pages ? A.c.at(layer, values, p, t - j * A.page.d, col, sizeof(W)) : nullptr;
-  };
-  for (long j0 = 0; j0 < count; j0 += UN * step) {
-    W x[UN];
-    char* to[UN];
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const long j = j0 + i * step + mine;
-      to[i] = nullptr;
-      if (mine < step && col < A.c.per && j < count) {
-        const long f = path[j];
-        if (f > j && f < n) {
-          const char* from = place(first + f);
-          to[i] = from ? place(first + j) : nullptr;
-          if (to[i]) x[i] = *reinterpret_cast<const W*>(from);
+  const int round = min(UN * step, kThreads);
+  for (long j0 = 0; j0 < count; j0 += round) {
+    Move m{-1, 0, -1, 0};
+    if (tid < round && j0 + tid < count) {
+      const long j = j0 + tid, f = path[j];
+      if (f > j && f < n) {
+        const long pf = A.page(first + f), pt = A.page(first + j);
+        if (pf < A.M) {  // (and pt, which is not behind it)
+          const int from = A.table[(long)b * A.M + pf], to = A.table[(long)b * A.M + pt];
+          if (from >= 0 && from < A.pages && to >= 0 && to < A.pages)
+            m = {from, (int)(first + f - pf * A.page.d), to, (int)(first + j - pt * A.page.d)};
         }
       }
+    }
+    smove[tid] = m;
+    // (none: everybody is at the same place, or before it)
+    if (!__syncthreads_or(m.from >= 0)) continue;
+    W x[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const int t = i * step + mine;
+      if (mine < step && col < A.c.per && t < round && smove[t].from >= 0)
+        x[i] = *reinterpret_cast<const W*>(A.c.at(layer, values, smove[t].from, smove[t].from_in, col, sizeof(W)));
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): read by all before it is written by any
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < UN; ++i)
-      if (to[i]) *reinterpret_cast<W*>(to[i]) = x[i];
+    for (int i = 0; i < UN; ++i) {
+      const int t = i * step + mine;
+      if (mine < step && col < A.c.per && t < round && smove[t].from >= 0)
+        *reinterpret_cast<W*>(A.c.at(layer, values, smove[t].to, smove[t].to_in, col, sizeof(W))) = x[i];
+    }
     __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------- forks
+// What an old place loses: its pages from `kept` on, those that the first new place going on from it does not keep
+struct ForkOld {
+  int kept, held;
+};
+// What a new place goes on with: its source, pages, the page that it writes on in (or -1), and whether its pages are counted: the
+// first new place of a source has them from it, and nothing is counted for that
+struct ForkNew {
+  int source, pages, last, counted;
+};
+
 struct ForkArgs {
   int B, B2, M, pages;  // places of the old and the new table
   long n_free;
   Div page;
   const int32_t *table, *lengths, *sources, *keep, *free, *taken, *shared;  // keep: null for all
   int32_t *table_out, *lengths_out, *free_out, *taken_out, *shared_out;
+  ForkOld* old;
+  ForkNew* fresh;
   // of each page: the new places that write on in it, and the first of them; the first of the old table's entries that leave it
   int32_t *writers, *writer, *entry;
   int32_t *freed, *copied;  // of each old place, the pages given back; of each new one, whether it takes a copy of its last page
-  int32_t* where;           // and where that stands on the free list, or -1
+  int32_t* where;           // and where that stands on the free list, or (k_fork_one) the page itself; -1: none
 };
 
 __device__ __forceinline__ int fork_pages(const ForkArgs& A, long n) {
@@ -108,109 +134,253 @@ __device__ __forceinline__ int fork_pages(const ForkArgs& A, long n) {
 }
 __device__ __forceinline__ bool is_page(const ForkArgs& A, int p) { return p >= 0 && p < A.pages; }
 
-// What a place of the new table goes on with
-struct Going {
-  int source, pages, last;  // last: the page that it writes on in, or -1
-  long keep;
-};
-__device__ __forceinline__ Going going(const ForkArgs& A, int i) {
-  Going g{-1, 0, -1, 0};
-  if (i >= A.B2) return g;
-  const int s = A.sources[i];
+// What place r goes on with, and how many tokens; `counted` is not known yet
+__device__ __forceinline__ ForkNew going(const ForkArgs& A, int r, long& keep) {
+  ForkNew g{-1, 0, -1, 0};
+  keep = 0;
+  if (r >= A.B2) return g;
+  const int s = A.sources[r];
   if (s < 0 || s >= A.B) return g;
   g.source = s;
   const long len = max(A.lengths[s], 0);
-  g.keep = A.keep ? min((long)max(A.keep[i], 0), len) : len;
-  g.pages = fork_pages(A, g.keep);
-  const long j = A.page(g.keep);
-  if (g.keep > j * A.page.d && j < A.M) {
+  keep = A.keep ? min((long)max(A.keep[r], 0), len) : len;
+  g.pages = fork_pages(A, keep);
+  const long j = A.page(keep);
+  if (keep > j * A.page.d && j < A.M) {
     const int p = A.table[(long)s * A.M + j];
     if (is_page(A, p)) g.last = p;
   }
   return g;
 }
 
-// the first new place that goes on from old place b, or B2; by a workgroup
-__device__ __forceinline__ int heir_of(const ForkArgs& A, int b, int* sheir) {
-  int mine = A.B2;
-  for (int i = threadIdx.x; i < A.B2; i += kThreads)
-    if (A.sources[i] == b) mine = min(mine, i);
-  __syncthreads();
-  if (threadIdx.x == 0) *sheir = A.B2;
-  __syncthreads();
-  if (mine < A.B2) atomicMin(sheir, mine);
-  __syncthreads();
-  return *sheir;
-}
-
+// A workgroup per place: what the old place of that number loses, what the new one goes on with, and its row of the table. The
+// list, the counts and the notes of all pages are shared out.
 __global__ __launch_bounds__(kThreads) void k_fork_init(ForkArgs A) {
-  const long stride = (long)gridDim.x * kThreads, id = (long)blockIdx.x * kThreads + threadIdx.x;
+  __shared__ int sfirst[2];
+  GDN_POISON_LDS(sfirst);
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const long stride = (long)gridDim.x * kThreads, id = (long)r * kThreads + tid;
   for (long i = id; i < A.pages; i += stride) {
     A.shared_out[i] = A.shared[i];
     A.writers[i] = 0;
     A.writer[i] = A.entry[i] = 0x7fffffff;
   }
   for (long i = id; i < A.n_free; i += stride) A.free_out[i] = A.free[i];
-}
-
-// A workgroup per place: what the old place of that number loses, and what the new one takes on. The first new place that goes on
-// from an old one keeps what it has, and nothing is counted for that.
-__global__ __launch_bounds__(kThreads) void k_fork_count(ForkArgs A) {
-  __shared__ int sheir;
-  GDN_POISON_LDS(sheir);
-  const int r = blockIdx.x, tid = threadIdx.x;
-  if (r < A.B) {
-    const int heir = heir_of(A, r, &sheir);
-    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
-    for (int j = kept + tid; j < held; j += kThreads) {
-      const int p = A.table[(long)r * A.M + j];
-      if (!is_page(A, p)) continue;
-      atomicSub(&A.shared_out[p], 1);
-      atomicMin(&A.entry[p], r * A.M + j);
+  if (r >= max(A.B, A.B2)) return;
+  long keep;
+  ForkNew g = going(A, r, keep);
+  if (tid < 2) sfirst[tid] = A.B2;
+  __syncthreads();
+  // the first new place that goes on from old place r, and the first that goes on from r's own source
+  int heir = A.B2, mine = A.B2;
+  for (int i = tid; i < A.B2; i += kThreads) {
+    const int s = A.sources[i];
+    if (s == r) heir = min(heir, i);
+    if (s == g.source) mine = min(mine, i);
+  }
+  if (heir < A.B2) atomicMin(&sfirst[0], heir);
+  if (mine < A.B2) atomicMin(&sfirst[1], mine);
+  __syncthreads();
+  heir = sfirst[0];
+  if (r < A.B2) {
+    for (int j = tid; j < A.M; j += kThreads) A.table_out[(long)r * A.M + j] = j < g.pages ? A.table[(long)g.source * A.M + j] : -1;
+    if (tid == 0) {
+      g.counted = g.source >= 0 && sfirst[1] != r;
+      A.fresh[r] = g;
+      A.lengths_out[r] = (int)keep;
     }
   }
-  const Going g = going(A, r);
-  if (g.source < 0) return;
-  if (heir_of(A, g.source, &sheir) != r)
-    for (int j = tid; j < g.pages; j += kThreads) {
-      const int p = A.table[(long)g.source * A.M + j];
-      if (is_page(A, p)) atomicAdd(&A.shared_out[p], 1);
+  if (r < A.B && tid == 0) {
+    const int kept = heir < A.B2 ? going(A, heir, keep).pages : 0;
+    A.old[r] = {kept, max(kept, fork_pages(A, max(A.lengths[r], 0)))};
+  }
+}
+
+// the old table's entry r, j loses its page; the new place's has one more holder
+__device__ __forceinline__ void drop(const ForkArgs& A, int r, int j) {
+  const int p = A.table[(long)r * A.M + j];
+  if (!is_page(A, p)) return;
+  atomicSub(&A.shared_out[p], 1);
+  atomicMin(&A.entry[p], r * A.M + j);
+}
+__device__ __forceinline__ void add(const ForkArgs& A, int source, int j) {
+  const int p = A.table[(long)source * A.M + j];
+  if (is_page(A, p)) atomicAdd(&A.shared_out[p], 1);
+}
+// (k_fork_one reads what its own workgroup counted)
+__device__ __forceinline__ int counted(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+// whether the old table's entry gives its page back
+__device__ __forceinline__ bool gives_back(const ForkArgs& A, int r, int j, int& p) {
+  p = A.table[(long)r * A.M + j];
+  return is_page(A, p) && counted(&A.entry[p]) == r * A.M + j && counted(&A.shared_out[p]) == -1;
+}
+// A last page with room has one holder: the first of those that write on in it, if all of its holders do. The others take copies.
+__device__ __forceinline__ bool takes_copy(const ForkArgs& A, int r, const ForkNew& g) {
+  return g.last >= 0 && !(counted(&A.shared_out[g.last]) + 1 == counted(&A.writers[g.last]) && counted(&A.writer[g.last]) == r);
+}
+// the page at this place of the whole free list, or -1
+__device__ __forceinline__ int page_at(const ForkArgs& A, long at) {
+  const int got = at >= 0 && at < A.n_free ? counted(&A.free_out[at]) : -1;
+  return is_page(A, got) ? got : -1;
+}
+__device__ __forceinline__ void take(const ForkArgs& A, int r, const ForkNew& g, int got) {
+  A.table_out[(long)r * A.M + g.pages - 1] = got;
+  if (got >= 0) A.shared_out[got] = 0;
+}
+
+// Few places and entries: the rest in one workgroup of a thread per place, whose barriers stand for the ends of three launches.
+constexpr int kOne = 1024, kOneTurns = 64;  // the most threads; of each, entries
+
+// running sums over the workgroup's threads of two numbers of 32 bits, and the whole
+__device__ __forceinline__ long scan_one(long v, long* swave, long& total) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const long t = __shfl_up(v, d);
+    if (lane() >= d) v += t;
+  }
+  __syncthreads();
+  if (lane() == 63) swave[wave()] = v;
+  __syncthreads();
+  total = 0;
+  long before = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / 64; ++w) {
+    if (w < wave()) before += swave[w];
+    total += swave[w];
+  }
+  return v + before;
+}
+__device__ __forceinline__ long pair(int hi, int lo) { return (long)hi << 32 | lo; }
+__device__ __forceinline__ int hi_of(long v) { return (int)(v >> 32); }
+__device__ __forceinline__ int lo_of(long v) { return (int)v; }
+// the place whose run of numbers holds e: the last of those that begin at or before it
+__device__ __forceinline__ int run_of(const int* begin, int n, int e) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (begin[mid] <= e) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
+  __shared__ int sdrop[kOne], sadd[kOne], skept[kOne], ssource[kOne];
+  __shared__ long swave[kOne / 64];
+  GDN_POISON_LDS(sdrop, sadd, skept, ssource, swave);
+  const int tid = threadIdx.x;
+  const ForkOld o = tid < A.B ? A.old[tid] : ForkOld{0, 0};
+  const ForkNew g = tid < A.B2 ? A.fresh[tid] : ForkNew{-1, 0, -1, 0};
+  const long had = min((long)max(A.taken[0], 0), A.n_free);
+  const int drops = o.held - o.kept, adds = g.counted ? g.pages : 0;
+  long all;
+  const long upto = scan_one(pair(drops, adds), swave, all);
+  const int n_drop = hi_of(all), n_add = lo_of(all);
+  sdrop[tid] = hi_of(upto) - drops;
+  sadd[tid] = lo_of(upto) - adds;
+  skept[tid] = o.kept;
+  ssource[tid] = g.source;
+  if (g.last >= 0) {
+    atomicAdd(&A.writers[g.last], 1);
+    atomicMin(&A.writer[g.last], tid);
+  }
+  __syncthreads();
+  int r0 = 0, j0 = 0;  // the thread's first entry, kept: most calls have no more
+  if (tid < n_drop) {
+    r0 = run_of(sdrop, A.B, tid);
+    j0 = skept[r0] + tid - sdrop[r0];
+  }
+  auto dropped = [&](int e, int& r, int& j) {
+    r = e == tid ? r0 : run_of(sdrop, A.B, e);
+    j = e == tid ? j0 : skept[r] + e - sdrop[r];
+  };
+  for (int e = tid; e < n_drop; e += kOne) {
+    int r, j;
+    dropped(e, r, j);
+    drop(A, r, j);
+  }
+  for (int e = tid; e < n_add; e += kOne) {
+    const int r = run_of(sadd, A.B2, e);
+    add(A, ssource[r], e - sadd[r]);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): all is counted
+  __syncthreads();
+  const bool copy = takes_copy(A, tid, g);
+  uint64_t back_here = 0;  // of the thread's entries, up to kOneTurns of them
+  for (int e = tid, i = 0; e < n_drop; e += kOne, ++i) {
+    int r, j, p;
+    dropped(e, r, j);
+    if (gives_back(A, r, j, p)) back_here |= 1ull << i;
+  }
+  const long ranks = scan_one(pair(__builtin_popcountll(back_here), copy), swave, all);
+  const int n_back = hi_of(all), n_copy = lo_of(all), rank = lo_of(ranks) - copy;
+  const long back = min((long)n_back, had);  // what the list has room for
+  if (tid == 0) A.taken_out[0] = (int)min(had - back + n_copy, 0x7fffffffl);
+  if (n_back) {
+    long before = 0;
+    for (int e = tid, i = 0; i * kOne < n_drop; e += kOne, ++i) {
+      const bool gone = back_here >> i & 1;
+      const long at = before + (n_drop <= kOne ? hi_of(ranks) : lo_of(scan_one(gone, swave, all))) - 1;
+      before += lo_of(all);
+      if (gone) {
+        int r, j;
+        dropped(e, r, j);
+        const int p = A.table[(long)r * A.M + j];
+        A.shared_out[p] = 0;
+        if (at < back) A.free_out[had - back + at] = p;
+      }
     }
+  }
+  if (copy) atomicSub(&A.shared_out[g.last], 1);  // others hold it on: it is not given back
+  if (n_copy) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // the list is whole
+    __syncthreads();
+  }
+  if (tid < A.B2) {
+    int got = -1;
+    if (copy) {
+      got = page_at(A, had - back + rank);
+      take(A, tid, g, got);
+    }
+    A.where[tid] = got;
+  }
+}
+
+// The same of many, each step a launch of a workgroup per place
+__global__ __launch_bounds__(kThreads) void k_fork_count(ForkArgs A) {
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r < A.B) {
+    const ForkOld o = A.old[r];
+    for (int j = o.kept + tid; j < o.held; j += kThreads) drop(A, r, j);
+  }
+  if (r >= A.B2) return;
+  const ForkNew g = A.fresh[r];
+  if (g.counted)
+    for (int j = tid; j < g.pages; j += kThreads) add(A, g.source, j);
   if (tid == 0 && g.last >= 0) {
     atomicAdd(&A.writers[g.last], 1);
     atomicMin(&A.writer[g.last], r);
   }
 }
 
-// whether the old table's entry gives its page back
-__device__ __forceinline__ bool gives_back(const ForkArgs& A, int r, int j, int& p) {
-  p = A.table[(long)r * A.M + j];
-  return is_page(A, p) && A.entry[p] == r * A.M + j && A.shared_out[p] == -1;
-}
-
 __global__ __launch_bounds__(kThreads) void k_fork_decide(ForkArgs A) {
-  __shared__ int sheir, scount;
-  GDN_POISON_LDS(sheir, scount);
+  __shared__ int scount;
+  GDN_POISON_LDS(scount);
   const int r = blockIdx.x, tid = threadIdx.x;
-  if (r < A.B) {
-    const int heir = heir_of(A, r, &sheir);
-    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
-    if (tid == 0) scount = 0;
-    __syncthreads();
-    int n = 0, p;
-    for (int j = kept + tid; j < held; j += kThreads) n += gives_back(A, r, j, p);
-    if (n) atomicAdd(&scount, n);
-    __syncthreads();
-    if (tid == 0) A.freed[r] = scount;
-  }
-  if (r < A.B2 && tid == 0) {
-    const Going g = going(A, r);
-    // a last page with room has one holder: the first of those that write on in it, if all of its holders do
-    A.copied[r] = g.last >= 0 && !(A.shared_out[g.last] + 1 == A.writers[g.last] && A.writer[g.last] == r);
-  }
+  if (r < A.B2 && tid == 0) A.copied[r] = takes_copy(A, r, A.fresh[r]);
+  if (r >= A.B) return;
+  const ForkOld o = A.old[r];
+  if (tid == 0) scount = 0;
+  __syncthreads();
+  int n = 0, p;
+  for (int j = o.kept + tid; j < o.held; j += kThreads) n += gives_back(A, r, j, p);
+#pragma unroll
+  for (int d = 32; d; d /= 2) n += __shfl_xor(n, d);
+  if (lane() == 0) atomicAdd(&scount, n);
+  __syncthreads();
+  if (tid == 0) A.freed[r] = scount;
 }
 
-// sums of freed before place r, of copied before it, and of all freed
+// sums of freed and of copied before place r, and of all of them
 struct Sums {
   int freed, copied, all_freed, all_copied;
 };
@@ -244,47 +414,40 @@ __device__ __forceinline__ Sums sums_before(const ForkArgs& A, int r, int (*ssum
   return s;
 }
 
-__global__ __launch_bounds__(kThreads) void k_fork_tables(ForkArgs A) {
-  __shared__ int sheir, ssum[kThreads / 64][4], srank[kThreads / 64];
-  GDN_POISON_LDS(sheir, ssum, srank);
+__global__ __launch_bounds__(kThreads) void k_fork_push(ForkArgs A) {
+  __shared__ int ssum[kThreads / 64][4], srank[kThreads / 64];
+  GDN_POISON_LDS(ssum, srank);
   const int r = blockIdx.x, tid = threadIdx.x;
   const Sums s = sums_before(A, r, ssum);
   const long had = min((long)max(A.taken[0], 0), A.n_free);
   const long back = min((long)s.all_freed, had);  // what the list has room for
   if (r == 0 && tid == 0) A.taken_out[0] = (int)min(had - back + s.all_copied, 0x7fffffffl);
-  if (r < A.B) {
-    const int heir = heir_of(A, r, &sheir);
-    const int kept = heir < A.B2 ? going(A, heir).pages : 0, held = fork_pages(A, max(A.lengths[r], 0));
-    long rank = s.freed;
-    for (int j0 = kept; j0 < held; j0 += kThreads) {
-      const int j = j0 + tid;
-      int p = -1;
-      const bool gone = j < held && gives_back(A, r, j, p);
-      const uint64_t mask = __ballot(gone);
-      if (lane() == 0) srank[wave()] = __builtin_popcountll(mask);
-      __syncthreads();
-      long at = rank + __builtin_popcountll(mask & ((1ull << lane()) - 1));
-#pragma unroll
-      for (int w = 0; w < kThreads / 64; ++w) {
-        if (w < wave()) at += srank[w];
-        rank += srank[w];
-      }
-      if (gone) {
-        A.shared_out[p] = 0;  // (read by this entry alone from here on)
-        if (at < back) A.free_out[had - back + at] = p;
-      }
-      __syncthreads();
-    }
-  }
-  if (r >= A.B2) return;
-  const Going g = going(A, r);
-  const bool copy = A.copied[r] != 0;
-  for (int j = tid; j < A.M; j += kThreads)
-    A.table_out[(long)r * A.M + j] = j < g.pages ? A.table[(long)g.source * A.M + j] : -1;
-  if (tid == 0) {
-    A.lengths_out[r] = (int)g.keep;
+  if (r < A.B2 && tid == 0) {
+    const bool copy = A.copied[r] != 0;
     A.where[r] = copy ? (int)min(had - back + s.copied, 0x7fffffffl) : -1;
-    if (copy) atomicSub(&A.shared_out[g.last], 1);  // others hold it on: it is not given back
+    if (copy) atomicSub(&A.shared_out[A.fresh[r].last], 1);  // others hold it on: it is not given back
+  }
+  if (r >= A.B) return;
+  const ForkOld o = A.old[r];
+  long rank = s.freed;
+  for (int j0 = o.kept; j0 < o.held; j0 += kThreads) {
+    const int j = j0 + tid;
+    int p = -1;
+    const bool gone = j < o.held && gives_back(A, r, j, p);
+    const uint64_t mask = __ballot(gone);
+    if (lane() == 0) srank[wave()] = __builtin_popcountll(mask);
+    __syncthreads();
+    long at = rank + __builtin_popcountll(mask & ((1ull << lane()) - 1));
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      if (w < wave()) at += srank[w];
+      rank += srank[w];
+    }
+    if (gone) {
+      A.shared_out[p] = 0;  // (read by this entry alone from here on)
+      if (at < back) A.free_out[had - back + at] = p;
+    }
+    __syncthreads();
   }
 }
 
@@ -292,39 +455,38 @@ struct ForkCopyArgs {
   Caches c;
   ForkArgs f;
   int layers;
-  bool first;  // of the launches: it writes the table
+  bool known, first;  // where names pages; of the launches (the first takes them)
 };
 
-// The copies: a workgroup per new place, cache and group of columns. The free list is whole by now: a copy may take a page that
+// The copies: a workgroup per new place, cache, group of columns and kCopyTurns times the tokens that its threads have on their way at
+// once. The free list is whole by now: a copy may take a page that
 // was given back (which no copy is made of: what writers leave is held by others).
+constexpr int kCopyTurns = 4, UN = 4;
 template <class W>
 __global__ __launch_bounds__(kThreads) void k_fork_copy(ForkCopyArgs A) {
   const ForkArgs& F = A.f;
   const int r = blockIdx.x, tid = threadIdx.x;
-  if (r >= F.B2) return;
   const int at = F.where[r];
   if (at < 0) return;
-  const Going g = going(F, r);
-  const int got = at < F.n_free ? F.free_out[at] : -1;
-  const long j = F.page(g.keep);
-  if (A.first && blockIdx.y == 0 && tid == 0) {
-    F.table_out[(long)r * F.M + j] = is_page(F, got) ? got : -1;
-    if (is_page(F, got)) F.shared_out[got] = 0;
-  }
-  if (!A.layers || !is_page(F, got)) return;
+  const ForkNew g = F.fresh[r];
+  const int got = A.known ? at : page_at(F, at);
+  if (!A.known && A.first && blockIdx.y == 0 && tid == 0) take(F, r, g, got);
+  if (!A.layers || got < 0) return;
   const int group = blockIdx.y % A.c.groups, cache = blockIdx.y / A.c.groups, layer = cache / 2;
   const bool values = cache % 2;
   const int cols = A.c.cols, step = kThreads / cols, mine = tid / cols, col = group * cols + tid % cols;
   if (mine >= step || col >= A.c.per) return;
-  const int count = (int)(g.keep - j * F.page.d);
-  for (int t0 = mine; t0 < count; t0 += 4 * step) {
-    W x[4];
+  const long keep = F.lengths_out[r];
+  const int count = (int)(keep - (g.pages - 1) * F.page.d);
+  const int z0 = blockIdx.z * kCopyTurns * UN * step, z1 = min(count, z0 + kCopyTurns * UN * step);
+  for (int t0 = z0 + mine; t0 < z1; t0 += UN * step) {
+    W x[UN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t0 + i * step < count) x[i] = *reinterpret_cast<const W*>(A.c.at(layer, values, g.last, t0 + i * step, col, sizeof(W)));
+    for (int i = 0; i < UN; ++i)
+      if (t0 + i * step < z1) x[i] = *reinterpret_cast<const W*>(A.c.at(layer, values, g.last, t0 + i * step, col, sizeof(W)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t0 + i * step < count) *reinterpret_cast<W*>(A.c.at(layer, values, got, t0 + i * step, col, sizeof(W))) = x[i];
+    for (int i = 0; i < UN; ++i)
+      if (t0 + i * step < z1) *reinterpret_cast<W*>(A.c.at(layer, values, got, t0 + i * step, col, sizeof(W))) = x[i];
   }
 }
 
@@ -414,7 +576,8 @@ int tjev_gdn_paged_compact(const tjev_gdn_pages_params* p, void* stream, void* c
 
 size_t tjev_gdn_fork_workspace_bytes(const tjev_gdn_pages_params* p) {
   if (gdn::check(p, nullptr, nullptr, false) || p->new_requests < 1) return 0;
-  return sizeof(int32_t) * (3 * (size_t)p->pages + p->requests + 2 * (size_t)p->new_requests);
+  return sizeof(gdn::ForkNew) * p->new_requests + sizeof(gdn::ForkOld) * p->requests +
+         sizeof(int32_t) * (3 * (size_t)p->pages + p->requests + 2 * (size_t)p->new_requests);
 }
 
 int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches, void* const* v_caches,
@@ -435,30 +598,44 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   if (!workspace || workspace_bytes < need) return fail(TJEV_GDN_EWORKSPACE, "forks need a workspace of tjev_gdn_fork_workspace_bytes");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TJEV_GDN_EINVAL, "the workspace must be 256-byte aligned");
   if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
-  int32_t* ws = static_cast<int32_t*>(workspace);
   gdn::ForkCopyArgs C{};
   gdn::ForkArgs& A = C.f;
   A = {p->requests, p->new_requests, p->table_width, p->pages, p->n_free, gdn::div_by(p->page_size), block_table, lengths, sources, keep,
        free_pages, taken, shared, table_out, lengths_out, free_out, taken_out, shared_out};
-  A.writers = ws;
+  A.fresh = static_cast<gdn::ForkNew*>(workspace);
+  A.old = reinterpret_cast<gdn::ForkOld*>(A.fresh + p->new_requests);
+  A.writers = reinterpret_cast<int32_t*>(A.old + p->requests);
   A.writer = A.writers + p->pages;
   A.entry = A.writer + p->pages;
   A.freed = A.entry + p->pages;
   A.copied = A.freed + p->requests;
   A.where = A.copied + p->new_requests;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const long most = p->pages > p->n_free ? p->pages : p->n_free, blocks = (most + gdn::kThreads - 1) / gdn::kThreads;
-  const dim3 places((unsigned)(A.B > A.B2 ? A.B : A.B2)), block(gdn::kThreads);
-  hipLaunchKernelGGL(gdn::k_fork_init, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), block, 0, st, A);
-  hipLaunchKernelGGL(gdn::k_fork_count, places, block, 0, st, A);
-  hipLaunchKernelGGL(gdn::k_fork_decide, places, block, 0, st, A);
-  hipLaunchKernelGGL(gdn::k_fork_tables, places, block, 0, st, A);
+  const int places = A.B > A.B2 ? A.B : A.B2;
+  const long most = p->pages > p->n_free ? p->pages : p->n_free, blocks = (most + 4 * gdn::kThreads - 1) / (4 * gdn::kThreads);
+  const dim3 block(gdn::kThreads);
+  hipLaunchKernelGGL(gdn::k_fork_init, dim3((unsigned)std::max((long)places, std::min(blocks, 1024l))), block, 0, st, A);
+  const long entries = (long)std::max(A.B, A.B2) * A.M;
+  C.known = places <= gdn::kOne && entries <= gdn::kOne * gdn::kOneTurns;
+  if (C.known) {
+    hipLaunchKernelGGL(gdn::k_fork_one, dim3(1), dim3(gdn::kOne), 0, st, A);
+    if (!p->layers) {
+      const hipError_t e = hipGetLastError();
+      return e == hipSuccess ? 0 : fail(TJEV_GDN_EHIP, hipGetErrorString(e));
+    }
+  } else {
+    hipLaunchKernelGGL(gdn::k_fork_count, dim3(places), block, 0, st, A);
+    hipLaunchKernelGGL(gdn::k_fork_decide, dim3(places), block, 0, st, A);
+    hipLaunchKernelGGL(gdn::k_fork_push, dim3(places), block, 0, st, A);
+  }
   return gdn::by_layers(p, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
     C.c = c;
     C.layers = layers;
     C.first = first;
     const int y = 2 * layers * c.groups;
-    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1), block, 0, st, C);
+    
+    const int turn = gdn::kCopyTurns * gdn::UN * (gdn::kThreads / c.cols);
+    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, (p->page_size + turn - 1) / turn), block, 0, st, C);
   });
 }
 

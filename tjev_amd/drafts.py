@@ -73,8 +73,7 @@ def draft_tree(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tenso
                      (parents.get_device(), starts.get_device(), lengths.get_device()))
     dev = parents.device
     parents, starts, lengths = _int32_near(parents), _int32(starts), _int32(lengths)
-    ancestors = torch.empty((parents.shape[0], (int(max_new) + 63) // 64), dtype=torch.int64, device=dev)
-    positions = torch.empty(parents.shape[0], dtype=torch.int32, device=dev)
+    ancestors, positions = torch.empty((parents.shape[0], (int(max_new) + 63) // 64), dtype=torch.int64, device=dev), torch.empty_like(parents)
     with _lib.on_device(dev):
         _lib.check_status(_lib.load().tjev_gdn_draft_tree(
             p, _lib.current_stream(dev), parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), ancestors.data_ptr(), positions.data_ptr()))
@@ -147,11 +146,11 @@ def verify_drafts(tokens: torch.Tensor, target_probs: torch.Tensor, starts: torc
     dev, requests, most = target_probs.device, starts.shape[0] - 1, int(max_new)
     tokens, starts, uniforms = _int32_near(tokens), _int32(starts), uniforms.contiguous()
     parents = None if parents is None else _int32_near(parents)
-    out, path, kept = torch.empty(requests * (2 * most + 1), dtype=torch.int32, device=dev).split((requests * most, requests * most, requests))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out, ws = tokens.new_empty((requests, most)), torch.empty(need, dtype=torch.uint8, device=dev)
+    path, kept = torch.empty_like(out), tokens.new_empty(requests)
     with _lib.on_device(dev):
         _lib.check_status(lib.tjev_gdn_verify_drafts(
             p, _lib.current_stream(dev), tokens.data_ptr(), None if parents is None else parents.data_ptr(), starts.data_ptr(),
             uniforms.data_ptr(), target_probs.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), out.data_ptr(),
             path.data_ptr(), kept.data_ptr(), ws.data_ptr(), need))
-    return Verified(out.view(requests, most), path.view(requests, most), kept)
+    return Verified(out, path, kept)

@@ -25,8 +25,10 @@ graphs, have their own. Calls recorded by jit tracing or make_fx raise.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import operator
 from typing import NamedTuple
 
 import torch
@@ -312,51 +314,53 @@ class Forked(NamedTuple):
     shared: torch.Tensor
 
 
-def _layer(pair) -> tuple:
-    k, v = pair
-    return k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, k.get_device(), v.get_device()
+_alike = operator.attrgetter("dtype", "requires_grad")
+_size, _stride, _get_device, _address = torch.Tensor.size, torch.Tensor.stride, torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
-@functools.lru_cache(maxsize=256)
-def _caches_params(what: str, like, layers: int, page_size, pages: int | None):
-    """The caches' part of a call's parameters, from the first layer's (None: there are no layers)."""
-    if like is None:
-        return dict(pages=1 if pages is None else pages, page_size=1 if page_size is None else page_size, layers=0)
-    k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype = like[:6]
-    if len(k_shape) != 4 or k_dtype not in _DTYPES:
-        raise ValueError(f"caches are [pages, page_size, heads, dim], float32 or bfloat16, not {tuple(k_shape)} {k_dtype}")
-    _check_caches(k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype, k_shape[2], k_shape[3])
-    if min(k_shape) < 1:
-        raise ValueError(f"caches {tuple(k_shape)} without pages, heads or values")
-    if page_size not in (None, k_shape[1]) or pages not in (None, k_shape[0]):
-        raise ValueError(f"{what}: {pages} pages of {page_size} tokens, and caches {tuple(k_shape)}")
-    if any(s == 0 and n > 1 for strides in (k_stride, v_stride) for s, n in zip(strides, k_shape)):
-        raise ValueError("an expanded cache cannot be written")
-    return dict(pages=k_shape[0], page_size=k_shape[1], kv_heads=k_shape[2], dim=k_shape[3], dtype=_DTYPES[k_dtype], layers=layers,
-                k_stride=k_stride[:3], v_stride=v_stride[:3])
-
-
-def _layers(what: str, caches, page_size, pages):
-    """The layers' caches as the library takes them: their part of the parameters, their addresses, their devices."""
-    pairs = [tuple(pair) for pair in caches]
-    like = None
-    for pair in pairs:
-        if len(pair) != 2:
-            raise ValueError(f"{what} takes pairs of caches, k and v of every layer")
-        if like is None:
-            like = _layer(pair)
-        elif _layer(pair) != like:
-            raise ValueError(f"the layers' caches are alike in shape, strides, type and device: {like} and {_layer(pair)}")
-    flat = [x for pair in pairs for x in pair]
-    if any(x.requires_grad for x in flat) or _lib.dual_level():
+def _layers(what: str, caches):
+    """The layers' caches as the library takes them: what they have in common (kept checks go by it), and the addresses of k's and
+    of v's. A look at each tensor in C, for all at once: 0.5 us a layer."""
+    pairs = list(caches)
+    if not pairs:
+        return None, 0, _NO_LAYERS, _NO_LAYERS
+    if set(map(len, pairs)) != {2}:
+        raise ValueError(f"{what} takes pairs of caches, k and v of every layer")
+    ks, vs = zip(*pairs)
+    flat = ks + vs
+    sizes, k_strides, v_strides, alike, devices = (set(map(_size, flat)), set(map(_stride, ks)), set(map(_stride, vs)), set(map(_alike, flat)),
+                                                   set(map(_get_device, flat)))
+    if _lib.dual_level() or any(grad for _, grad in alike):
         _lib.inference_only(what, *flat)
-    n = len(pairs)
-    ks, vs = ((ctypes.c_void_p * max(1, n))(*(pair[i].data_ptr() for pair in pairs)) for i in (0, 1))
-    return _caches_params(what, like, n, page_size, pages), ks, vs, () if like is None else like[6:]
+    if len(sizes) > 1 or len(k_strides) > 1 or len(v_strides) > 1 or len({dt for dt, _ in alike}) > 1:
+        raise ValueError(f"the layers' caches are alike in shape, strides and type, not {sizes} {k_strides} {v_strides} {[dt for dt, _ in alike]}")
+    return ((sizes.pop(), k_strides.pop(), v_strides.pop(), alike.pop()[0], *devices), len(pairs), array.array("Q", map(_address, ks)),
+            array.array("Q", map(_address, vs)))
+
+
+_NO_LAYERS = array.array("Q", (0,))
+
+
+def _pages_params(what: str, like, layers: int, page_size, pages, **kw):
+    """The library's parameters, the caches' part from what they have in common (None: there are none)."""
+    if like is None:
+        return _lib.PagesParams(pages=1 if pages is None else pages, page_size=1 if page_size is None else page_size, **kw)
+    shape, k_stride, v_stride, dtype = like[:4]
+    if len(shape) != 4 or dtype not in _DTYPES:
+        raise ValueError(f"caches are [pages, page_size, heads, dim], float32 or bfloat16, not {tuple(shape)} {dtype}")
+    _check_caches(shape, k_stride, dtype, shape, v_stride, dtype, shape[2], shape[3])
+    if min(shape) < 1:
+        raise ValueError(f"caches {tuple(shape)} without pages, heads or values")
+    if page_size not in (None, shape[1]) or pages not in (None, shape[0]):
+        raise ValueError(f"{what}: {pages} pages of {page_size} tokens, and caches {tuple(shape)}")
+    if any(s == 0 and n > 1 for strides in (k_stride, v_stride) for s, n in zip(strides, shape)):
+        raise ValueError("an expanded cache cannot be written")
+    return _lib.PagesParams(pages=shape[0], page_size=shape[1], kv_heads=shape[2], dim=shape[3], dtype=_DTYPES[dtype], layers=layers,
+                            k_stride=k_stride[:3], v_stride=v_stride[:3], **kw)
 
 
 @functools.lru_cache(maxsize=256)
-def _check_compact(t_shape, t_dtype, s_shape, s_dtype, l_shape, l_dtype, p_shape, p_dtype, k_shape, k_dtype, devices) -> None:
+def _compact_params(like, layers: int, t_shape, t_dtype, s_shape, s_dtype, l_shape, l_dtype, p_shape, p_dtype, k_shape, k_dtype, devices):
     if len(t_shape) != 2 or t_dtype != torch.int32 or not 1 <= t_shape[0] <= _lib.MAX_REQUESTS or t_shape[1] < 1:
         raise ValueError(f"block_table is [requests, pages] int32 of 1 to {_lib.MAX_REQUESTS} requests, not {tuple(t_shape)} {t_dtype}")
     requests = t_shape[0]
@@ -369,7 +373,9 @@ def _check_compact(t_shape, t_dtype, s_shape, s_dtype, l_shape, l_dtype, p_shape
     for dt in (s_dtype, l_dtype, p_dtype, k_dtype):
         if dt not in (torch.int32, torch.int64):
             raise ValueError(f"starts, lengths, path and kept are int32 or int64, not {dt}")
-    _lib.one_gpu("paged_compact", devices)
+    p = _pages_params("paged_compact", like, layers, None, None, max_new=p_shape[1], requests=requests, table_width=t_shape[1])
+    _lib.one_gpu("paged_compact", (*devices, *like[4:]) if like else devices)
+    return ctypes.byref(p)
 
 
 def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor,
@@ -382,31 +388,31 @@ def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengt
     place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct. What
     stands behind a request's kept tokens is left as it was."""
     _lib.not_recorded("paged_compact")
-    params, ks, vs, devices = _layers("paged_compact", caches, None, None)
-    _check_compact(block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, path.shape, path.dtype,
-                   kept.shape, kept.dtype, (block_table.get_device(), starts.get_device(), lengths.get_device(), path.get_device(),
-                                            kept.get_device(), *devices))
+    like, layers, ks, vs = _layers("paged_compact", caches)
+    p = _compact_params(
+        like, layers, block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, path.shape, path.dtype,
+        kept.shape, kept.dtype, (block_table.get_device(), starts.get_device(), lengths.get_device(), path.get_device(), kept.get_device()))
     dev = block_table.device
     table, starts, lengths, path, kept = block_table.contiguous(), _int32(starts), _int32(lengths), _int32_near(path), _int32_near(kept)
-    out = torch.empty(table.shape[0], dtype=torch.int32, device=dev)
-    p = _lib.PagesParams(max_new=path.shape[1], requests=table.shape[0], table_width=table.shape[1], **params)
+    out = torch.empty_like(lengths)
     with _lib.on_device(dev):
         _lib.check_status(_lib.load().tjev_gdn_paged_compact(
-            ctypes.byref(p), _lib.current_stream(dev), ks, vs, table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), path.data_ptr(),
-            kept.data_ptr(), out.data_ptr()))
+            p, _lib.current_stream(dev), ks.buffer_info()[0], vs.buffer_info()[0], table.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
+            path.data_ptr(), kept.data_ptr(), out.data_ptr()))
     return out
 
 
 @functools.lru_cache(maxsize=256)
-def _check_fork(t_shape, t_dtype, l_shape, l_dtype, s_shape, s_dtype, keep, f_shape, f_dtype, taken, sh_shape, sh_dtype, page_size: int,
-                devices) -> None:
+def _fork_params(lib, like, layers: int, t_shape, t_dtype, l_shape, l_dtype, s_shape, s_dtype, keep, f_shape, f_dtype, taken, sh_shape, sh_dtype,
+                 page_size: int, devices):
+    """The library's view of a call and its workspace. keep: its (shape, dtype) or None; taken: its (size, dtype)."""
     if len(t_shape) != 2 or t_dtype != torch.int32 or not 1 <= t_shape[0] <= _lib.MAX_REQUESTS or t_shape[1] < 1:
         raise ValueError(f"block_table is [requests, pages] int32 of 1 to {_lib.MAX_REQUESTS} requests, not {tuple(t_shape)} {t_dtype}")
     if page_size < 1:
         raise ValueError(f"pages of at least one token, not {page_size}")
     if l_shape != (t_shape[0],):
         raise ValueError(f"lengths {tuple(l_shape)} of {t_shape[0]} requests")
-    if len(s_shape) != 1 or not 1 <= s_shape[0] <= _lib.MAX_REQUESTS or keep not in (None, (s_shape, keep and keep[1])):
+    if len(s_shape) != 1 or not 1 <= s_shape[0] <= _lib.MAX_REQUESTS or (keep is not None and keep[0] != s_shape):
         raise ValueError(f"sources and keep are [new requests] of 1 to {_lib.MAX_REQUESTS}, not {tuple(s_shape)} and {keep and tuple(keep[0])}")
     if len(f_shape) != 1 or len(sh_shape) != 1 or sh_shape[0] < 1 or taken[0] != 1:
         raise ValueError("free_pages is a list of pages, taken one number, and shared a number for every page")
@@ -414,7 +420,10 @@ def _check_fork(t_shape, t_dtype, l_shape, l_dtype, s_shape, s_dtype, keep, f_sh
         if dt not in (torch.int32, torch.int64):
             raise ValueError(f"lengths, sources, keep, pages and their numbers are int32 or int64, not {dt}")
     _check_sizes(t_shape[0] * t_shape[1], s_shape[0] * t_shape[1], f_shape[0], sh_shape[0], page_size)
-    _lib.one_gpu("paged_fork", devices)
+    p = ctypes.byref(_pages_params("paged_fork", like, layers, page_size, sh_shape[0], n_free=f_shape[0], requests=t_shape[0],
+                                   new_requests=s_shape[0], table_width=t_shape[1]))
+    _lib.one_gpu("paged_fork", (*devices, *like[4:]) if like else devices)
+    return p, lib.tjev_gdn_fork_workspace_bytes(p)
 
 
 def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources: torch.Tensor, keep: torch.Tensor | None,
@@ -434,27 +443,24 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
 
     Nothing given is changed but the caches: the new table, lengths, list, ``taken`` and ``shared`` come back."""
     _lib.not_recorded("paged_fork")
-    page_size = int(page_size)
-    params, ks, vs, devices = _layers("paged_fork", caches, page_size, shared.shape[0] if shared.dim() == 1 else None)
-    _check_fork(block_table.shape, block_table.dtype, lengths.shape, lengths.dtype, sources.shape, sources.dtype,
-                None if keep is None else (keep.shape, keep.dtype), free_pages.shape, free_pages.dtype, (taken.numel(), taken.dtype),
-                shared.shape, shared.dtype, page_size,
-                (block_table.get_device(), lengths.get_device(), sources.get_device(), _device(keep, lengths), free_pages.get_device(),
-                 taken.get_device(), shared.get_device(), *devices))
-    lib, dev = _lib.load(), block_table.device
+    lib = _lib.load()
+    like, layers, ks, vs = _layers("paged_fork", caches)
+    p, need = _fork_params(
+        lib, like, layers, block_table.shape, block_table.dtype, lengths.shape, lengths.dtype, sources.shape, sources.dtype,
+        None if keep is None else (keep.shape, keep.dtype), free_pages.shape, free_pages.dtype, (taken.numel(), taken.dtype), shared.shape,
+        shared.dtype, int(page_size),
+        (block_table.get_device(), lengths.get_device(), sources.get_device(), _device(keep, lengths), free_pages.get_device(),
+         taken.get_device(), shared.get_device()))
+    dev = block_table.device
     table, lengths, sources, free, taken, shared = (block_table.contiguous(), _int32(lengths), _int32_near(sources), _int32(free_pages),
                                                     _int32(taken), _int32(shared))
     keep = None if keep is None else _int32_near(keep)
-    requests, width, new, n_free, pages = *table.shape, sources.shape[0], free.shape[0], shared.shape[0]
-    table_out = torch.empty((new, width), dtype=torch.int32, device=dev)
-    free_out, shared_out, lengths_out, taken_out = torch.empty(n_free + pages + new + 1, dtype=torch.int32, device=dev).split(
-        (n_free, pages, new, 1))
-    p = _lib.PagesParams(n_free=n_free, requests=requests, new_requests=new, table_width=width, **params)
-    need = lib.tjev_gdn_fork_workspace_bytes(ctypes.byref(p))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    # (tensors of their own: a part of a larger one takes longer to make)
+    table_out, ws = table.new_empty((sources.shape[0], table.shape[1])), torch.empty(need, dtype=torch.uint8, device=dev)
+    lengths_out, free_out, taken_out, shared_out = torch.empty_like(sources), torch.empty_like(free), taken.new_empty(1), torch.empty_like(shared)
     with _lib.on_device(dev):
         _lib.check_status(lib.tjev_gdn_paged_fork(
-            ctypes.byref(p), _lib.current_stream(dev), ks, vs, table.data_ptr(), lengths.data_ptr(), sources.data_ptr(),
+            p, _lib.current_stream(dev), ks.buffer_info()[0], vs.buffer_info()[0], table.data_ptr(), lengths.data_ptr(), sources.data_ptr(),
             None if keep is None else keep.data_ptr(), free.data_ptr(), taken.data_ptr(), shared.data_ptr(), table_out.data_ptr(),
             lengths_out.data_ptr(), free_out.data_ptr(), taken_out.data_ptr(), shared_out.data_ptr(), ws.data_ptr(), need))
     return Forked(table_out, lengths_out, free_out, taken_out, shared_out)
