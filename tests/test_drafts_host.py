@@ -34,7 +34,7 @@ def library(monkeypatch):
     lib.tjev_gdn_paged_compact = compact
     lib.tjev_gdn_verify_workspace_bytes = lambda p: 256
     lib.tjev_gdn_fork_workspace_bytes = lambda p: 256
-    lib.tjev_gdn_paged_workspace_bytes = lambda p: 256
+    lib.tjev_gdn_paged_tree_workspace_bytes = lambda p: 256
     monkeypatch.setattr(_lib, "load", lambda: lib)
     monkeypatch.setattr(_lib, "one_gpu", lambda what, devices: None)
     monkeypatch.setattr(_lib, "current_stream", lambda device: 0)
@@ -309,7 +309,8 @@ def test_tree_attention_c_abi():
     lib, f = _lib.load(), _fake(12)
     p = _lib.PagedParams(tokens=3, requests=2, table_width=3, pages=4, page_size=16, heads=4, kv_heads=2, dim=64, dtype=1, scale=0.125, q_stride=(256, 64),
                          out_stride=(256, 64), k_stride=(2048, 128, 64), v_stride=(2048, 128, 64))
-    need = lib.tjev_gdn_paged_workspace_bytes(ctypes.byref(p))
+    need = lib.tjev_gdn_paged_tree_workspace_bytes(ctypes.byref(p))
+    assert need > 0 and lib.tjev_gdn_paged_tree_workspace_bytes(None) == 0
     call = lambda a, words, n=need: lib.tjev_gdn_paged_tree_attention(ctypes.byref(p), None, *a[:7], words, None, a[8], a[9], n)  # noqa: E731
     assert call(f, 0) == 1 and "word" in lib.tjev_gdn_last_error().decode()
     assert call(f, 1, need - 1) == 3

@@ -54,6 +54,7 @@ EXPORTS = (
     "tjev_gdn_paged_append",
     "tjev_gdn_paged_workspace_bytes",
     "tjev_gdn_paged_attention",
+    "tjev_gdn_paged_tree_workspace_bytes",
     "tjev_gdn_paged_tree_attention",
     "tjev_gdn_draft_tree",
     "tjev_gdn_verify_workspace_bytes",
@@ -243,6 +244,8 @@ def open_library(path: Path) -> ctypes.CDLL:
     lib.tjev_gdn_paged_workspace_bytes.restype = sz
     lib.tjev_gdn_paged_attention.argtypes = [gpp, vp] + [vp] * 9 + [sz]
     lib.tjev_gdn_paged_attention.restype = i32
+    lib.tjev_gdn_paged_tree_workspace_bytes.argtypes = [gpp]
+    lib.tjev_gdn_paged_tree_workspace_bytes.restype = sz
     lib.tjev_gdn_paged_tree_attention.argtypes = [gpp, vp] + [vp] * 7 + [ctypes.c_int32] + [vp] * 3 + [sz]
     lib.tjev_gdn_paged_tree_attention.restype = i32
     dpp, hpp = ctypes.POINTER(DraftParams), ctypes.POINTER(PagesParams)

@@ -17,7 +17,7 @@ namespace {
 int ranges_of(const tjev_gdn_paged_params* p) { return p->dtype == TJEV_GDN_BF16 && p->dim <= 64 ? kMostRanges : 512; }
 
 // What the host knows: the rows and requests of the call, not how they are shared out.
-AttnPlan plan_of(const tjev_gdn_paged_params* p) {
+AttnPlan plan_of(const tjev_gdn_paged_params* p, bool tree) {
   const bool bf = p->dtype == TJEV_GDN_BF16;
   const int dt = p->dim <= 64 ? 64 : p->dim <= 128 ? 128 : 256;
   const long g = p->heads / p->kv_heads, rows = p->tokens * g;
@@ -35,12 +35,17 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p) {
   // of 128: 50.5 us, with 16 rows 55.0; 20 of 6 after 1858, 8/1 heads: 22.4, with 16 rows 17.6).
   auto few = [](long n) { return n > 16 && n <= 32; };
   r.nq = (bf ? dt == 64 && (few(mean) || (p->max_new && few(top))) : mean > 16 && dt <= 128 && rows / 32 * p->kv_heads >= 128) ? 2 : 1;
-  r.mixed = bf && top > 16 * r.nq;
-  const int kb = bf ? 128 : 64;
-  // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
-  const long tiles = (rows / (r.mixed ? kWideRows : 16 * r.nq) + active) * p->kv_heads;
+  const int kb = bf ? 128 : 64, most = ranges_of(p);
   const long blocks = ((long)p->table_width * p->page_size + kb - 1) / kb + kWideExtra + kGateExtra;
-  const int most = ranges_of(p);
+  // a request's rows are one streamed tile (mixed) or tiles of one kind, of which its last may be short
+  auto tiles_of = [&](int tile_rows) { return (rows / tile_rows + active) * p->kv_heads; };
+  r.mixed = bf && top > 16 * r.nq;
+  // Trees whose streamed tiles are at most kFewTurns units to a workgroup are streamed, and read their keys a few times: the many
+  // small parts are worked on at once (16/4 heads of 256: one tree of 12 over 4000, 22.4 us instead of 26.1; 4 of 12 over 1000, 24.4 and 34.1;
+  // 16 of 6 over 1000, 30.6 and 40.9; with twice the limit 16 of 12 over 1000 would take 44.7, and 43.7 in tiles of 128).
+  constexpr int kFewTurns = 2;
+  if (tree && r.mixed && tiles_of(16 * r.nq) * blocks <= kFewTurns * (long)most) r.mixed = false;
+  const long tiles = tiles_of(r.mixed ? kWideRows : 16 * r.nq);
   r.G = tiles >= most || blocks * tiles >= most ? most : (int)(blocks * tiles);
   // so few tiles that a workgroup each would leave most CUs idle, and take parts by the dozen; or rows for so few, in a batch
   // whose other requests may bring none
@@ -81,9 +86,11 @@ int attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const
   if (int s = validate(p)) return s;
   if (!p->tokens) return 0;
   if (!q || !k_cache || !v_cache || !block_table || !starts || !lengths || !out) return fail(TJEV_GDN_EINVAL, "null tensor argument");
-  const size_t need = plan_of(p).bytes;
+  const AttnPlan plan = plan_of(p, ancestors != nullptr);
+  const size_t need = plan.bytes;
   if (!workspace || workspace_bytes < need)
-    return fail(TJEV_GDN_EWORKSPACE, "paged attention needs a workspace of tjev_gdn_paged_workspace_bytes");
+    return fail(TJEV_GDN_EWORKSPACE, ancestors ? "paged tree attention needs a workspace of tjev_gdn_paged_tree_workspace_bytes"
+                                               : "paged attention needs a workspace of tjev_gdn_paged_workspace_bytes");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TJEV_GDN_EINVAL, "the workspace must be 256-byte aligned");
   const long e = p->dtype == TJEV_GDN_BF16 ? 2 : 4;
   AttnArgs A{};
@@ -118,7 +125,6 @@ int attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const
   if (A.ks > (1l << 26) || A.vs > (1l << 26)) return fail(TJEV_GDN_EUNSUPPORTED, "cache slots more than 64 MB apart");
   if (any % 16) return fail(TJEV_GDN_EINVAL, "q, gate, out and the caches must be 16-byte aligned, with strides that keep their rows so");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const AttnPlan plan = plan_of(p);
   // (the parts: the ranges' notes behind them, which say how many there are, are never NaN)
   if (int s = poison_workspace(workspace, plan.bytes - (size_t)plan.G * kSplitBytes, stream)) return s;
   A.tree = ancestors;
@@ -138,7 +144,12 @@ extern "C" {
 
 size_t tjev_gdn_paged_workspace_bytes(const tjev_gdn_paged_params* p) {
   if (gdn::validate(p)) return 0;
-  return gdn::plan_of(p).bytes;
+  return gdn::plan_of(p, false).bytes;
+}
+
+size_t tjev_gdn_paged_tree_workspace_bytes(const tjev_gdn_paged_params* p) {
+  if (gdn::validate(p)) return 0;
+  return gdn::plan_of(p, true).bytes;
 }
 
 int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const void* q, const void* k_cache, const void* v_cache,

@@ -211,7 +211,8 @@ def _attention_params(lib, q_shape, q_stride, q_dtype, kc_shape, kc_stride, kc_d
                          dim ** -0.5 if scale is None else scale, _strides(q_shape, q_stride),
                          (0, 0) if gate is None else _strides(*gate[:2]), (heads * dim, dim) if out is None else _strides(*out[:2]),
                          _strides(kc_shape, kc_stride), _strides(vc_shape, vc_stride), max_new=max_new or 0)
-    return ctypes.byref(p), lib.tjev_gdn_paged_workspace_bytes(ctypes.byref(p))
+    need = lib.tjev_gdn_paged_workspace_bytes if what == "paged_attention" else lib.tjev_gdn_paged_tree_workspace_bytes
+    return ctypes.byref(p), need(ctypes.byref(p))
 
 
 def _strides(shape, stride):
