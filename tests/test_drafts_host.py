@@ -6,7 +6,11 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import os
 import random
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -318,6 +322,38 @@ def test_tree_attention_c_abi():
         a = list(f)
         a[i] = None
         assert call(a, 1) == 1 and "null" in lib.tjev_gdn_last_error().decode(), i
+
+
+def test_the_keys_of_a_tree_under_asan(tmp_path):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not Path(hipcc).exists():
+        pytest.skip("hipcc not available")
+    exe = tmp_path / "tree_asan"
+    build = subprocess.run([hipcc, "--offload-arch=gfx950", "-O1", "-g", "-std=c++17", "-Xarch_host", "-fsanitize=address",
+                            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                            str(Path(__file__).parent / "asan" / "tree_driver.hip"), "-o", str(exe)], capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr[-3000:]
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=0:halt_on_error=1:exitcode=86")
+    run = subprocess.run([str(exe)], capture_output=True, text=True, env=env, timeout=300)
+    assert run.returncode == 0 and "0 wrong" in run.stdout, (run.stdout + run.stderr)[-3000:]
+
+
+def _tree_workspace(**kw):
+    from tjev_amd import _lib
+
+    p = dict(tokens=12, requests=1, table_width=254, pages=64, page_size=16, heads=16, kv_heads=4, dim=256, dtype=_lib.BF16, scale=1.0)
+    p = _lib.PagedParams(**{**p, **kw})
+    return _lib.load().tjev_gdn_paged_tree_workspace_bytes(ctypes.byref(p)), _lib.load().tjev_gdn_paged_workspace_bytes(ctypes.byref(p))
+
+
+def test_small_batches_of_trees_are_streamed():
+    """Places of 16 rows, not of 128: within two units to a workgroup; beyond that, in fp32 and in few rows as causal rows are."""
+    place = lambda rows: 2 * rows * (256 + 2) * 4 + 32  # noqa: E731
+    tree, causal = _tree_workspace()
+    assert tree % place(16) == 0 and causal % place(128) == 0
+    for kw in (dict(table_width=4000), dict(tokens=400), dict(tokens=4), dict(dtype=0)):
+        tree, causal = _tree_workspace(**kw)
+        assert tree == causal > 0
 
 
 # ---------------------------------------------------------------- the plain forms

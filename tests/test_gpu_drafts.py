@@ -143,10 +143,10 @@ def test_verified_tokens_have_the_targets_distribution(drawn):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-def test_verify_degenerate_rows(dtype):
+@pytest.mark.parametrize("vocab", [300, 66000])
+def test_verify_degenerate_rows(dtype, vocab):
     """Rows without a positive number, NaN, infinities and negative numbers, a draft like the target, tokens outside the vocabulary,
     the same token twice among siblings, numbers of 0, 1, over 1, below 0 and NaN."""
-    vocab = 300
     nan, inf = math.nan, math.inf
     base = torch.softmax(torch.randn(vocab, generator=torch.Generator().manual_seed(1)), -1)
     one = torch.zeros(vocab)
@@ -155,7 +155,7 @@ def test_verify_degenerate_rows(dtype):
     odd[[3, 50, 99]] = torch.tensor([nan, inf, -1.0])
     for name, row in (("plain", base), ("zeros", torch.zeros(vocab)), ("nan", torch.full((vocab,), nan)), ("one", one), ("odd", odd),
                       ("tiny", base * 1e-38)):
-        for u0 in (0.0, 0.3, 1.0, 7.0, -1.0, nan):
+        for u0 in (0.0, 0.3, 1.0, 7.0, -1.0, nan)[::1 if vocab < 1000 else 2]:
             for up, x in (([-1, 0, 0, 0, 1], [0, 17, 17, 5, 9]), ([-1, 0, 0, 0, 0], [0, -1, vocab, 2 ** 31 - 1, 17]), ([-1, -1, 1, 0, 3], [0, 3, 17, 50, 99])):
                 u = torch.tensor([u0, 0.9999, 0.5, 0.01, 0.2])
                 case = dict(tokens=torch.tensor(x), target_probs=row.repeat(5, 1).to(dtype), starts=torch.tensor([0, 5]), uniforms=u,
@@ -170,13 +170,14 @@ def test_verify_degenerate_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-def test_verify_borders(dtype):
-    """Powers of two, whose sums are exact: numbers on the border of a token take the next one, at both sides of a slice's end."""
-    vocab = 1 << 14
-    row = torch.full((1, vocab), 2.0 ** -14, dtype=dtype)
-    ks = [0, 1, 2, 255, 256, 4094, 4095, 4096, 4097, 8191, 8192, 12288, vocab - 1]
-    us = [k * 2.0 ** -14 for k in ks]
-    print(f"verify borders {dtype}", flush=True)
+@pytest.mark.parametrize("bits", [14, 16, 17, 21])
+def test_verify_borders(dtype, bits):
+    """Powers of two, whose sums are exact: numbers on the border of a token take the next one, at both sides of a part's end."""
+    vocab = 1 << bits
+    row = torch.full((1, vocab), 2.0 ** -bits, dtype=dtype)
+    ks = [0, 1, 2, 255, 256, 1023, 1024, 1025, 4094, 4095, 4096, 4097, 8191, 8192, 12288, vocab // 2, vocab // 2 + 1, vocab - 1]
+    us = [k * 2.0 ** -bits for k in ks]
+    print(f"verify borders {dtype} vocab={vocab}", flush=True)
     from tjev_amd import verify_drafts
 
     v = verify_drafts(torch.zeros(len(ks), dtype=torch.int32, device="cuda"), row.cuda().expand(len(ks), vocab), torch.arange(len(ks) + 1).cuda(),
@@ -437,6 +438,8 @@ def _calls():
     parents = i32([p for n in sizes for p in random_tree(rng, n)[:n]])
     case = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in _verify(random.Random(9), sizes, 9001, "tree", F32, False).items()}
     drawn = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in _verify(random.Random(9), sizes, 9001, "chain", BF, True).items()}
+    large = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in _verify(random.Random(9), sizes, 70001, "tree", BF, False).items()}
+    large_drawn = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in _verify(random.Random(9), sizes, 70001, "chain", F32, True).items()}
     lens = [30, 11, 64, 90]
     table, free, taken, shared = _pool(rng, lens, 8, 12, 20, common=1)
     given = [i32(x) for x in (table, lens, [0, 0, 1, 3, 3, 3], [30, 29, 5, 90, 88, 3], free, [taken], shared)]
@@ -447,6 +450,16 @@ def _calls():
         f = paged_fork(caches, *given, page_size=8)
         return [*f, *(c for pair in caches for c in pair)]
 
+    many = [rng.randint(0, 40) for _ in range(1500)]
+    table, free, taken, shared = _pool(rng, many, 4, 10, 900, common=1)
+    given_many = [i32(x) for x in (table, many, [rng.randrange(-1, 1500) for _ in range(1200)], [rng.randint(0, 40) for _ in range(1200)], free, [taken],
+                                   shared)]
+    small = _caches(torch.Generator().manual_seed(6), 1, len(shared), 4, 1, 8, BF)
+
+    def fork_many(*_):
+        caches = [tuple(c.clone() for c in pair) for pair in small]
+        return [*paged_fork(caches, *given_many, page_size=4), *caches[0]]
+
     path = i32([[0, 2, 3, -1], [0, 3, 6, 7], [-1] * 4, [0, 1, 2, 10]])
     kept = i32([3, 4, 0, 4])
     wide = i32([table[b][:11] for b in range(4)])
@@ -456,10 +469,11 @@ def _calls():
         return [paged_compact(caches, wide, starts, lengths, path, kept), *(c for pair in caches for c in pair)]
 
     return {"tree": lambda: list(draft_tree(parents, starts, lengths, max_new=70)), "verify": lambda: list(verify_drafts(**case, max_new=70)),
-            "drawn": lambda: list(verify_drafts(**drawn, max_new=70)), "fork": fork, "compact": compact}
+            "drawn": lambda: list(verify_drafts(**drawn, max_new=70)), "verify, large": lambda: list(verify_drafts(**large, max_new=70)),
+            "drawn, large": lambda: list(verify_drafts(**large_drawn, max_new=70)), "fork": fork, "fork, many": fork_many, "compact": compact}
 
 
-@pytest.mark.parametrize("what", ["tree", "verify", "drawn", "fork", "compact"])
+@pytest.mark.parametrize("what", ["tree", "verify", "drawn", "verify, large", "drawn, large", "fork", "fork, many", "compact"])
 def test_calls_at_once_and_captured(monkeypatch, what):
     """Calls on two streams without a wait, captured ones replayed with eager work between, poisoned workspaces and LDS: the same bits."""
     from tjev_amd import _lib

@@ -86,6 +86,39 @@ def test_rows_may_name_any_token(dtype, heads, words):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,lens,requests", [
+    (8, 2, 64, [(700, 6), (0, 1), (90, 40)], 60), (16, 4, 256, [(1200, 64)], 64), (6, 3, 40, [(2000, 90), (5, 9)], 200),
+    (4, 4, 200, [(77, 50), (1, 1)], 120), (16, 2, 128, [(4000, 3), (0, 200)], 9),
+])
+def test_unused_requests_and_the_most_new_tokens(dtype, heads, kv_heads, dim, lens, requests):
+    """More places than trees, and bounds on a tree's tokens: the true one, none, and (which costs time alone) wrong ones."""
+    case = _case(24, lens, heads=heads, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, gate=True)
+    want, room = tree_attention64(*(case[n] for n in NAMES), gate=case["gate"])
+    starts, lengths = torch.zeros(requests + 1, dtype=torch.int32), torch.zeros(requests, dtype=torch.int32)
+    table = torch.full((requests, case["block_table"].shape[1]), -1, dtype=torch.int32)
+    for b in range(len(lens)):
+        at = b * (requests - 1) // max(1, len(lens) - 1)
+        starts[at + 1:] = case["starts"][b + 1]
+        lengths[at], table[at] = case["lengths"][b], case["block_table"][b]
+    case.update(starts=starts, lengths=lengths, block_table=table)
+    for max_new in (None, max(n for _, n in lens), 1, 5, 10 ** 6):
+        print(f"tree attention {dtype} {heads}/{kv_heads} of {dim} {lens} in {requests} places, max_new={max_new}", flush=True)
+        compare(_attend(case, max_new=max_new), want, room)
+
+
+def test_no_tokens():
+    from tjev_amd import paged_tree_attention
+
+    c = torch.zeros(2, 16, 2, 64, device="cuda")
+    z = torch.zeros(3, dtype=torch.int32, device="cuda")
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    got = paged_tree_attention(torch.empty(0, 4, 64, device="cuda"), c, c, table, z, z[:2], torch.empty(0, 1, dtype=torch.int64, device="cuda"))
+    assert got.shape == (0, 4, 64)
+    got = paged_tree_attention(torch.ones(5, 4, 64, device="cuda"), c, c, table, z, z[:2], torch.full((5, 1), -1, device="cuda"))
+    assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("page", [16, 10])
 @pytest.mark.parametrize("heads", [4, 16])
 def test_pages_that_are_none(dtype, page, heads):
@@ -158,6 +191,7 @@ SPLIT = {
     "streamed, few": ([(9000, 2)], 8, 2, 128, None), "streamed, many": ([(900, 2)] * 70, 8, 2, 128, None),
     "wide, few": ([(3000, 64)], 16, 4, 256, None), "wide, many": ([(1500, 70)] * 6, 16, 4, 128, None),
     "wide, counted": ([(3000, 64)] + [(0, 0)] * 63, 16, 4, 256, 64), "32 rows": ([(700, 5)] * 40, 8, 2, 64, 8),
+    "32 rows, many": ([(50, 20)] * 40, 8, 8, 64, None), "small, streamed": ([(1500, 12)], 16, 4, 256, None),
 }
 
 

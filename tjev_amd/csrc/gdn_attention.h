@@ -439,21 +439,7 @@ __device__ __forceinline__ int range_of(int block, int G) { return G % 8 ? block
 // TREE: a row attends to all keys before the request's new tokens, and of those to the ones that its bits name. Which of the
 // 64 keys from k0 on that is; rows behind the request's last attend to none.
 __device__ __forceinline__ uint64_t tree_keys(const AttnArgs& A, const Request& q, int row, int k0) {
-  if (row >= q.rows) return 0;
-  const uint64_t* bits = A.tree + (long)(q.s0 + A.by_g(row)) * A.words;
-  const long at = k0 - q.first;  // of the first of them among the new tokens
-  uint64_t s;
-  if (at <= -64) {
-    s = ~0ull;
-  } else if (at < 0) {
-    s = ((1ull << -at) - 1) | bits[0] << -at;
-  } else {
-    const long i = at >> 6;
-    const int sh = at & 63;
-    s = (i < A.words ? bits[i] >> sh : 0) | (sh && i + 1 < A.words ? bits[i + 1] << (64 - sh) : 0);
-  }
-  const int left = q.keys - k0;
-  return left >= 64 ? s : left > 0 ? s & ((1ull << left) - 1) : 0;
+  return row < q.rows ? keys_of_bits(A.tree + (long)(q.s0 + A.by_g(row)) * A.words, A.words, k0 - q.first, q.keys - k0) : 0;
 }
 // the keys that all rows attend to
 __device__ __forceinline__ int tree_first(const Request& q) { return q.first < 0 ? 0 : q.first < q.keys ? (int)q.first : q.keys; }

@@ -150,6 +150,22 @@ __host__ __device__ __forceinline__ int row_limit(const Batch& A, const Request&
   return last < 0 ? 0 : last < q.keys ? (int)last : q.keys;
 }
 
+// Which of 64 keys a row of a tree attends to: the first of them is number `at` of its request's new tokens (negative: it stands
+// before them, where the row attends to all), and `left` of them are keys of the request.
+__host__ __device__ __forceinline__ uint64_t keys_of_bits(const uint64_t* bits, long words, long at, int left) {
+  uint64_t s;
+  if (at <= -64) {
+    s = ~0ull;
+  } else if (at < 0) {
+    s = ((1ull << -at) - 1) | bits[0] << -at;
+  } else {
+    const long i = at >> 6;
+    const int sh = at & 63;
+    s = (i < words ? bits[i] >> sh : 0) | (sh && i + 1 < words ? bits[i + 1] << (64 - sh) : 0);
+  }
+  return left >= 64 ? s : left > 0 ? s & ((1ull << left) - 1) : 0;
+}
+
 // A key's place. Keys behind the last are taken at the last (their weights are 0); an entry that is no page
 // of the cache reads page 0 and is not good.
 struct Place {
