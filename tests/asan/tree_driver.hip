@@ -40,12 +40,14 @@ int main() {
     const int32_t starts[2] = {(int32_t)(rng() % 400) - 50, (int32_t)(rng() % 400) - 50}, lengths[1] = {(int32_t)(rng() % 700) - 50};
     A.starts = starts;
     A.lengths = lengths;
-    const gdn::Request q = gdn::request<16, 128, true>(A, 0);
+    const bool pairs = rng() % 2;  // a streamed tile's unit is two blocks
+    const gdn::Request q = pairs ? gdn::request<16, 128, true, 2>(A, 0) : gdn::request<16, 128, true>(A, 0);
+    const long unit = pairs && q.tile_rows == 16 ? 256 : 128;
     bad += q.rows && !(q.s0 >= 0 && q.s0 + (q.rows - 1) / A.g < A.N);
     bad += q.keys < 0 || q.keys > (long)A.M * A.page;
     long sum = 0;
     for (int t = 0; t < q.tiles; ++t) {
-      bad += q.before_tile(t) != sum || (long)q.tile_blocks(t) * 128 < q.keys || q.tile_blocks(t) < 1;
+      bad += q.before_tile(t) != sum || (long)q.tile_blocks(t) * unit < q.keys || (q.keys && (long)(q.tile_blocks(t) - 1) * unit >= q.keys) || q.tile_blocks(t) < 1;
       sum += q.extra + q.tile_blocks(t);
     }
     bad += sum != q.per_head || q.cost != q.per_head * A.Hk;

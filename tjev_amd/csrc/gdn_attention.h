@@ -127,11 +127,11 @@ struct FoundLds {
 };
 
 // Up to 64 requests are read and summed by each wave for itself, more of them by the workgroup, in turns, twice.
-template <int R, int KB, bool TREE>
+template <int R, int KB, bool TREE, int W>
 __device__ __forceinline__ Found find_range(const AttnArgs& A, int range, FoundLds& f) {
   const int tid = threadIdx.x;
   Found r;
-  auto load = [&](int b) { return b < A.B ? request<R, KB, TREE>(A, b) : Request{}; };
+  auto load = [&](int b) { return b < A.B ? request<R, KB, TREE, W>(A, b) : Request{}; };
   if (A.B <= 64) {
     const Request q = load(lane());
     const long upto = scan_wave(q.cost);
@@ -1215,12 +1215,21 @@ __device__ __forceinline__ void clear_rest(const AttnArgs& A) {
   }
 }
 
+// The blocks of keys in a unit of a streamed tile (gdn_paged.h). In batches of trees with tiles of both kinds at a head dim of 256
+// a block takes a streamed tile half of what it takes a wide one (7.5 us, 15.3), so its unit is two of them. The wide tiles' loop
+// then also holds its queries without scratch, which the compiler's allocation decides: 16/4 heads, pages of 64, 32 trees of 24
+// over 16384, 176 us instead of 189 (all lengths alike 413, 459); 32 of 64 over 8192, 354 and 447; 8 of 200 over 2000 111 and 133; but 32
+// of 12 over 2000 47.7 and 45.2. With pages that are no whole tiles' (24: 127 us instead of 105) or padded heads (dim 200: 169
+// and 116) two cost more, at 128 too, where a block takes both kinds the same.
+template <class T, int DT, bool PAD, bool WHOLE, bool MIXED, bool TREE>
+constexpr int kTreeUnit = MIXED && TREE && DT == 256 && WHOLE && !PAD ? 2 : 1;
+
 // MIXED: the batch may hold requests of more than A.wide packed rows, which take the wide tiles. TREE: see tree_keys.
 template <class T, int DT, int NQ, bool PAD, bool WHOLE, bool MIXED, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
   using S = Shape<T, DT>;
   using L = StreamLds<T, DT, NQ>;
-  constexpr int R = 16 * NQ, KB = S::KB;
+  constexpr int R = 16 * NQ, KB = S::KB, W = kTreeUnit<T, DT, PAD, WHOLE, MIXED, TREE>;
   constexpr int BUF = MIXED ? Wide<DT>::TK * DT / 8 : 0;  // pieces of 16 bytes
   constexpr int NA = L::ACC > 2 * BUF ? L::ACC : 2 * BUF, NB = L::Q > BUF ? L::Q : BUF;
   __shared__ FoundLds sfound;
@@ -1242,7 +1251,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
 
   {
     const int range = range_of(blockIdx.x, A.G);
-    const Found f = find_range<R, KB, TREE>(A, range, sfound);
+    const Found f = find_range<R, KB, TREE, W>(A, range, sfound);
     if (threadIdx.x == 0) split_of(A, range)->parts = 0;
     if (A.fill) clear_rest<T>(A);
     if (f.b < 0) return;
@@ -1283,7 +1292,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
         if (local < q.cost) {
           st.at = at.tile + 1 < q.tiles ? Unit{at.head, at.tile + 1, 0} : Unit{at.head + 1, 0, 0};
         } else if (u + seg < u1) {
-          const Request n = b + 1 < A.B ? request<R, KB, TREE>(A, b + 1) : Request{};
+          const Request n = b + 1 < A.B ? request<R, KB, TREE, W>(A, b + 1) : Request{};
           local = 0;
           st.q = n;
           st.b = b + 1;
@@ -1298,7 +1307,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
             wide_tile<DT, PAD, WHOLE, TREE>(q, b, part, k0, keys, pa, pa + Wide<DT>::TK * DT, reinterpret_cast<uint16_t*>(sb),
                                       reinterpret_cast<uint16_t*>(sc), sd, sbad);
         } else {
-          stream_tile<T, DT, NQ, PAD, WHOLE, TREE>(q, b, part, k0, keys, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
+          stream_tile<T, DT, NQ, PAD, WHOLE, TREE>(q, b, part, W * k0, W * keys, sb, reinterpret_cast<f32x4*>(sa), sm, sl);
         }
       }
     }
@@ -1309,7 +1318,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention(AttnArgs A) {
       if (uniform(wave()) == 0) {
         int b = uniform(st.b) + 1;
         for (; b < A.B; b += 64) {
-          const Request n = b + lane() < A.B ? request<R, KB, TREE>(A, b + lane()) : Request{};
+          const Request n = b + lane() < A.B ? request<R, KB, TREE, W>(A, b + lane()) : Request{};
           const uint64_t here = __ballot(n.cost > 0);
           if (here) {
             const int first = __builtin_ctzll(here);

@@ -90,8 +90,9 @@ struct Request {
   }
 };
 
-// TREE: a tree's rows may attend to any of the request's new tokens, so every tile has all of its keys.
-template <int R, int KB, bool TREE = false>
+// TREE: a tree's rows may attend to any of the request's new tokens, so every tile has all of its keys. W: a streamed tile's unit
+// has W * KB keys (a tree's, where it takes less time than a wide tile's of KB).
+template <int R, int KB, bool TREE = false, int W = 1>
 __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   Request q;
   const long n = A.N, a = A.starts[b], e = A.starts[b + 1], len = A.lengths[b];
@@ -107,7 +108,8 @@ __host__ __device__ __forceinline__ Request request(const Batch& A, int b) {
   q.first = len - (e - a);
   q.by_g = A.by_g_long;
   q.y = 0;
-  q.blocks = keys ? (int)((keys + KB - 1) / KB) : 1;  // a row without keys is written too
+  const int unit = wide ? KB : W * KB;
+  q.blocks = keys ? (int)((keys + unit - 1) / unit) : 1;  // a row without keys is written too
   if (!TREE && wide && q.first >= 0 && keys == len) {
     // Tile t's last row may attend to first + (kWideRows (t + 1) - 1) / g + 1 keys, which are
     // floor((first g + kWideRows (t + 1) - 1) / (KB g)) + 1 blocks, and with KB = kWideRows floor((y + t) / g)
