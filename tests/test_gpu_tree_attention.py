@@ -106,6 +106,20 @@ def test_unused_requests_and_the_most_new_tokens(dtype, heads, kv_heads, dim, le
         compare(_attend(case, max_new=max_new), want, room)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(16, 4, 256, 16), (16, 4, 256, 64), (16, 4, 256, 24), (16, 4, 200, 16), (16, 4, 128, 32),
+                                                     (24, 4, 64, 16)])
+@pytest.mark.parametrize("longest", [128, 385, 900])
+def test_many_trees_in_tiles_of_both_kinds(heads, kv_heads, dim, page, longest):
+    """Trees of a few tokens beside ones of up to 40, more of them than are streamed; keys that end in the first and the second
+    block of a pair, one key, and none."""
+    rng = random.Random(longest + page)
+    lens = [(rng.choice((0, 1, 127, 128, 129, 255, 256, 257, longest)) % (longest + 1), rng.choice((0, 1, 2, 4, 5, 9, 33, 40))) for _ in range(44)]
+    print(f"many trees, {heads}/{kv_heads} of {dim}, page={page}, up to {longest} keys", flush=True)
+    case = _case(longest, lens, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=BF, gate=dim == 256, pad_rows=2)
+    want, room = tree_attention64(*(case[n] for n in NAMES), gate=case["gate"])
+    compare(_attend(case), want, room)
+
+
 def test_no_tokens():
     from tjev_amd import paged_tree_attention
 
