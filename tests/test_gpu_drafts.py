@@ -118,6 +118,23 @@ def test_verify(dtype, kind, drawn, sizes, vocab, max_new):
         assert int(v.kept.min()) == 1 and int(v.kept.max()) > 1
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("kind,drawn", [("tree", False), ("chain", False), ("chain", True)])
+@pytest.mark.parametrize("requests,vocab", [(257, 1), (300, 6), (256, 33), (261, 1025), (270, 5000)])
+def test_verify_many(dtype, kind, drawn, requests, vocab):
+    """More requests than are verified by a workgroup each, of small vocabularies too."""
+    rng = random.Random(requests + vocab)
+    sizes = [rng.choice([0, 1, 1, 2, 3, 5]) for _ in range(requests)]
+    print(f"verify {dtype} {kind} drawn={drawn} {requests} requests vocab={vocab}", flush=True)
+    _check(_verify(rng, sizes, vocab, kind, dtype, drawn, front=2, behind=1), 4)
+
+
+@pytest.mark.parametrize("dtype,drawn,vocab", [(F32, True, 32768), (F32, True, 32769), (F32, False, 65536), (BF, True, 65536), (BF, False, 65537)])
+def test_verify_at_the_largest_rows_of_a_launch(dtype, drawn, vocab):
+    print(f"verify {dtype} drawn={drawn} vocab={vocab}", flush=True)
+    _check(_verify(random.Random(vocab), [3, 1, 4], vocab, "chain" if drawn else "tree", dtype, drawn, front=0, behind=0), 4)
+
+
 @pytest.mark.parametrize("drawn", [False, True])
 def test_verified_tokens_have_the_targets_distribution(drawn):
     """A grid of numbers for the draft and for the drawn token: the first emitted token has the target's probabilities up to the grid's
@@ -368,6 +385,20 @@ def test_fork_of_many(requests, new, width, page):
     keep = [rng.randint(0, width * page) for _ in range(new)]
     table, free, taken, shared = _pool(rng, lens, page, width, new, common=1)
     print(f"fork of {requests} places into {new}", flush=True)
+    _fork([], table, lens, sources, keep, free, taken, shared, page)
+
+
+@pytest.mark.parametrize("requests,new,width,page", [(64, 1000, 4, 4), (1000, 64, 4, 4), (16, 3, 256, 1), (1, 2, 2048, 1), (1024, 1024, 4, 3), (1024, 1024, 64, 3), (5, 1, 819, 2),
+                                                     (1025, 9, 4, 3), (70, 70, 300, 2)])
+@pytest.mark.parametrize("kind", ["end", "any", "twice"])
+def test_fork_of_many_pages(requests, new, width, page, kind):
+    """Pages given back and shared by the thousand, in and past what one workgroup does."""
+    rng = random.Random(requests + new)
+    lens = [rng.randint(width * page // 2, width * page) for _ in range(requests)]
+    sources = [-1 if kind == "end" and i % 9 else rng.randrange(-1, requests) if kind == "any" else i // 2 % requests for i in range(new)]
+    keep = [rng.randint(0, width * page) for _ in range(new)]
+    table, free, taken, shared = _pool(rng, lens, page, width, new, common=3)
+    print(f"fork of {requests} places into {new} of {width} pages, {kind}", flush=True)
     _fork([], table, lens, sources, keep, free, taken, shared, page)
 
 

@@ -493,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void k_verify_draw(VerifyArgs A) {
   }
 }
 
-// Vocabularies of up to kOneRow: the walk and both passes over the row in one launch, a request to a workgroup of kOne threads.
+// The walk and both passes over the row in one launch, a request to a workgroup of kOne threads, whose numbers' sums LDS holds.
 constexpr int kOne = 1024, kOneRow = 1 << 16;
 
 template <class T, bool CHOSEN>
@@ -612,6 +612,15 @@ int check_verify(const tjev_gdn_draft_params* p) {
   return 0;
 }
 
+// Whether a call's requests are verified by a workgroup each, in one launch: where a row is read in about the time that the second
+// launch would take (chosen tokens of 50257 in bf16, 1 to 256 requests: 12.1 us, in two launches 14.1; of 65536 in fp32, 64: 13.4, 14.3; drawn
+// ones, two rows of it, 16.6, 14.8), and every CU has one request at most, which is as many workgroups as its LDS holds (1024 requests of
+// drawn ones of 32000 in bf16: 39.3, 29.5).
+constexpr int kOneRequests = 256, kOneBytes = 1 << 18;
+bool in_one(const tjev_gdn_draft_params* p, long row_bytes) {
+  return p->vocab <= kOneRow && p->requests <= kOneRequests && row_bytes <= kOneBytes;
+}
+
 long slices_of(const tjev_gdn_draft_params* p) { return ((long)p->vocab + kSlice - 1) / kSlice; }
 long parts_of(const tjev_gdn_draft_params* p) { return ((long)p->vocab + kPart - 1) / kPart; }
 // the workspace: the ends, the parts' sums, the slices' bits and marks
@@ -683,7 +692,7 @@ int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const i
   auto one = [&](auto type, auto chosen) {
     hipLaunchKernelGGL((gdn::k_verify_one<decltype(type), chosen.value>), draw, dim3(gdn::kOne), 0, st, A);
   };
-  if (p->vocab <= gdn::kOneRow) {
+  if (gdn::in_one(p, p->vocab * e * (draft ? 2 : 1))) {
     if (e == 2) {
       draft ? one(uint16_t{}, std::false_type{}) : one(uint16_t{}, std::true_type{});
     } else {

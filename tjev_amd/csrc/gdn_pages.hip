@@ -228,8 +228,12 @@ __device__ __forceinline__ void take(const ForkArgs& A, int r, const ForkNew& g,
   if (got >= 0) A.shared_out[got] = 0;
 }
 
-// Few places and entries: the rest in one workgroup of a thread per place, whose barriers stand for the ends of three launches.
-constexpr int kOne = 1024, kOneTurns = 64;  // the most threads; of each, entries
+// Few places and entries: the rest in one workgroup of a thread per place, whose barriers stand for the ends of three launches. An entry
+// that loses its holder costs one CU 5 ns (two atomics, two loads and two stores, each lane's of a line of its own), so this is for few:
+// 16 places of 64 pages, all given back, 18.6 us a call, in launches of their own 26.4; 64 of 64 all of them 26.2 and 26.4, one page of each place
+// 18.7 and 26.6; and 64 of 512 would take 182 and 26.5 (a page of each 18.1: how many are given back the host does not know, and
+// where beams go on from each other it is half of them at every step).
+constexpr int kOne = 1024, kBatch = 4;  // the most threads; of each, entries
 
 // running sums over the workgroup's threads of two numbers of 32 bits, and the whole
 __device__ __forceinline__ long scan_one(long v, long* swave, long& total) {
@@ -253,21 +257,16 @@ __device__ __forceinline__ long scan_one(long v, long* swave, long& total) {
 __device__ __forceinline__ long pair(int hi, int lo) { return (long)hi << 32 | lo; }
 __device__ __forceinline__ int hi_of(long v) { return (int)(v >> 32); }
 __device__ __forceinline__ int lo_of(long v) { return (int)v; }
-// the place whose run of numbers holds e: the last of those that begin at or before it
-__device__ __forceinline__ int run_of(const int* begin, int n, int e) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (begin[mid] <= e) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
+// The entries that lose or gain a holder are numbered through, place by place, kOne to a turn. Each is a chain of latencies (its place, the
+// table, the counts), so all turns are on their way at once; the entries' ranks among those given back come from
+// one running sum over the turns' and waves' numbers of them.
 __global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
-  __shared__ int sdrop[kOne], sadd[kOne], skept[kOne], ssource[kOne];
+  __shared__ int sdrop[kOne], sadd[kOne];    // the first number of each place's entries
+  __shared__ int sfrom[kOne], ssource[kOne];  // the table's index of an entry, less its number
+  __shared__ int sback[kBatch][kOne / 64];
   __shared__ long swave[kOne / 64];
-  GDN_POISON_LDS(sdrop, sadd, skept, ssource, swave);
-  const int tid = threadIdx.x;
+  GDN_POISON_LDS(sdrop, sadd, sfrom, ssource, sback, swave);
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(wave());
   const ForkOld o = tid < A.B ? A.old[tid] : ForkOld{0, 0};
   const ForkNew g = tid < A.B2 ? A.fresh[tid] : ForkNew{-1, 0, -1, 0};
   const long had = min((long)max(A.taken[0], 0), A.n_free);
@@ -277,58 +276,79 @@ __global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
   const int n_drop = hi_of(all), n_add = lo_of(all);
   sdrop[tid] = hi_of(upto) - drops;
   sadd[tid] = lo_of(upto) - adds;
-  skept[tid] = o.kept;
-  ssource[tid] = g.source;
+  sfrom[tid] = tid * A.M + o.kept - sdrop[tid];
+  ssource[tid] = g.source * A.M - sadd[tid];
   if (g.last >= 0) {
     atomicAdd(&A.writers[g.last], 1);
     atomicMin(&A.writer[g.last], tid);
   }
   __syncthreads();
-  int r0 = 0, j0 = 0;  // the thread's first entry, kept: most calls have no more
-  if (tid < n_drop) {
-    r0 = run_of(sdrop, A.B, tid);
-    j0 = skept[r0] + tid - sdrop[r0];
-  }
-  auto dropped = [&](int e, int& r, int& j) {
-    r = e == tid ? r0 : run_of(sdrop, A.B, e);
-    j = e == tid ? j0 : skept[r] + e - sdrop[r];
+  // the thread's entries of `n`: the index of each in the table, and its page (-1: none)
+  auto entries = [&](const int* begin, const int* base, int places, int n, int (&at)[kBatch], int (&page)[kBatch]) {
+    // each one's place: the last of those whose entries begin at or before it
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) at[u] = 0;
+    for (int step = kOne / 2; step; step /= 2)
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (at[u] + step < places && begin[at[u] + step] <= u * kOne + tid) at[u] += step;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int e = u * kOne + tid;
+      at[u] = e < n ? base[at[u]] + e : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      page[u] = at[u] >= 0 ? A.table[at[u]] : -1;
+      if (!is_page(A, page[u])) page[u] = -1;
+    }
   };
-  for (int e = tid; e < n_drop; e += kOne) {
-    int r, j;
-    dropped(e, r, j);
-    drop(A, r, j);
+  int at[kBatch], page[kBatch];
+  if (n_add) {
+    entries(sadd, ssource, A.B2, n_add, at, page);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (page[u] >= 0) atomicAdd(&A.shared_out[page[u]], 1);
   }
-  for (int e = tid; e < n_add; e += kOne) {
-    const int r = run_of(sadd, A.B2, e);
-    add(A, ssource[r], e - sadd[r]);
-  }
+  entries(sdrop, sfrom, A.B, n_drop, at, page);
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u)
+    if (page[u] >= 0) {
+      atomicSub(&A.shared_out[page[u]], 1);
+      atomicMin(&A.entry[page[u]], at[u]);
+    }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): all is counted
   __syncthreads();
   const bool copy = takes_copy(A, tid, g);
-  uint64_t back_here = 0;  // of the thread's entries, up to kOneTurns of them
-  for (int e = tid, i = 0; e < n_drop; e += kOne, ++i) {
-    int r, j, p;
-    dropped(e, r, j);
-    if (gives_back(A, r, j, p)) back_here |= 1ull << i;
+  int first[kBatch], holders[kBatch];
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    first[u] = page[u] >= 0 ? counted(&A.entry[page[u]]) : -1;
+    holders[u] = page[u] >= 0 ? counted(&A.shared_out[page[u]]) : 0;
   }
-  const long ranks = scan_one(pair(__builtin_popcountll(back_here), copy), swave, all);
+  uint64_t gone[kBatch];  // of the wave's entries of each turn, those that give their page back
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    gone[u] = __ballot(page[u] >= 0 && first[u] == at[u] && holders[u] == -1);
+    if (lane() == 0) sback[u][w] = __builtin_popcountll(gone[u]);
+  }
+  __syncthreads();
+  int* const backs = &sback[0][0];
+  const int mine = tid < kBatch * (kOne / 64) ? backs[tid] : 0;
+  const long ranks = scan_one(pair(mine, copy), swave, all);
   const int n_back = hi_of(all), n_copy = lo_of(all), rank = lo_of(ranks) - copy;
   const long back = min((long)n_back, had);  // what the list has room for
   if (tid == 0) A.taken_out[0] = (int)min(had - back + n_copy, 0x7fffffffl);
   if (n_back) {
-    long before = 0;
-    for (int e = tid, i = 0; i * kOne < n_drop; e += kOne, ++i) {
-      const bool gone = back_here >> i & 1;
-      const long at = before + (n_drop <= kOne ? hi_of(ranks) : lo_of(scan_one(gone, swave, all))) - 1;
-      before += lo_of(all);
-      if (gone) {
-        int r, j;
-        dropped(e, r, j);
-        const int p = A.table[(long)r * A.M + j];
-        A.shared_out[p] = 0;
-        if (at < back) A.free_out[had - back + at] = p;
+    if (tid < kBatch * (kOne / 64)) backs[tid] = hi_of(ranks) - mine;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (gone[u] >> lane() & 1) {
+        const long place = sback[u][w] + __builtin_popcountll(gone[u] & ((1ull << lane()) - 1));
+        A.shared_out[page[u]] = 0;
+        if (place < back) A.free_out[had - back + place] = page[u];
       }
-    }
   }
   if (copy) atomicSub(&A.shared_out[g.last], 1);  // others hold it on: it is not given back
   if (n_copy) {
@@ -616,7 +636,7 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   const dim3 block(gdn::kThreads);
   hipLaunchKernelGGL(gdn::k_fork_init, dim3((unsigned)std::max((long)places, std::min(blocks, 1024l))), block, 0, st, A);
   const long entries = (long)std::max(A.B, A.B2) * A.M;
-  C.known = places <= gdn::kOne && entries <= gdn::kOne * gdn::kOneTurns;
+  C.known = places <= gdn::kOne && entries <= gdn::kOne * gdn::kBatch;
   if (C.known) {
     hipLaunchKernelGGL(gdn::k_fork_one, dim3(1), dim3(gdn::kOne), 0, st, A);
     if (!p->layers) {
@@ -633,7 +653,6 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
     C.layers = layers;
     C.first = first;
     const int y = 2 * layers * c.groups;
-    
     const int turn = gdn::kCopyTurns * gdn::UN * (gdn::kThreads / c.cols);
     hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, (p->page_size + turn - 1) / turn), block, 0, st, C);
   });
