@@ -388,15 +388,17 @@ def test_fork_of_many(requests, new, width, page):
     _fork([], table, lens, sources, keep, free, taken, shared, page)
 
 
-@pytest.mark.parametrize("requests,new,width,page", [(64, 1000, 4, 4), (1000, 64, 4, 4), (16, 3, 256, 1), (1, 2, 2048, 1), (1024, 1024, 4, 3), (1024, 1024, 64, 3), (5, 1, 819, 2),
-                                                     (1025, 9, 4, 3), (70, 70, 300, 2)])
-@pytest.mark.parametrize("kind", ["end", "any", "twice"])
+@pytest.mark.parametrize("requests,new,width,page", [
+    (64, 1000, 4, 4), (1000, 64, 4, 4), (16, 3, 256, 1), (1, 2, 2048, 1), (1024, 1024, 4, 3), (5, 1, 819, 2), (64, 1000, 65, 4), (1000, 64, 65, 4),
+    (16, 3, 4096, 1), (1, 2, 20000, 1), (1024, 1024, 64, 3), (1025, 9, 4, 3), (70, 70, 300, 2),
+])
+@pytest.mark.parametrize("kind", ["end", "any", "twice", "all kept"])
 def test_fork_of_many_pages(requests, new, width, page, kind):
     """Pages given back and shared by the thousand, in and past what one workgroup does."""
     rng = random.Random(requests + new)
     lens = [rng.randint(width * page // 2, width * page) for _ in range(requests)]
     sources = [-1 if kind == "end" and i % 9 else rng.randrange(-1, requests) if kind == "any" else i // 2 % requests for i in range(new)]
-    keep = [rng.randint(0, width * page) for _ in range(new)]
+    keep = None if kind == "all kept" else [rng.randint(0, width * page) for _ in range(new)]
     table, free, taken, shared = _pool(rng, lens, page, width, new, common=3)
     print(f"fork of {requests} places into {new} of {width} pages, {kind}", flush=True)
     _fork([], table, lens, sources, keep, free, taken, shared, page)

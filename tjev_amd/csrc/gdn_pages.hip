@@ -53,6 +53,7 @@ struct Move {
   int from, from_in, to, to_in;
 };
 
+// One tree of 16, 6 layers of 4 heads of 256: 5.0 us; 128 of up to 60, 8 layers of 8 heads of 128, 7.3 MB: 9.8.
 template <class W>
 __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactArgs A) {
   constexpr int UN = 8;
@@ -229,11 +230,14 @@ __device__ __forceinline__ void take(const ForkArgs& A, int r, const ForkNew& g,
 }
 
 // Few places and entries: the rest in one workgroup of a thread per place, whose barriers stand for the ends of three launches. An entry
-// that loses its holder costs one CU 5 ns (two atomics, two loads and two stores, each lane's of a line of its own), so this is for few:
-// 16 places of 64 pages, all given back, 18.6 us a call, in launches of their own 26.4; 64 of 64 all of them 26.2 and 26.4, one page of each place
-// 18.7 and 26.6; and 64 of 512 would take 182 and 26.5 (a page of each 18.1: how many are given back the host does not know, and
-// where beams go on from each other it is half of them at every step).
-constexpr int kOne = 1024, kBatch = 4;  // the most threads; of each, entries
+// that loses its holder costs one CU 5 ns (two atomics, two loads and two stores, each lane's of a line of its own), so this is for calls
+// that change few, which the host does not know and guesses. With lengths to keep (a step's roll back: most places go on, with
+// what they had) tables of up to kOneTurns * kOne entries: 64 places of 512 pages, a page of each given back, 18.6 us a call, in
+// launches of their own 26.7; with three whole rows 21.4 and 26.4, with twenty 70 and 26; all given back 178 and 26.5. Without (beams that go on from each other, samples)
+// up to kFewTurns * kOne: 64 of 64, all given back, 26.2 and 26.4, a page of each 18.7 and 26.6; half of 64 of 512, the rest twice,
+// would take 152 and 26.6.
+constexpr int kOne = 1024, kOneTurns = 64, kFewTurns = 4;
+constexpr int kBatch = 4;  // entries that a thread has on their way at once
 
 // running sums over the workgroup's threads of two numbers of 32 bits, and the whole
 __device__ __forceinline__ long scan_one(long v, long* swave, long& total) {
@@ -257,14 +261,25 @@ __device__ __forceinline__ long scan_one(long v, long* swave, long& total) {
 __device__ __forceinline__ long pair(int hi, int lo) { return (long)hi << 32 | lo; }
 __device__ __forceinline__ int hi_of(long v) { return (int)(v >> 32); }
 __device__ __forceinline__ int lo_of(long v) { return (int)v; }
+// of each of the entries e0, e0 + kOne, ... the place whose run of numbers holds it: the last of those that begin at or before it
+__device__ __forceinline__ void runs_of(const int* begin, int n, int e0, int (&r)[kBatch]) {
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) r[u] = 0;
+  for (int step = kOne / 2; step; step /= 2)
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (r[u] + step < n && begin[r[u] + step] <= e0 + u * kOne) r[u] += step;
+}
+
 // The entries that lose or gain a holder are numbered through, place by place, kOne to a turn. Each is a chain of latencies (its place, the
-// table, the counts), so all turns are on their way at once; the entries' ranks among those given back come from
-// one running sum over the turns' and waves' numbers of them.
+// table, the counts), so a thread has kBatch on their way at once; the entries' ranks among those given back come from one running
+// sum over all turns' and waves' numbers of them.
 __global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
   __shared__ int sdrop[kOne], sadd[kOne];    // the first number of each place's entries
   __shared__ int sfrom[kOne], ssource[kOne];  // the table's index of an entry, less its number
-  __shared__ int sback[kBatch][kOne / 64];
+  __shared__ int sback[kOneTurns][kOne / 64];
   __shared__ long swave[kOne / 64];
+  static_assert(kOneTurns * (kOne / 64) == kOne && kOneTurns % kBatch == 0, "a thread per number");
   GDN_POISON_LDS(sdrop, sadd, sfrom, ssource, sback, swave);
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(wave());
   const ForkOld o = tid < A.B ? A.old[tid] : ForkOld{0, 0};
@@ -274,27 +289,23 @@ __global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
   long all;
   const long upto = scan_one(pair(drops, adds), swave, all);
   const int n_drop = hi_of(all), n_add = lo_of(all);
+  int* const backs = &sback[0][0];
   sdrop[tid] = hi_of(upto) - drops;
   sadd[tid] = lo_of(upto) - adds;
   sfrom[tid] = tid * A.M + o.kept - sdrop[tid];
   ssource[tid] = g.source * A.M - sadd[tid];
+  backs[tid] = 0;
   if (g.last >= 0) {
     atomicAdd(&A.writers[g.last], 1);
     atomicMin(&A.writer[g.last], tid);
   }
   __syncthreads();
-  // the thread's entries of `n`: the index of each in the table, and its page (-1: none)
-  auto entries = [&](const int* begin, const int* base, int places, int n, int (&at)[kBatch], int (&page)[kBatch]) {
-    // each one's place: the last of those whose entries begin at or before it
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) at[u] = 0;
-    for (int step = kOne / 2; step; step /= 2)
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (at[u] + step < places && begin[at[u] + step] <= u * kOne + tid) at[u] += step;
+  // the thread's entries of a batch: the index of each in the table, and its page (-1: none)
+  auto entries = [&](const int* begin, const int* base, int places, int n, int e0, int (&at)[kBatch], int (&page)[kBatch]) {
+    runs_of(begin, places, e0 + tid, at);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int e = u * kOne + tid;
+      const int e = e0 + u * kOne + tid;
       at[u] = e < n ? base[at[u]] + e : -1;
     }
 #pragma unroll
@@ -303,52 +314,83 @@ __global__ __launch_bounds__(kOne) void k_fork_one(ForkArgs A) {
       if (!is_page(A, page[u])) page[u] = -1;
     }
   };
-  int at[kBatch], page[kBatch];
-  if (n_add) {
-    entries(sadd, ssource, A.B2, n_add, at, page);
+  for (int e0 = 0; e0 < n_add; e0 += kBatch * kOne) {
+    int at[kBatch], page[kBatch];
+    entries(sadd, ssource, A.B2, n_add, e0, at, page);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
       if (page[u] >= 0) atomicAdd(&A.shared_out[page[u]], 1);
   }
-  entries(sdrop, sfrom, A.B, n_drop, at, page);
+  int at0[kBatch], page0[kBatch];  // the first batch's, kept: most calls have no more
+  entries(sdrop, sfrom, A.B, n_drop, 0, at0, page0);
+  auto drop_all = [&](const int (&at)[kBatch], const int (&page)[kBatch]) {
 #pragma unroll
-  for (int u = 0; u < kBatch; ++u)
-    if (page[u] >= 0) {
-      atomicSub(&A.shared_out[page[u]], 1);
-      atomicMin(&A.entry[page[u]], at[u]);
-    }
+    for (int u = 0; u < kBatch; ++u)
+      if (page[u] >= 0) {
+        atomicSub(&A.shared_out[page[u]], 1);
+        atomicMin(&A.entry[page[u]], at[u]);
+      }
+  };
+  drop_all(at0, page0);
+  for (int e0 = kBatch * kOne; e0 < n_drop; e0 += kBatch * kOne) {
+    int at[kBatch], page[kBatch];
+    entries(sdrop, sfrom, A.B, n_drop, e0, at, page);
+    drop_all(at, page);
+  }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): all is counted
   __syncthreads();
   const bool copy = takes_copy(A, tid, g);
-  int first[kBatch], holders[kBatch];
+  uint64_t back_here = 0;  // of the thread's entries, by their turn
+  auto look = [&](int e0, const int (&at)[kBatch], const int (&page)[kBatch]) {
+    int first[kBatch], holders[kBatch];
 #pragma unroll
-  for (int u = 0; u < kBatch; ++u) {
-    first[u] = page[u] >= 0 ? counted(&A.entry[page[u]]) : -1;
-    holders[u] = page[u] >= 0 ? counted(&A.shared_out[page[u]]) : 0;
-  }
-  uint64_t gone[kBatch];  // of the wave's entries of each turn, those that give their page back
+    for (int u = 0; u < kBatch; ++u) {
+      first[u] = page[u] >= 0 ? counted(&A.entry[page[u]]) : -1;
+      holders[u] = page[u] >= 0 ? counted(&A.shared_out[page[u]]) : 0;
+    }
 #pragma unroll
-  for (int u = 0; u < kBatch; ++u) {
-    gone[u] = __ballot(page[u] >= 0 && first[u] == at[u] && holders[u] == -1);
-    if (lane() == 0) sback[u][w] = __builtin_popcountll(gone[u]);
+    for (int u = 0; u < kBatch; ++u) {
+      const int turn = e0 / kOne + u;
+      const bool gone = page[u] >= 0 && first[u] == at[u] && holders[u] == -1;
+      const uint64_t mask = __ballot(gone);
+      if (gone) back_here |= 1ull << turn;
+      if (mask && lane() == 0) sback[turn][w] = __builtin_popcountll(mask);
+    }
+  };
+  look(0, at0, page0);
+  for (int e0 = kBatch * kOne; e0 < n_drop; e0 += kBatch * kOne) {
+    int at[kBatch], page[kBatch];
+    entries(sdrop, sfrom, A.B, n_drop, e0, at, page);
+    look(e0, at, page);
   }
   __syncthreads();
-  int* const backs = &sback[0][0];
-  const int mine = tid < kBatch * (kOne / 64) ? backs[tid] : 0;
+  const int mine = backs[tid];
   const long ranks = scan_one(pair(mine, copy), swave, all);
   const int n_back = hi_of(all), n_copy = lo_of(all), rank = lo_of(ranks) - copy;
   const long back = min((long)n_back, had);  // what the list has room for
   if (tid == 0) A.taken_out[0] = (int)min(had - back + n_copy, 0x7fffffffl);
   if (n_back) {
-    if (tid < kBatch * (kOne / 64)) backs[tid] = hi_of(ranks) - mine;
+    backs[tid] = hi_of(ranks) - mine;
     __syncthreads();
+    auto give = [&](int e0, const int (&page)[kBatch]) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (gone[u] >> lane() & 1) {
-        const long place = sback[u][w] + __builtin_popcountll(gone[u] & ((1ull << lane()) - 1));
-        A.shared_out[page[u]] = 0;
-        if (place < back) A.free_out[had - back + place] = page[u];
+      for (int u = 0; u < kBatch; ++u) {
+        const int turn = e0 / kOne + u;
+        const bool gone = back_here >> turn & 1;
+        const uint64_t mask = __ballot(gone);
+        if (gone) {
+          const long place = sback[turn][w] + __builtin_popcountll(mask & ((1ull << lane()) - 1));
+          A.shared_out[page[u]] = 0;
+          if (place < back) A.free_out[had - back + place] = page[u];
+        }
       }
+    };
+    give(0, page0);
+    for (int e0 = kBatch * kOne; e0 < n_drop; e0 += kBatch * kOne) {
+      int at[kBatch], page[kBatch];
+      entries(sdrop, sfrom, A.B, n_drop, e0, at, page);
+      give(e0, page);
+    }
   }
   if (copy) atomicSub(&A.shared_out[g.last], 1);  // others hold it on: it is not given back
   if (n_copy) {
@@ -478,6 +520,7 @@ struct ForkCopyArgs {
   bool known, first;  // where names pages; of the launches (the first takes them)
 };
 
+// Bound by memory: the last pages of 192 samples, 6 layers of 4 heads of 256 in pages of 64, 215 MB, 50 us, 4.3 TB/s (a large copy has 5.0).
 // The copies: a workgroup per new place, cache, group of columns and kCopyTurns times the tokens that its threads have on their way at
 // once. The free list is whole by now: a copy may take a page that
 // was given back (which no copy is made of: what writers leave is held by others).
@@ -636,7 +679,7 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   const dim3 block(gdn::kThreads);
   hipLaunchKernelGGL(gdn::k_fork_init, dim3((unsigned)std::max((long)places, std::min(blocks, 1024l))), block, 0, st, A);
   const long entries = (long)std::max(A.B, A.B2) * A.M;
-  C.known = places <= gdn::kOne && entries <= gdn::kOne * gdn::kBatch;
+  C.known = places <= gdn::kOne && entries <= gdn::kOne * (keep ? gdn::kOneTurns : gdn::kFewTurns);
   if (C.known) {
     hipLaunchKernelGGL(gdn::k_fork_one, dim3(1), dim3(gdn::kOne), 0, st, A);
     if (!p->layers) {

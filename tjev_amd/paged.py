@@ -442,6 +442,9 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
     table's order, and are the first to be taken again; the list needs room for them there, as it has where all of them were
     taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
 
+    A call with ``keep`` is taken to be a step's roll back, where few pages change hands; it is right with any, but slower than one without
+    where thousands do (64 places of 512 pages, all given back: 180 us instead of 27).
+
     Nothing given is changed but the caches: the new table, lengths, list, ``taken`` and ``shared`` come back."""
     _lib.not_recorded("paged_fork")
     lib = _lib.load()
