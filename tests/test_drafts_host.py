@@ -129,6 +129,19 @@ def test_refusals(library, what, bad, match):
     assert not [c for c in library.calls if not c[0].endswith("bytes")]
 
 
+@pytest.mark.parametrize("what", ["paged_compact", "paged_fork"])
+def test_a_cache_given_twice(library, what):
+    """Its tokens would be moved twice. Keys and values in one tensor are two caches."""
+    joint, other = torch.zeros(4, 16, 2, 2, 64), torch.zeros(4, 16, 2, 64)
+    k, v = joint[..., 0, :], joint[..., 1, :]
+    for caches in ([(k, k)], [(k, v), (k, v)], [(k, v), (v, k)]):
+        with pytest.raises(ValueError, match="twice"):
+            _call(what, caches=caches)
+    assert not [c for c in library.calls if not c[0].endswith("bytes")]
+    _call(what, caches=[(k, v)])
+    _call(what, caches=[(other, other + 1)])
+
+
 def test_products_past_32_bits(library):
     """A table of 2^31 entries: its rows are counted in 32 bits."""
     table = torch.zeros(1, 1, dtype=torch.int32).expand(2048, 1 << 20)
@@ -143,7 +156,7 @@ def test_products_past_32_bits(library):
 def test_gradients_are_not_lost(library, what, which):
     x = {"target_probs": torch.zeros(5, 11), "draft_probs": torch.zeros(5, 11), "uniforms": torch.zeros(5), "q": torch.zeros(3, 4, 64), "k_cache": CACHE.clone(),
          "gate": torch.zeros(3, 4, 64), "out": torch.zeros(3, 4, 64), "caches": CACHE.clone()}[which]
-    give = (lambda t: dict(caches=[(CACHE, CACHE), (CACHE, t)])) if which == "caches" else (lambda t: {which: t})
+    give = (lambda t: dict(caches=[(CACHE, CACHE + 1), (CACHE + 2, t)])) if which == "caches" else (lambda t: {which: t})
     with forward_ad.dual_level(), torch.no_grad():
         with pytest.raises(RuntimeError, match=f"{what} has no gradient"):
             _call(what, **give(forward_ad.make_dual(x, torch.ones_like(x))))

@@ -339,6 +339,12 @@ def _layers(what: str, caches):
             array.array("Q", map(_address, vs)))
 
 
+def _distinct(what: str, layers: int, ks, vs) -> None:
+    """Tokens of a cache that is listed twice would be moved twice, by workgroups at once."""
+    if layers and len({*ks, *vs}) < 2 * layers:
+        raise ValueError(f"{what}: a cache is given twice (layers that share one name it once)")
+
+
 _NO_LAYERS = array.array("Q", (0,))
 
 
@@ -384,7 +390,7 @@ def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengt
     """Moves the kept ones of every request's new tokens to the front of them, in all layers' caches at once, in place, and
     returns the lengths that are left [B] int32: token path[b, j] becomes the j-th, j < kept[b], as ``verify_drafts`` names them.
 
-    ``caches``: the (k_cache, v_cache) of every layer, alike in shape and strides (none: the lengths alone). ``starts`` and
+    ``caches``: the (k_cache, v_cache) of every layer, alike in shape and strides, none of them twice or part of another (none: the lengths alone). ``starts`` and
     ``lengths`` are the step's, with the new tokens. A request's numbers in ``path`` [B, max_new] grow; those that are less than their
     place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct. What
     stands behind a request's kept tokens is left as it was."""
@@ -393,6 +399,7 @@ def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengt
     p = _compact_params(
         like, layers, block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, path.shape, path.dtype,
         kept.shape, kept.dtype, (block_table.get_device(), starts.get_device(), lengths.get_device(), path.get_device(), kept.get_device()))
+    _distinct("paged_compact", layers, ks, vs)
     dev = block_table.device
     table, starts, lengths, path, kept = block_table.contiguous(), _int32(starts), _int32(lengths), _int32_near(path), _int32_near(kept)
     out = torch.empty_like(lengths)
@@ -437,7 +444,7 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
 
     ``shared`` [pages]: how many hold each page beside its first holder (0 in the beginning). Places share pages; but a last page with room
     in it, where the next tokens go, has one holder: the first place that goes on in it where nobody holds it otherwise, and for each
-    other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides;
+    other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides, none of them twice;
     those may be none). Pages that nobody holds any more come back in front of index ``taken`` of ``free_pages`` [F], in the
     table's order, and are the first to be taken again; the list needs room for them there, as it has where all of them were
     taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
@@ -455,6 +462,7 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
         shared.dtype, int(page_size),
         (block_table.get_device(), lengths.get_device(), sources.get_device(), _device(keep, lengths), free_pages.get_device(),
          taken.get_device(), shared.get_device()))
+    _distinct("paged_fork", layers, ks, vs)
     dev = block_table.device
     table, lengths, sources, free, taken, shared = (block_table.contiguous(), _int32(lengths), _int32_near(sources), _int32(free_pages),
                                                     _int32(taken), _int32(shared))
