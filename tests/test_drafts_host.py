@@ -360,7 +360,7 @@ def _tree_workspace(**kw):
 
 
 def test_small_batches_of_trees_are_streamed():
-    """Places of 16 rows, not of 128: within two units to a workgroup; beyond that, in fp32 and in few rows as causal rows are."""
+    """Places of 16 rows, not of 128: within a few units to a workgroup; beyond that, in fp32 and in few rows as causal rows are."""
     place = lambda rows: 2 * rows * (256 + 2) * 4 + 32  # noqa: E731
     tree, causal = _tree_workspace()
     assert tree % place(16) == 0 and causal % place(128) == 0

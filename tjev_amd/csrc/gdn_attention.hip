@@ -41,9 +41,10 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p, bool tree) {
   auto tiles_of = [&](int tile_rows) { return (rows / tile_rows + active) * p->kv_heads; };
   r.mixed = bf && top > 16 * r.nq;
   // Trees whose streamed tiles are at most kFewTurns units to a workgroup are streamed, and read their keys a few times: the many
-  // small parts are worked on at once (16/4 heads of 256: one tree of 12 over 4000, 22.4 us instead of 26.1; 4 of 12 over 1000, 24.4 and 34.1;
-  // 16 of 6 over 1000, 30.6 and 40.9; with twice the limit 16 of 12 over 1000 would take 44.7, and 43.7 in tiles of 128).
-  constexpr int kFewTurns = 2;
+  // small parts are worked on at once (16/4 heads of 256: 8 trees of 12 over 1000, 28.4 us instead of 36.1 in tiles of 128; 8 of up to 8 over up to
+  // 3000, 19.3 and 37.2; 2 of 12 over 4000, 27.3 and 25.7. With a limit of 6, 16 of 12 over 1000 would take 40.0 instead of 37.7, one of 32 over
+  // 4000 at 32/8 of 128 25.6 instead of 21.9, but 32 of up to 12 over up to 1000 26.1 instead of 37.9: how even they are the host does not know).
+  constexpr int kFewTurns = 4;
   if (tree && r.mixed && tiles_of(16 * r.nq) * blocks <= kFewTurns * (long)most) r.mixed = false;
   const long tiles = tiles_of(r.mixed ? kWideRows : 16 * r.nq);
   r.G = tiles >= most || blocks * tiles >= most ? most : (int)(blocks * tiles);

@@ -320,11 +320,11 @@ _size, _stride, _get_device, _address = torch.Tensor.size, torch.Tensor.stride, 
 
 
 def _layers(what: str, caches):
-    """The layers' caches as the library takes them: what they have in common (kept checks go by it), and the addresses of k's and
-    of v's. A look at each tensor in C, for all at once: 0.5 us a layer."""
+    """The layers' caches as the library takes them: what they have in common (kept checks go by it), their number, and the addresses
+    of all k's, then of all v's. A look at each tensor in C, for all at once: 0.5 us a layer."""
     pairs = list(caches)
     if not pairs:
-        return None, 0, _NO_LAYERS, _NO_LAYERS
+        return None, 0, _NO_LAYERS
     if set(map(len, pairs)) != {2}:
         raise ValueError(f"{what} takes pairs of caches, k and v of every layer")
     ks, vs = zip(*pairs)
@@ -335,14 +335,16 @@ def _layers(what: str, caches):
         _lib.inference_only(what, *flat)
     if len(sizes) > 1 or len(k_strides) > 1 or len(v_strides) > 1 or len({dt for dt, _ in alike}) > 1:
         raise ValueError(f"the layers' caches are alike in shape, strides and type, not {sizes} {k_strides} {v_strides} {[dt for dt, _ in alike]}")
-    return ((sizes.pop(), k_strides.pop(), v_strides.pop(), alike.pop()[0], *devices), len(pairs), array.array("Q", map(_address, ks)),
-            array.array("Q", map(_address, vs)))
+    return (sizes.pop(), k_strides.pop(), v_strides.pop(), alike.pop()[0], *devices), len(pairs), array.array("Q", map(_address, flat))
 
 
-def _distinct(what: str, layers: int, ks, vs) -> None:
-    """Tokens of a cache that is listed twice would be moved twice, by workgroups at once."""
-    if layers and len({*ks, *vs}) < 2 * layers:
+def _of_layers(what: str, layers: int, addresses) -> tuple[int, int]:
+    """Where the library finds the addresses of k's and of v's. Tokens of a cache that is listed twice would be moved twice, by
+    workgroups at once."""
+    if len(set(addresses)) < 2 * layers:
         raise ValueError(f"{what}: a cache is given twice (layers that share one name it once)")
+    at = addresses.buffer_info()[0]
+    return at, at + 8 * layers
 
 
 _NO_LAYERS = array.array("Q", (0,))
@@ -395,17 +397,17 @@ def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengt
     place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct. What
     stands behind a request's kept tokens is left as it was."""
     _lib.not_recorded("paged_compact")
-    like, layers, ks, vs = _layers("paged_compact", caches)
+    like, layers, addresses = _layers("paged_compact", caches)
     p = _compact_params(
         like, layers, block_table.shape, block_table.dtype, starts.shape, starts.dtype, lengths.shape, lengths.dtype, path.shape, path.dtype,
         kept.shape, kept.dtype, (block_table.get_device(), starts.get_device(), lengths.get_device(), path.get_device(), kept.get_device()))
-    _distinct("paged_compact", layers, ks, vs)
+    k_at, v_at = _of_layers("paged_compact", layers, addresses)
     dev = block_table.device
     table, starts, lengths, path, kept = block_table.contiguous(), _int32(starts), _int32(lengths), _int32_near(path), _int32_near(kept)
     out = torch.empty_like(lengths)
     with _lib.on_device(dev):
         _lib.check_status(_lib.load().tjev_gdn_paged_compact(
-            p, _lib.current_stream(dev), ks.buffer_info()[0], vs.buffer_info()[0], table.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
+            p, _lib.current_stream(dev), k_at, v_at, table.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
             path.data_ptr(), kept.data_ptr(), out.data_ptr()))
     return out
 
@@ -455,14 +457,14 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
     Nothing given is changed but the caches: the new table, lengths, list, ``taken`` and ``shared`` come back."""
     _lib.not_recorded("paged_fork")
     lib = _lib.load()
-    like, layers, ks, vs = _layers("paged_fork", caches)
+    like, layers, addresses = _layers("paged_fork", caches)
     p, need = _fork_params(
         lib, like, layers, block_table.shape, block_table.dtype, lengths.shape, lengths.dtype, sources.shape, sources.dtype,
         None if keep is None else (keep.shape, keep.dtype), free_pages.shape, free_pages.dtype, (taken.numel(), taken.dtype), shared.shape,
         shared.dtype, int(page_size),
         (block_table.get_device(), lengths.get_device(), sources.get_device(), _device(keep, lengths), free_pages.get_device(),
          taken.get_device(), shared.get_device()))
-    _distinct("paged_fork", layers, ks, vs)
+    k_at, v_at = _of_layers("paged_fork", layers, addresses)
     dev = block_table.device
     table, lengths, sources, free, taken, shared = (block_table.contiguous(), _int32(lengths), _int32_near(sources), _int32(free_pages),
                                                     _int32(taken), _int32(shared))
@@ -472,7 +474,7 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
     lengths_out, free_out, taken_out, shared_out = torch.empty_like(sources), torch.empty_like(free), taken.new_empty(1), torch.empty_like(shared)
     with _lib.on_device(dev):
         _lib.check_status(lib.tjev_gdn_paged_fork(
-            p, _lib.current_stream(dev), ks.buffer_info()[0], vs.buffer_info()[0], table.data_ptr(), lengths.data_ptr(), sources.data_ptr(),
+            p, _lib.current_stream(dev), k_at, v_at, table.data_ptr(), lengths.data_ptr(), sources.data_ptr(),
             None if keep is None else keep.data_ptr(), free.data_ptr(), taken.data_ptr(), shared.data_ptr(), table_out.data_ptr(),
             lengths_out.data_ptr(), free_out.data_ptr(), taken_out.data_ptr(), shared_out.data_ptr(), ws.data_ptr(), need))
     return Forked(table_out, lengths_out, free_out, taken_out, shared_out)
