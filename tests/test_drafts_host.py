@@ -299,6 +299,8 @@ def test_pages_c_abi():
     for k in (odd, none, None):
         assert compact(_pages(), k=k) == 1 and compact(_pages(), v=k) == 1
     assert fork(_pages(), k=none) == 1 and fork(_pages(), v=None) == 1
+    assert fork(_pages(), k=odd) == 1 and fork(_pages(), v=odd) == 1 and "aligned" in said()  # (before anything is launched)
+    assert fork(_pages(page_size=1 << 20)) == 2 and "2^20" in said()
     for i in range(6):
         a = list(f[:6])
         a[i] = None

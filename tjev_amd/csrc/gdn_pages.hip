@@ -586,14 +586,18 @@ int fill(Caches& c, const tjev_gdn_pages_params* p, void* const* k, void* const*
   return w;
 }
 
-// launch(W, caches of the launch, layers of the launch, whether it is the first) for every kLayers layers, once at least
-template <class F>
-int by_layers(const tjev_gdn_pages_params* p, void* const* k, void* const* v, F launch) {
-  Caches c{};
+// the same, refused before anything is launched; without layers there is one column of nothing
+int layout(Caches& c, int& w, const tjev_gdn_pages_params* p, void* const* k, void* const* v) {
   c.groups = c.cols = 1;
-  int w = 16;
+  w = 16;
   if (p->layers && !(w = fill(c, p, k, v))) return fail(TJEV_GDN_EINVAL, "the caches must be aligned to their elements");
   if (2l * kLayers * c.groups > 65535) return fail(TJEV_GDN_EUNSUPPORTED, "kv_heads * dim too large");
+  return 0;
+}
+
+// launch(W, caches of the launch, layers of the launch, whether it is the first) for every kLayers layers, once at least
+template <class F>
+int by_layers(const tjev_gdn_pages_params* p, Caches c, int w, void* const* k, void* const* v, F launch) {
   for (int l0 = 0; l0 == 0 || l0 < p->layers; l0 += kLayers) {
     const int n = p->layers - l0 < kLayers ? p->layers - l0 : kLayers;
     for (int l = 0; l < n; ++l) c.k[l] = static_cast<char*>(k[l0 + l]), c.v[l] = static_cast<char*>(v[l0 + l]);
@@ -628,7 +632,10 @@ int tjev_gdn_paged_compact(const tjev_gdn_pages_params* p, void* stream, void* c
   A.B = p->requests, A.M = p->table_width, A.pages = p->pages, A.most = p->max_new;
   A.page = gdn::div_by(p->page_size);
   A.table = block_table, A.starts = starts, A.lengths = lengths, A.path = path, A.kept = kept;
-  return gdn::by_layers(p, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
+  gdn::Caches caches{};
+  int w = 0;
+  if (int s = gdn::layout(caches, w, p, k_caches, v_caches)) return s;
+  return gdn::by_layers(p, caches, w, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
     A.c = c;
     A.layers = layers;
     A.lengths_out = first ? lengths_out : nullptr;
@@ -652,6 +659,7 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   if (p->new_requests < 1 || p->n_free < 0) return fail(TJEV_GDN_EINVAL, "new_requests must be positive, n_free not negative");
   if (p->n_free >= (1l << 31) || (long)p->requests * p->table_width >= (1l << 31) || (long)p->new_requests * p->table_width >= (1l << 31))
     return fail(TJEV_GDN_EINVAL, "problem too large");
+  if (p->layers && p->page_size >= (1 << 20)) return fail(TJEV_GDN_EUNSUPPORTED, "forks copy last pages of less than 2^20 tokens");
   if (!block_table || !lengths || !sources || !taken || !shared || !table_out || !lengths_out || !taken_out || !shared_out ||
       (p->n_free && (!free_pages || !free_out)))
     return fail(TJEV_GDN_EINVAL, "null tensor argument");
@@ -660,6 +668,9 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   const size_t need = tjev_gdn_fork_workspace_bytes(p);
   if (!workspace || workspace_bytes < need) return fail(TJEV_GDN_EWORKSPACE, "forks need a workspace of tjev_gdn_fork_workspace_bytes");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TJEV_GDN_EINVAL, "the workspace must be 256-byte aligned");
+  gdn::Caches caches{};
+  int w = 0;
+  if (int s = gdn::layout(caches, w, p, k_caches, v_caches)) return s;
   if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
   gdn::ForkCopyArgs C{};
   gdn::ForkArgs& A = C.f;
@@ -691,13 +702,13 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
     hipLaunchKernelGGL(gdn::k_fork_decide, dim3(places), block, 0, st, A);
     hipLaunchKernelGGL(gdn::k_fork_push, dim3(places), block, 0, st, A);
   }
-  return gdn::by_layers(p, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
+  return gdn::by_layers(p, caches, w, k_caches, v_caches, [&](auto w, const gdn::Caches& c, int layers, bool first) {
     C.c = c;
     C.layers = layers;
     C.first = first;
     const int y = 2 * layers * c.groups;
     const int turn = gdn::kCopyTurns * gdn::UN * (gdn::kThreads / c.cols);
-    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, (p->page_size + turn - 1) / turn), block, 0, st, C);
+    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, layers ? (p->page_size + turn - 1) / turn : 1), block, 0, st, C);
   });
 }
 
