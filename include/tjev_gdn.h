@@ -464,7 +464,8 @@ int tjev_gdn_paged_compact(const tjev_gdn_pages_params* p, void* stream, void* c
  *   table_out  [new_requests, table_width]  -1 behind a place's pages, and for a copy that finds the list at its end
  *   lengths_out [new_requests], free_out [n_free], shared_out [pages]
  *   taken_out  [1]  more than n_free means a shortage
- * aliasing none of the inputs. Pages of caches hold less than 2^20 tokens. The workspace (256-byte aligned) needs no clearing. */
+ * aliasing none of the inputs. Pages of caches hold less than 2^20 tokens, and up to 2^20 - 16 where a token has more than 128 vectors (of 16
+ * bytes, or of one element where an address or stride is no multiple of that). The workspace (256-byte aligned) needs no clearing. */
 size_t tjev_gdn_fork_workspace_bytes(const tjev_gdn_pages_params* p);
 int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* const* k_caches,
                         void* const* v_caches, const int32_t* block_table, const int32_t* lengths,

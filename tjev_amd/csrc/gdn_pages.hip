@@ -553,6 +553,12 @@ __global__ __launch_bounds__(kThreads) void k_fork_copy(ForkCopyArgs A) {
   }
 }
 
+// the workgroups that share out a page's tokens
+long copy_parts(int page, int cols) {
+  const long turn = kCopyTurns * UN * (kThreads / cols);
+  return (page + turn - 1) / turn;
+}
+
 int check(const tjev_gdn_pages_params* p, void* const* k, void* const* v, bool caches) {
   if (!p) return fail(TJEV_GDN_EINVAL, "null params");
   if (p->requests < 1 || p->table_width < 1 || p->page_size < 1 || p->pages < 1 || p->layers < 0)
@@ -671,6 +677,8 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
   gdn::Caches caches{};
   int w = 0;
   if (int s = gdn::layout(caches, w, p, k_caches, v_caches)) return s;
+  const long parts = p->layers ? gdn::copy_parts(p->page_size, caches.cols) : 1;
+  if (parts > 65535) return fail(TJEV_GDN_EUNSUPPORTED, "forks copy last pages of up to 2^20 - 16 tokens of more than 128 vectors each");
   if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
   gdn::ForkCopyArgs C{};
   gdn::ForkArgs& A = C.f;
@@ -707,8 +715,7 @@ int tjev_gdn_paged_fork(const tjev_gdn_pages_params* p, void* stream, void* cons
     C.layers = layers;
     C.first = first;
     const int y = 2 * layers * c.groups;
-    const int turn = gdn::kCopyTurns * gdn::UN * (gdn::kThreads / c.cols);
-    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, layers ? (p->page_size + turn - 1) / turn : 1), block, 0, st, C);
+    hipLaunchKernelGGL((gdn::k_fork_copy<decltype(w)>), dim3(A.B2, y ? y : 1, (unsigned)parts), block, 0, st, C);
   });
 }
 

@@ -447,7 +447,7 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
     ``shared`` [pages]: how many hold each page beside its first holder (0 in the beginning). Places share pages; but a last page with room
     in it, where the next tokens go, has one holder: the first place that goes on in it where nobody holds it otherwise, and for each
     other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides, none of them twice, in
-    pages of less than 2^20 tokens; those may be none). Pages that nobody holds any more come back in front of index ``taken`` of ``free_pages`` [F], in the
+    pages of up to 2^20 - 16 tokens; those may be none). Pages that nobody holds any more come back in front of index ``taken`` of ``free_pages`` [F], in the
     table's order, and are the first to be taken again; the list needs room for them there, as it has where all of them were
     taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
 
