@@ -12,8 +12,16 @@
     f = paged_fork(caches, t.block_table, t.lengths, places, lengths, free_pages, t.taken, shared, page_size=P)
 
 A request's new tokens are a tree. Token 0 is its root, the token that the last step ended with; ``parents`` holds for every other the
-number within the request of the one that it was drafted behind, which comes before it. (GDN layers keep a state and no keys: they run such a
-step a level at a time with ``gdn_decode_step``, each token from its parent's state.)
+number within the request of the one that it was drafted behind, which comes before it.
+
+GDN layers keep a state and no keys. They run such a step a level of the trees at a time with ``gdn_decode_step``, each token from its
+parent's state and conv history; none of the calls above moves those, the caller does, who made the trees and knows their levels:
+
+    for at, above in levels:       # rows of the batch, and their parents' (of the first level: the requests' places)
+        out[at], conv[at], state[at] = gdn_decode_step(qkv[at], ..., conv[above], state[above], ...)
+
+and after verification request b goes on with those of row t.starts[b] + v.path[b, v.kept[b] - 1], or, in place i of a fork, of request
+places[i]. A level reads and writes whole states (4 H Dk Dv bytes a token), and its indexing copies them once more each way.
 """
 
 from __future__ import annotations
