@@ -390,7 +390,8 @@ int tjev_gdn_paged_attention(const tjev_gdn_paged_params* p, void* stream, const
 /* The same for trees of new tokens (drafts): a row attends to all keys before its request's new tokens and, of those, to the
  * ones named by its bits: bit j % 64 of ancestors[row, j / 64] (int64 [tokens, words]; see tjev_gdn_draft_tree) is the request's new token j,
  * whose key stands at lengths[b] - (starts[b + 1] - starts[b]) + j. A row may name any of them, or none; tokens from 64 words on cannot
- * be named. All else as above; the workspace has a size of its own. */
+ * be named. All else as above; the workspace has a size of its own. The kernels are chosen by table_width * page_size too, the most keys
+ * that a request may have: small batches in tables with room for many more than they hold take up to 60% longer. */
 size_t tjev_gdn_paged_tree_workspace_bytes(const tjev_gdn_paged_params* p);
 int tjev_gdn_paged_tree_attention(const tjev_gdn_paged_params* p, void* stream, const void* q,
                                   const void* k_cache, const void* v_cache,

@@ -41,9 +41,12 @@ AttnPlan plan_of(const tjev_gdn_paged_params* p, bool tree) {
   auto tiles_of = [&](int tile_rows) { return (rows / tile_rows + active) * p->kv_heads; };
   r.mixed = bf && top > 16 * r.nq;
   // Trees whose streamed tiles are at most kFewTurns units to a workgroup are streamed, and read their keys a few times: the many
-  // small parts are worked on at once (16/4 heads of 256: 8 trees of 12 over 1000, 28.4 us instead of 36.1 in tiles of 128; 8 of up to 8 over up to
-  // 3000, 19.3 and 37.2; 2 of 12 over 4000, 27.3 and 25.7. With a limit of 6, 16 of 12 over 1000 would take 40.0 instead of 37.7, one of 32 over
-  // 4000 at 32/8 of 128 25.6 instead of 21.9, but 32 of up to 12 over up to 1000 26.1 instead of 37.9: how even they are the host does not know).
+  // small parts are worked on at once. The host knows no lengths, so every tile is counted with keys to the table's end: in a table
+  // with room for many more keys than the requests have (32768, say) the same batches go to the tiles of 128, the slower ones for them.
+  // Streamed and in tiles of 128, 16/4 heads of 256: 8 trees of 12 over 1000 27.7 us and 36.0; 8 of up to 8 over up to 3000 26.3 and 38.4;
+  // one of 12 over 4000 19.8 and 26.2; 2 of 12 over 4000 25.6 and 25.5. Past the limit: 16 of 12 over 1000 39.5 and 37.5; one of 32 over 4000
+  // at 32/8 of 128 24.7 and 21.2; one of 12 over 30000 65.8 and 48.9; but 32 of up to 12 over up to 1000 32.4 and 36.8: how even they are
+  // the host does not know.
   constexpr int kFewTurns = 4;
   if (tree && r.mixed && tiles_of(16 * r.nq) * blocks <= kFewTurns * (long)most) r.mixed = false;
   const long tiles = tiles_of(r.mixed ? kWideRows : 16 * r.nq);

@@ -131,7 +131,9 @@ struct WalkEnd {
 };
 
 // The walk of a request, by one wave: the node it ends in, the child whose draft distribution is taken off (or -1), and how many
-// tokens it has. write: its path, accepted tokens and their number too.
+// tokens it has. write: its path, accepted tokens and their number too. Children that are looked at stand in a chain, and each behind the
+// first 64 tokens reads the ones before its group again (one tree of 50257 tokens in bf16, all but the root rejected: 16 of them
+// 13.7 us, 64 23, 128 51, 256 146, 512 495).
 struct End {
   long node, off, count;
 };

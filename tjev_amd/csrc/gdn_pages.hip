@@ -233,9 +233,9 @@ __device__ __forceinline__ void take(const ForkArgs& A, int r, const ForkNew& g,
 // that loses its holder costs one CU 5 ns (two atomics, two loads and two stores, each lane's of a line of its own), so this is for calls
 // that change few, which the host does not know and guesses. With lengths to keep (a step's roll back: most places go on, with
 // what they had) tables of up to kOneTurns * kOne entries: 64 places of 512 pages, a page of each given back, 18.6 us a call, in
-// launches of their own 26.7; with three whole rows 21.4 and 26.4, with twenty 70 and 26; all given back 178 and 26.5. Without (beams that go on from each other, samples)
-// up to kFewTurns * kOne: 64 of 64, all given back, 26.2 and 26.4, a page of each 18.7 and 26.6; half of 64 of 512, the rest twice,
-// would take 152 and 26.6.
+// launches of their own 26.7; with three whole rows 21.4 and 26.4, with twenty 70 and 26; all given back 178 and 26.5. Without (beams
+// that go on from each other, samples) up to kFewTurns * kOne: 64 of 64, all given back, 26.2 and 26.4, a page of each 18.7 and 26.6; half
+// of 64 of 512, the rest twice, would take 152 and 26.6. (Entries are the table's, not the requests': lengths are on the GPU.)
 constexpr int kOne = 1024, kOneTurns = 64, kFewTurns = 4;
 constexpr int kBatch = 4;  // entries that a thread has on their way at once
 
@@ -520,7 +520,7 @@ struct ForkCopyArgs {
   bool known, first;  // where names pages; of the launches (the first takes them)
 };
 
-// Bound by memory: the last pages of 192 samples, 6 layers of 4 heads of 256 in pages of 64, 215 MB, 50 us, 4.3 TB/s (a large copy has 5.0).
+// Bound by memory: the last pages of 192 samples, 6 layers of 4 heads of 256 in pages of 64, 215 MB, 51 us, 4.2 TB/s (a large copy has 5.0).
 // The copies: a workgroup per new place, cache, group of columns and kCopyTurns times the tokens that its threads have on their way at
 // once. The free list is whole by now: a copy may take a page that
 // was given back (which no copy is made of: what writers leave is held by others).

@@ -9,7 +9,7 @@
     ...
     v = verify_drafts(tokens, target_probs, t.starts, uniforms, parents=parents, max_new=M)
     lengths = paged_compact(caches, t.block_table, t.starts, t.lengths, v.path, v.kept)
-    f = paged_fork(caches, t.block_table, t.lengths, places, lengths, free_pages, t.taken, shared, page_size=P)
+    f = paged_fork(caches, t.block_table, t.lengths, places, lengths[places], free_pages, t.taken, shared, page_size=P)
 
 A request's new tokens are a tree. Token 0 is its root, the token that the last step ended with; ``parents`` holds for every other the
 number within the request of the one that it was drafted behind, which comes before it.

@@ -290,7 +290,13 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ones that its row of ``ancestors`` [N, W] int64 names (bit j % 64 of word j / 64: the request's j-th), in whatever order they
     stand; as ``draft_tree`` makes them these are its ancestors and itself. A row may name any of them, or none (one that then
     has no keys is 0); a request's tokens from 64 W on cannot be named. ``max_new``: the most new tokens of one request; it
-    chooses kernels and no row's keys. All else as for ``paged_attention``."""
+    chooses kernels and no row's keys. All else as for ``paged_attention``, but for which rows have their weights rounded in bf16:
+
+    Kernels are chosen by the table's width too, the only bound on the keys that the host has. Batches that may hold a request of more
+    than 16 tokens times query heads per key head (32 as there) go to the kernel for many rows, for those requests, except where all of
+    them in tiles of 16 (32) rows, each counted with M * page_size keys in blocks of 128, are at most 2048 blocks (3072 at head dims up
+    to 64): small batches in tables not much wider than they need, which take up to a third less time for it (one tree of 12 over 4000,
+    16/4 heads of 256: 20 us, in a table for 16384 keys or more 26)."""
     if ancestors.dim() != 2 or ancestors.shape[0] != q.shape[0] or ancestors.shape[1] < 1 or ancestors.dtype != torch.int64:
         raise ValueError(f"ancestors are [{q.shape[0]}, words] int64, not {tuple(ancestors.shape)} {ancestors.dtype}")
     _check_sizes(ancestors.shape[1])
@@ -392,10 +398,10 @@ def paged_compact(caches, block_table: torch.Tensor, starts: torch.Tensor, lengt
     """Moves the kept ones of every request's new tokens to the front of them, in all layers' caches at once, in place, and
     returns the lengths that are left [B] int32: token path[b, j] becomes the j-th, j < kept[b], as ``verify_drafts`` names them.
 
-    ``caches``: the (k_cache, v_cache) of every layer, alike in shape and strides, none of them twice or part of another (none: the lengths alone). ``starts`` and
-    ``lengths`` are the step's, with the new tokens. A request's numbers in ``path`` [B, max_new] grow; those that are less than their
-    place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct. What
-    stands behind a request's kept tokens is left as it was."""
+    ``caches``: the (k_cache, v_cache) of every layer, alike in shape and strides, none of them twice or part of another (none: the
+    lengths alone). ``starts`` and ``lengths`` are the step's, with the new tokens. A request's numbers in ``path`` [B, max_new] grow; those
+    that are less than their place, or no new token, are left out. A page that holds new tokens is held by one request; those are distinct.
+    What stands behind a request's kept tokens is left as it was."""
     _lib.not_recorded("paged_compact")
     like, layers, addresses = _layers("paged_compact", caches)
     p = _compact_params(
@@ -441,15 +447,15 @@ def paged_fork(caches, block_table: torch.Tensor, lengths: torch.Tensor, sources
     """Which requests go on, with what: place i of the new table with the first ``keep[i]`` tokens (None: all) of place
     ``sources[i]`` [B'] of ``block_table`` [B, M] (-1: it is unused). That is a batch's samples or beams (a source several times),
     a roll back behind rejected drafts (``keep`` shorter), requests that end (no place goes on from them) and a table made dense, all at
-    once, on the GPU. ``lengths`` [B] are those that the places have pages for: after a step the step's own (``PagedTables.lengths``), not what
-    was kept of it, or the pages of the rest would be nobody's.
+    once, on the GPU. ``lengths`` [B] are those that the places have pages for: after a step the step's own (``PagedTables.lengths``), not
+    what was kept of it, or the pages of the rest would be nobody's.
 
     ``shared`` [pages]: how many hold each page beside its first holder (0 in the beginning). Places share pages; but a last page with room
     in it, where the next tokens go, has one holder: the first place that goes on in it where nobody holds it otherwise, and for each
-    other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides, none of them twice, in
-    pages of up to 2^20 - 16 tokens; those may be none). Pages that nobody holds any more come back in front of index ``taken`` of ``free_pages`` [F], in the
-    table's order, and are the first to be taken again; the list needs room for them there, as it has where all of them were
-    taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
+    other one a page is taken and the tokens are copied in all layers' ``caches`` ((k_cache, v_cache) pairs, alike in shape and strides,
+    none of them twice, in pages of up to 2^20 - 16 tokens; those may be none). Pages that nobody holds any more come back in front of index
+    ``taken`` of ``free_pages`` [F], in the table's order, and are the first to be taken again; the list needs room for them there, as it
+    has where all of them were taken from it. A copy that finds no page gets -1, and ``taken`` is over F.
 
     A call with ``keep`` is taken to be a step's roll back, where few pages change hands; it is right with any, but slower than one without
     where thousands do (64 places of 512 pages, all given back: 180 us instead of 27).
