@@ -742,8 +742,8 @@ __device__ __forceinline__ void stream_tile(const Request& q, int b, const Part&
 // fragments by transposing LDS reads. The pieces of a row of K or V lie in LDS in an order that depends on the row
 // (swz), which spreads both kinds of read over the banks (no conflicts counted). Bound by the products and what
 // stands between them: 2048 tokens over 30000 at head dims 256, 128, 64 run at 945, 944, 810 TFLOP/s (a
-// warmer card 873, 877, 739), the matrix units busy for half of the cycles. The queries stay in registers (three fragments at 256 in LDS), the results too;
-// two workgroups to a CU cover each other's softmax and barriers.
+// warmer card 873, 877, 739), the matrix units busy for half of the cycles. The queries stay in registers (three fragments at 256 in LDS),
+// the results too; two workgroups to a CU cover each other's softmax and barriers.
 // The base of the powers follows the running maximum only when that has grown by more than 2^8: the rescaling
 // of the results is skipped otherwise (a softmax does not depend on its base; weights up to 2^8 have bf16's
 // relative precision like all others).

@@ -688,8 +688,8 @@ int tjev_gdn_verify_drafts(const tjev_gdn_draft_params* p, void* stream, const i
     return fail(TJEV_GDN_EINVAL, "the probabilities must be aligned to their elements");
   if (int s = gdn::poison_workspace(workspace, need, stream)) return s;
   const long slices = gdn::slices_of(p);
-  gdn::VerifyArgs A{p->tokens, p->max_new, p->target_stride, p->draft_stride, p->requests, p->vocab, (int)slices, (int)gdn::parts_of(p), tokens, parents, starts,
-                    uniforms, static_cast<const char*>(target), static_cast<const char*>(draft), tokens_out, path, kept};
+  gdn::VerifyArgs A{p->tokens, p->max_new, p->target_stride, p->draft_stride, p->requests, p->vocab, (int)slices, (int)gdn::parts_of(p), tokens,
+                    parents, starts, uniforms, static_cast<const char*>(target), static_cast<const char*>(draft), tokens_out, path, kept};
   gdn::lay_out(p, &A, static_cast<char*>(workspace));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 sums((unsigned)slices, (unsigned)p->requests), draw((unsigned)p->requests), block(gdn::kThreads);

@@ -294,9 +294,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
 
     Kernels are chosen by the table's width too, the only bound on the keys that the host has. Batches that may hold a request of more
     than 16 tokens times query heads per key head (32 as there) go to the kernel for many rows, for those requests, except where all of
-    them in tiles of 16 (32) rows, each counted with M * page_size keys in blocks of 128, are at most 2048 blocks (3072 at head dims up
-    to 64): small batches in tables not much wider than they need, which take up to a third less time for it (one tree of 12 over 4000,
-    16/4 heads of 256: 20 us, in a table for 16384 keys or more 26)."""
+    them in tiles of 16 (32) rows, each counted as M * page_size keys in blocks of 128 and three blocks more, are at most four blocks to
+    a workgroup, of which there are 512 (768 at head dims up to 64): small batches in tables not much wider than they need, which take up
+    to a third less time for it (one tree of 12 over 4000, 16/4 heads of 256: 20 us, in a table for 16384 keys or more 26)."""
     if ancestors.dim() != 2 or ancestors.shape[0] != q.shape[0] or ancestors.shape[1] < 1 or ancestors.dtype != torch.int64:
         raise ValueError(f"ancestors are [{q.shape[0]}, words] int64, not {tuple(ancestors.shape)} {ancestors.dtype}")
     _check_sizes(ancestors.shape[1])
